@@ -384,6 +384,40 @@ int teeny_argmax_rows(const void* x, int64_t* out, int rows, int cols, int dtype
 int teeny_argmax_rows_advance(const void* x, int64_t* out, int rows, int cols, int dtype,
                               int* advance, hipStream_t stream);
 
+/* Sampling: one token per row of logits [rows, cols] (rows ld elements apart;
+ * ld 0: one row for all) from the random number u[row] in [0, 1).  Replaces
+ * temperature_sample (examples/llama_generate.rs:254-275), a host loop over
+ * softmax(logits / T); the filters have no counterpart there.
+ *   order     higher logit first, lower index first among equal ones
+ *   top_k     keeps the first k of the order (0, or cols and more: all)
+ *   top_p     of those, every token before which less than top_p of their
+ *             probability lies (1: all)
+ *   min_p     of those, tokens at least min_p times as probable as the first
+ *             (0: all)
+ *   out[row]  the first kept token, in index order, whose running probability
+ *             exceeds u times the kept probability
+ * temperature 0 takes the first of the order (the lowest index of the maximum,
+ * where teeny_argmax_rows takes the last).  -inf and NaN logits are never drawn;
+ * a row with no other gives -1; +inf logits share a row among themselves.
+ * Probabilities are held as whole numbers of 2^-44 of the row's largest and
+ * summed exactly: the result does not depend on timing or on the other rows, and
+ * a token below 2^-45 of the most probable one is not drawn.
+ * Each setting is a value for every row, or (temperature_rows, ... not null) one
+ * per row in device memory, read when the kernel runs: there a temperature that
+ * is not above 0 counts as 0, a top_k below 1 as off, a top_p not below 1 as
+ * off and one not above 0 as keeping one token, a min_p not above 0 as off.  u
+ * outside [0, 1) or NaN is taken as its nearest border (NaN as 0).
+ * dtype of the logits: fp32 or bf16.  cols <= 2^19, rows <= 65535.
+ * advance: as teeny_argmax_rows_advance; may be null.  workspace:
+ * teeny_sample_rows_workspace_bytes(rows, cols) bytes, 16-byte aligned. */
+size_t teeny_sample_rows_workspace_bytes(int rows, int cols);
+int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int cols,
+                      double temperature, const float* temperature_rows, int top_k,
+                      const int32_t* top_k_rows, double top_p, const float* top_p_rows,
+                      double min_p, const float* min_p_rows, int64_t* out, int dtype,
+                      int32_t* advance, void* workspace, size_t workspace_bytes,
+                      hipStream_t stream);
+
 /* Linear layer y[M, N] = x[M, K] . w[N, K]^T in bf16, any M >= 1: replaces
  * the external teeny-core Linear behind sym_linear (src/layers/mod.rs:54-58).
  * Up to 16 rows (a KV-cached decode step) with N % 128 == 0 and K % 128 == 0

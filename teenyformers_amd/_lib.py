@@ -34,6 +34,8 @@ _fns: dict = {}  # entry points by name, for call()
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_d = ctypes.c_double
+_l = ctypes.c_long
 _sz = ctypes.c_size_t
 
 _SIGNATURES = {
@@ -87,6 +89,9 @@ _SIGNATURES = {
     "teeny_embed_rmsnorm_fwd": ([_p] * 5 + [_i, _i, _i, _f, _i, _i, _p], _i),
     "teeny_argmax_rows_advance": ([_p, _p, _i, _i, _i, _p, _p], _i),
     "teeny_argmax_rows": ([_p, _p, _i, _i, _i, _p], _i),
+    "teeny_sample_rows_workspace_bytes": ([_i, _i], _sz),
+    "teeny_sample_rows": ([_p, _l, _p, _i, _i, _d, _p, _i, _p, _d, _p, _d, _p, _p, _i, _p, _p, _sz,
+                           _p], _i),
     "teeny_linear_bf16": ([_p, _p, _p, _i, _i, _i, _p], _i),
     "teeny_gemm_bf16": ([_p, _p, _p, _i, _i, _i, _p], _i),
     "teeny_linear_swiglu_bf16": ([_p, _p, _p, _i, _i, _i, _p], _i),

@@ -36,6 +36,7 @@
   X(fa2_bwd_bf16)        \
   X(llama)               \
   X(decode_bf16)         \
+  X(sample)              \
   X(linear_bf16)         \
   X(gemm_bf16)           \
   X(gemm_f32)
@@ -1292,6 +1293,65 @@ int teeny_argmax_rows_advance(const void* x, int64_t* out, int rows, int cols, i
   snprintf(name, sizeof name, "teeny_argmax_rows_%s", dtype_tag(dtype));
   void* args[] = {&x, &out, &cols, &advance};
   return launch(name, dim3(rows), dim3(1024), 0, stream, args);
+}
+
+// Sampling (sample.hip): the records of the chunks that a row is summed in, and
+// with filters the chunks' weights and counts by bin.
+namespace {
+constexpr int kSampleChunk = 8192, kSampleBins = 180;
+constexpr int kSampleCols = 1 << 19;  // weights of 2^44 at most: no sum overflows
+constexpr size_t kSampleRec = 32;     // Chunk in sample.hip
+struct SampleArgs {                   // Args in sample.hip
+  double t, p, m;
+  const float *ts, *ps, *ms;
+  const int32_t* ks;
+  int k;
+};
+// (a row may start up to 7 elements past a 16-byte boundary)
+int sample_chunks(int cols) { return (cols + 7 + kSampleChunk - 1) / kSampleChunk; }
+}  // namespace
+
+size_t teeny_sample_rows_workspace_bytes(int rows, int cols) {
+  if (rows <= 0 || rows > 65535 || cols <= 0 || cols > kSampleCols) return 0;
+  const size_t n = (size_t)rows * sample_chunks(cols);
+  return align256(n * kSampleRec) + align256(n * kSampleBins * sizeof(uint64_t)) +
+         align256(n * kSampleBins * sizeof(uint32_t));
+}
+
+int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int cols,
+                      double temperature, const float* temperature_rows, int top_k,
+                      const int32_t* top_k_rows, double top_p, const float* top_p_rows,
+                      double min_p, const float* min_p_rows, int64_t* out, int dtype,
+                      int32_t* advance, void* workspace, size_t workspace_bytes,
+                      hipStream_t stream) {
+  if (!logits || !u || !out) return TEENY_ERR_NULL_POINTER;
+  if (!dtype_ok(dtype)) return TEENY_ERR_UNSUPPORTED;
+  if (rows <= 0 || rows > 65535 || cols <= 0 || cols > kSampleCols || ld < 0 ||
+      (ld < cols && ld != 0))
+    return TEENY_ERR_INVALID_SHAPE;
+  if ((uintptr_t)logits % dtype_size(dtype) != 0) return TEENY_ERR_INVALID_VALUE;
+  if (!temperature_rows && !(temperature >= 0.0)) return TEENY_ERR_INVALID_VALUE;
+  if (!top_k_rows && top_k < 0) return TEENY_ERR_INVALID_VALUE;
+  if (!top_p_rows && !(top_p > 0.0 && top_p <= 1.0)) return TEENY_ERR_INVALID_VALUE;
+  if (!min_p_rows && !(min_p >= 0.0 && min_p <= 1.0)) return TEENY_ERR_INVALID_VALUE;
+  if (!workspace || workspace_bytes < teeny_sample_rows_workspace_bytes(rows, cols))
+    return TEENY_ERR_WORKSPACE;
+  if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
+  int n_ch = sample_chunks(cols);
+  const size_t n = (size_t)rows * n_ch;
+  char* rec = (char*)workspace;
+  char* mass = rec + align256(n * kSampleRec);
+  char* cnt = mass + align256(n * kSampleBins * sizeof(uint64_t));
+  SampleArgs a{temperature, top_p, min_p, temperature_rows, top_p_rows, min_p_rows, top_k_rows,
+               top_k};
+  char name[48];
+  snprintf(name, sizeof name, "teeny_sample_scan_%s", dtype_tag(dtype));
+  void* a0[] = {&logits, &ld, &cols, &a, &rec, &cnt, &mass};
+  int rc = launch(name, dim3((unsigned)n_ch, (unsigned)rows), dim3(1024), 0, stream, a0);
+  if (rc) return rc;
+  snprintf(name, sizeof name, "teeny_sample_draw_%s", dtype_tag(dtype));
+  void* a1[] = {&logits, &ld, &cols, &a, &u, &rec, &cnt, &mass, &n_ch, &out, &advance};
+  return launch(name, dim3((unsigned)rows), dim3(1024), 0, stream, a1);
 }
 
 // Decode-step linear layers (linear_bf16.hip): 512 threads, 128 W rows per

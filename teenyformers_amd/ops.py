@@ -604,6 +604,93 @@ def argmax_rows(x, out=None, advance=None):
     return out
 
 
+def _on_device_of(t: torch.Tensor):
+    """The context in which a call on t runs: t's device current (its current
+    stream then is the one that _stream gives)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _per_row(name: str, value, rows: int, dtype, like: torch.Tensor):
+    """A sampling setting as (number, device tensor or None)."""
+    if not isinstance(value, torch.Tensor):
+        return value, None
+    if (value.dtype != dtype or value.numel() != rows or value.device != like.device
+            or not value.is_contiguous()):
+        raise ValueError(f"sample_rows: {name} is a number or a contiguous {dtype} tensor with a "
+                         "value per row, on the logits' device")
+    return 0, value
+
+
+def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+                min_p=0.0, out: torch.Tensor | None = None, advance: torch.Tensor | None = None,
+                workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row of logits [..., V] (fp32 or bf16) from the random
+    numbers u (fp32, one per row, in [0, 1)) -> int64 [...].
+
+    softmax(logits / temperature), cut by top_k, then top_p (the shortest leading
+    part, by probability, that holds top_p of what top_k left), then min_p (tokens
+    at least min_p times as probable as the first); the first kept token in index
+    order whose running probability exceeds u times the kept probability, the
+    reference's walk (examples/llama_generate.rs:254-275).  Equal logits are
+    ordered by index, the lowest first.  temperature 0: the lowest index of the
+    row's maximum (argmax_rows: the last).  -inf and NaN logits are never drawn;
+    a row without any other gives -1.
+
+    temperature, top_k (0: off), top_p (1: off) and min_p (0: off) are numbers, or
+    device tensors with a value per row (fp32; top_k int32), read when the
+    kernels run, so a captured call can be replayed with others.  Rows may lie
+    apart (a slice of padded columns) or be one row (expand).  advance: as
+    argmax_rows.  workspace: teeny_sample_rows_workspace_bytes bytes (uint8) that
+    no call on another stream uses at the same time; by default a fresh one."""
+    if not logits.is_cuda:
+        raise ValueError("teenyformers_amd ops take device tensors (no CPU fallback)")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("sample_rows: logits are [..., V] with V >= 1")
+    code = _code(logits)
+    shape, V = logits.shape[:-1], logits.shape[-1]
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    if x.stride(1) != 1 and V > 1 or 0 < x.stride(0) < V:
+        x = x.contiguous()
+    rows = x.shape[0]
+    _dev(u, out, advance, workspace)
+    if u.dtype != torch.float32 or u.numel() != rows or u.device != x.device:
+        raise ValueError("sample_rows: u is fp32 with a value per row, on the logits' device")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int64, device=x.device)
+    elif out.dtype != torch.int64 or out.numel() != rows or out.device != x.device:
+        raise ValueError("sample_rows: out is int64 with a value per row, on the logits' device")
+    if advance is not None and (advance.dtype != torch.int32 or advance.numel() != 1
+                                or advance.device != x.device):
+        raise ValueError("sample_rows: advance is one int32 on the logits' device")
+    t, ts = _per_row("temperature", temperature, rows, torch.float32, x)
+    k, ks = _per_row("top_k", top_k, rows, torch.int32, x)
+    p, ps = _per_row("top_p", top_p, rows, torch.float32, x)
+    m, ms = _per_row("min_p", min_p, rows, torch.float32, x)
+    if ts is None and not t >= 0.0:
+        raise ValueError("sample_rows: temperature must be at least 0")
+    if ks is None and k < 0:
+        raise ValueError("sample_rows: top_k must be at least 0 (0: off)")
+    if ps is None and not 0.0 < p <= 1.0:
+        raise ValueError("sample_rows: top_p must be in (0, 1]")
+    if ms is None and not 0.0 <= m <= 1.0:
+        raise ValueError("sample_rows: min_p must be in [0, 1]")
+    if rows == 0:
+        return out
+    need = _lib.lib().teeny_sample_rows_workspace_bytes(rows, V)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    elif workspace.device != x.device:
+        raise ValueError("sample_rows: workspace must be on the logits' device")
+    with _on_device_of(x):
+        call("teeny_sample_rows", _p(x), x.stride(0) if rows > 1 else V, _p(u), rows, V, float(t),
+             _p(ts), min(int(k), 2 ** 31 - 1), _p(ks), float(p), _p(ps), float(m), _p(ms), _p(out),
+             code, _p(advance), _p(workspace), workspace.numel() * workspace.element_size(),
+             _stream())
+    return out
+
+
 def _no_grad(x2: torch.Tensor, w: torch.Tensor) -> bool:
     # the library's linear kernels have no backward: autograd uses torch's GEMM
     return not (torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad))

@@ -397,3 +397,28 @@ def test_fused_decode_cache_limit(monkeypatch):
     monkeypatch.setattr(ops, "decode_qkv_splits", lambda *a: 16)
     assert model._fused_decode(qkv, SimpleNamespace(capacity=8_388_607))
     assert not model._fused_decode(qkv, SimpleNamespace(capacity=8_388_608))
+
+
+def test_sample_rows_validation(L):
+    """The sampler's refusals, and the workspace sizes of shapes that it does not take."""
+    def f(**kw):
+        a = dict(x=P, ld=100, u=P, rows=4, cols=100, t=1.0, ts=None, k=0, ks=None, p=1.0, ps=None, m=0.0,
+                 ms=None, out=P, dtype=BF16, adv=None, ws=P, wsb=1 << 40)
+        a.update(kw)
+        return L.teeny_sample_rows(a["x"], a["ld"], a["u"], a["rows"], a["cols"], a["t"], a["ts"], a["k"],
+                                   a["ks"], a["p"], a["ps"], a["m"], a["ms"], a["out"], a["dtype"],
+                                   a["adv"], a["ws"], a["wsb"], None)
+    nan = float("nan")
+    for kw in (dict(x=None), dict(u=None), dict(out=None)):
+        assert f(**kw) == NULLP
+    assert f(dtype=7) == UNSUP
+    for kw in (dict(rows=0), dict(rows=65536), dict(cols=0), dict(cols=(1 << 19) + 1), dict(ld=99),
+               dict(ld=-100)):
+        assert f(**kw) == SHAPE
+    for kw in (dict(t=-1.0), dict(t=nan), dict(k=-1), dict(p=0.0), dict(p=1.01), dict(p=nan), dict(m=-0.1),
+               dict(m=1.1), dict(m=nan), dict(x=P + 1), dict(ws=P + 8)):
+        assert f(**kw) == VALUE
+    need = L.teeny_sample_rows_workspace_bytes(4, 100)
+    assert need > 0 and f(wsb=need - 1) == WS and f(ws=None) == WS
+    for rows, cols in ((0, 5), (65536, 5), (5, 0), (5, (1 << 19) + 1)):
+        assert L.teeny_sample_rows_workspace_bytes(rows, cols) == 0
