@@ -373,6 +373,36 @@ int teeny_decode_attention_dev(const void* q, const void* k_cache, const void* v
                                int dtype, void* workspace, size_t workspace_bytes,
                                hipStream_t stream);
 
+/* Attention of sequences that share a prefix (n samples of one prompt, requests
+ * behind one system prompt), whose keys and values are stored and read once for
+ * the batch: q [B, Hq, n_new, D] holds n_new new tokens per sequence, k/v_prefix
+ * [Hkv, prefix_len, D] the prefix in rows 0 .. n_prefix-1 (a cache of one
+ * sequence; n_prefix 0: none, the pointers may be null), k/v_cache [B, Hkv,
+ * cache_len, D] each sequence's own rows.  Row s of sequence b attends to the
+ * prefix and to cache rows 0 .. n_past[b] + s (the new tokens' own rows are in
+ * the cache already); rows past cache_len do not exist, and a row that sees no
+ * key at all gives zeros.  n_past: int32 device memory read when the kernels run,
+ * n_past_stride 1 for one value per sequence, 0 for one for all; or null, and
+ * n_past_host (0 .. cache_len - n_new) counts for all.
+ * o [B, Hq, n_new, D], or with merged [B, n_new, Hq * D]
+ * (teeny_merge_heads of the former, the same bits).  softmax_scale as the
+ * forwards'.  head_dim: fp32 8, 16, 32, 64, 128; bf16 64, 128; bf16 tensors are
+ * 16-byte aligned.  bf16, n_new > 1: the rows n_past[b] .. n_past[b] + n_new - 1
+ * must be finite, as the causal forward's; cache rows past them and prefix rows
+ * past n_prefix are never read.  workspace:
+ * teeny_shared_prefix_attention_workspace_bytes bytes, 16-byte aligned.  No
+ * reference counterpart (it has no KV cache). */
+size_t teeny_shared_prefix_attention_workspace_bytes(int batch, int n_heads_q, int n_heads_kv,
+                                                     int n_new, int n_prefix, int cache_len,
+                                                     int head_dim, int dtype);
+int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix,
+                                  const void* k_cache, const void* v_cache, void* o, int batch,
+                                  int n_heads_q, int n_heads_kv, int n_new, int n_prefix,
+                                  int prefix_len, const int32_t* n_past, int n_past_stride,
+                                  int n_past_host, int cache_len, int head_dim,
+                                  float softmax_scale, int merged, int dtype, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream);
+
 /* Row argmax of x [rows, cols] -> out[rows] (int64): the reference's greedy
  * choice (examples/llama_generate.rs:252-257), the LAST index among equal
  * maxima (Rust's Iterator::max_by); NaN, on which the reference's comparison

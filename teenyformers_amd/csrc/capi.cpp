@@ -36,6 +36,7 @@
   X(fa2_bwd_bf16)        \
   X(llama)               \
   X(decode_bf16)         \
+  X(prefix_attn)         \
   X(sample)              \
   X(linear_bf16)         \
   X(gemm_bf16)           \
@@ -1276,6 +1277,112 @@ int teeny_decode_attention_dev(const void* q, const void* k_cache, const void* v
   return decode_attention_impl(q, k_cache, v_cache, o, batch, n_heads_q, n_heads_kv, n_past,
                                max_keys, cache_len, head_dim, softmax_scale, dtype, workspace,
                                workspace_bytes, stream);
+}
+
+// Attention over a shared prefix (prefix_attn.hip): shares of the prefix for each
+// tile of a kv head's rows, shares of each sequence's own keys, and a merge.
+namespace {
+struct PrefixShape {  // Shape in prefix_attn.hip
+  int batch, hkv, gs, s;
+  int n_prefix, prefix_len, cache_len;
+  const int32_t* past;
+  int past_stride, past_imm;
+  int p_splits, p_keys, row_tiles, o_splits;
+  float scale;
+};
+struct PrefixParts {  // Parts in prefix_attn.hip
+  float *m, *l, *o;
+};
+struct PrefixPlan {
+  int nw, rows;  // wavefronts per workgroup, rows per row tile
+  int row_tiles, p_splits, p_keys, o_splits;
+  long groups;   // of 32 (fp32: 16) rows of a sequence and kv head
+};
+PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_new, int n_prefix, int cache_len,
+                       int dtype) {
+  PrefixPlan p{};
+  const long gs = (long)(hq / hkv) * n_new, rows = batch * gs, cus = device_cus();
+  const bool f32 = dtype == TEENY_F32;
+  p.nw = f32 ? 1 : rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
+  p.rows = f32 ? 16 : 32 * p.nw;
+  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
+  const long slots = cus * (f32 ? 4 : p.nw == 8 ? 1 : p.nw == 4 ? 2 : 3);
+  if (n_prefix > 0) {
+    const long want = std::max(1L, slots / ((long)p.row_tiles * hkv));
+    const long per = ((n_prefix + want - 1) / want + 31) / 32 * 32;
+    p.p_keys = (int)std::max(per, f32 ? 32L : 64L);
+    p.p_splits = (n_prefix + p.p_keys - 1) / p.p_keys;
+  }
+  p.groups = (gs + (f32 ? 15 : 31)) / (f32 ? 16 : 32);
+  const long items = (long)batch * hkv * p.groups;
+  const long most = (cache_len + 128L * p.nw - 1) / (128L * p.nw);
+  p.o_splits = (int)std::max(1L, std::min(std::min(most, 16L), slots / std::max(1L, items)));
+  return p;
+}
+}  // namespace
+
+size_t teeny_shared_prefix_attention_workspace_bytes(int batch, int n_heads_q, int n_heads_kv,
+                                                     int n_new, int n_prefix, int cache_len,
+                                                     int head_dim, int dtype) {
+  if (batch <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0 ||
+      n_new <= 0 || n_prefix < 0 || cache_len <= 0 || head_dim <= 0 || !dtype_ok(dtype))
+    return 0;
+  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
+  const size_t rows = (size_t)batch * n_heads_q * n_new * (p.p_splits + p.o_splits);
+  return 2 * align256(rows * sizeof(float)) + align256(rows * head_dim * sizeof(float));
+}
+
+int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix,
+                                  const void* k_cache, const void* v_cache, void* o, int batch,
+                                  int n_heads_q, int n_heads_kv, int n_new, int n_prefix,
+                                  int prefix_len, const int32_t* n_past, int n_past_stride,
+                                  int n_past_host, int cache_len, int head_dim,
+                                  float softmax_scale, int merged, int dtype, void* workspace,
+                                  size_t workspace_bytes, hipStream_t stream) {
+  if (!q || !k_cache || !v_cache || !o) return TEENY_ERR_NULL_POINTER;
+  if (n_prefix > 0 && (!k_prefix || !v_prefix)) return TEENY_ERR_NULL_POINTER;
+  if (!dtype_ok(dtype) || !fa2_head_dim_ok(head_dim, dtype)) return TEENY_ERR_UNSUPPORTED;
+  if (batch <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0 ||
+      n_new <= 0 || n_prefix < 0 || prefix_len < n_prefix || cache_len < n_new ||
+      (long)batch * n_heads_q * n_new >= kMaxElems / head_dim ||
+      (long)prefix_len * head_dim * 2 >= kMaxElems || (long)cache_len * head_dim * 2 >= kMaxElems)
+    return TEENY_ERR_INVALID_SHAPE;
+  if (n_past ? (n_past_stride != 0 && n_past_stride != 1)
+             : (n_past_host < 0 || n_past_host > cache_len - n_new))
+    return TEENY_ERR_INVALID_VALUE;
+  if (!scale_ok(softmax_scale, dtype)) return TEENY_ERR_INVALID_VALUE;
+  const uintptr_t at = (uintptr_t)q | (uintptr_t)o | (uintptr_t)k_cache | (uintptr_t)v_cache |
+                       (n_prefix > 0 ? (uintptr_t)k_prefix | (uintptr_t)v_prefix : 0);
+  if (at % (dtype == TEENY_BF16 ? 16 : 4) != 0) return TEENY_ERR_INVALID_VALUE;
+  if (!workspace || workspace_bytes < teeny_shared_prefix_attention_workspace_bytes(
+                                          batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len,
+                                          head_dim, dtype))
+    return TEENY_ERR_WORKSPACE;
+  if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
+  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
+  const int shares = p.p_splits + p.o_splits;
+  const size_t rows = (size_t)batch * n_heads_q * n_new;
+  PrefixParts parts{(float*)workspace,
+                    (float*)((char*)workspace + align256(rows * shares * sizeof(float))),
+                    (float*)((char*)workspace + 2 * align256(rows * shares * sizeof(float)))};
+  PrefixShape a{batch,      n_heads_kv, n_heads_q / n_heads_kv * n_new, n_new, n_prefix, prefix_len,
+                cache_len,  n_past,     n_past_stride, n_past_host,
+                p.p_splits, p.p_keys,   p.row_tiles,   p.o_splits,  softmax_scale};
+  const long wgs = (long)p.p_splits * p.row_tiles * n_heads_kv +
+                   (long)p.o_splits * batch * n_heads_kv * p.groups;
+  if (wgs >= (1L << 31) || (long)rows >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+  char name[64];
+  if (dtype == TEENY_BF16)
+    snprintf(name, sizeof name, "teeny_prefix_attn_bf16_d%d_w%d", head_dim, p.nw);
+  else
+    snprintf(name, sizeof name, "teeny_prefix_attn_f32_d%d", head_dim);
+  void* a0[] = {&q, &k_prefix, &v_prefix, &k_cache, &v_cache, &a, &parts};
+  int rc = launch(name, dim3((unsigned)wgs), dim3(64 * p.nw), 0, stream, a0);
+  if (rc) return rc;
+  snprintf(name, sizeof name, "teeny_prefix_merge_%s", dtype_tag(dtype));
+  void* a1[] = {&parts, &o, &a, &head_dim, &merged};
+  const unsigned lds = ((unsigned)(shares + 3) / 4 * 4 + 1024) * 4;
+  return launch(name, dim3((unsigned)rows), dim3(256), lds, stream, a1);
 }
 
 int teeny_argmax_rows(const void* x, int64_t* out, int rows, int cols, int dtype,

@@ -586,6 +586,82 @@ def decode_qkv_attention(qkv: "Partials", k_cache, v_cache, n_past, n_heads_q: i
     return out
 
 
+def _on_device_of(t: torch.Tensor):
+    """The context in which a call on t runs: t's device current (its current
+    stream then is the one that _stream gives)."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: int, n_past,
+                            softmax_scale: float | None = None, merged: bool = False, out=None,
+                            workspace=None):
+    """Attention of sequences that share a prefix, whose keys and values are
+    stored and read once for the batch (teeny_shared_prefix_attention): q
+    [B, Hq, D] (one new token a sequence) or [B, Hq, S, D]; k/v_prefix
+    [Hkv, Lp, D] (or [1, Hkv, Lp, D], a one-sequence cache), rows 0 ..
+    n_prefix-1; k/v_cache [B, Hkv, L, D], each sequence's own rows, the new
+    tokens' among them.  Row s of sequence b attends to the prefix and to its
+    cache rows 0 .. n_past[b] + s.  n_past: an int, or an int32 device tensor of
+    one value or one per sequence, read when the kernels run (for captured
+    graphs).  Returns o in q's shape, or with merged [B, S, Hq*D].  No gradients.
+    workspace: uint8, teeny_shared_prefix_attention_workspace_bytes, that no call
+    on another stream uses at the same time; by default a fresh one."""
+    if q.dim() not in (3, 4):
+        raise ValueError("shared_prefix_attention: q is [B, Hq, D] or [B, Hq, S, D]")
+    if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4:
+        k_prefix, v_prefix = k_prefix[0], v_prefix[0]
+    _dev(q, k_prefix, v_prefix, k_cache, v_cache, out, workspace)
+    B, Hq, D = q.shape[0], q.shape[1], q.shape[-1]
+    S = q.shape[2] if q.dim() == 4 else 1
+    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[0] != B
+            or k_cache.shape[3] != D):
+        raise ValueError("shared_prefix_attention: the caches are [B, Hkv, L, D] matching q")
+    Hkv, L = k_cache.shape[1], k_cache.shape[2]
+    if (k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != Hkv
+            or k_prefix.shape[2] != D):
+        raise ValueError("shared_prefix_attention: the prefix is [Hkv, Lp, D] matching the caches")
+    ts = (k_prefix, v_prefix, k_cache, v_cache)
+    if any(t.dtype != q.dtype for t in ts):
+        raise TypeError("shared_prefix_attention: q, the prefix and the caches share a dtype")
+    if any(t.device != q.device for t in ts):
+        raise ValueError("shared_prefix_attention: all tensors are on one device")
+    if not 0 <= n_prefix <= k_prefix.shape[1]:
+        raise ValueError("shared_prefix_attention: n_prefix must lie in the prefix's rows")
+    code = _code(q)
+    past, stride, past_host = None, 0, 0
+    if isinstance(n_past, torch.Tensor):
+        if (n_past.dtype != torch.int32 or n_past.device != q.device or not n_past.is_contiguous()
+                or n_past.numel() not in (1, B)):
+            raise TypeError("n_past must be an int, or an int32 tensor of one value or one per "
+                            "sequence on q's device")
+        past, stride = n_past, int(n_past.numel() == B)
+    else:
+        past_host = int(n_past)
+        if not 0 <= past_host <= L - S:
+            raise ValueError("shared_prefix_attention: rows n_past .. n_past + S - 1 must lie in "
+                             "the cache")
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    shape = (B, S, Hq * D) if merged else tuple(q.shape)
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError(f"shared_prefix_attention: out must be {shape} of q's type and device")
+    if workspace is None:
+        need = _lib.lib().teeny_shared_prefix_attention_workspace_bytes(B, Hq, Hkv, S, n_prefix, L, D,
+                                                                        code)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.device != q.device:
+        raise ValueError("shared_prefix_attention: workspace must be on q's device")
+    with _on_device_of(q):
+        call("teeny_shared_prefix_attention", _p(q), _p(k_prefix), _p(v_prefix), _p(k_cache),
+             _p(v_cache), _p(out), B, Hq, Hkv, S, n_prefix, k_prefix.shape[1], _p(past), stride,
+             past_host, L, D, scale, int(bool(merged)), code, _p(workspace),
+             workspace.numel() * workspace.element_size(), _stream())
+    return out
+
+
 def argmax_rows(x, out=None, advance=None):
     """x [rows, cols] -> int64 [rows]: the last index of each row's maximum,
     the reference's greedy choice (examples/llama_generate.rs:252-257,
@@ -602,14 +678,6 @@ def argmax_rows(x, out=None, advance=None):
     call("teeny_argmax_rows_advance", _p(x2), _p(out), rows, cols, _code(x2), _p(advance),
          _stream())
     return out
-
-
-def _on_device_of(t: torch.Tensor):
-    """The context in which a call on t runs: t's device current (its current
-    stream then is the one that _stream gives)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
 
 
 def _per_row(name: str, value, rows: int, dtype, like: torch.Tensor):

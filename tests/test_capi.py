@@ -422,3 +422,30 @@ def test_sample_rows_validation(L):
     assert need > 0 and f(wsb=need - 1) == WS and f(ws=None) == WS
     for rows, cols in ((0, 5), (65536, 5), (5, 0), (5, (1 << 19) + 1)):
         assert L.teeny_sample_rows_workspace_bytes(rows, cols) == 0
+
+
+def test_shared_prefix_attention_validation(L):
+    """Refusals of the attention over a shared prefix."""
+    def f(**kw):
+        a = dict(q=P, kp=P, vp=P, k=P, v=P, o=P, b=2, hq=4, hkv=2, s=1, np=100, lp=128, past=None, st=0,
+                 host=5, L=64, d=64, scale=0.125, merged=0, dtype=BF16, ws=P, wsb=1 << 40)
+        a.update(kw)
+        return L.teeny_shared_prefix_attention(
+            a["q"], a["kp"], a["vp"], a["k"], a["v"], a["o"], a["b"], a["hq"], a["hkv"], a["s"], a["np"],
+            a["lp"], a["past"], a["st"], a["host"], a["L"], a["d"], a["scale"], a["merged"], a["dtype"],
+            a["ws"], a["wsb"], None)
+    for n in ("q", "kp", "vp", "k", "v", "o"):
+        assert f(**{n: None}) == NULLP
+    for kw in (dict(d=96), dict(d=32), dict(dtype=7), dict(d=256, dtype=F32)):
+        assert f(**kw) == UNSUP
+    for kw in (dict(b=0), dict(hq=3), dict(hkv=0), dict(s=0), dict(np=-1), dict(np=129), dict(L=0),
+               dict(s=65), dict(L=1 << 24), dict(lp=1 << 24), dict(b=1 << 25)):
+        assert f(**kw) == SHAPE, kw
+    for kw in (dict(host=-1), dict(host=64), dict(past=P, st=2), dict(scale=0.0), dict(q=P + 2),
+               dict(o=P + 8), dict(kp=P + 4), dict(ws=P + 8), dict(scale=float("inf"))):
+        assert f(**kw) == VALUE, kw
+    assert f(q=P + 2, dtype=F32) == VALUE
+    need = L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 100, 64, 64, BF16)
+    assert need > 0 and f(wsb=need - 1) == WS and f(ws=None) == WS
+    assert L.teeny_shared_prefix_attention_workspace_bytes(2, 3, 2, 1, 100, 64, 64, BF16) == 0
+    assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, -1, 64, 64, BF16) == 0
