@@ -552,6 +552,18 @@ int teeny_qkv_rope_split_partials_dev(const float* parts, int n_parts, void* q_o
                                       int n_heads_kv, int head_dim, float ln_rope_base,
                                       int dtype, hipStream_t stream);
 
+/* The QKV split of sequences behind a shared prefix: token s of sequence b goes
+ * to cache row r = row0[b row0_stride] + s (row0: int32 device memory,
+ * row0_stride 1 or 0 as n_past of teeny_shared_prefix_attention; null:
+ * row0_host for all), its rotary position being rope_offset + r (the prefix's
+ * length).  qkv as teeny_qkv_rope_split takes it, or (qkv null) parts as
+ * teeny_qkv_rope_split_partials_dev; otherwise as those, with q_out required. */
+int teeny_qkv_rope_split_rows(const void* qkv, const float* parts, int n_parts, void* q_out,
+                              void* k_cache, void* v_cache, int batch, int seq_len,
+                              const int32_t* row0, int row0_stride, int row0_host,
+                              int rope_offset, int cache_len, int n_heads_q, int n_heads_kv,
+                              int head_dim, float ln_rope_base, int dtype, hipStream_t stream);
+
 /* teeny_decode_qkv_attention_dev: a one-token decode step's attention in
  * one launch, for position p = *n_past (read when the kernel runs): the
  * QKV projection's K-split slabs parts[n_parts][batch][(Hq + 2 Hkv) D] are

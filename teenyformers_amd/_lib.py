@@ -89,6 +89,7 @@ _SIGNATURES = {
     "teeny_embed_rmsnorm_fwd": ([_p] * 5 + [_i, _i, _i, _f, _i, _i, _p], _i),
     "teeny_argmax_rows_advance": ([_p, _p, _i, _i, _i, _p, _p], _i),
     "teeny_argmax_rows": ([_p, _p, _i, _i, _i, _p], _i),
+    "teeny_qkv_rope_split_rows": ([_p, _p, _i] + [_p] * 3 + [_i, _i, _p] + [_i] * 7 + [_f, _i, _p], _i),
     "teeny_shared_prefix_attention_workspace_bytes": ([_i] * 8, _sz),
     "teeny_shared_prefix_attention": ([_p] * 6 + [_i] * 6 + [_p] + [_i] * 4 + [_f, _i, _i, _p, _sz,
                                                                            _p], _i),

@@ -1092,6 +1092,40 @@ int teeny_qkv_rope_split_partials_dev(const float* parts, int n_parts, void* q_o
                 dim3(256), shmem, stream, args);
 }
 
+int teeny_qkv_rope_split_rows(const void* qkv, const float* parts, int n_parts, void* q_out,
+                              void* k_cache, void* v_cache, int batch, int seq_len,
+                              const int32_t* row0, int row0_stride, int row0_host,
+                              int rope_offset, int cache_len, int n_heads_q, int n_heads_kv,
+                              int head_dim, float ln_rope_base, int dtype, hipStream_t stream) {
+  if (!q_out || (qkv == nullptr) == (parts == nullptr)) return TEENY_ERR_NULL_POINTER;
+  int rc = qkv_rope_split_check(qkv ? qkv : parts, q_out, k_cache, v_cache, batch, seq_len,
+                                row0 ? 0 : row0_host, cache_len, n_heads_q, n_heads_kv, head_dim,
+                                ln_rope_base, dtype);
+  if (rc) return rc;
+  if (row0 && row0_stride != 0 && row0_stride != 1) return TEENY_ERR_INVALID_VALUE;
+  if (rope_offset < 0 || rope_offset > (1 << 30)) return TEENY_ERR_INVALID_VALUE;
+  const int htot = n_heads_q + 2 * n_heads_kv;
+  int pos_imm = row0 ? 0 : row0_host;
+  char name[48];
+  snprintf(name, sizeof name, "teeny_qkv_%srope_split_rows_%s", qkv ? "" : "parts_",
+           dtype_tag(dtype));
+  if (qkv) {  // the grid of teeny_qkv_rope_split
+    const int ppw = 256 / (head_dim / (dtype == TEENY_BF16 ? 8 : 4));
+    void* args[] = {&qkv,       &q_out,      &k_cache,  &v_cache,      &seq_len,     &row0, &pos_imm,
+                    &cache_len, &n_heads_q, &n_heads_kv, &head_dim, &ln_rope_base, &row0_stride,
+                    &rope_offset};
+    return launch(name, dim3((seq_len + ppw - 1) / ppw, (unsigned)((long)batch * ((htot + 7) / 8))),
+                  dim3(256), 0, stream, args);
+  }
+  long part_stride = (long)batch * seq_len * htot * head_dim;
+  if (n_parts <= 0 || part_stride * n_parts >= kMaxElems) return TEENY_ERR_INVALID_SHAPE;
+  void* args[] = {&parts,     &n_parts,   &part_stride, &q_out,       &k_cache,    &v_cache,
+                  &seq_len,   &row0,      &pos_imm,     &cache_len,   &n_heads_q,  &n_heads_kv,
+                  &head_dim,  &ln_rope_base, &row0_stride, &rope_offset};
+  return launch(name, dim3((seq_len + 3) / 4, (unsigned)((long)batch * ((htot + 3) / 4))),
+                dim3(256), 4u * (unsigned)(head_dim / 2) * 8u, stream, args);
+}
+
 // Workgroups that share the keys of a (b, kv head) in the one-launch decode
 // attention: a key tile (32) per wavefront at full cache at the finest, until
 // every CU has a workgroup, at most 16 (32 was 0-50 % slower than 16).

@@ -35,7 +35,7 @@ __device__ void qkv_rope_split(const T* __restrict__ qkv, T* __restrict__ q_out,
                                const int* __restrict__ pos_dev, int pos0, int cache_len, int hq,
                                int hkv, int head_dim, float ln_base,
                                const float* __restrict__ parts = nullptr, int n_parts = 0,
-                               long part_stride = 0) {
+                               long part_stride = 0, int pos_stride = 0, int rope_offset = 0) {
   extern __shared__ float2 cs_tab[];  // [kPos][head_dim / 2]
   const int half = head_dim / 2;
   const int s0 = blockIdx.x * kPos;
@@ -68,13 +68,13 @@ __device__ void qkv_rope_split(const T* __restrict__ qkv, T* __restrict__ q_out,
   const bool first = (int)threadIdx.x < total && source(threadIdx.x, v, p, hh, s);
   if (first) load(v, hh, s, in);
 
-  if (pos_dev) pos0 += *pos_dev;
+  if (pos_dev) pos0 += pos_dev[b * pos_stride];
   const float c = rope_c(ln_base, head_dim);
   for (int i = threadIdx.x; i < kPos * half; i += kThreads) {
     int pp = i / half, k = i - pp * half;
     if (s0 + pp >= seq) break;  // i grows with pp: no later entry is needed either
     float sn, cn;
-    rope_cos_sin(pos0 + s0 + pp, k, c, cn, sn);
+    rope_cos_sin(pos0 + rope_offset + s0 + pp, k, c, cn, sn);
     cs_tab[i] = make_float2(cn, sn);
   }
   __syncthreads();
@@ -122,7 +122,8 @@ template <typename T>
 __device__ void qkv_rope_rows(const T* __restrict__ qkv, T* __restrict__ q_out,
                               T* __restrict__ k_cache, T* __restrict__ v_cache, int seq,
                               const int* __restrict__ pos_dev, int pos0, int cache_len, int hq,
-                              int hkv, int head_dim, float ln_base) {
+                              int hkv, int head_dim, float ln_base, int pos_stride = 0,
+                              int rope_offset = 0) {
   constexpr int VN = Vec16<T>::N;
   const int vpr = head_dim / VN;  // vectors per head row (the host keeps it <= kThreads)
   const int ppw = kThreads / vpr;
@@ -141,13 +142,14 @@ __device__ void qkv_rope_rows(const T* __restrict__ qkv, T* __restrict__ q_out,
   for (int h = 0; h < kQkvHeads; ++h)
     if (h0 + h < htot) Vec16<T>::load(src + (long)h * head_dim, in[h]);
 
-  if (pos_dev) pos0 += *pos_dev;
+  if (pos_dev) pos0 += pos_dev[b * pos_stride];
   const int pos = pos0 + s;
   float cn[VN / 2], sn[VN / 2];
   if (h0 < hq + hkv) {  // some head of the group is rotated
     const float c = rope_c(ln_base, head_dim);
 #pragma unroll
-    for (int j = 0; j < VN / 2; ++j) rope_cos_sin(pos, v * (VN / 2) + j, c, cn[j], sn[j]);
+    for (int j = 0; j < VN / 2; ++j)
+      rope_cos_sin(pos + rope_offset, v * (VN / 2) + j, c, cn[j], sn[j]);
   }
 #pragma unroll
   for (int h = 0; h < kQkvHeads; ++h) {
@@ -597,6 +599,25 @@ extern "C" __global__ __launch_bounds__(256) void teeny_rope_table_f32(float2* c
                                   cache_len, hq, hkv, head_dim, ln_base, parts, n_parts,        \
                                   part_stride);                                                 \
   }
+// ... a position per sequence, the rotary position rope_offset past the cache row
+#define TEENY_QKV_ROWS_INST(TN, T)                                                              \
+  extern "C" __global__ __launch_bounds__(256) void teeny_qkv_parts_rope_split_rows_##TN(      \
+      const float* parts, int n_parts, long part_stride, T* q_out, T* k_cache, T* v_cache,      \
+      int seq, const int* pos_dev, int pos0, int cache_len, int hq, int hkv, int head_dim,      \
+      float ln_base, int pos_stride, int rope_offset) {                                         \
+    qkv_rope_split<T, true, 4, 4>(nullptr, q_out, k_cache, v_cache, seq, pos_dev, pos0,        \
+                                  cache_len, hq, hkv, head_dim, ln_base, parts, n_parts,        \
+                                  part_stride, pos_stride, rope_offset);                        \
+  }                                                                                             \
+  extern "C" __global__ __launch_bounds__(256) void teeny_qkv_rope_split_rows_##TN(            \
+      const T* qkv, T* q_out, T* k_cache, T* v_cache, int seq, const int* pos_dev, int pos0,    \
+      int cache_len, int hq, int hkv, int head_dim, float ln_base, int pos_stride,              \
+      int rope_offset) {                                                                        \
+    qkv_rope_rows<T>(qkv, q_out, k_cache, v_cache, seq, pos_dev, pos0, cache_len, hq, hkv,      \
+                     head_dim, ln_base, pos_stride, rope_offset);                               \
+  }
+TEENY_QKV_ROWS_INST(f32, float)
+TEENY_QKV_ROWS_INST(bf16, bf16)
 TEENY_QKV_PARTS_INST(f32, float)
 TEENY_QKV_PARTS_INST(bf16, bf16)
 

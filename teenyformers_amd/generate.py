@@ -15,6 +15,12 @@ random N(0, 0.02) weights and random prompt ids, prints one JSON line of
 timings, and is the workload of the decode kernel profiles:
 
   python -m teenyformers_amd.generate --preset llama3-8b --batch 16 --prompt-len 512
+
+--num-samples N draws N continuations of the prompt, which runs and is stored
+once (Llama.generate_samples); --top-k, --top-p and --min-p cut the
+distribution.  Any of them draws on the device (ops.sample_rows, random
+numbers from torch's generator with --seed); without them, --temperature keeps
+the reference's sampler on the host.
 """
 from __future__ import annotations
 
@@ -91,6 +97,9 @@ def generate_text(args) -> int:
     eos = eos_id(tok)
     print(args.prompt, end="", flush=True)
     prompt = torch.tensor([ids], dtype=torch.int64, device="cuda")
+    if args.on_device:
+        print()
+        return print_samples(args, model, prompt, tok, eos)
     cache, logits = model.prefill(prompt, len(ids) + args.max_new_tokens)
     if not args.no_stream_layout:
         model.stream_layout()
@@ -120,6 +129,51 @@ def generate_text(args) -> int:
     return 0
 
 
+def random_numbers(args) -> torch.Tensor:
+    """u of every step and sample, fp32 in [0, 1)."""
+    g = torch.Generator(device="cuda").manual_seed(args.seed)
+    return torch.rand((args.max_new_tokens, args.num_samples), generator=g, device="cuda")
+
+
+def print_samples(args, model, prompt, tok, eos: int) -> int:
+    """--num-samples continuations, each up to its end-of-sequence token."""
+    if not args.no_stream_layout:
+        model.stream_layout()
+    out = model.generate_samples(prompt, random_numbers(args), args.temperature, args.top_k,
+                                 args.top_p, args.min_p).tolist()
+    for i, row in enumerate(out):
+        row = row[:row.index(eos)] if eos in row else row
+        if args.num_samples > 1:
+            print(f"--- {i + 1}")
+        print(tok.decode(row, skip_special_tokens=True))
+    return 0
+
+
+def bench_samples(args, model, ids) -> int:
+    """--preset with --num-samples: one prompt, its continuations drawn on the device."""
+    u = random_numbers(args)
+    cache, logits = model.share_prefix(ids[:1], args.num_samples, args.max_new_tokens)
+    if not args.no_stream_layout:
+        model.stream_layout()
+    how = (args.temperature, args.top_k, args.top_p, args.min_p)
+    first = ops.sample_rows(logits.expand(args.num_samples, -1), u[0], *how).view(-1, 1)
+    ms = 0.0
+    if args.max_new_tokens > 1:
+        sg = llama.SampleGraph(model, cache, first, u[1], *how)
+        torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        for i in range(2, args.max_new_tokens):
+            sg.replay(u[i])
+        torch.cuda.synchronize()
+        ms = (time.perf_counter() - t0) * 1e3 / max(1, args.max_new_tokens - 2)
+    print(json.dumps({"preset": args.preset, "num_samples": args.num_samples,
+                      "prompt_len": args.prompt_len, "new_tokens": args.max_new_tokens,
+                      "decode_ms_per_step": round(ms, 3),
+                      "decode_tokens_per_s": round(args.num_samples / ms * 1e3, 1) if ms else None}),
+          flush=True)
+    return 0
+
+
 def bench_preset(args) -> int:
     cfg = llama.LlamaConfig(**PRESETS[args.preset])
     w = llama.init_weights(cfg, dtype=torch.bfloat16, seed=args.seed)
@@ -127,6 +181,8 @@ def bench_preset(args) -> int:
     g = torch.Generator(device="cuda").manual_seed(args.seed)
     ids = torch.randint(0, cfg.vocab_size, (args.batch, args.prompt_len), generator=g,
                         device="cuda")
+    if args.on_device:
+        return bench_samples(args, model, ids)
     torch.cuda.synchronize()
     t0 = time.perf_counter()
     cache, logits = model.prefill(ids, args.prompt_len + args.max_new_tokens)
@@ -155,6 +211,11 @@ def main(argv=None) -> int:
     ap.add_argument("--prompt", default="The quick brown fox")
     ap.add_argument("--max-new-tokens", type=int, default=128)
     ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--num-samples", type=int, default=1,
+                    help="continuations of the prompt, drawn on the device")
+    ap.add_argument("--top-k", type=int, default=0, help="0: off")
+    ap.add_argument("--top-p", type=float, default=1.0, help="1: off")
+    ap.add_argument("--min-p", type=float, default=0.0, help="0: off")
     ap.add_argument("--seed", type=int, default=42)
     ap.add_argument("--dtype", choices=["bf16", "f32"], default="bf16")
     ap.add_argument("--preset", choices=sorted(PRESETS), help="random weights, timing only")
@@ -165,6 +226,12 @@ def main(argv=None) -> int:
     args = ap.parse_args(argv)
     if args.max_new_tokens < 1:
         ap.error("--max-new-tokens must be at least 1")
+    if not (args.temperature >= 0.0 and args.num_samples >= 1 and 0 <= args.top_k < 2 ** 31
+            and 0.0 < args.top_p <= 1.0 and 0.0 <= args.min_p <= 1.0):
+        ap.error("--temperature and --top-k are at least 0, --num-samples at least 1, --top-p in "
+                 "(0, 1], --min-p in [0, 1]")
+    args.on_device = (args.num_samples > 1 or args.top_k > 0 or args.top_p < 1.0
+                      or args.min_p > 0.0)
     if args.preset:
         return bench_preset(args)
     if not args.model_dir:

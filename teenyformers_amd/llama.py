@@ -19,7 +19,10 @@ MI355X-specific structure (same arithmetic):
     KV-cache write in one pass;
   * every residual add is fused into the next RMSNorm (teeny_fused_add_rmsnorm);
   * prefill runs the causal FA2 kernel over the cache; each decode step runs
-    teeny_decode_attention over the cached keys;
+    teeny_decode_attention over the cached keys; sequences that go on from one
+    prompt (share_prefix, extend, generate_samples) run
+    teeny_shared_prefix_attention over the prompt's one cache and their own;
+  * tokens are drawn on the device (teeny_sample_rows);
   * Linear layers (teeny-core's external `Linear`, src/layers/mod.rs:54-58,
     y = x W^T with W [out, in]) run through the library's linear entry
     points: a prompt's products through hipBLASLt (teeny_linear_bf16 /
@@ -183,6 +186,29 @@ class KVCache:
         self.length = 0
 
 
+class SharedPrefixCache:
+    """K/V of sequences that go on from one prompt: the prompt's cache (of one
+    sequence, read by all of them), and per layer the sequences' own rows [B, Hkv,
+    capacity, D].  length: the own rows written (of the longest sequence);
+    lengths: int32 [B] on the device where the sequences differ, else None.
+    Rotary positions go on from the prompt's length."""
+
+    def __init__(self, cfg: LlamaConfig, prefix: KVCache, batch: int, capacity: int):
+        if prefix.k[0].shape[0] != 1:
+            raise ValueError("SharedPrefixCache: the prefix is a cache of one sequence")
+        shape = (batch, cfg.n_kv_heads(), capacity, cfg.head_dim())
+        like = prefix.k[0]
+        self.prefix, self.n_prefix = prefix, prefix.length
+        # rows are written before any query sees them
+        self.k = [torch.zeros(shape, dtype=like.dtype, device=like.device)
+                  for _ in range(cfg.n_layers)]
+        self.v = [torch.zeros(shape, dtype=like.dtype, device=like.device)
+                  for _ in range(cfg.n_layers)]
+        self.capacity = capacity
+        self.length = 0
+        self.lengths = None
+
+
 class Llama:
     """Forward passes of the Llama model (src/llama.rs:40-82) on the HIP ops."""
 
@@ -233,6 +259,13 @@ class Llama:
         rows = ops.split_rows()
         qkv = ops.linear_split(n1, self._lw(p + "qkv_proj.weight"), rows=rows)
         scale = cfg.softmax_scale()
+        if isinstance(cache, SharedPrefixCache):
+            q = torch.empty((B, Hq, S, D), dtype=n1.dtype, device=n1.device)
+            ops.qkv_rope_split(qkv, q, cache.k[i], cache.v[i], pos0, Hq, Hkv, cfg.rope_base,
+                               rope_offset=cache.n_prefix)
+            att = ops.shared_prefix_attention(q, cache.prefix.k[i], cache.prefix.v[i], cache.k[i],
+                                              cache.v[i], cache.n_prefix, pos0, scale, merged=True)
+            return ops.linear_split(att, self._lw(p + "o_proj.weight"), rows=rows)
         if isinstance(pos0, torch.Tensor) and self._fused_decode(qkv, cache):
             # one launch: QKV split, RoPE, cache write and attention
             o = ops.decode_qkv_attention(qkv, cache.k[i], cache.v[i], pos0, Hq, Hkv,
@@ -330,7 +363,8 @@ class Llama:
         x, n1 = ops.embed_rmsnorm(ids, w["model.embed_tokens.weight"],
                                   w["model.layers.0.input_layernorm.weight"], eps)
         pos = pos0
-        if ids.shape[1] == 1 and not isinstance(pos0, torch.Tensor) and pos0 > 0:
+        if (ids.shape[1] == 1 and not isinstance(pos0, torch.Tensor) and pos0 > 0
+                and not isinstance(cache, SharedPrefixCache)):
             # a one-token step takes its position from device memory, as the
             # captured graph does, so both run the same kernels
             pos = torch.tensor([pos0], dtype=torch.int32, device=ids.device)
@@ -370,11 +404,80 @@ class Llama:
         h = self.hidden(ids, cache, 0)
         return cache, self.logits(h[:, -1])
 
-    def decode_step(self, cache: KVCache, ids: torch.Tensor) -> torch.Tensor:
+    def decode_step(self, cache: KVCache | SharedPrefixCache, ids: torch.Tensor) -> torch.Tensor:
         """One token per sequence (ids [B, 1]) -> next-token logits [B, vocab]."""
+        lengths = getattr(cache, "lengths", None)
+        if lengths is not None and cache.length >= cache.capacity:
+            raise ValueError("decode_step: the cache is full")  # device lengths: not checked there
         with ops.own_gemm():  # the kernels of the graph-captured step
-            h = self.hidden(ids, cache, cache.length)
+            h = self.hidden(ids, cache, cache.length if lengths is None else lengths)
+            if lengths is not None:
+                cache.lengths = lengths + 1
+                cache.length += 1
             return self.logits(h[:, -1])
+
+    def share_prefix(self, prompt: torch.Tensor, batch: int, capacity: int
+                     ) -> tuple[SharedPrefixCache, torch.Tensor]:
+        """Prompt pass of one prompt [1, P] that `batch` sequences go on from, each
+        with `capacity` rows of its own: the cache and the last position's logits
+        [1, vocab]."""
+        if prompt.dim() != 2 or prompt.shape[0] != 1:
+            raise ValueError("share_prefix: one prompt, [1, P]")
+        prefix, logits = self.prefill(prompt, prompt.shape[1])
+        return SharedPrefixCache(self.cfg, prefix, batch, capacity), logits
+
+    def extend(self, cache: SharedPrefixCache, ids: torch.Tensor,
+               lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Prompts behind the shared prefix: ids [B, S] become the sequences' first
+        own rows; returns the logits [B, vocab] after each sequence's last token.
+        lengths [B] (1 .. S): the real tokens of a batch padded at its end; later
+        steps overwrite the padding's rows, which no real token sees."""
+        if cache.length != 0:
+            raise ValueError("extend: the sequences have rows already")
+        B, S = ids.shape
+        if S > cache.capacity or B != cache.k[0].shape[0]:
+            raise ValueError("extend: ids are [B, S] of the cache's sequences and capacity")
+        if lengths is not None:
+            if lengths.shape != (B,) or lengths.is_floating_point():
+                raise ValueError("extend: lengths holds a whole number per sequence")
+            if int(lengths.min()) < 1 or int(lengths.max()) > S:
+                raise ValueError("extend: lengths must lie in 1 .. S")
+        h = self.hidden(ids, cache, 0)
+        if lengths is None:
+            return self.logits(h[:, -1])
+        lengths = lengths.to(device=ids.device, dtype=torch.int32)
+        cache.lengths, cache.length = lengths, int(lengths.max())
+        rows = (lengths.to(torch.int64) - 1).view(B, 1, 1).expand(B, 1, h.shape[2])
+        return self.logits(h.gather(1, rows)[:, 0])
+
+    def generate_samples(self, prompt: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
+                         top_p=1.0, min_p=0.0, ids: torch.Tensor | None = None,
+                         lengths: torch.Tensor | None = None, graph: bool = True) -> torch.Tensor:
+        """Continuations of one prompt [1, P], drawn with the random numbers u
+        [n_new, B] (fp32, in [0, 1)) -> ids [B, n_new].  The prompt runs once and its
+        keys are stored once.  ids [B, S] (with lengths, as extend): each sequence's
+        own text behind the prompt.  Settings as ops.sample_rows.  graph: the step
+        is captured once and replayed (the same tokens)."""
+        n_new, B = u.shape
+        if n_new < 1 or u.dtype != torch.float32:
+            raise ValueError("generate_samples: u is fp32 [n_new, B]")
+        own = 0 if ids is None else ids.shape[1]
+        cache, logits = self.share_prefix(prompt, B, own + n_new)
+        logits = logits.expand(B, -1) if ids is None else self.extend(cache, ids, lengths)
+        how = (temperature, top_k, top_p, min_p)
+        nxt = ops.sample_rows(logits, u[0].contiguous(), *how).view(B, 1)
+        out = [nxt]
+        if n_new > 1 and graph:
+            sg = SampleGraph(self, cache, nxt, u[1].contiguous(), *how)
+            out.append(sg.ids.clone())
+            for i in range(2, n_new):
+                sg.replay(u[i])
+                out.append(sg.ids.clone())
+        for i in range(1, n_new if not graph else 0):
+            logits = self.decode_step(cache, nxt)
+            nxt = ops.sample_rows(logits, u[i].contiguous(), *how).view(B, 1)
+            out.append(nxt)
+        return torch.cat(out, dim=1)
 
     def generate(self, prompt: torch.Tensor, n_new: int) -> torch.Tensor:
         """Greedy decoding with the KV cache -> generated ids [B, n_new]."""
@@ -467,8 +570,11 @@ class DecodeGraph:
                  trace: list | None = None):
         self.model, self.cache = model, cache
         self.ids = ids.to(torch.int64).clone()
-        self.pos = torch.full((1,), cache.length, dtype=torch.int32, device=ids.device)
-        model._decode_ws(ids.shape[0], cache, ids.device)
+        lengths = getattr(cache, "lengths", None)  # (a copy: replays move it on)
+        self.pos = (torch.full((1,), cache.length, dtype=torch.int32, device=ids.device)
+                    if lengths is None else lengths.clone())
+        if not isinstance(cache, SharedPrefixCache):
+            model._decode_ws(ids.shape[0], cache, ids.device)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
@@ -476,6 +582,8 @@ class DecodeGraph:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         cache.length += 1
+        if lengths is not None:
+            cache.lengths = self.pos
         self.logits = torch.empty_like(self.first_logits)
         self.graph = None
         self._graphs = {}  # by the number of key splits
@@ -493,7 +601,8 @@ class DecodeGraph:
         """The key splits of a step that attends n_keys rows (1 where the step
         does not run the fused attention)."""
         cfg, cache = self.model.cfg, self.cache
-        if cache.k[0].dtype != torch.bfloat16 or cfg.head_dim() not in (64, 128):
+        if (isinstance(cache, SharedPrefixCache) or cache.k[0].dtype != torch.bfloat16
+                or cfg.head_dim() not in (64, 128)):
             return 1
         return ops.decode_qkv_splits(self.ids.shape[0], cfg.n_kv_heads(), cache.capacity,
                                      cfg.head_dim(), n_keys)
@@ -509,11 +618,42 @@ class DecodeGraph:
             # the greedy choice lands in the ids the next replay embeds (the
             # embedding read them at the start of this step)
             # (and the position moves on: every kernel that reads it came before)
-            ops.argmax_rows(logits, out=self.ids.view(-1), advance=self.pos)
+            self._choose(logits)
         return logits
+
+    def _choose(self, logits: torch.Tensor):
+        one = self.pos.numel() == 1
+        ops.argmax_rows(logits, out=self.ids.view(-1), advance=self.pos if one else None)
+        if not one:
+            self.pos.add_(1)
 
     def replay(self):
         if self.cache.length >= self.cache.capacity:
             raise RuntimeError("KV cache is full")
         self._graphs.get(self._splits(self.cache.length + 1), self.graph).replay()
         self.cache.length += 1
+        if getattr(self.cache, "lengths", None) is not None:
+            self.cache.lengths = self.pos
+
+
+class SampleGraph(DecodeGraph):
+    """DecodeGraph whose tokens are drawn (ops.sample_rows, settings as there: a
+    tensor's values may be changed between replays) with the random numbers of
+    each step: u [B] for the first, replay(u) for the next."""
+
+    def __init__(self, model: Llama, cache: KVCache | SharedPrefixCache, ids: torch.Tensor,
+                 u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        self.u = u.clone()
+        self.how = (temperature, top_k, top_p, min_p)
+        super().__init__(model, cache, ids)
+
+    def _choose(self, logits: torch.Tensor):
+        one = self.pos.numel() == 1
+        ops.sample_rows(logits, self.u, *self.how, out=self.ids.view(-1),
+                        advance=self.pos if one else None)
+        if not one:
+            self.pos.add_(1)
+
+    def replay(self, u: torch.Tensor):
+        self.u.copy_(u)
+        super().replay()

@@ -490,11 +490,17 @@ def _ln(rope_base) -> float:
 
 
 def qkv_rope_split(qkv, q_out, k_cache, v_cache, pos0, n_heads_q: int, n_heads_kv: int,
-                   rope_base: float):
+                   rope_base: float, rope_offset: int = 0):
     """qkv [B, S, (Hq+2Hkv)*D] -> q_out [B, Hq, S, D] (RoPE) and K (RoPE) / V
     written to caches [B, Hkv, L, D] at rows pos0 .. pos0+S-1.  pos0: an int,
     or a one-element int32 device tensor read when the kernel runs (for
-    captured graphs).  q_out None (a dense qkv only): the caches only."""
+    captured graphs).  q_out None (a dense qkv only): the caches only.
+    Behind a shared prefix (shared_prefix_attention): rope_offset, the prefix's
+    length, is added to the rotary positions (not to the rows), and pos0 may hold
+    a value per sequence."""
+    if rope_offset or isinstance(pos0, torch.Tensor) and pos0.numel() > 1:
+        return _qkv_rope_split_rows(qkv, q_out, k_cache, v_cache, pos0, n_heads_q, n_heads_kv,
+                                    rope_base, rope_offset)
     if isinstance(qkv, Partials):
         _dev(qkv.slabs, q_out, k_cache, v_cache)
         B, S, _ = qkv.shape
@@ -519,6 +525,31 @@ def qkv_rope_split(qkv, q_out, k_cache, v_cache, pos0, n_heads_q: int, n_heads_k
         return
     call("teeny_qkv_rope_split", _p(qkv), _p(q_out), _p(k_cache), _p(v_cache), B, S, pos0,
          k_cache.shape[2], n_heads_q, n_heads_kv, D, _ln(rope_base), _code(qkv), _stream())
+
+
+def _qkv_rope_split_rows(qkv, q_out, k_cache, v_cache, pos0, n_heads_q: int, n_heads_kv: int,
+                         rope_base: float, rope_offset: int):
+    parts = isinstance(qkv, Partials)
+    src = qkv.slabs if parts else qkv
+    _dev(src, q_out, k_cache, v_cache)
+    B, S, W = qkv.shape
+    D, L = k_cache.shape[3], k_cache.shape[2]
+    if (W != (n_heads_q + 2 * n_heads_kv) * D or q_out.shape != (B, n_heads_q, S, D)
+            or k_cache.shape != (B, n_heads_kv, L, D) or v_cache.shape != k_cache.shape):
+        raise ValueError("qkv_rope_split: qkv [B, S, (Hq+2Hkv)*D], q_out [B, Hq, S, D] and caches "
+                         "[B, Hkv, L, D] must match")
+    if qkv.dtype != q_out.dtype or k_cache.dtype != q_out.dtype or v_cache.dtype != q_out.dtype:
+        raise TypeError("qkv_rope_split: qkv, q_out and the caches share a dtype")
+    row0, host = (pos0, 0) if isinstance(pos0, torch.Tensor) else (None, int(pos0))
+    if row0 is not None and (row0.dtype != torch.int32 or not row0.is_cuda
+                             or row0.numel() not in (1, B) or not row0.is_contiguous()):
+        raise TypeError("a device position must be an int32 CUDA tensor of one value or one per "
+                        "sequence")
+    with _on_device_of(q_out):
+        call("teeny_qkv_rope_split_rows", None if parts else _p(src), _p(src) if parts else None,
+             qkv.n if parts else 0, _p(q_out), _p(k_cache), _p(v_cache), B, S, _p(row0),
+             int(row0 is not None and row0.numel() == B), host, int(rope_offset), L, n_heads_q,
+             n_heads_kv, D, _ln(rope_base), _code(q_out), _stream())
 
 
 def decode_attention(q, k_cache, v_cache, n_keys: int, softmax_scale: float | None = None,

@@ -449,3 +449,30 @@ def test_shared_prefix_attention_validation(L):
     assert need > 0 and f(wsb=need - 1) == WS and f(ws=None) == WS
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 3, 2, 1, 100, 64, 64, BF16) == 0
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, -1, 64, 64, BF16) == 0
+
+
+def test_qkv_rope_split_rows_validation(L):
+    """Refusals of the QKV split behind a prefix."""
+    def f(**kw):
+        a = dict(qkv=P, parts=None, n=0, q=P, k=P, v=P, b=2, s=1, row0=None, st=0, host=3, off=10, L=64,
+                 hq=4, hkv=2, d=64, ln=9.2, dtype=BF16)
+        a.update(kw)
+        return L.teeny_qkv_rope_split_rows(a["qkv"], a["parts"], a["n"], a["q"], a["k"], a["v"], a["b"],
+                                           a["s"], a["row0"], a["st"], a["host"], a["off"], a["L"],
+                                           a["hq"], a["hkv"], a["d"], a["ln"], a["dtype"], None)
+    for kw in (dict(qkv=None), dict(parts=P, n=1), dict(q=None), dict(k=None), dict(v=None)):
+        assert f(**kw) == NULLP, kw
+    for kw in (dict(host=-1), dict(host=64), dict(s=0), dict(hq=5), dict(qkv=None, parts=P, n=0)):
+        assert f(**kw) == SHAPE, kw
+    for kw in (dict(off=-1), dict(off=(1 << 30) + 1), dict(row0=P, st=2), dict(ln=float("nan"))):
+        assert f(**kw) == VALUE, kw
+    assert f(dtype=7) == UNSUP and f(d=12) == UNSUP
+
+
+def test_generate_command_refuses(capsys):
+    """Arguments out of their ranges end the command before anything is loaded."""
+    from teenyformers_amd import generate
+    for bad in (["--num-samples", "0"], ["--top-k", "-1"], ["--top-p", "0"], ["--top-p", "1.5"],
+                ["--min-p", "-0.1"], ["--min-p", "2"], ["--temperature", "-1"], ["--temperature", "nan"]):
+        with pytest.raises(SystemExit):
+            generate.main(["--preset", "llama3-8b", *bad])
