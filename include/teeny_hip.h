@@ -437,7 +437,7 @@ int teeny_argmax_rows_advance(const void* x, int64_t* out, int rows, int cols, i
  * is not above 0 counts as 0, a top_k below 1 as off, a top_p not below 1 as
  * off and one not above 0 as keeping one token, a min_p not above 0 as off.  u
  * outside [0, 1) or NaN is taken as its nearest border (NaN as 0).
- * dtype of the logits: fp32 or bf16.  cols <= 2^19, rows <= 65535.
+ * dtype of the logits: fp32 or bf16.  cols <= 524280, rows <= 65535.
  * advance: as teeny_argmax_rows_advance; may be null.  workspace:
  * teeny_sample_rows_workspace_bytes(rows, cols) bytes, 16-byte aligned. */
 size_t teeny_sample_rows_workspace_bytes(int rows, int cols);

@@ -69,8 +69,10 @@ def _run(cmd, verbose):
 
 
 # Per-file additions.  The forward's row maxima read MFMA results: without
-# NaNs to honour, fmaxf needs no canonicalising v_max per operand.
-EXTRA_FLAGS: dict[str, list[str]] = {"fa2_fwd_bf16": ["-fno-honor-nans"]}
+# NaNs to honour, fmaxf needs no canonicalising v_max per operand.  The sampler's
+# fixed-point weights want each product rounded where it is written.
+EXTRA_FLAGS: dict[str, list[str]] = {"fa2_fwd_bf16": ["-fno-honor-nans"],
+                                     "sample": ["-ffp-contract=off"]}
 
 
 def _hipcc(name, verbose):

@@ -1439,24 +1439,25 @@ int teeny_argmax_rows_advance(const void* x, int64_t* out, int rows, int cols, i
 // Sampling (sample.hip): the records of the chunks that a row is summed in, and
 // with filters the chunks' weights and counts by bin.
 namespace {
-constexpr int kSampleChunk = 8192, kSampleBins = 180;
-constexpr int kSampleCols = 1 << 19;  // weights of 2^44 at most: no sum overflows
-constexpr size_t kSampleRec = 32;     // Chunk in sample.hip
+constexpr int kSampleChunk = 8192;
+// 64 chunks, a row starting up to 7 elements past a 16-byte boundary (and
+// weights of 2^44 at most: no sum overflows)
+constexpr int kSampleCols = 64 * kSampleChunk - 8;
+constexpr size_t kSampleRec = 32;                                    // Chunk in sample.hip
+constexpr size_t kSampleBins = 8 * 180 + 8 * 1024 + 4 * (180 + 4);   // Bins in sample.hip
 struct SampleArgs {                   // Args in sample.hip
   double t, p, m;
   const float *ts, *ps, *ms;
   const int32_t* ks;
   int k;
 };
-// (a row may start up to 7 elements past a 16-byte boundary)
 int sample_chunks(int cols) { return (cols + 7 + kSampleChunk - 1) / kSampleChunk; }
 }  // namespace
 
 size_t teeny_sample_rows_workspace_bytes(int rows, int cols) {
   if (rows <= 0 || rows > 65535 || cols <= 0 || cols > kSampleCols) return 0;
   const size_t n = (size_t)rows * sample_chunks(cols);
-  return align256(n * kSampleRec) + align256(n * kSampleBins * sizeof(uint64_t)) +
-         align256(n * kSampleBins * sizeof(uint32_t));
+  return align256(n * kSampleRec) + align256(n * kSampleBins);
 }
 
 int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int cols,
@@ -1481,18 +1482,17 @@ int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int
   int n_ch = sample_chunks(cols);
   const size_t n = (size_t)rows * n_ch;
   char* rec = (char*)workspace;
-  char* mass = rec + align256(n * kSampleRec);
-  char* cnt = mass + align256(n * kSampleBins * sizeof(uint64_t));
+  char* bins = rec + align256(n * kSampleRec);
   SampleArgs a{temperature, top_p, min_p, temperature_rows, top_p_rows, min_p_rows, top_k_rows,
                top_k};
   char name[48];
   snprintf(name, sizeof name, "teeny_sample_scan_%s", dtype_tag(dtype));
-  void* a0[] = {&logits, &ld, &cols, &a, &rec, &cnt, &mass};
+  void* a0[] = {&logits, &ld, &cols, &a, &rec, &bins};
   int rc = launch(name, dim3((unsigned)n_ch, (unsigned)rows), dim3(1024), 0, stream, a0);
   if (rc) return rc;
   snprintf(name, sizeof name, "teeny_sample_draw_%s", dtype_tag(dtype));
-  void* a1[] = {&logits, &ld, &cols, &a, &u, &rec, &cnt, &mass, &n_ch, &out, &advance};
-  return launch(name, dim3((unsigned)rows), dim3(1024), 0, stream, a1);
+  void* a1[] = {&logits, &ld, &cols, &a, &u, &rec, &bins, &n_ch, &out, &advance};
+  return launch(name, dim3((unsigned)rows), dim3(256), 0, stream, a1);
 }
 
 // Decode-step linear layers (linear_bf16.hip): 512 threads, 128 W rows per

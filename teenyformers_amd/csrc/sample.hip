@@ -15,52 +15,72 @@
 // first whose running weight exceeds u times the kept weight.
 //
 // Numbers: the border between two tokens among 1e5 is narrower than fp32 sums
-// resolve, and sums of floats depend on their order.  So L = x log2(e) / T and
-// 2^-d are evaluated in fp64 and a weight is held as a whole number of 2^-44
-// (64 bits; at most 2^19 columns, so no sum overflows): sums are exact, in any
-// order, with atomics too.  A weight that rounds to zero cannot be drawn.
-// Weights are relative to the largest logit of the token's CHUNK (8192 columns)
-// where chunks are summed alone, and a chunk's sum is brought to the row's
-// scale by one fp64 factor, so one pass over the logits serves.
+// resolve, and sums of floats depend on their order.  So q = 4 x log2(e) / T (a
+// token's place in quarter octaves) and 2^(q/4) are evaluated in fp64, and a
+// weight is held as a whole number of 2^-44 of the largest (64 bits; at most
+// 524280 columns, so no sum overflows): sums are exact, in any order, with
+// atomics too.  A weight that rounds to zero cannot be drawn.
+//   With filters, floor(q) is a token's bin and 2^(frac(q)/4), of one scale in
+// every bin of the row, its weight there: bins are summed over chunks as they
+// are and scaled once.  Without, weights are relative to the largest logit of
+// the token's CHUNK (8192 columns), and a chunk's sum is brought to the row's
+// scale by one fp64 factor.  Either way one pass over the logits serves.
 //
 // Two launches:
 //   scan   (chunk, row): one 16-byte load a thread (8 bf16; two for fp32), the
-//          chunk's maximum, and its weight; with filters its weights and
-//          counts by bins of d a quarter octave wide (192 LDS bins).
-//   draw   (row): merges the chunks; without filters picks the chunk, and the
-//          token in it.  With filters: finds the bin that a filter's border
-//          lies in, collects that bin's tokens (in LDS, or by passing over the
-//          row again where they are too many), narrows the border to one key
-//          by a radix select of 1024 sub-bins, and to an index among equal
-//          keys; then the kept weight of every chunk, the chunk, the token.
+//          chunk's maximum, and its weight by 512 columns.  With filters: its
+//          tokens weighed and counted by bins below the chunk's maximum, in LDS,
+//          and the tokens of its first bins, up to 1024, written out bin by bin.
+//          A top-k of up to 512 needs no more than the chunk's own first k and
+//          no weight: only those are handled.
+//   draw   (row, 256 threads): without filters picks the chunk, the 512 columns
+//          and the token.  With a small top-k: everything that the chunks wrote
+//          out, in LDS.  Else: merges the chunks' bins, finds the bin that a
+//          filter's border lies in, and collects that bin's tokens.  The border
+//          is narrowed to one key by a radix select of 1024 sub-bins, and to an
+//          index among equal keys; then the kept weight of every chunk, the
+//          chunk, 64 columns of it, the token.  What does not fit (a bin with
+//          thousands of tokens) is read from the row again.
 #include "common.h"
 
 namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the scan
 constexpr int kTok = 8;                   // tokens per thread and chunk
 constexpr int kChunk = kThreads * kTok;   // columns per chunk
-constexpr int kMaxChunks = 65;            // 2^19 columns and a misaligned start
+constexpr int kMaxChunks = 64;            // a lane each
 constexpr int kBins = 180;                // quarter octaves below the row's maximum: 45 octaves
+constexpr int kFirstBins = 48;            // of them those that are counted first: 12 octaves
+constexpr int kCand = 1024;               // tokens that a chunk writes out
+constexpr int kSmallK = 512;              // a top-k that the chunk's own first k settle
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr int kFrac = 44;                 // fraction bits of a weight
-constexpr int kList = 8192;               // tokens that a border's bin may hold in LDS
+constexpr u64 kLow52 = (1ull << 52) - 1;
 
 struct Chunk {
-  double lref;  // L of the chunk's maximum
-  u64 mass;     // sum of the chunk's weights (without filters)
-  float xmax;   // the chunk's maximum; -inf: no token
-  int pad[3];
+  double lref;   // without filters: log2 weight of the chunk's maximum
+  u64 mass;      // ... and the sum of the chunk's weights below it
+  float xmax;    // the chunk's maximum; -inf: no token
+  int last;      // with filters: the last bin whose tokens are written out
+  int n_out;     // ... how many they are
+  int complete;  // ... and whether a small top-k needs no other
 };
 static_assert(sizeof(Chunk) == 32, "the host sizes the workspace by it");
+struct Bins {
+  u64 mass[kBins];           // weights by bin; without filters by 512 columns
+  u64 list[kCand];           // key << 32 | column, bin by bin
+  uint32_t first[kBins + 4]; // tokens before each bin (of those counted)
+};
+static_assert(sizeof(Bins) == 8 * kBins + 8 * kCand + 4 * (kBins + 4), "as the host has it");
 
 struct Settings {
-  double c;       // log2(e) / T
-  double p, lmin; // top-p; log2(min_p), -inf without
+  double c;        // log2(e) / T
+  double p, lmin;  // top-p; log2(min_p), -inf without
   int k;
   bool fk, fp, filters;
+  bool few;        // a top-k of up to kSmallK: the chunks' first tokens alone
 };
 
 // One row's settings: a value for all rows, or a device array of one per row.
@@ -86,11 +106,12 @@ DEVI Settings settings(const Args& a, int row, int cols) {
   s.p = p > 0.0 ? p : 0.0;
   s.lmin = m > 0.0 && !greedy ? (m < 1.0 ? log2(m) : 0.0) : -INFINITY;
   s.filters = s.fk || s.fp || s.lmin > -INFINITY;
+  s.few = s.fk && k <= kSmallK;
   return s;
 }
 
 // 2^-d for d in [0, 46): 2^-d = 2^i 2^f, f in [0, 1), and 2^f from the series
-// of exp around f = 1/2 (eleven terms leave 2^-47 relative).
+// of exp around f = 1/2 (terms to the eleventh leave 2^-47 relative).
 DEVI double exp2_neg(double d) {
   const double y = -d, i = floor(y);
   const double r = (y - i - 0.5) * 0.69314718055994530942;
@@ -114,7 +135,40 @@ DEVI u64 weight(double d) {
   if (d == 0.0) return 1ull << kFrac;
   // adding 2^52 rounds to a whole number, which is then in the low bits
   const double w = exp2_neg(d) * (double)(1ull << kFrac) + 4503599627370496.0;
-  return __builtin_bit_cast(u64, w) & ((1ull << 52) - 1);
+  return __builtin_bit_cast(u64, w) & kLow52;
+}
+// The weight of a token within its bin, 2^((f - 1) / 4) for f = frac(q), from the
+// series around f = 1/2: |t ln 2 / 4| < 0.087, terms to the eighth leave 2^-50.
+// (The last sum is at 2^52, which rounds it to a whole number.)
+constexpr double kLn2Q = 0.69314718055994530942 / 4;
+constexpr double kC0 = 17592186044416.0 * 0.91700404320467123175;  // 2^(44 - 1/8)
+constexpr double kC1 = kC0 * kLn2Q, kC2 = kC1 * kLn2Q / 2, kC3 = kC2 * kLn2Q / 3,
+                 kC4 = kC3 * kLn2Q / 4, kC5 = kC4 * kLn2Q / 5, kC6 = kC5 * kLn2Q / 6,
+                 kC7 = kC6 * kLn2Q / 7, kC8 = kC7 * kLn2Q / 8;
+DEVI u64 bin_weight(double f) {
+  const double t = f - 0.5;
+  double s = kC8;
+  s = fma(s, t, kC7);
+  s = fma(s, t, kC6);
+  s = fma(s, t, kC5);
+  s = fma(s, t, kC4);
+  s = fma(s, t, kC3);
+  s = fma(s, t, kC2);
+  s = fma(s, t, kC1);
+  return __builtin_bit_cast(u64, fma(s, t, kC0 + 4503599627370496.0)) & kLow52;
+}
+// A token's bin below that of xmax (kBins: it does not count) and its weight in
+// it.  q4 = 4 c.  (Compiled without contraction: x q4 - floor(x q4) with the
+// product unrounded has no place in [0, 1) where logits are masked with -1e38,
+// and gave equal logits other weights in one place than in another.)  The largest token is in bin 0 also where its q is not finite
+// (+inf; 0 * inf), and then alone with its equals.
+DEVI int bin_of(float x, float xmax, double q4, u64* w) {
+  const double top = floor((double)xmax * q4), q = (double)x * q4, fl = floor(q);
+  const double r = top - fl;
+  const bool fin = fabs(top) < INFINITY;
+  *w = bin_weight(fin ? q - fl : 0.5);
+  if (x == xmax) return 0;
+  return x > -INFINITY && fin && r < (double)kBins ? (int)r : kBins;
 }
 
 // Order-preserving unsigned key of a logit (no NaN, no -0) and back.
@@ -151,21 +205,174 @@ template <typename T> DEVI int misaligned(const T* row) {
   return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
 }
 
-DEVI u64 shfl_up64(u64 v, int d) {
-  const uint32_t lo = __shfl_up((uint32_t)v, d, 64), hi = __shfl_up((uint32_t)(v >> 32), d, 64);
-  return (u64)hi << 32 | lo;
+// Wavefront sums through DPP (every lane active): within rows of 16 lanes, then
+// lane 15 of a row into the next, then lane 31 into the upper half.
+template <int CTRL, int ROWS> DEVI uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
 }
-DEVI u64 wave_scan(u64 v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 o = shfl_up64(v, d);
-    if (lane >= d) v += o;
-  }
+template <int CTRL, int ROWS> DEVI u64 dpp(u64 v) {
+  return (u64)dpp<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)v);
+}
+template <typename V> DEVI V wave_scan(V v) {  // inclusive
+  v += dpp<0x111, 0xf>(v);  // row_shr:1
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v);  // row_bcast:15
+  v += dpp<0x143, 0xc>(v);  // row_bcast:31
   return v;
 }
-// Exclusive prefix sum over the workgroup; total in *total.  tmp: kWaves words
-// of LDS that no earlier phase still reads.
+DEVI uint32_t lane_value(uint32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+DEVI u64 lane_value(u64 v, int lane) {
+  return (u64)lane_value((uint32_t)(v >> 32), lane) << 32 | lane_value((uint32_t)v, lane);
+}
+template <typename V> DEVI V wave_total(V v) { return lane_value(wave_scan(v), 63); }
+
+// ---------------------------------------------------------------------------
+// scan: grid (chunks, rows)
+// ---------------------------------------------------------------------------
+struct ScanSmem {
+  u64 mass[kBins];
+  uint32_t cnt[192];
+  uint32_t first[192];  // tokens before each bin
+  float red[kWaves];
+  u64 sums[kWaves];
+  int last;
+};
+
+template <typename T>
+__device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, const Args a,
+                            Chunk* __restrict__ rec, Bins* __restrict__ bins) {
+  __shared__ ScanSmem sm;
+  const int tid = threadIdx.x, lane = tid & 63, ch = blockIdx.x, row_i = blockIdx.y;
+  const long slot = (long)row_i * gridDim.x + ch;
+  const T* row = logits + row_i * ld;
+  float x[kTok];
+  const int col = load8(row, cols, misaligned(row), ch, tid, x);
+  const Settings s = settings(a, row_i, cols);
+  if (tid < 192) {
+    sm.cnt[tid] = 0;
+    if (tid < kBins) sm.mass[tid] = 0;
+  }
+  float mx = x[0];
+#pragma unroll
+  for (int j = 1; j < kTok; ++j) mx = fmaxf(mx, x[j]);
+  mx = wave_max(mx);
+  if (lane == 0) sm.red[tid >> 6] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm.red[w]);
+  Bins& to = bins[slot];
+  if (!s.filters) {
+    const double lref = (double)mx * s.c;
+    u64 sum = 0;
+#pragma unroll
+    for (int j = 0; j < kTok; ++j)
+      if (x[j] > -INFINITY) sum += weight(x[j] == mx ? 0.0 : lref - (double)x[j] * s.c);
+    sum = wave_total(sum);
+    if (lane == 0) sm.sums[tid >> 6] = sum;
+    __syncthreads();
+    if (tid < 64) {
+      const u64 w = lane < kWaves ? sm.sums[lane] : 0, all = wave_total(w);
+      if (lane < kWaves) to.mass[lane] = w;
+      if (lane == 0) rec[slot] = Chunk{lref, all, mx, 0, 0, 0};
+    }
+    return;
+  }
+  // Without top-p, tokens that min-p drops even by the chunk's own maximum do not
+  // count.
+  const double q4 = 4.0 * s.c, least = s.fp ? -INFINITY : (double)mx * s.c + s.lmin;
+  const int counted = s.fk && !s.few ? kBins : kFirstBins;
+  int bin[kTok];
+  uint32_t rank[kTok];
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    u64 w;
+    bin[j] = bin_of(x[j], mx, q4, &w);
+    if (mx == -INFINITY || ((double)x[j] * s.c < least && x[j] != mx)) bin[j] = kBins;
+    if (!s.few && bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
+    if (bin[j] < counted) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
+  }
+  __syncthreads();
+  uint32_t have = 0;
+  if (s.few) {  // too few in the first bins: the others too
+    have = wave_total(lane < kFirstBins ? sm.cnt[lane] : 0);
+    if (have < (uint32_t)s.k) {
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kTok; ++j)
+        if (bin[j] >= counted && bin[j] < kBins) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
+      __syncthreads();
+    }
+  }
+  const int known = s.few && have < (uint32_t)s.k ? kBins : counted;  // bins counted
+  if (tid < 64) {  // three bins a lane
+    uint32_t n[3], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sum += n[i] = sm.cnt[3 * lane + i];
+    const uint32_t inc = wave_scan(sum);
+    uint32_t before = inc - sum;
+    // written out: whole bins while they fit, up to the one that completes a
+    // small top-k
+    int last = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int b = 3 * lane + i;
+      sm.first[b] = before;
+      last += b < known && before + n[i] <= (uint32_t)kCand &&
+              !(s.few && before >= (uint32_t)s.k);
+      before += n[i];
+    }
+    // (the bins for which that holds are the first ones)
+    last = (int)wave_total((uint32_t)last) - 1;
+    const uint32_t all = lane_value(inc, 63);
+    if (lane == 0) sm.last = last;
+    // written above by this wavefront: LDS keeps its order
+    const uint32_t n_out = last + 1 < 192 ? sm.first[last + 1] : all;
+    if (lane == 0)
+      rec[slot] = Chunk{0.0, 0, mx, last, (int)n_out,
+                        s.few && (n_out >= (uint32_t)s.k || n_out == all)};
+  }
+  __syncthreads();
+  const int last = sm.last;
+#pragma unroll
+  for (int j = 0; j < kTok; ++j)
+    if (bin[j] <= last)
+      to.list[sm.first[bin[j]] + rank[j]] = (u64)key_of(x[j]) << 32 | (uint32_t)(col + j);
+  if (s.few) return;
+  if (tid <= kBins) to.first[tid] = sm.first[tid];
+  if (tid < kBins) to.mass[tid] = sm.mass[tid];
+}
+
+// ---------------------------------------------------------------------------
+// draw: grid (rows)
+// ---------------------------------------------------------------------------
+constexpr int kDraw = 256, kDrawWaves = kDraw / 64;
+constexpr int kSub = 1024;      // sub-bins of the radix select
+constexpr int kList = 4096;     // tokens collected in LDS
+constexpr int kCell = 64, kCells = kChunk / kCell;  // columns of a chunk's cells
+
+struct DrawSmem {
+  u64 list[kList];              // key << 32 | column of the collected tokens
+  u64 sub_mass[kSub];           // radix select: weight and count by sub-bin
+  uint32_t sub_cnt[kSub];
+  u64 mass[kBins];              // the row's bins, weights in the row's scale
+  uint32_t cnt[kBins];
+  double scale[kBins];          // a bin's scale: 2^(-bin / 4)
+  int off[kMaxChunks];          // bins that the chunk's maximum lies below the row's; kBins: out
+  int last[kMaxChunks];
+  uint32_t from[kMaxChunks], base[kMaxChunks + 1];  // collecting: where in a chunk's list, and ours
+  u64 kept[kMaxChunks];         // kept weight of a chunk
+  uint32_t tie[kMaxChunks];
+  u64 cell[kCells];             // ... of a chunk's 64 columns
+  u64 tmp[kDrawWaves];
+  uint32_t kmin, kmax;
+  u64 a, b;                     // a value that one thread hands to all
+  float xr;
+  int i, j;
+};
+
+// Exclusive prefix sum over the workgroup; total in *total.
 DEVI u64 block_scan(u64 v, u64* tmp, u64* total) {
   const int wave = threadIdx.x >> 6;
   const u64 inc = wave_scan(v);
@@ -173,7 +380,7 @@ DEVI u64 block_scan(u64 v, u64* tmp, u64* total) {
   __syncthreads();
   u64 base = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
+  for (int w = 0; w < kDrawWaves; ++w) {
     const u64 t = tmp[w];
     base += w < wave ? t : 0;
     all += t;
@@ -183,294 +390,363 @@ DEVI u64 block_scan(u64 v, u64* tmp, u64* total) {
   return base + inc - v;
 }
 
-// ---------------------------------------------------------------------------
-// scan: grid (chunks, rows)
-// ---------------------------------------------------------------------------
-template <typename T>
-__device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, const Args a,
-                            Chunk* __restrict__ rec, uint32_t* __restrict__ cnt,
-                            u64* __restrict__ mass) {
-  __shared__ uint32_t h_cnt[kBins];
-  __shared__ u64 h_mass[kBins];
-  __shared__ float red[kWaves];
-  __shared__ u64 sums[kWaves];
-  const int tid = threadIdx.x, ch = blockIdx.x, row_i = blockIdx.y;
-  const long slot = (long)row_i * gridDim.x + ch;
-  const T* row = logits + row_i * ld;
-  float x[kTok];
-  load8(row, cols, misaligned(row), ch, tid, x);
-  const Settings s = settings(a, row_i, cols);
-  if (s.filters && tid < kBins) {
-    h_cnt[tid] = 0;
-    h_mass[tid] = 0;
-  }
-  float mx = x[0];
-#pragma unroll
-  for (int j = 1; j < kTok; ++j) mx = fmaxf(mx, x[j]);
-  mx = wave_max(mx);
-  if ((tid & 63) == 0) red[tid >> 6] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red[w]);
-  const double lref = (double)mx * s.c;
-  if (!s.filters) {
-    u64 sum = 0;
-#pragma unroll
-    for (int j = 0; j < kTok; ++j)
-      if (x[j] > -INFINITY) sum += weight(x[j] == mx ? 0.0 : lref - (double)x[j] * s.c);
-    const u64 inc = wave_scan(sum);
-    if ((tid & 63) == 63) sums[tid >> 6] = inc;
-    __syncthreads();
-    if (tid == 0) {
-      u64 all = 0;
-      for (int w = 0; w < kWaves; ++w) all += sums[w];
-      rec[slot] = Chunk{lref, all, mx, {}};
-    }
-    return;
-  }
-  const double bmax = floor(4.0 * lref);
-#pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    if (!(x[j] > -INFINITY)) continue;
-    const double l = (double)x[j] * s.c;
-    const bool top = x[j] == mx;
-    const double r = top ? 0.0 : bmax - floor(4.0 * l);
-    if (r < (double)kBins) {  // false for NaN
-      atomicAdd(&h_cnt[(int)r], 1u);
-      atomicAdd(&h_mass[(int)r], weight(top ? 0.0 : lref - l));
-    }
-  }
-  __syncthreads();
-  if (tid < kBins) {
-    cnt[slot * kBins + tid] = h_cnt[tid];
-    mass[slot * kBins + tid] = h_mass[tid];
-  }
-  if (tid == 0) rec[slot] = Chunk{lref, 0, mx, {}};
+// floor(x total) for x in [0, 1), in whole numbers: fp64 would round totals past
+// 2^53, and a border of equal weights would move.
+DEVI u64 share(double x, u64 total) {
+  return __umul64hi((u64)(x * 18446744073709551616.0), total);
+}
+// The weight that top-p's part holds at least: p total, less the rounding of p
+// itself (0.9 of 40 equal tokens are 36 of them, though the nearest fp64 to 0.9
+// is above it).
+DEVI u64 part_of(double p, u64 total) {
+  const u64 n = share(p, total), slack = total >> 50;
+  return n > slack ? n - slack : 1;
+}
+// u times a total, as the running weight that the drawn token exceeds.
+DEVI u64 target_of(float u, u64 total) {
+  return u < 1.0f ? (u > 0.0f ? share(u, total) : 0) : u >= 1.0f ? total - 1 : 0;
 }
 
-// ---------------------------------------------------------------------------
-// draw: grid (rows)
-// ---------------------------------------------------------------------------
-struct DrawSmem {
-  u64 list[kList];              // key << 32 | column of the collected tokens
-  u64 sub_mass[kThreads];       // radix select: weight and count by sub-bin
-  uint32_t sub_cnt[kThreads];
-  u64 mass[kBins];              // the row's bins
-  uint32_t cnt[kBins];
-  double f[kMaxChunks];         // chunk scale -> row scale; 0: the chunk does not count
-  double lref[kMaxChunks];
-  float xmax[kMaxChunks];
-  int off[kMaxChunks];          // bins that the chunk's maximum lies below the row's
-  u64 kept[kMaxChunks];         // kept weight of a chunk, in its own scale
-  uint32_t tie[kMaxChunks];
-  u64 tmp[kWaves];
-  uint32_t n_list, kmin, kmax;
-  u64 a, b;                     // a value that one thread hands to all
-  int i, j;
-};
+// Without filters, by one wavefront: the chunk, its 512 columns, the token.
+template <typename T>
+DEVI void draw_plain(const T* row, int cols, int mis, const Settings& s, float u,
+                     const Chunk* rec, const Bins* bins, int n_ch, long long* out) {
+  const int lane = threadIdx.x & 63;
+  Chunk r{};
+  r.xmax = -INFINITY;
+  if (lane < n_ch) r = rec[lane];
+  const float xr = wave_max(r.xmax);
+  if (xr == -INFINITY) {  // no token to draw
+    if (lane == 0) *out = -1;
+    return;
+  }
+  const double d = r.xmax == xr ? 0.0 : (double)xr * s.c - r.lref;
+  const bool in = r.xmax > -INFINITY && d < 46.0;
+  const double f = in ? (d == 0.0 ? 1.0 : exp2_neg(d)) : 0.0;  // chunk scale -> row scale
+  const u64 w = !in ? 0 : f == 1.0 ? r.mass : (u64)((double)r.mass * f + 0.5);
+  const u64 inc = wave_scan(w);
+  u64 t = target_of(u, lane_value(inc, 63));
+  // one lane: the running sums are increasing
+  const int ch = __builtin_ctzll(__ballot(inc - w <= t && t < inc));
+  t -= lane_value(inc - w, ch);
+  const double fc = __builtin_bit_cast(double, lane_value(__builtin_bit_cast(u64, f), ch));
+  t = min((u64)((double)t / fc), lane_value(r.mass, ch) - 1);  // in the chunk's scale
+  const double lref = __builtin_bit_cast(double, lane_value(__builtin_bit_cast(u64, r.lref), ch));
+  const float xmax = __builtin_bit_cast(float, lane_value(__builtin_bit_cast(uint32_t, r.xmax), ch));
+  const u64 part = lane < kWaves ? bins[ch].mass[lane] : 0, pinc = wave_scan(part);
+  const int sub = __builtin_ctzll(__ballot(pinc - part <= t && t < pinc));
+  t -= lane_value(pinc - part, sub);
+  float x[kTok];
+  const int col = load8(row, cols, mis, ch, sub * 64 + lane, x);
+  u64 v[kTok], mine = 0;
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) {
+    v[j] = x[j] > -INFINITY ? weight(x[j] == xmax ? 0.0 : lref - (double)x[j] * s.c) : 0;
+    mine += v[j];
+  }
+  u64 run = wave_scan(mine) - mine;
+  if (run <= t && t < run + mine) {
+    int at = col;
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {  // tokens whose running weight does not exceed t
+      run += v[j];
+      at += run <= t;
+    }
+    *out = at;
+  }
+}
+
+// The tokens of bins lo .. hi of a half chunk, into the list (by the workgroup; a
+// call of its own, because few rows need it and each place that may is code).
+template <typename T>
+__device__ __attribute__((noinline)) void refill(const T* row, int cols, int mis, float xr,
+                                                 double q4, int lo, int hi, int part,
+                                                 DrawSmem& sm) {
+  static_assert(kChunk / 2 <= kList, "a half chunk fits");
+  __syncthreads();
+  if (threadIdx.x == 0) sm.base[64] = 0;
+  __syncthreads();
+  for (int it = 0; it < kChunk / 2 / (kDraw * kTok); ++it) {
+    float x[kTok];
+    const int col = load8(row, cols, mis, part >> 1,
+                          (part & 1) * (kThreads / 2) + it * kDraw + threadIdx.x, x);
+    for (int j = 0; j < kTok; ++j) {
+      u64 w;
+      const int b = x[j] > -INFINITY ? bin_of(x[j], xr, q4, &w) : kBins + 1;
+      if (b >= lo && b <= hi)
+        sm.list[atomicAdd(&sm.base[64], 1u)] = (u64)key_of(x[j]) << 32 | (uint32_t)(col + j);
+    }
+  }
+  __syncthreads();
+}
 
 template <typename T>
 __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, const Args a,
                             const float* __restrict__ us, const Chunk* __restrict__ rec,
-                            const uint32_t* __restrict__ cnt, const u64* __restrict__ mass,
-                            int n_ch, long long* __restrict__ out, int* __restrict__ advance) {
+                            const Bins* __restrict__ bins, int n_ch, long long* __restrict__ out,
+                            int* __restrict__ advance) {
   __shared__ DrawSmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row_i = blockIdx.x;
   if (advance && row_i == 0 && tid == 0) *advance += 1;
   const T* row = logits + row_i * ld;
   const int mis = misaligned(row);
-  const Settings s = settings(a, row_i, cols);
-  const double c = s.c;
   rec += (long)row_i * n_ch;
-  cnt += (long)row_i * n_ch * kBins;
-  mass += (long)row_i * n_ch * kBins;
-
-  // ---- the row's maximum, and each chunk's place below it -------------------
-  float xr = -INFINITY;
-  for (int i = 0; i < n_ch; ++i) xr = fmaxf(xr, rec[i].xmax);
-  if (xr == -INFINITY) {  // no token left to draw
-    if (tid == 0) out[row_i] = -1;
+  bins += (long)row_i * n_ch;
+  out += row_i;
+  const float u = us[row_i];
+  const Settings s = settings(a, row_i, cols);
+  if (!s.filters) {
+    if (wave == 0) draw_plain(row, cols, mis, s, u, rec, bins, n_ch, out);
     return;
   }
-  const double lrow = (double)xr * c, brow = floor(4.0 * lrow);
-  if (tid < n_ch) {
-    const Chunk r = rec[tid];
-    const double d = r.xmax == xr ? 0.0 : lrow - r.lref;
-    const bool in = r.xmax > -INFINITY && d < 46.0;
-    sm.f[tid] = in ? (d == 0.0 ? 1.0 : exp2_neg(d)) : 0.0;
-    sm.off[tid] = in && d != 0.0 ? (int)(brow - floor(4.0 * r.lref)) : 0;
-    sm.lref[tid] = r.lref;
-    sm.xmax[tid] = r.xmax;
-    sm.kept[tid] = r.mass;
-  }
-  __syncthreads();
+  const double c = s.c, q4 = 4.0 * c;
 
-  // A token's bin below the row's maximum; kBins or more: it does not count.
-  auto bin_of = [&](float x) {
-    if (x == xr) return 0;
-    const double r = brow - floor(4.0 * ((double)x * c));
-    return r < (double)kBins ? (int)r : kBins;
+  // ---- the row's maximum, and each chunk's place below it -------------------
+  if (wave == 0) {
+    Chunk r{};
+    r.xmax = -INFINITY;
+    if (lane < n_ch) r = rec[lane];
+    const float m = wave_max(r.xmax);
+    u64 w;
+    const int off = r.xmax > -INFINITY ? bin_of(r.xmax, m, q4, &w) : kBins;
+    sm.off[lane] = off;
+    sm.last[lane] = r.last;
+    sm.from[lane] = 0;
+    // what a small top-k collects: all that the chunks wrote out
+    const uint32_t n = off < kBins ? r.n_out : 0, inc = wave_scan(n);
+    sm.base[lane] = inc - n;
+    if (lane == 63) sm.base[64] = inc;
+    const bool all = __all(off >= kBins || r.complete);
+    if (lane == 0) {
+      sm.xr = m;
+      sm.i = all;
+    }
+  }
+  for (int i = tid; i < kBins; i += kDraw) {
+    sm.cnt[i] = 0;
+    sm.mass[i] = 0;
+    sm.scale[i] = exp2_neg(0.25 * i);
+  }
+  if (tid < kMaxChunks) sm.kept[tid] = 0;
+  if (tid < kCells) sm.cell[tid] = 0;
+  __syncthreads();
+  const float xr = sm.xr;
+  if (xr == -INFINITY) {  // no token to draw
+    if (tid == 0) *out = -1;
+    return;
+  }
+  const double lmin = (double)xr * c + s.lmin;  // min-p in terms of L
+  // a small top-k whose chunks wrote out all that it needs, and that fits
+  const bool fast = s.few && sm.i && sm.base[64] <= (uint32_t)kList;
+
+  auto weight_of = [&](float x, int* b) __attribute__((always_inline)) {  // in the row's scale
+    u64 w;
+    *b = bin_of(x, xr, q4, &w);
+    return *b == 0 ? w : *b < kBins ? (u64)((double)w * sm.scale[*b] + 0.5) : 0;
   };
-  auto row_weight = [&](float x) { return weight(x == xr ? 0.0 : lrow - (double)x * c); };
-  auto chunk_weight = [&](int ch, float x) {
-    return weight(x == sm.xmax[ch] ? 0.0 : sm.lref[ch] - (double)x * c);
+  auto row_weight = [&](float x) __attribute__((always_inline)) {
+    int b;
+    return weight_of(x, &b);
+  };
+  auto bin_at = [&](float x) __attribute__((always_inline)) {
+    u64 w;
+    return bin_of(x, xr, q4, &w);
   };
 
   // the border that top-k and top-p leave: tokens with a higher key, or the same
   // key and a column up to cut_col; jc: its bin (kBins: no border)
   uint32_t cut_key = 0;
   int cut_col = 0x7fffffff, jc = kBins;
-  const double lmin = lrow + s.lmin;  // min-p in terms of L
-  auto keeps = [&](float x, int col) {
+  auto above_cut = [&](float x, int col) __attribute__((always_inline)) {
     const uint32_t key = key_of(x);
-    return (key > cut_key || (key == cut_key && col <= cut_col)) &&
-           (x == xr || (double)x * c >= lmin || s.lmin == -INFINITY);
+    return key > cut_key || (key == cut_key && col <= cut_col);
+  };
+  auto keeps = [&](float x, int col) __attribute__((always_inline)) {
+    return above_cut(x, col) && (x == xr || (double)x * c >= lmin || s.lmin == -INFINITY);
   };
 
-  if (s.filters) {
-    // ---- the row's bins ------------------------------------------------------
-    if (tid < kBins) {
-      uint32_t n = 0;
-      u64 m = 0;
-      for (int ch = 0; ch < n_ch; ++ch) {
-        const int r = tid - sm.off[ch];
-        const double f = sm.f[ch];
-        if (f > 0.0 && r >= 0) {
-          n += cnt[ch * kBins + r];
-          const u64 v = mass[ch * kBins + r];
-          m += f == 1.0 ? v : (u64)((double)v * f + 0.5);
-        }
+  // Copies the chunks' list entries [from, from + base[ch + 1] - base[ch]) into
+  // ours: 16 lanes a chunk.
+  auto gather = [&]() __attribute__((always_inline)) {
+    const int l16 = tid & 15;
+    for (int ch = tid >> 4; ch < n_ch; ch += kDraw / 16) {
+      const uint32_t b0 = sm.base[ch], n = sm.base[ch + 1] - b0;
+      const u64* src = bins[ch].list + sm.from[ch];
+      for (uint32_t i = l16; i < n; i += 64) {
+        u64 e[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) e[t] = src[min(i + 16 * t, n - 1)];
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (i + 16 * t < n) sm.list[b0 + i + 16 * t] = e[t];
       }
-      sm.cnt[tid] = n;
-      sm.mass[tid] = m;
     }
     __syncthreads();
-    // exclusive prefix sums over the bins, in registers of threads 0 .. kBins-1
-    u64 total_n, total_m;
-    const u64 n_here = tid < kBins ? sm.cnt[tid] : 0, m_here = tid < kBins ? sm.mass[tid] : 0;
-    const u64 n_before = block_scan(n_here, sm.tmp, &total_n);
-    const u64 m_before = block_scan(m_here, sm.tmp, &total_m);
+  };
 
-    int list_lo = 1, list_hi = 0;  // the bins whose tokens the list holds
-    // f(x, column) for every token of bins lo .. hi, from the list or the row
-    auto each = [&](int lo, int hi, auto&& f) {
-      if (lo >= list_lo && hi <= list_hi) {
-        const int n = sm.n_list;
-        for (int i = tid; i < n; i += kThreads) {
-          const u64 e = sm.list[i];
-          const float x = of_key((uint32_t)(e >> 32));
-          const int b = bin_of(x);
-          if (b >= lo && b <= hi) f(x, (int)(uint32_t)e);
-        }
-        return;
+  int list_lo = 1, list_hi = 0;  // the bins whose tokens the LDS list holds
+  // f(x, column) for every token of bins lo .. hi: from the list, or passing over
+  // the row, half a chunk at a time through the list
+  auto each = [&](int lo, int hi, auto&& f) __attribute__((always_inline)) {
+    const bool listed = lo >= list_lo && hi <= list_hi;
+    const bool all = !listed || (lo == list_lo && hi == list_hi);
+    for (int part = 0; part < (listed ? 1 : 2 * n_ch); ++part) {
+      if (!listed) {
+        list_lo = 1;
+        list_hi = 0;
+        const int off = sm.off[part >> 1];
+        if (off > hi || off >= kBins) continue;
+        refill(row, cols, mis, xr, q4, lo, hi, part, sm);
       }
-      for (int ch = wave; ch < n_ch; ch += kWaves) {  // a wavefront takes whole chunks
-        if (!(sm.f[ch] > 0.0) || sm.off[ch] > hi) continue;
-        for (int it = 0; it < kThreads / 64; ++it) {
-          float x[kTok];
-          const int col = load8(row, cols, mis, ch, it * 64 + lane, x);
-#pragma unroll
-          for (int j = 0; j < kTok; ++j)
-            if (x[j] > -INFINITY) {
-              const int b = bin_of(x[j]);
-              if (b >= lo && b <= hi) f(x[j], col + j);
-            }
-        }
+      const uint32_t n = sm.base[64];
+      for (uint32_t i = tid; i < n; i += kDraw) {
+        const u64 e = sm.list[i];
+        const float x = of_key((uint32_t)(e >> 32));
+        const int b = all ? lo : bin_at(x);
+        if (b >= lo && b <= hi) f(x, (int)(uint32_t)e);
       }
-    };
-    // collects the tokens of bins lo .. hi, n of them, in LDS if they fit
-    auto collect = [&](int lo, int hi, u64 n) {
-      if ((lo >= list_lo && hi <= list_hi) || n > (u64)kList) return;
-      __syncthreads();
-      if (tid == 0) sm.n_list = 0;
-      __syncthreads();
+    }
+  };
+  // collects the tokens of bins lo .. hi in LDS where the chunks wrote them out
+  // and they fit
+  auto collect = [&](int lo, int hi) __attribute__((always_inline)) {
+    if (lo >= list_lo && hi <= list_hi) return;
+    __syncthreads();
+    if (wave == 0) {
+      uint32_t f0 = 0, n = 0;
+      const int off = lane < n_ch ? sm.off[lane] : kBins;
+      const bool in = off <= hi && off < kBins;
+      if (in && hi - off <= sm.last[lane]) {
+        f0 = bins[lane].first[max(lo - off, 0)];
+        n = bins[lane].first[hi - off + 1] - f0;
+      }
+      const uint32_t inc = wave_scan(n);
+      sm.from[lane] = f0;
+      sm.base[lane] = inc - n;
+      const bool ok = __all(!in || hi - off <= sm.last[lane]);
+      if (lane == 63) sm.base[64] = inc;
+      if (lane == 0) sm.i = ok && lane_value(inc, 63) <= (uint32_t)kList;
+    }
+    __syncthreads();
+    if (!sm.i) {
       list_lo = 1;
-      list_hi = 0;  // read from the row
+      list_hi = 0;  // from the row
+      return;
+    }
+    gather();
+    list_lo = lo;
+    list_hi = hi;
+  };
+  // The border among the tokens of bins lo .. hi that are above the present cut:
+  // the one at which their running count (by_count) or weight, in the order,
+  // reaches need.  Sets the cut.
+  auto border = [&](int lo, int hi, u64 need, bool by_count) __attribute__((always_inline)) {
+    constexpr int KS = sizeof(T) == 2 ? 16 : 0;  // low bits that every key shares
+    __syncthreads();
+    if (tid == 0) {
+      sm.kmin = 0xffffffffu;
+      sm.kmax = 0;
+    }
+    __syncthreads();
+    uint32_t k0 = 0xffffffffu, k1 = 0;
+    each(lo, hi, [&](float x, int col) {
+      if (!above_cut(x, col)) return;
+      k0 = min(k0, key_of(x) >> KS);
+      k1 = max(k1, key_of(x) >> KS);
+    });
+    if (k0 <= k1) {
+      atomicMin(&sm.kmin, k0);
+      atomicMax(&sm.kmax, k1);
+    }
+    __syncthreads();
+    k0 = sm.kmin;
+    k1 = sm.kmax;
+    u64 ties = 0;
+    do {
+      const uint32_t span = k1 - k0;
+      const int sh = span < (uint32_t)kSub ? 0 : 22 - __builtin_clz(span);
+      for (int i = tid; i < kSub; i += kDraw) {
+        sm.sub_mass[i] = 0;
+        sm.sub_cnt[i] = 0;
+      }
+      __syncthreads();
       each(lo, hi, [&](float x, int col) {
-        const uint32_t at = atomicAdd(&sm.n_list, 1u);
-        sm.list[at & (kList - 1)] = (u64)key_of(x) << 32 | (uint32_t)col;
-      });
-      __syncthreads();
-      list_lo = lo;
-      list_hi = hi;
-    };
-    // The border in bin j: the token at which the running count (BY_COUNT) or
-    // weight of the bin's tokens, in the order, reaches need.  Sets the cut.
-    auto border = [&](int j, u64 need, bool by_count) {
-      __syncthreads();
-      if (tid == 0) {
-        sm.kmin = 0xffffffffu;
-        sm.kmax = 0;
-      }
-      __syncthreads();
-      each(j, j, [&](float x, int) {
-        atomicMin(&sm.kmin, key_of(x));
-        atomicMax(&sm.kmax, key_of(x));
-      });
-      __syncthreads();
-      uint32_t k0 = sm.kmin, k1 = sm.kmax;
-      u64 ties = 0;
-      do {
-        const uint32_t span = k1 - k0;
-        const int sh = span < (uint32_t)kThreads ? 0 : 22 - __builtin_clz(span);
-        sm.sub_mass[tid] = 0;
-        sm.sub_cnt[tid] = 0;
-        __syncthreads();
-        each(j, j, [&](float x, int) {
-          const uint32_t k = key_of(x);
-          if (k >= k0 && k <= k1) {
-            atomicAdd(&sm.sub_cnt[(k1 - k) >> sh], 1u);
-            if (!by_count) atomicAdd(&sm.sub_mass[(k1 - k) >> sh], row_weight(x));
-          }
-        });
-        __syncthreads();
-        const u64 n = sm.sub_cnt[tid], v = by_count ? n : sm.sub_mass[tid];
-        u64 all;
-        const u64 before = block_scan(v, sm.tmp, &all);
-        if (need > all) need = all;  // the merged bin's sum was rounded up
-        if (need == 0) break;        // every weight here rounds to zero: all are kept
-        if (v > 0 && before < need && need <= before + v) {
-          sm.i = tid;
-          sm.a = need - before;
-          sm.b = n;
+        const uint32_t k = key_of(x) >> KS;
+        if (k >= k0 && k <= k1 && above_cut(x, col)) {
+          atomicAdd(&sm.sub_cnt[(k1 - k) >> sh], 1u);
+          if (!by_count) atomicAdd(&sm.sub_mass[(k1 - k) >> sh], row_weight(x));
         }
-        __syncthreads();
-        const uint32_t sub = sm.i;
-        need = sm.a;
-        ties = sm.b;
-        __syncthreads();
-        const uint32_t top = k1 - (sub << sh);
-        k0 = top - k0 < (1u << sh) ? k0 : top - (1u << sh) + 1;
-        k1 = top;
-      } while (k0 < k1);
-      cut_key = k0;
-      cut_col = 0x7fffffff;
-      jc = j;
-      if (need == 0) return;
-      const float x = of_key(k0);
-      if (!by_count) {  // as many of the equal tokens as their weight needs
-        const u64 w = row_weight(x);
-        need = (need + w - 1) / w;
-      }
-      if (need >= ties) return;
-      // the column of the need-th of the equal tokens: its chunk, then in it
-      if (tid < kMaxChunks) sm.tie[tid] = 0;
-      __syncthreads();
-      each(j, j, [&](float y, int col) {
-        if (key_of(y) == k0) atomicAdd(&sm.tie[(col + mis) / kChunk], 1u);
       });
       __syncthreads();
-      if (tid == 0) {
-        u64 left = need;
-        int ch = 0;
-        while (ch < n_ch - 1 && left > sm.tie[ch]) left -= sm.tie[ch++];
-        sm.i = ch;
-        sm.a = left;
+      u64 v[4], sum = 0, all;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sum += v[i] = by_count ? sm.sub_cnt[4 * tid + i] : sm.sub_mass[4 * tid + i];
+      u64 before = block_scan(sum, sm.tmp, &all);
+      if (need > all) need = all;  // the merged bin's sum was rounded up
+      if (need == 0) break;        // every weight here rounds to zero: all are kept
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (v[i] > 0 && before < need && need <= before + v[i]) {
+          sm.i = 4 * tid + i;
+          sm.a = need - before;
+          sm.b = sm.sub_cnt[4 * tid + i];
+        }
+        before += v[i];
       }
       __syncthreads();
+      const uint32_t sub = sm.i;
+      need = sm.a;
+      ties = sm.b;
+      __syncthreads();
+      const uint32_t top = k1 - (sub << sh);
+      k0 = top - k0 < (1u << sh) ? k0 : top - (1u << sh) + 1;
+      k1 = top;
+    } while (k0 < k1);
+    // (bf16: the low half of a key is all zeros, of a negative logit's all ones)
+    k0 = KS ? k0 << 16 | (k0 & 0x8000u ? 0u : 0xffffu) : k0;
+    if (need == 0) {
+      if (k0 > cut_key) {
+        cut_key = k0;
+        cut_col = 0x7fffffff;
+      }
+      return;
+    }
+    const float x = of_key(k0);
+    if (!by_count) {  // as many of the equal tokens as their weight needs
+      const u64 w = row_weight(x);
+      need = (need + w - 1) / w;
+    }
+    if (need >= ties) {  // all that were above the cut
+      if (k0 > cut_key) {
+        cut_key = k0;
+        cut_col = 0x7fffffff;
+      }
+      return;
+    }
+    cut_key = k0;
+    // the column of the need-th of the equal tokens (those above a cut among them
+    // are the first): its chunk, then in it
+    if (tid < kMaxChunks) sm.tie[tid] = 0;
+    __syncthreads();
+    each(lo, hi, [&](float y, int col) {
+      if (y == x) atomicAdd(&sm.tie[(col + mis) / kChunk], 1u);
+    });
+    __syncthreads();
+    if (wave == 0) {
+      const u64 n = lane < n_ch ? sm.tie[lane] : 0, before = wave_scan(n) - n;
+      if (before < need && need <= before + n) {
+        sm.i = lane;
+        sm.a = need - before;
+      }
+    }
+    __syncthreads();
+    const int ch = sm.i;
+    u64 left = sm.a;
+    __syncthreads();
+    for (int it = 0; it < kChunk / (kDraw * kTok); ++it) {
       float y[kTok];
-      const int col = load8(row, cols, mis, sm.i, tid, y);
-      const u64 left = sm.a;
+      const int col = load8(row, cols, mis, ch, it * kDraw + tid, y);
       u64 here = 0, all;
 #pragma unroll
       for (int t = 0; t < kTok; ++t) here += y[t] == x;
@@ -481,137 +757,188 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
         for (int t = 0; t < kTok; ++t)
           if (y[t] == x && ++n == left) sm.j = col + t;
       }
-      __syncthreads();
-      cut_col = sm.j;
-    };
-    // the bin at which a running sum over the bins reaches need (thread j holds
-    // bin j's sum and what lies before it); what is needed within the bin, and
-    // what it holds, in sm.a and sm.b
-    auto find_bin = [&](u64 before, u64 here, u64 need) {
-      __syncthreads();
-      if (here > 0 && before < need && need <= before + here) {
-        sm.i = tid;
-        sm.a = need - before;
-      }
-      __syncthreads();
-      return sm.i;
-    };
+      if (left <= all) break;
+      left -= all;
+    }
+    __syncthreads();
+    cut_col = sm.j;
+  };
 
-    u64 m_left = total_m;  // the weight that top-k leaves
-    if (s.fk && (u64)s.k < total_n) {
-      const int jk = find_bin(n_before, n_here, (u64)s.k);
-      const u64 need = sm.a;
-      __syncthreads();
-      if (tid == jk) {
-        sm.b = n_before + n_here;
-        sm.a = m_before;
-      }
-      __syncthreads();
-      const u64 up_to = sm.b, above = sm.a;
-      // every token up to the border's bin where that is few, else the bin's
-      collect(up_to <= (u64)kList ? 0 : jk, jk, up_to <= (u64)kList ? up_to : sm.cnt[jk]);
-      border(jk, need, true);
-      if (s.fp) {
-        u64 mine = 0, part;
-        each(jk, jk, [&](float x, int col) {
-          const uint32_t key = key_of(x);
-          if (key > cut_key || (key == cut_key && col <= cut_col)) mine += row_weight(x);
-        });
-        block_scan(mine, sm.tmp, &part);
-        m_left = above + part;
-      }
-    }
-    if (s.fp) {
-      u64 need = (u64)ceil(s.p * (double)m_left);
-      need = max(1ull, min(need, min(m_left, total_m)));
-      // (bins past top-k's border hold weight too, but the need is met before)
-      const int jp = find_bin(m_before, m_here, need);
-      const u64 in_bin = sm.a;
-      const uint32_t old_key = cut_key;
-      const int old_col = cut_col, old_bin = jc;
-      collect(jp, jp, sm.cnt[jp]);
-      border(jp, in_bin, false);
-      // never past top-k's border (the sums around it are rounded)
-      if (old_bin < kBins && (cut_key < old_key || (cut_key == old_key && cut_col > old_col))) {
-        cut_key = old_key;
-        cut_col = old_col;
-        jc = old_bin;
-      }
-    }
-    if (s.lmin > -INFINITY) {
-      const double r = brow - floor(4.0 * lmin);
-      jc = min(jc, r < (double)kBins ? (int)r : kBins);
-    }
-    // ---- each chunk's kept weight: whole bins, and the border's bin ----------
-    __syncthreads();
-    const int whole = jc;  // bins 0 .. whole - 1 are kept
-    for (int ch = wave; ch < n_ch; ch += kWaves) {
-      u64 v = 0;
-      if (sm.f[ch] > 0.0)
-        for (int r = lane; r < whole - sm.off[ch]; r += 64) v += mass[ch * kBins + r];
-      v = wave_scan(v);
-      if (lane == 63) sm.kept[ch] = v;
-    }
-    __syncthreads();
-    if (jc < kBins)
-      each(jc, jc, [&](float x, int col) {
-        if (keeps(x, col)) {
-          const int ch = (col + mis) / kChunk;
-          atomicAdd(&sm.kept[ch], chunk_weight(ch, x));
-        }
+  u64 m_before = 0, m_here = 0;  // thread b: the weight before bin b, and in it
+  u64 n_before = 0, n_here = 0;  // ... and tokens
+  u64 total_n = 0, total_m = 0;
+  if (fast) {
+    gather();
+    list_lo = 0;
+    list_hi = kBins;
+  } else {
+    // ---- the row's bins ------------------------------------------------------
+    if (s.few) {  // too many for what the chunks wrote out: by passing over the row
+      if (tid < kMaxChunks) sm.last[tid] = -1;
+      each(0, kBins - 1, [&](float x, int) {
+        int b;
+        const u64 w = weight_of(x, &b);
+        atomicAdd(&sm.cnt[b], 1u);
+        atomicAdd(&sm.mass[b], w);
       });
-    __syncthreads();
-  }
-
-  // ---- the chunk that u falls into -------------------------------------------
-  if (tid == 0) {
-    u64 total = 0;
-    for (int ch = 0; ch < n_ch; ++ch)
-      total += (u64)((double)sm.kept[ch] * sm.f[ch] + 0.5);
-    const double u = (double)us[row_i];
-    const double at = (u > 0.0 ? u : 0.0) * (double)total;
-    u64 t = at < (double)total ? (u64)at : total;
-    if (t >= total) t = total - 1;
-    int pick = -1;
-    u64 rest = 0;
-    for (int ch = 0; ch < n_ch; ++ch) {
-      const u64 w = (u64)((double)sm.kept[ch] * sm.f[ch] + 0.5);
-      if (w == 0) continue;
-      pick = ch;
-      if (t < w) {
-        rest = (u64)((double)t / sm.f[ch]);  // in the chunk's scale
-        break;
+    } else {
+      const int counted = s.fk ? kBins : 0;
+      for (int i = tid; i < n_ch * kBins; i += kDraw) {
+        const int ch = i / kBins, b = i - ch * kBins, r = b + sm.off[ch];
+        const u64 m = bins[ch].mass[b];
+        if (r >= kBins) continue;
+        if (m > 0) atomicAdd(&sm.mass[r], m);
+        if (b < counted) atomicAdd(&sm.cnt[r], bins[ch].first[b + 1] - bins[ch].first[b]);
       }
-      t -= w;
+      __syncthreads();
+      if (tid > 0 && tid < kBins)
+        sm.mass[tid] = (u64)((double)sm.mass[tid] * sm.scale[tid] + 0.5);
     }
-    if (rest >= sm.kept[pick]) rest = sm.kept[pick] - 1;
-    sm.i = pick;
-    sm.a = rest;
+    __syncthreads();
+    if (tid < kBins) {
+      m_here = sm.mass[tid];
+      n_here = sm.cnt[tid];
+    }
+    m_before = block_scan(m_here, sm.tmp, &total_m);
+    if (s.fk) n_before = block_scan(n_here, sm.tmp, &total_n);
+  }
+  // ---- the borders: top-k's by count, then top-p's by weight --------------------
+  for (int stage = s.fk ? 0 : 1; stage < (s.fp ? 2 : 1); ++stage) {
+    const bool by_count = stage == 0;
+    u64 need, left = total_m;  // left: the weight that top-k leaves
+    if (!by_count && s.fk) {
+      u64 mine = 0;
+      each(fast ? 0 : jc, fast ? kBins : jc, [&](float x, int col) {
+        if (above_cut(x, col)) mine += row_weight(x);
+      });
+      if (!fast && tid == jc) mine += m_before;  // and the bins above
+      block_scan(mine, sm.tmp, &left);
+    }
+    // (fewer tokens than k: all of them)
+    if (by_count) need = min((u64)s.k, fast ? (u64)sm.base[64] : total_n);
+    else need = max(1ull, min(part_of(s.p, left), left));
+    if (fast) {
+      border(0, kBins, need, by_count);
+      continue;
+    }
+    // the bin at which the running sum over the bins reaches need
+    const u64 before = by_count ? n_before : m_before, here = by_count ? n_here : m_here;
+    if (!by_count) need = min(need, total_m);
+    __syncthreads();
+    if (here > 0 && before < need && need <= before + here) {
+      sm.i = tid;
+      sm.a = need - before;
+    }
+    __syncthreads();
+    const int j = sm.i;
+    need = sm.a;
+    if (j > jc) break;  // (by rounding) past top-k's border: that one holds
+    collect(j, j);
+    border(j, j, need, by_count);
+    jc = j;
+  }
+  if (!fast && s.lmin > -INFINITY) {
+    const double r = floor((double)xr * q4) - floor(4.0 * lmin);
+    jc = min(jc, r < (double)kBins ? (int)r : kBins);
+  }
+  // ---- each chunk's kept weight: whole bins, and the border's bin --------------
+  if (!fast && jc < kBins) collect(jc, jc);
+  __syncthreads();
+  if (!fast && !s.few) {
+    const int l16 = tid & 15;
+    for (int ch = tid >> 4; ch < n_ch; ch += kDraw / 16) {
+      const int off = sm.off[ch];
+      u64 v = 0;
+#pragma unroll 4
+      for (int r = l16; r < jc - off; r += 16)
+        v += r + off == 0 ? bins[ch].mass[r]
+                          : (u64)((double)bins[ch].mass[r] * sm.scale[r + off] + 0.5);
+      if (v > 0) atomicAdd(&sm.kept[ch], v);
+    }
+  }
+  if (fast || s.few || jc < kBins)
+    each(fast || s.few ? 0 : jc, fast ? kBins : min(jc, kBins - 1), [&](float x, int col) {
+      if (keeps(x, col)) atomicAdd(&sm.kept[(col + mis) / kChunk], row_weight(x));
+    });
+  __syncthreads();
+
+  // ---- the chunk that u falls into, and where in it ---------------------------
+  if (wave == 0) {
+    const u64 w = lane < n_ch ? sm.kept[lane] : 0, inc = wave_scan(w);
+    const u64 t = target_of(u, lane_value(inc, 63));
+    if (inc - w <= t && t < inc) {
+      sm.i = lane;
+      sm.a = t - (inc - w);
+    }
+    if (lane == 0) sm.kmin = kChunk - 1;
   }
   __syncthreads();
-  // ---- the token in it ---------------------------------------------------------
   const int ch = sm.i;
-  const u64 target = sm.a;
-  float x[kTok];
-  const int col = load8(row, cols, mis, ch, tid, x);
-  u64 w[kTok], mine = 0, all;
-#pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    const bool in = x[j] > -INFINITY && (!s.filters || (bin_of(x[j]) < kBins && keeps(x[j], col + j)));
-    w[j] = in ? chunk_weight(ch, x[j]) : 0;
-    mine += w[j];
-  }
-  u64 before = block_scan(mine, sm.tmp, &all);
-  if (before <= target && target < before + mine) {
-    int at = 0;
-#pragma unroll
-    for (int j = kTok - 1; j >= 0; --j) {  // the first whose running weight exceeds target
-      u64 run = before;
-#pragma unroll
-      for (int t = 0; t <= j; ++t) run += w[t];
-      if (run > target) at = col + j;
+  u64 t = sm.a;
+  // f(column in the chunk, weight) for the chunk's kept tokens
+  auto kept_in = [&](auto&& f) __attribute__((always_inline)) {
+    auto one = [&](float x, int col) {
+      if (!keeps(x, col)) return;
+      int b;
+      const u64 w = weight_of(x, &b);
+      if (b < kBins) f(col + mis - ch * kChunk, w);
+    };
+    if (fast) {
+      const uint32_t end = sm.base[ch + 1];
+      for (uint32_t i = sm.base[ch] + tid; i < end; i += kDraw) {
+        const u64 e = sm.list[i];
+        one(of_key((uint32_t)(e >> 32)), (int)(uint32_t)e);
+      }
+    } else if (jc - sm.off[ch] <= sm.last[ch]) {  // the chunk wrote them out
+      const uint32_t end = bins[ch].first[jc - sm.off[ch] + 1];
+      for (uint32_t i = tid; i < end; i += kDraw) {
+        const u64 e = bins[ch].list[i];
+        one(of_key((uint32_t)(e >> 32)), (int)(uint32_t)e);
+      }
+    } else {
+      for (int part = 2 * ch; part < 2 * ch + 2; ++part) {
+        refill(row, cols, mis, xr, q4, 0, min(jc, kBins - 1), part, sm);
+        for (uint32_t i = tid; i < sm.base[64]; i += kDraw) {
+          const u64 e = sm.list[i];
+          one(of_key((uint32_t)(e >> 32)), (int)(uint32_t)e);
+        }
+      }
     }
-    out[row_i] = at;
+  };
+  // ---- 64 columns of it, and the token in them ---------------------------------
+  kept_in([&](int at, u64 w) {
+    if (w > 0) atomicAdd(&sm.cell[at / kCell], w);
+    else atomicMin(&sm.kmin, (uint32_t)at);
+  });
+  __syncthreads();
+  if (wave == 0) {
+    const u64 w0 = sm.cell[2 * lane], w1 = sm.cell[2 * lane + 1];
+    const u64 inc = wave_scan(w0 + w1), before = inc - w0 - w1;
+    // (the kept weight's whole bins were rounded as such: t may lie past the sum)
+    const u64 all = lane_value(inc, 63);
+    if (all == 0) {  // and even where no token's own weight is above zero
+      if (lane == 0) {
+        sm.j = -1;
+        *out = (long long)ch * kChunk + (int)sm.kmin - mis;
+      }
+    } else if (t = min(t, all - 1); before <= t && t < inc) {
+      const bool second = t >= before + w0;
+      sm.j = 2 * lane + second;
+      sm.b = t - before - (second ? w0 : 0);
+    }
+  }
+  if (tid < kCell) sm.sub_mass[tid] = 0;
+  __syncthreads();
+  const int cell = sm.j;
+  if (cell < 0) return;
+  kept_in([&](int at, u64 w) {
+    if (at / kCell == cell) sm.sub_mass[at % kCell] = w;
+  });
+  __syncthreads();
+  if (wave == 0) {
+    const u64 w = sm.sub_mass[lane], inc = wave_scan(w);
+    const u64 left = sm.b;
+    if (inc - w <= left && left < inc) *out = (long long)ch * kChunk + cell * kCell + lane - mis;
   }
 }
 
@@ -619,13 +946,13 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
 
 #define TEENY_SAMPLE_INST(TN, T)                                                                  \
   extern "C" __global__ __launch_bounds__(1024) void teeny_sample_scan_##TN(                     \
-      const T* logits, long ld, int cols, Args a, Chunk* rec, uint32_t* cnt, u64* mass) {         \
-    sample_scan<T>(logits, ld, cols, a, rec, cnt, mass);                                          \
+      const T* logits, long ld, int cols, Args a, Chunk* rec, Bins* bins) {                       \
+    sample_scan<T>(logits, ld, cols, a, rec, bins);                                               \
   }                                                                                               \
-  extern "C" __global__ __launch_bounds__(1024) void teeny_sample_draw_##TN(                     \
+  extern "C" __global__ __launch_bounds__(256) void teeny_sample_draw_##TN(                      \
       const T* logits, long ld, int cols, Args a, const float* u, const Chunk* rec,               \
-      const uint32_t* cnt, const u64* mass, int n_ch, long long* out, int* advance) {             \
-    sample_draw<T>(logits, ld, cols, a, u, rec, cnt, mass, n_ch, out, advance);                   \
+      const Bins* bins, int n_ch, long long* out, int* advance) {                                 \
+    sample_draw<T>(logits, ld, cols, a, u, rec, bins, n_ch, out, advance);                        \
   }
 TEENY_SAMPLE_INST(f32, float)
 TEENY_SAMPLE_INST(bf16, bf16)

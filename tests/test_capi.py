@@ -412,7 +412,7 @@ def test_sample_rows_validation(L):
     for kw in (dict(x=None), dict(u=None), dict(out=None)):
         assert f(**kw) == NULLP
     assert f(dtype=7) == UNSUP
-    for kw in (dict(rows=0), dict(rows=65536), dict(cols=0), dict(cols=(1 << 19) + 1), dict(ld=99),
+    for kw in (dict(rows=0), dict(rows=65536), dict(cols=0), dict(cols=524281), dict(ld=99),
                dict(ld=-100)):
         assert f(**kw) == SHAPE
     for kw in (dict(t=-1.0), dict(t=nan), dict(k=-1), dict(p=0.0), dict(p=1.01), dict(p=nan), dict(m=-0.1),
@@ -420,7 +420,7 @@ def test_sample_rows_validation(L):
         assert f(**kw) == VALUE
     need = L.teeny_sample_rows_workspace_bytes(4, 100)
     assert need > 0 and f(wsb=need - 1) == WS and f(ws=None) == WS
-    for rows, cols in ((0, 5), (65536, 5), (5, 0), (5, (1 << 19) + 1)):
+    for rows, cols in ((0, 5), (65536, 5), (5, 0), (5, 524281)):
         assert L.teeny_sample_rows_workspace_bytes(rows, cols) == 0
 
 
