@@ -43,6 +43,8 @@
 //          thousands of tokens) is read from the row again.
 #include "common.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef unsigned long long u64;
@@ -226,6 +228,15 @@ DEVI uint32_t lane_value(uint32_t v, int lane) { return __builtin_amdgcn_readlan
 DEVI u64 lane_value(u64 v, int lane) {
   return (u64)lane_value((uint32_t)(v >> 32), lane) << 32 | lane_value((uint32_t)v, lane);
 }
+DEVI uint32_t wave_max_u32(uint32_t v) {
+  v = max(v, dpp<0x111, 0xf>(v));
+  v = max(v, dpp<0x112, 0xf>(v));
+  v = max(v, dpp<0x114, 0xf>(v));
+  v = max(v, dpp<0x118, 0xf>(v));
+  v = max(v, dpp<0x142, 0xa>(v));
+  v = max(v, dpp<0x143, 0xc>(v));
+  return lane_value(v, 63);
+}
 template <typename V> DEVI V wave_total(V v) { return lane_value(wave_scan(v), 63); }
 
 // ---------------------------------------------------------------------------
@@ -350,10 +361,24 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
 constexpr int kDraw = 256, kDrawWaves = kDraw / 64;
 constexpr int kSub = 1024;      // sub-bins of the radix select
 constexpr int kList = 4096;     // tokens collected in LDS
+constexpr int kMost = kList - kSmallK;  // ... for a small top-k, what it leaves behind them
 constexpr int kCell = 64, kCells = kChunk / kCell;  // columns of a chunk's cells
+
+// A pass over (a part of) the row, by the workgroup, for its tokens between two
+// keys: what bins with too many tokens for the list are worked on with.
+enum PassMode { kCollect, kSubs, kKeep, kBinsOf, kCellsOf };
+struct Pass {
+  int step, sh, by_count;        // kSubs: as the border's step
+  uint32_t k0, k1;               // the keys
+  uint32_t top;                  // the greatest key's part that is compared
+  int col0, table;
+  uint32_t cut_key;              // kSubs, kKeep, kCellsOf: tokens above this cut
+  int cut_col, min_p;            // ... and (but kSubs) that min-p keeps
+};
 
 struct DrawSmem {
   u64 list[kList];              // key << 32 | column of the collected tokens
+  u64 few_w[kSmallK];           // weights of what a small top-k leaves
   u64 sub_mass[kSub];           // radix select: weight and count by sub-bin
   uint32_t sub_cnt[kSub];
   u64 mass[kBins];              // the row's bins, weights in the row's scale
@@ -363,12 +388,13 @@ struct DrawSmem {
   int last[kMaxChunks];
   uint32_t from[kMaxChunks], base[kMaxChunks + 1];  // collecting: where in a chunk's list, and ours
   u64 kept[kMaxChunks];         // kept weight of a chunk
-  uint32_t tie[kMaxChunks];
   u64 cell[kCells];             // ... of a chunk's 64 columns
   u64 tmp[kDrawWaves];
-  uint32_t kmin, kmax;
+  uint32_t ends[2];             // keys of the first and last logit of some bins
+  uint32_t kmin, kmax, n_few;
   u64 a, b;                     // a value that one thread hands to all
   float xr;
+  double c, lmin;               // log2(e) / T; min-p in terms of L = x c, -inf without
   int i, j;
 };
 
@@ -389,6 +415,63 @@ DEVI u64 block_scan(u64 v, u64* tmp, u64* total) {
   *total = all;
   return base + inc - v;
 }
+
+// One round of a radix select by N threads (a wavefront, or the workgroup): clear
+// the sub-bins, add the tokens to sm.sub_cnt and sm.sub_mass at sub_at<N>(sub-bin),
+// and pick the sub-bin at which the running sum of counts, or weights, reaches
+// *need, which becomes what is needed in it (0: no sum at all); *n: its count.
+// sub_at: a thread's kSub / N consecutive sub-bins, N apart (no bank conflicts).
+template <int N> DEVI uint32_t sub_at(uint32_t sub) { return sub % (kSub / N) * N + sub / (kSub / N); }
+template <int N>
+struct Select {
+  static constexpr int PER = kSub / N;
+  DEVI static void sync() {
+    if (N > 64) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+  DEVI static void clear(DrawSmem& sm) {
+    const int r = threadIdx.x % N;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      sm.sub_mass[i * N + r] = 0;
+      sm.sub_cnt[i * N + r] = 0;
+    }
+    sync();
+  }
+  DEVI static uint32_t pick(DrawSmem& sm, bool by_count, u64* need, u64* n) {
+    const int r = threadIdx.x % N;
+    sync();
+    u64 sum = 0, all, before;
+    for (int i = 0; i < PER; ++i)
+      sum += by_count ? sm.sub_cnt[i * N + r] : sm.sub_mass[i * N + r];
+    if constexpr (N > 64) {
+      before = block_scan(sum, sm.tmp, &all);
+    } else {
+      const u64 inc = wave_scan(sum);
+      before = inc - sum;
+      all = lane_value(inc, 63);
+    }
+    const u64 want = min(*need, all);  // (a merged bin's sum may have been rounded up)
+    if (before < want && want <= before + sum) {  // one thread: find it among its own
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t cnt = sm.sub_cnt[i * N + r];
+        const u64 v = by_count ? cnt : sm.sub_mass[i * N + r];
+        if (before < want && want <= before + v) {
+          sm.i = r * PER + i;
+          sm.a = want - before;
+          sm.b = cnt;
+        }
+        before += v;
+      }
+    }
+    sync();
+    const uint32_t sub = sm.i;
+    *need = want > 0 ? sm.a : 0;
+    *n = sm.b;
+    sync();
+    return sub;
+  }
+};
 
 // floor(x total) for x in [0, 1), in whole numbers: fp64 would round totals past
 // 2^53, and a border of equal weights would move.
@@ -430,7 +513,8 @@ DEVI void draw_plain(const T* row, int cols, int mis, const Settings& s, float u
   const int ch = __builtin_ctzll(__ballot(inc - w <= t && t < inc));
   t -= lane_value(inc - w, ch);
   const double fc = __builtin_bit_cast(double, lane_value(__builtin_bit_cast(u64, f), ch));
-  t = min((u64)((double)t / fc), lane_value(r.mass, ch) - 1);  // in the chunk's scale
+  if (fc != 1.0) t = (u64)((double)t / fc);  // in the chunk's scale
+  t = min(t, lane_value(r.mass, ch) - 1);
   const double lref = __builtin_bit_cast(double, lane_value(__builtin_bit_cast(u64, r.lref), ch));
   const float xmax = __builtin_bit_cast(float, lane_value(__builtin_bit_cast(uint32_t, r.xmax), ch));
   const u64 part = lane < kWaves ? bins[ch].mass[lane] : 0, pinc = wave_scan(part);
@@ -456,25 +540,111 @@ DEVI void draw_plain(const T* row, int cols, int mis, const Settings& s, float u
   }
 }
 
-// The tokens of bins lo .. hi of a half chunk, into the list (by the workgroup; a
-// call of its own, because few rows need it and each place that may is code).
-template <typename T>
-__device__ __attribute__((noinline)) void refill(const T* row, int cols, int mis, float xr,
-                                                 double q4, int lo, int hi, int part,
-                                                 DrawSmem& sm) {
-  static_assert(kChunk / 2 <= kList, "a half chunk fits");
+// A token's bin below the row's maximum and its weight in the row's scale (0
+// past the bins).
+DEVI u64 row_weight(const DrawSmem& sm, float x, int* b) {
+  u64 w;
+  *b = bin_of(x, sm.xr, 4.0 * sm.c, &w);
+  return *b == 0 ? w : *b < kBins ? (u64)((double)w * sm.scale[*b] + 0.5) : 0;
+}
+DEVI bool above(uint32_t key, int col, uint32_t cut_key, int cut_col) {
+  return key > cut_key || (key == cut_key && col <= cut_col);
+}
+DEVI bool min_p_keeps(const DrawSmem& sm, float x) {
+  return x == sm.xr || (double)x * sm.c >= sm.lmin || sm.lmin == -INFINITY;
+}
+
+// The least and one past the greatest key of the logits of bins lo .. hi, into
+// sm.ends: a bin falls with the logit, so each end is found by a search over the
+// keys, 64 at a time (wavefronts 0 and 1).
+DEVI void find_ends(int lo, int hi, DrawSmem& sm) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
-  if (threadIdx.x == 0) sm.base[64] = 0;
-  __syncthreads();
-  for (int it = 0; it < kChunk / 2 / (kDraw * kTok); ++it) {
-    float x[kTok];
-    const int col = load8(row, cols, mis, part >> 1,
-                          (part & 1) * (kThreads / 2) + it * kDraw + threadIdx.x, x);
-    for (int j = 0; j < kTok; ++j) {
+  if (wave < 2) {
+    // wave 0: the least key of a bin up to hi; wave 1: the least of a bin below lo
+    const int bound = wave == 0 ? hi : lo - 1;
+    uint32_t first = key_of(-INFINITY) + 1, end = key_of(sm.xr) + 1;  // it lies in [first, end]
+    while (first < end) {
+      const uint32_t step = (end - first) / 64 + 1;
+      const uint32_t k = first + (uint32_t)min((u64)step * lane, (u64)(end - first - 1));
       u64 w;
-      const int b = x[j] > -INFINITY ? bin_of(x[j], xr, q4, &w) : kBins + 1;
-      if (b >= lo && b <= hi)
-        sm.list[atomicAdd(&sm.base[64], 1u)] = (u64)key_of(x[j]) << 32 | (uint32_t)(col + j);
+      const u64 yes = __ballot(bin_of(of_key(k), sm.xr, 4.0 * sm.c, &w) <= bound);
+      // lanes from the first yes on; the answer is that lane's key or before it
+      const int n = yes ? __builtin_ctzll(yes) : 64;
+      if (n < 64) end = lane_value(k, n);
+      if (n == 0) break;
+      first = lane_value(k, n - 1) + 1;
+    }
+    if (lane == 0) sm.ends[wave] = end;
+  }
+  __syncthreads();
+}
+
+// The pass over columns of parts [part, end) (half chunks).  kCollect: into the
+// list, sm.base[64] counting them, past what fits too.  kKeep with p.table: the
+// weight of key k is sm.sub_mass[p.top - k].  Calls of their own, because few rows
+// need them and each place that may is code.
+template <typename T, int MODE>
+__device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, int part, int end,
+                                               Pass p, DrawSmem& sm) {
+  const int lane = threadIdx.x & 63;
+  __syncthreads();
+  if (MODE == kCollect) {
+    if (threadIdx.x == 0) sm.base[64] = 0;
+    __syncthreads();
+  }
+  constexpr int U = 4;  // loads in flight
+  constexpr int KS = sizeof(T) == 2 ? 16 : 0;
+  const float x0 = of_key(p.k0), x1 = of_key(p.k1);
+  u64 kept = 0;
+  auto token = [&](float y, int c) __attribute__((always_inline)) {
+    if (!(y >= x0 && y <= x1)) return;
+    const uint32_t key = key_of(y);
+    int b;
+    if (MODE == kCollect) {
+      const uint32_t at = atomicAdd(&sm.base[64], 1u);
+      if (at < (uint32_t)kList) sm.list[at] = (u64)key << 32 | (uint32_t)c;
+    } else if (MODE == kSubs) {
+      if (!above(key, c, p.cut_key, p.cut_col) || (p.step == 2 && (c ^ p.col0) >> 9)) return;
+      const uint32_t sub = sub_at<kDraw>(p.step == 0   ? (p.top - (key >> KS)) >> p.sh
+                                         : p.step == 1 ? c >> 9
+                                                       : c & 511);
+      atomicAdd(&sm.sub_cnt[sub], 1u);
+      if (!p.by_count) atomicAdd(&sm.sub_mass[sub], row_weight(sm, y, &b));
+    } else if (MODE == kBinsOf) {
+      const u64 w = row_weight(sm, y, &b);
+      atomicAdd(&sm.cnt[b], 1u);
+      atomicAdd(&sm.mass[b], w);
+    } else {
+      if (!above(key, c, p.cut_key, p.cut_col) || (p.min_p && !min_p_keeps(sm, y))) return;
+      if (MODE == kKeep) {
+        kept += p.table ? sm.sub_mass[p.top - (key >> KS)] : row_weight(sm, y, &b);
+      } else {  // kCellsOf
+        const u64 w = row_weight(sm, y, &b);
+        if (w > 0) atomicAdd(&sm.cell[(c + mis) % kChunk / kCell], w);
+        else atomicMin(&sm.kmin, (uint32_t)((c + mis) % kChunk));
+      }
+    }
+  };
+  const int slots = end * (kThreads / 2);
+  for (int s0 = part * (kThreads / 2) + threadIdx.x; s0 < slots; s0 += U * kDraw) {
+    float x[U][kTok];
+    int col[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      // (past the end, and past the row: no column)
+      const int slot = s0 + i * kDraw < slots ? s0 + i * kDraw : kMaxChunks * kThreads + 1;
+      col[i] = load8(row, cols, mis, 0, slot, x[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) token(x[i][j], col[i] + j);
+      if (MODE == kKeep) {  // (a wavefront's 512 columns lie in one chunk)
+        kept = wave_total(kept);
+        if (lane == 0 && kept > 0) atomicAdd(&sm.kept[(s0 + i * kDraw) / kThreads], kept);
+        kept = 0;
+      }
     }
   }
   __syncthreads();
@@ -512,6 +682,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     sm.off[lane] = off;
     sm.last[lane] = r.last;
     sm.from[lane] = 0;
+    sm.kept[lane] = 0;
     // what a small top-k collects: all that the chunks wrote out
     const uint32_t n = off < kBins ? r.n_out : 0, inc = wave_scan(n);
     sm.base[lane] = inc - n;
@@ -519,7 +690,10 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     const bool all = __all(off >= kBins || r.complete);
     if (lane == 0) {
       sm.xr = m;
+      sm.c = c;
+      sm.lmin = s.lmin > -INFINITY ? (double)m * c + s.lmin : -INFINITY;
       sm.i = all;
+      sm.kmin = sm.kmax = sm.n_few = 0;
     }
   }
   for (int i = tid; i < kBins; i += kDraw) {
@@ -527,7 +701,6 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     sm.mass[i] = 0;
     sm.scale[i] = exp2_neg(0.25 * i);
   }
-  if (tid < kMaxChunks) sm.kept[tid] = 0;
   if (tid < kCells) sm.cell[tid] = 0;
   __syncthreads();
   const float xr = sm.xr;
@@ -535,34 +708,15 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     if (tid == 0) *out = -1;
     return;
   }
-  const double lmin = (double)xr * c + s.lmin;  // min-p in terms of L
   // a small top-k whose chunks wrote out all that it needs, and that fits
-  const bool fast = s.few && sm.i && sm.base[64] <= (uint32_t)kList;
-
-  auto weight_of = [&](float x, int* b) __attribute__((always_inline)) {  // in the row's scale
-    u64 w;
-    *b = bin_of(x, xr, q4, &w);
-    return *b == 0 ? w : *b < kBins ? (u64)((double)w * sm.scale[*b] + 0.5) : 0;
-  };
-  auto row_weight = [&](float x) __attribute__((always_inline)) {
-    int b;
-    return weight_of(x, &b);
-  };
-  auto bin_at = [&](float x) __attribute__((always_inline)) {
-    u64 w;
-    return bin_of(x, xr, q4, &w);
-  };
+  const bool fast = s.few && sm.i && sm.base[64] <= (uint32_t)kMost;
 
   // the border that top-k and top-p leave: tokens with a higher key, or the same
   // key and a column up to cut_col; jc: its bin (kBins: no border)
   uint32_t cut_key = 0;
   int cut_col = 0x7fffffff, jc = kBins;
-  auto above_cut = [&](float x, int col) __attribute__((always_inline)) {
-    const uint32_t key = key_of(x);
-    return key > cut_key || (key == cut_key && col <= cut_col);
-  };
-  auto keeps = [&](float x, int col) __attribute__((always_inline)) {
-    return above_cut(x, col) && (x == xr || (double)x * c >= lmin || s.lmin == -INFINITY);
+  auto above_cut = [&](uint32_t key, int col) __attribute__((always_inline)) {
+    return above(key, col, cut_key, cut_col);
   };
 
   // Copies the chunks' list entries [from, from + base[ch + 1] - base[ch]) into
@@ -584,246 +738,310 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     __syncthreads();
   };
 
-  int list_lo = 1, list_hi = 0;  // the bins whose tokens the LDS list holds
-  // f(x, column) for every token of bins lo .. hi: from the list, or passing over
-  // the row, half a chunk at a time through the list
-  auto each = [&](int lo, int hi, auto&& f) __attribute__((always_inline)) {
-    const bool listed = lo >= list_lo && hi <= list_hi;
-    const bool all = !listed || (lo == list_lo && hi == list_hi);
-    for (int part = 0; part < (listed ? 1 : 2 * n_ch); ++part) {
-      if (!listed) {
-        list_lo = 1;
-        list_hi = 0;
-        const int off = sm.off[part >> 1];
-        if (off > hi || off >= kBins) continue;
-        refill(row, cols, mis, xr, q4, lo, hi, part, sm);
+  // The border among the tokens between keys k0 and k1 that are above the present
+  // cut: the one at which their running count (by_count) or weight, in the order,
+  // reaches need.  Sets the cut.  A round finds a sub-bin: by key, until one is
+  // left (step 0), then among its equals by column / 512 (1) and column (2).
+  // N threads; subs(k0, k1, sh, step, col0, by_count): adds the tokens' sub-bins;
+  // narrowed(k0, k1, n): called when n tokens are left between two new keys.
+  constexpr int KS = sizeof(T) == 2 ? 16 : 0;  // low bits that every key shares
+  // (bf16: the low half of a key is all zeros, of a negative logit's all ones)
+  auto key_back = [](uint32_t k) __attribute__((always_inline)) {
+    return KS ? k << 16 | (k & 0x8000u ? 0u : 0xffffu) : k;
+  };
+  auto border = [&](auto select, auto weighs, uint32_t k0, uint32_t k1, u64 need, bool by_count, auto&& subs,
+                    auto&& narrowed) __attribute__((always_inline)) {
+    constexpr bool WEIGH = decltype(weighs)::value;
+    k0 >>= KS;
+    k1 >>= KS;
+    int col0 = 0;
+    bool all_equals = true;
+    for (int step = 0; step < 3;) {
+      const uint32_t span = k1 - k0;
+      const int sh = span < (uint32_t)kSub ? 0 : 22 - __builtin_clz(span);
+      select.clear(sm);
+      // a key per sub-bin: counted, and weighed once for all its tokens
+      const bool weigh = WEIGH && !by_count && sh == 0;
+      subs(k0, k1, sh, step, col0, by_count || weigh);
+      if (weigh) {
+        __syncthreads();
+        for (uint32_t i = tid; i <= k1 - k0; i += kDraw) {
+          int b;
+          const uint32_t cnt = sm.sub_cnt[sub_at<kDraw>(i)];
+          if (cnt > 0)
+            sm.sub_mass[sub_at<kDraw>(i)] = cnt * row_weight(sm, of_key(key_back(k1 - i)), &b);
+        }
       }
-      const uint32_t n = sm.base[64];
-      for (uint32_t i = tid; i < n; i += kDraw) {
-        const u64 e = sm.list[i];
-        const float x = of_key((uint32_t)(e >> 32));
-        const int b = all ? lo : bin_at(x);
-        if (b >= lo && b <= hi) f(x, (int)(uint32_t)e);
+      u64 n = 0;
+      const uint32_t sub = select.pick(sm, by_count, &need, &n);
+      if (need == 0) break;  // every weight here rounds to zero: all are kept
+      if (step == 0) {
+        const uint32_t top = k1 - (sub << sh);
+        k0 = top - k0 < (1u << sh) ? k0 : top - (1u << sh) + 1;
+        k1 = top;
+        narrowed(KS ? k0 << 16 : k0, KS ? k1 << 16 | 0xffffu : k1, n);
+        if (k0 < k1) continue;
+        if (!by_count) {  // as many of the equal tokens as their weight needs
+          int b;
+          const u64 w = row_weight(sm, of_key(key_back(k0)), &b);
+          need = (need + w - 1) / w;
+          by_count = true;
+        }
+        if (need >= n) break;  // all of them
+        step = 1;
+      } else {
+        if (step == 1) col0 = sub << 9;
+        else col0 |= sub;
+        all_equals = ++step < 3;
       }
     }
+    k0 = key_back(k0);
+    if (!all_equals) {
+      cut_key = k0;
+      cut_col = col0;
+    } else if (k0 > cut_key) {  // (of equals of the cut those up to its column stay)
+      cut_key = k0;
+      cut_col = 0x7fffffff;
+    }
   };
-  // collects the tokens of bins lo .. hi in LDS where the chunks wrote them out
-  // and they fit
-  auto collect = [&](int lo, int hi) __attribute__((always_inline)) {
-    if (lo >= list_lo && hi <= list_hi) return;
+
+  if (fast) {
+    // ---- a small top-k: all that the chunks wrote out, then the k of them --------
+    gather();
+    const uint32_t n_all = sm.base[64];
+    uint32_t lo = 0, hi = 0;  // of ~key and key
+    for (uint32_t i = tid; i < n_all; i += kDraw) {
+      const uint32_t key = (uint32_t)(sm.list[i] >> 32);
+      lo = max(lo, ~key);
+      hi = max(hi, key);
+    }
+    lo = wave_max_u32(lo);
+    hi = wave_max_u32(hi);
+    if (lane == 0) {
+      atomicMax(&sm.kmin, lo);
+      atomicMax(&sm.kmax, hi);
+    }
+    __syncthreads();
+    const uint32_t key0 = ~sm.kmin, key1 = sm.kmax;
+    if (n_all > (uint32_t)s.k)
+      border(
+          Select<kDraw>{}, std::false_type{}, key0, key1, s.k, true,
+          [&](uint32_t k0, uint32_t k1, int sh, int step, int col0, bool)
+              __attribute__((always_inline)) {
+                for (uint32_t i = tid; i < n_all; i += kDraw) {
+                  const u64 e = sm.list[i];
+                  const uint32_t k = (uint32_t)(e >> 32) >> KS;
+                  const int col = (int)(uint32_t)e;
+                  if (k < k0 || k > k1 || (step == 2 && (col ^ col0) >> 9)) continue;
+                  const uint32_t sub = step == 0 ? (k1 - k) >> sh : step == 1 ? col >> 9 : col & 511;
+                  atomicAdd(&sm.sub_cnt[sub_at<kDraw>(sub)], 1u);
+                }
+              },
+          [](uint32_t, uint32_t, u64) {});
+    __syncthreads();
+    for (uint32_t i = tid; i < n_all; i += kDraw) {
+      const u64 e = sm.list[i];
+      if (!above_cut((uint32_t)(e >> 32), (int)(uint32_t)e)) continue;
+      const uint32_t at = atomicAdd(&sm.n_few, 1u);
+      int b;
+      sm.list[kMost + at] = e;
+      sm.few_w[at] = row_weight(sm, of_key((uint32_t)(e >> 32)), &b);
+    }
+    __syncthreads();
+    // the rest by one wavefront, without barriers
+    if (wave > 0) return;
+    constexpr int E = kSmallK / 64;  // tokens a lane
+    const uint32_t n = sm.n_few;
+    uint32_t key[E];
+    int col[E];
+    u64 w[E], mine = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const uint32_t at = lane + 64 * i;
+      const u64 e = at < n ? sm.list[kMost + at] : 0;
+      key[i] = (uint32_t)(e >> 32);
+      col[i] = (int)(uint32_t)e;
+      w[i] = at < n ? sm.few_w[at] : 0;
+      mine += w[i];
+    }
+    if (s.fp) {
+      const u64 total = wave_total(mine);
+      border(
+          Select<64>{}, std::false_type{}, max(key0, cut_key), key1,
+          max(1ull, min(part_of(s.p, total), total)), false,
+          [&](uint32_t k0, uint32_t k1, int sh, int step, int col0, bool by_count)
+              __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                  const uint32_t k = key[i] >> KS;
+                  if (lane + 64 * i >= n || k < k0 || k > k1 || (step == 2 && (col[i] ^ col0) >> 9))
+                    continue;
+                  const uint32_t sub = sub_at<64>(step == 0   ? (k1 - k) >> sh
+                                                  : step == 1 ? col[i] >> 9
+                                                              : col[i] & 511);
+                  atomicAdd(&sm.sub_cnt[sub], 1u);
+                  if (!by_count) atomicAdd(&sm.sub_mass[sub], w[i]);
+                }
+              },
+          [](uint32_t, uint32_t, u64) {});
+    }
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (lane + 64 * i < n && !(above_cut(key[i], col[i]) && min_p_keeps(sm, of_key(key[i]))))
+        w[i] = 0;
+      mine += w[i];
+    }
+    // the token, in index order: by columns of 512, then by column
+    u64 t = target_of(u, wave_total(mine)) + 1, unused;
+    int col0 = 0;
+    for (int step = 1; step < 3; ++step) {
+      Select<64>::clear(sm);
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (w[i] > 0 && (step == 1 || (col[i] ^ col0) >> 9 == 0))
+          atomicAdd(&sm.sub_mass[sub_at<64>(step == 1 ? col[i] >> 9 : col[i] & 511)], w[i]);
+      const int sub = Select<64>::pick(sm, false, &t, &unused);
+      col0 = step == 1 ? sub << 9 : col0 | sub;
+    }
+    if (lane == 0) *out = col0;
+    return;
+  }
+
+  // ---- the row's bins ----------------------------------------------------------
+  u64 m_before, m_here = 0;      // thread b: the weight before bin b, and in it
+  u64 n_before = 0, n_here = 0;  // ... and tokens
+  u64 total_n = 0, total_m;
+  Pass p{};
+  if (s.few) {  // too many for what the chunks wrote out: by passing over the row
+    if (tid < kMaxChunks) sm.last[tid] = -1;
+    find_ends(0, kBins - 1, sm);
+    p.k0 = sm.ends[0];
+    p.k1 = sm.ends[1] - 1;
+    pass<T, kBinsOf>(row, cols, mis, 0, 2 * n_ch, p, sm);
+  } else {
+    const int counted = s.fk ? kBins : 0, all = n_ch * kBins;
+    for (int i0 = tid; i0 < all; i0 += 4 * kDraw) {
+      u64 m[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {  // (past the end: the last one again)
+        const int i = min(i0 + t * kDraw, all - 1), ch = i / kBins;
+        m[t] = bins[ch].mass[i - ch * kBins];
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = i0 + t * kDraw, ch = i / kBins, b = i - ch * kBins;
+        const int r = i < all ? b + sm.off[ch] : kBins;
+        if (r >= kBins) continue;
+        if (m[t] > 0) atomicAdd(&sm.mass[r], m[t]);
+        if (b < counted) atomicAdd(&sm.cnt[r], bins[ch].first[b + 1] - bins[ch].first[b]);
+      }
+    }
+    __syncthreads();
+    if (tid > 0 && tid < kBins)
+      sm.mass[tid] = (u64)((double)sm.mass[tid] * sm.scale[tid] + 0.5);
+  }
+  __syncthreads();
+  if (tid < kBins) {
+    m_here = sm.mass[tid];
+    n_here = sm.cnt[tid];
+  }
+  m_before = block_scan(m_here, sm.tmp, &total_m);
+  if (s.fk) n_before = block_scan(n_here, sm.tmp, &total_n);
+
+  // The list holds the tokens between keys list0 and list1 (none: list0 > list1).
+  uint32_t list0 = 1, list1 = 0;
+  // collects the tokens of bin j in the list, from what the chunks wrote out or
+  // else from the row, if they fit; k0, k1: the bin's keys
+  uint32_t bin0 = 0, bin1 = 0;
+  auto collect = [&](int j) __attribute__((always_inline)) {
+    find_ends(j, j, sm);
+    bin0 = sm.ends[0];
+    bin1 = sm.ends[1] - 1;
+    if (bin0 >= list0 && bin1 <= list1) return;
     __syncthreads();
     if (wave == 0) {
       uint32_t f0 = 0, n = 0;
-      const int off = lane < n_ch ? sm.off[lane] : kBins;
-      const bool in = off <= hi && off < kBins;
-      if (in && hi - off <= sm.last[lane]) {
-        f0 = bins[lane].first[max(lo - off, 0)];
-        n = bins[lane].first[hi - off + 1] - f0;
+      const int b = lane < n_ch && sm.off[lane] < kBins ? j - sm.off[lane] : -1;
+      if (b >= 0 && b <= sm.last[lane]) {
+        f0 = bins[lane].first[b];
+        n = bins[lane].first[b + 1] - f0;
       }
       const uint32_t inc = wave_scan(n);
       sm.from[lane] = f0;
       sm.base[lane] = inc - n;
-      const bool ok = __all(!in || hi - off <= sm.last[lane]);
+      const bool ok = __all(b < 0 || b <= sm.last[lane]);
       if (lane == 63) sm.base[64] = inc;
       if (lane == 0) sm.i = ok && lane_value(inc, 63) <= (uint32_t)kList;
     }
     __syncthreads();
-    if (!sm.i) {
-      list_lo = 1;
-      list_hi = 0;  // from the row
-      return;
+    list0 = 1;
+    list1 = 0;
+    if (sm.i) {
+      gather();
+    } else {
+      p.k0 = bin0;
+      p.k1 = bin1;
+      pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p, sm);
+      if (sm.base[64] > (uint32_t)kList) return;
     }
-    gather();
-    list_lo = lo;
-    list_hi = hi;
+    list0 = bin0;
+    list1 = bin1;
   };
-  // The border among the tokens of bins lo .. hi that are above the present cut:
-  // the one at which their running count (by_count) or weight, in the order,
-  // reaches need.  Sets the cut.
-  auto border = [&](int lo, int hi, u64 need, bool by_count) __attribute__((always_inline)) {
-    constexpr int KS = sizeof(T) == 2 ? 16 : 0;  // low bits that every key shares
-    __syncthreads();
-    if (tid == 0) {
-      sm.kmin = 0xffffffffu;
-      sm.kmax = 0;
+  // f(key, column) for the list's tokens between two keys
+  auto listed = [&](uint32_t k0, uint32_t k1, auto&& f) __attribute__((always_inline)) {
+    const uint32_t n = sm.base[64];
+    for (uint32_t i = tid; i < n; i += kDraw) {
+      const u64 e = sm.list[i];
+      const uint32_t key = (uint32_t)(e >> 32);
+      if (key >= k0 && key <= k1) f(key, (int)(uint32_t)e);
     }
-    __syncthreads();
-    uint32_t k0 = 0xffffffffu, k1 = 0;
-    each(lo, hi, [&](float x, int col) {
-      if (!above_cut(x, col)) return;
-      k0 = min(k0, key_of(x) >> KS);
-      k1 = max(k1, key_of(x) >> KS);
-    });
-    if (k0 <= k1) {
-      atomicMin(&sm.kmin, k0);
-      atomicMax(&sm.kmax, k1);
-    }
-    __syncthreads();
-    k0 = sm.kmin;
-    k1 = sm.kmax;
-    u64 ties = 0;
-    do {
-      const uint32_t span = k1 - k0;
-      const int sh = span < (uint32_t)kSub ? 0 : 22 - __builtin_clz(span);
-      for (int i = tid; i < kSub; i += kDraw) {
-        sm.sub_mass[i] = 0;
-        sm.sub_cnt[i] = 0;
-      }
-      __syncthreads();
-      each(lo, hi, [&](float x, int col) {
-        const uint32_t k = key_of(x) >> KS;
-        if (k >= k0 && k <= k1 && above_cut(x, col)) {
-          atomicAdd(&sm.sub_cnt[(k1 - k) >> sh], 1u);
-          if (!by_count) atomicAdd(&sm.sub_mass[(k1 - k) >> sh], row_weight(x));
-        }
-      });
-      __syncthreads();
-      u64 v[4], sum = 0, all;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sum += v[i] = by_count ? sm.sub_cnt[4 * tid + i] : sm.sub_mass[4 * tid + i];
-      u64 before = block_scan(sum, sm.tmp, &all);
-      if (need > all) need = all;  // the merged bin's sum was rounded up
-      if (need == 0) break;        // every weight here rounds to zero: all are kept
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (v[i] > 0 && before < need && need <= before + v[i]) {
-          sm.i = 4 * tid + i;
-          sm.a = need - before;
-          sm.b = sm.sub_cnt[4 * tid + i];
-        }
-        before += v[i];
-      }
-      __syncthreads();
-      const uint32_t sub = sm.i;
-      need = sm.a;
-      ties = sm.b;
-      __syncthreads();
-      const uint32_t top = k1 - (sub << sh);
-      k0 = top - k0 < (1u << sh) ? k0 : top - (1u << sh) + 1;
-      k1 = top;
-    } while (k0 < k1);
-    // (bf16: the low half of a key is all zeros, of a negative logit's all ones)
-    k0 = KS ? k0 << 16 | (k0 & 0x8000u ? 0u : 0xffffu) : k0;
-    if (need == 0) {
-      if (k0 > cut_key) {
-        cut_key = k0;
-        cut_col = 0x7fffffff;
-      }
-      return;
-    }
-    const float x = of_key(k0);
-    if (!by_count) {  // as many of the equal tokens as their weight needs
-      const u64 w = row_weight(x);
-      need = (need + w - 1) / w;
-    }
-    if (need >= ties) {  // all that were above the cut
-      if (k0 > cut_key) {
-        cut_key = k0;
-        cut_col = 0x7fffffff;
-      }
-      return;
-    }
-    cut_key = k0;
-    // the column of the need-th of the equal tokens (those above a cut among them
-    // are the first): its chunk, then in it
-    if (tid < kMaxChunks) sm.tie[tid] = 0;
-    __syncthreads();
-    each(lo, hi, [&](float y, int col) {
-      if (y == x) atomicAdd(&sm.tie[(col + mis) / kChunk], 1u);
-    });
-    __syncthreads();
-    if (wave == 0) {
-      const u64 n = lane < n_ch ? sm.tie[lane] : 0, before = wave_scan(n) - n;
-      if (before < need && need <= before + n) {
-        sm.i = lane;
-        sm.a = need - before;
-      }
-    }
-    __syncthreads();
-    const int ch = sm.i;
-    u64 left = sm.a;
-    __syncthreads();
-    for (int it = 0; it < kChunk / (kDraw * kTok); ++it) {
-      float y[kTok];
-      const int col = load8(row, cols, mis, ch, it * kDraw + tid, y);
-      u64 here = 0, all;
-#pragma unroll
-      for (int t = 0; t < kTok; ++t) here += y[t] == x;
-      const u64 before = block_scan(here, sm.tmp, &all);
-      if (before < left && left <= before + here) {
-        u64 n = before;
-#pragma unroll
-        for (int t = 0; t < kTok; ++t)
-          if (y[t] == x && ++n == left) sm.j = col + t;
-      }
-      if (left <= all) break;
-      left -= all;
-    }
-    __syncthreads();
-    cut_col = sm.j;
   };
-
-  u64 m_before = 0, m_here = 0;  // thread b: the weight before bin b, and in it
-  u64 n_before = 0, n_here = 0;  // ... and tokens
-  u64 total_n = 0, total_m = 0;
-  if (fast) {
-    gather();
-    list_lo = 0;
-    list_hi = kBins;
-  } else {
-    // ---- the row's bins ------------------------------------------------------
-    if (s.few) {  // too many for what the chunks wrote out: by passing over the row
-      if (tid < kMaxChunks) sm.last[tid] = -1;
-      each(0, kBins - 1, [&](float x, int) {
+  // sm.kept[chunk] += the kept weight of bin jc's tokens (min_p: and that it keeps)
+  auto keep_bin = [&](bool min_p) __attribute__((always_inline)) {
+    __syncthreads();
+    if (bin0 >= list0 && bin1 <= list1) {
+      listed(bin0, bin1, [&](uint32_t key, int col) __attribute__((always_inline)) {
         int b;
-        const u64 w = weight_of(x, &b);
-        atomicAdd(&sm.cnt[b], 1u);
-        atomicAdd(&sm.mass[b], w);
+        const float x = of_key(key);
+        if (above_cut(key, col) && (!min_p || min_p_keeps(sm, x)))
+          atomicAdd(&sm.kept[(col + mis) / kChunk], row_weight(sm, x, &b));
       });
     } else {
-      const int counted = s.fk ? kBins : 0;
-      for (int i = tid; i < n_ch * kBins; i += kDraw) {
-        const int ch = i / kBins, b = i - ch * kBins, r = b + sm.off[ch];
-        const u64 m = bins[ch].mass[b];
-        if (r >= kBins) continue;
-        if (m > 0) atomicAdd(&sm.mass[r], m);
-        if (b < counted) atomicAdd(&sm.cnt[r], bins[ch].first[b + 1] - bins[ch].first[b]);
+      p.k0 = max(bin0, cut_key);
+      p.k1 = bin1;
+      p.cut_key = cut_key;
+      p.cut_col = cut_col;
+      p.min_p = min_p;
+      // few keys: their weights in a table (of them, not of thousands of tokens)
+      p.top = bin1 >> KS;
+      p.table = p.top - (p.k0 >> KS) < (uint32_t)kSub;
+      for (uint32_t i = tid; p.table && i <= p.top - (p.k0 >> KS); i += kDraw) {
+        int b;
+        sm.sub_mass[i] = row_weight(sm, of_key(key_back(p.top - i)), &b);
       }
-      __syncthreads();
-      if (tid > 0 && tid < kBins)
-        sm.mass[tid] = (u64)((double)sm.mass[tid] * sm.scale[tid] + 0.5);
+      pass<T, kKeep>(row, cols, mis, 0, 2 * n_ch, p, sm);
     }
     __syncthreads();
-    if (tid < kBins) {
-      m_here = sm.mass[tid];
-      n_here = sm.cnt[tid];
-    }
-    m_before = block_scan(m_here, sm.tmp, &total_m);
-    if (s.fk) n_before = block_scan(n_here, sm.tmp, &total_n);
-  }
+  };
   // ---- the borders: top-k's by count, then top-p's by weight --------------------
   for (int stage = s.fk ? 0 : 1; stage < (s.fp ? 2 : 1); ++stage) {
-    const bool by_count = stage == 0;
-    u64 need, left = total_m;  // left: the weight that top-k leaves
-    if (!by_count && s.fk) {
-      u64 mine = 0;
-      each(fast ? 0 : jc, fast ? kBins : jc, [&](float x, int col) {
-        if (above_cut(x, col)) mine += row_weight(x);
-      });
-      if (!fast && tid == jc) mine += m_before;  // and the bins above
-      block_scan(mine, sm.tmp, &left);
-    }
-    // (fewer tokens than k: all of them)
-    if (by_count) need = min((u64)s.k, fast ? (u64)sm.base[64] : total_n);
-    else need = max(1ull, min(part_of(s.p, left), left));
-    if (fast) {
-      border(0, kBins, need, by_count);
-      continue;
+    u64 need;
+    if (stage == 0) {
+      need = min((u64)s.k, total_n);  // (fewer tokens than k: all of them)
+    } else {
+      u64 left = total_m;  // the weight that top-k leaves
+      if (s.fk) {
+        keep_bin(false);
+        u64 mine = tid < kMaxChunks ? sm.kept[tid] : 0;
+        if (tid == jc) mine += m_before;  // and the bins above
+        block_scan(mine, sm.tmp, &left);
+        if (tid < kMaxChunks) sm.kept[tid] = 0;
+      }
+      need = max(1ull, min(part_of(s.p, left), min(left, total_m)));
     }
     // the bin at which the running sum over the bins reaches need
-    const u64 before = by_count ? n_before : m_before, here = by_count ? n_here : m_here;
-    if (!by_count) need = min(need, total_m);
+    const u64 before = stage == 0 ? n_before : m_before, here = stage == 0 ? n_here : m_here;
     __syncthreads();
     if (here > 0 && before < need && need <= before + here) {
       sm.i = tid;
@@ -833,20 +1051,60 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     const int j = sm.i;
     need = sm.a;
     if (j > jc) break;  // (by rounding) past top-k's border: that one holds
-    collect(j, j);
-    border(j, j, need, by_count);
+    collect(j);
+    border(
+        Select<kDraw>{}, std::true_type{}, bin0, bin1, need, stage == 0,
+        [&](uint32_t k0, uint32_t k1, int sh, int step, int col0, bool by_count)
+            __attribute__((always_inline)) {
+              const uint32_t a0 = k0 << KS, a1 = KS ? k1 << 16 | 0xffffu : k1;
+              // (a bin's first key may lie above the first of its low half)
+              if (max(a0, bin0) >= list0 && min(a1, bin1) <= list1) {
+                listed(a0, a1, [&](uint32_t key, int col) __attribute__((always_inline)) {
+                  if (!above_cut(key, col) || (step == 2 && (col ^ col0) >> 9)) return;
+                  const uint32_t sub = sub_at<kDraw>(step == 0   ? (k1 - (key >> KS)) >> sh
+                                                     : step == 1 ? col >> 9
+                                                                 : col & 511);
+                  int b;
+                  atomicAdd(&sm.sub_cnt[sub], 1u);
+                  if (!by_count)
+                    atomicAdd(&sm.sub_mass[sub], row_weight(sm, of_key(key), &b));
+                });
+              } else {
+                p.step = step;
+                p.sh = sh;
+                p.by_count = by_count;
+                p.k0 = max(a0, bin0);
+                p.k1 = min(a1, bin1);
+                p.top = k1;
+                p.col0 = col0;
+                p.cut_key = cut_key;
+                p.cut_col = cut_col;
+                pass<T, kSubs>(row, cols, mis, 0, 2 * n_ch, p, sm);
+              }
+            },
+        [&](uint32_t k0, uint32_t k1, u64 n) __attribute__((always_inline)) {
+          k0 = max(k0, bin0);
+          k1 = min(k1, bin1);
+          // (those below a top-k's cut are collected too, and may not fit)
+          if ((k0 >= list0 && k1 <= list1) || n > (u64)kList) return;
+          p.k0 = k0;
+          p.k1 = k1;
+          pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p, sm);
+          const bool fits = sm.base[64] <= (uint32_t)kList;
+          list0 = fits ? k0 : 1;
+          list1 = fits ? k1 : 0;
+        });
     jc = j;
   }
-  if (!fast && s.lmin > -INFINITY) {
-    const double r = floor((double)xr * q4) - floor(4.0 * lmin);
-    jc = min(jc, r < (double)kBins ? (int)r : kBins);
+  if (s.lmin > -INFINITY) {
+    const double r = floor((double)xr * q4) - floor(4.0 * sm.lmin);
+    const int jm = r < (double)kBins ? (int)r : kBins;
+    if (jm < jc) collect(jc = jm);
   }
   // ---- each chunk's kept weight: whole bins, and the border's bin --------------
-  if (!fast && jc < kBins) collect(jc, jc);
-  __syncthreads();
-  if (!fast && !s.few) {
+  {
     const int l16 = tid & 15;
-    for (int ch = tid >> 4; ch < n_ch; ch += kDraw / 16) {
+    for (int ch = tid >> 4; ch < n_ch && !s.few; ch += kDraw / 16) {
       const int off = sm.off[ch];
       u64 v = 0;
 #pragma unroll 4
@@ -856,10 +1114,14 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       if (v > 0) atomicAdd(&sm.kept[ch], v);
     }
   }
-  if (fast || s.few || jc < kBins)
-    each(fast || s.few ? 0 : jc, fast ? kBins : min(jc, kBins - 1), [&](float x, int col) {
-      if (keeps(x, col)) atomicAdd(&sm.kept[(col + mis) / kChunk], row_weight(x));
-    });
+  if (s.few) {  // (its chunks left no weights: every token up to the border)
+    find_ends(0, min(jc, kBins - 1), sm);
+    bin0 = sm.ends[0];
+    bin1 = sm.ends[1] - 1;
+    list0 = 1;
+    list1 = 0;
+  }
+  if (s.few || jc < kBins) keep_bin(true);
   __syncthreads();
 
   // ---- the chunk that u falls into, and where in it ---------------------------
@@ -873,73 +1135,54 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     if (lane == 0) sm.kmin = kChunk - 1;
   }
   __syncthreads();
-  const int ch = sm.i;
+  const int ch = sm.i, off = sm.off[ch];
   u64 t = sm.a;
-  // f(column in the chunk, weight) for the chunk's kept tokens
-  auto kept_in = [&](auto&& f) __attribute__((always_inline)) {
-    auto one = [&](float x, int col) {
-      if (!keeps(x, col)) return;
+  // ---- its kept weight by 64 columns ---------------------------------------------
+  if (jc - off <= sm.last[ch]) {  // the chunk wrote out what can be kept
+    const uint32_t end = bins[ch].first[jc - off + 1];
+    for (uint32_t i = tid; i < end; i += kDraw) {
+      const u64 e = bins[ch].list[i];
+      const uint32_t key = (uint32_t)(e >> 32);
+      const int col = (int)(uint32_t)e, at = col + mis - ch * kChunk;
+      const float x = of_key(key);
       int b;
-      const u64 w = weight_of(x, &b);
-      if (b < kBins) f(col + mis - ch * kChunk, w);
-    };
-    if (fast) {
-      const uint32_t end = sm.base[ch + 1];
-      for (uint32_t i = sm.base[ch] + tid; i < end; i += kDraw) {
-        const u64 e = sm.list[i];
-        one(of_key((uint32_t)(e >> 32)), (int)(uint32_t)e);
-      }
-    } else if (jc - sm.off[ch] <= sm.last[ch]) {  // the chunk wrote them out
-      const uint32_t end = bins[ch].first[jc - sm.off[ch] + 1];
-      for (uint32_t i = tid; i < end; i += kDraw) {
-        const u64 e = bins[ch].list[i];
-        one(of_key((uint32_t)(e >> 32)), (int)(uint32_t)e);
-      }
-    } else {
-      for (int part = 2 * ch; part < 2 * ch + 2; ++part) {
-        refill(row, cols, mis, xr, q4, 0, min(jc, kBins - 1), part, sm);
-        for (uint32_t i = tid; i < sm.base[64]; i += kDraw) {
-          const u64 e = sm.list[i];
-          one(of_key((uint32_t)(e >> 32)), (int)(uint32_t)e);
-        }
-      }
+      const u64 w = row_weight(sm, x, &b);
+      if (b >= kBins || !above_cut(key, col) || !min_p_keeps(sm, x)) continue;
+      if (w > 0) atomicAdd(&sm.cell[at / kCell], w);
+      else atomicMin(&sm.kmin, (uint32_t)at);
     }
-  };
-  // ---- 64 columns of it, and the token in them ---------------------------------
-  kept_in([&](int at, u64 w) {
-    if (w > 0) atomicAdd(&sm.cell[at / kCell], w);
-    else atomicMin(&sm.kmin, (uint32_t)at);
-  });
-  __syncthreads();
-  if (wave == 0) {
-    const u64 w0 = sm.cell[2 * lane], w1 = sm.cell[2 * lane + 1];
-    const u64 inc = wave_scan(w0 + w1), before = inc - w0 - w1;
-    // (the kept weight's whole bins were rounded as such: t may lie past the sum)
-    const u64 all = lane_value(inc, 63);
-    if (all == 0) {  // and even where no token's own weight is above zero
-      if (lane == 0) {
-        sm.j = -1;
-        *out = (long long)ch * kChunk + (int)sm.kmin - mis;
-      }
-    } else if (t = min(t, all - 1); before <= t && t < inc) {
-      const bool second = t >= before + w0;
-      sm.j = 2 * lane + second;
-      sm.b = t - before - (second ? w0 : 0);
-    }
+  } else {
+    find_ends(0, min(jc, kBins - 1), sm);
+    p.k0 = sm.ends[0];
+    p.k1 = sm.ends[1] - 1;
+    p.cut_key = cut_key;
+    p.cut_col = cut_col;
+    p.min_p = 1;
+    pass<T, kCellsOf>(row, cols, mis, 2 * ch, 2 * ch + 2, p, sm);
   }
-  if (tid < kCell) sm.sub_mass[tid] = 0;
   __syncthreads();
-  const int cell = sm.j;
-  if (cell < 0) return;
-  kept_in([&](int at, u64 w) {
-    if (at / kCell == cell) sm.sub_mass[at % kCell] = w;
-  });
-  __syncthreads();
-  if (wave == 0) {
-    const u64 w = sm.sub_mass[lane], inc = wave_scan(w);
-    const u64 left = sm.b;
-    if (inc - w <= left && left < inc) *out = (long long)ch * kChunk + cell * kCell + lane - mis;
+  // ---- the columns and the token, by one wavefront -------------------------------
+  if (wave > 0) return;
+  const u64 w0 = sm.cell[2 * lane], w1 = sm.cell[2 * lane + 1];
+  const u64 inc = wave_scan(w0 + w1), all = lane_value(inc, 63);
+  if (all == 0) {  // (a bin's weight was rounded as such, no token's own is above zero)
+    if (lane == 0) *out = (long long)ch * kChunk + (int)sm.kmin - mis;
+    return;
   }
+  t = min(t, all - 1);
+  const u64 b0 = inc - w0 - w1;
+  const int at = __builtin_ctzll(__ballot(b0 <= t && t < inc));
+  const u64 first = lane_value(b0, at), half = lane_value(w0, at);
+  const bool second = t >= first + half;
+  t -= first + (second ? half : 0);
+  const int col = ch * kChunk + (2 * at + second) * kCell + lane - mis;
+  float x = col >= 0 && col < cols ? (float)row[col] : -INFINITY;
+  x = x == x ? x + 0.0f : -INFINITY;
+  int b;
+  u64 w = row_weight(sm, x, &b);
+  if (b >= kBins || !above_cut(key_of(x), col) || !min_p_keeps(sm, x)) w = 0;
+  const u64 run = wave_scan(w);
+  if (run - w <= t && t < run) *out = col;
 }
 
 }  // namespace
