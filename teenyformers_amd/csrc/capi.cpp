@@ -1492,7 +1492,7 @@ int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int
   if (rc) return rc;
   snprintf(name, sizeof name, "teeny_sample_draw_%s", dtype_tag(dtype));
   void* a1[] = {&logits, &ld, &cols, &a, &u, &rec, &bins, &n_ch, &out, &advance};
-  return launch(name, dim3((unsigned)rows), dim3(256), 0, stream, a1);
+  return launch(name, dim3((unsigned)rows), dim3(512), 0, stream, a1);
 }
 
 // Decode-step linear layers (linear_bf16.hip): 512 threads, 128 W rows per

@@ -296,14 +296,18 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
   const int counted = s.fk && !s.few ? kBins : kFirstBins;
   int bin[kTok];
   uint32_t rank[kTok];
+  auto tokens = [&](auto weighs) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j = 0; j < kTok; ++j) {
-    u64 w;
-    bin[j] = bin_of(x[j], mx, q4, &w);
-    if (mx == -INFINITY || ((double)x[j] * s.c < least && x[j] != mx)) bin[j] = kBins;
-    if (!s.few && bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
-    if (bin[j] < counted) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
-  }
+    for (int j = 0; j < kTok; ++j) {
+      u64 w;
+      bin[j] = bin_of(x[j], mx, q4, &w);
+      if (mx == -INFINITY || ((double)x[j] * s.c < least && x[j] != mx)) bin[j] = kBins;
+      if (decltype(weighs)::value && bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
+      if (bin[j] < counted) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
+    }
+  };
+  if (s.few) tokens(std::false_type{});
+  else tokens(std::true_type{});
   __syncthreads();
   uint32_t have = 0;
   if (s.few) {  // too few in the first bins: the others too
@@ -358,7 +362,7 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
 // ---------------------------------------------------------------------------
 // draw: grid (rows)
 // ---------------------------------------------------------------------------
-constexpr int kDraw = 256, kDrawWaves = kDraw / 64;
+constexpr int kDraw = 512, kDrawWaves = kDraw / 64;
 constexpr int kSub = 1024;      // sub-bins of the radix select
 constexpr int kList = 4096;     // tokens collected in LDS
 constexpr int kMost = kList - kSmallK;  // ... for a small top-k, what it leaves behind them
@@ -367,15 +371,6 @@ constexpr int kCell = 64, kCells = kChunk / kCell;  // columns of a chunk's cell
 // A pass over (a part of) the row, by the workgroup, for its tokens between two
 // keys: what bins with too many tokens for the list are worked on with.
 enum PassMode { kCollect, kSubs, kKeep, kBinsOf, kCellsOf };
-struct Pass {
-  int step, sh, by_count;        // kSubs: as the border's step
-  uint32_t k0, k1;               // the keys
-  uint32_t top;                  // the greatest key's part that is compared
-  int col0, table;
-  uint32_t cut_key;              // kSubs, kKeep, kCellsOf: tokens above this cut
-  int cut_col, min_p;            // ... and (but kSubs) that min-p keeps
-};
-
 struct DrawSmem {
   u64 list[kList];              // key << 32 | column of the collected tokens
   u64 few_w[kSmallK];           // weights of what a small top-k leaves
@@ -398,16 +393,20 @@ struct DrawSmem {
   int i, j;
 };
 
+// (of the module, not the kernel: the calls below reach it as LDS, not through
+// generic pointers, whose accesses made a pass over a row 15 times as long)
+static __shared__ DrawSmem sm;
+
 // Exclusive prefix sum over the workgroup; total in *total.
-DEVI u64 block_scan(u64 v, u64* tmp, u64* total) {
+DEVI u64 block_scan(u64 v, u64* total) {
   const int wave = threadIdx.x >> 6;
   const u64 inc = wave_scan(v);
-  if ((threadIdx.x & 63) == 63) tmp[wave] = inc;
+  if ((threadIdx.x & 63) == 63) sm.tmp[wave] = inc;
   __syncthreads();
   u64 base = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kDrawWaves; ++w) {
-    const u64 t = tmp[w];
+    const u64 t = sm.tmp[w];
     base += w < wave ? t : 0;
     all += t;
   }
@@ -416,20 +415,39 @@ DEVI u64 block_scan(u64 v, u64* tmp, u64* total) {
   return base + inc - v;
 }
 
+// Which sub-bin a token falls in.  By key (cs < 0): keys top - sub << sh downwards.
+// By column, whose bits from prev on are those of col0: its bits from cs on.
+struct Digit {
+  uint32_t top;
+  int sh, cs, prev, col0;
+  DEVI bool skips(int col) const { return cs >= 0 && (col ^ col0) >> prev; }
+  DEVI uint32_t sub(uint32_t key, int col, int subs) const {
+    return cs < 0 ? (top - key) >> sh : (uint32_t)(col >> cs) & (subs - 1);
+  }
+};
+constexpr int kColBits = 19;
+struct Pass {
+  uint32_t k0, k1;               // the keys
+  Digit digit;                   // kSubs
+  int by_count, table, min_p;    // kSubs; kKeep: weights from a table, of keys to digit.top
+  uint32_t cut_key;              // kSubs, kKeep, kCellsOf: tokens above this cut
+  int cut_col;                   // ... and, with min_p, that min-p keeps
+};
 // One round of a radix select by N threads (a wavefront, or the workgroup): clear
-// the sub-bins, add the tokens to sm.sub_cnt and sm.sub_mass at sub_at<N>(sub-bin),
+// the sub-bins, add the tokens to sm.sub_cnt and sm.sub_mass at at(sub-bin),
 // and pick the sub-bin at which the running sum of counts, or weights, reaches
 // *need, which becomes what is needed in it (0: no sum at all); *n: its count.
-// sub_at: a thread's kSub / N consecutive sub-bins, N apart (no bank conflicts).
-template <int N> DEVI uint32_t sub_at(uint32_t sub) { return sub % (kSub / N) * N + sub / (kSub / N); }
-template <int N>
+// at: a thread's PER consecutive sub-bins, N apart (no bank conflicts).
+// A round is by a part of the key, or by LOG2 bits of the column: see Digit.
+template <int N, int LOG2>
 struct Select {
-  static constexpr int PER = kSub / N;
+  static constexpr int SUBS = 1 << LOG2, PER = SUBS / N;
+  DEVI static uint32_t at(uint32_t sub) { return sub % PER * N + sub / PER; }
   DEVI static void sync() {
     if (N > 64) __syncthreads();
     else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
-  DEVI static void clear(DrawSmem& sm) {
+  DEVI static void clear() {
     const int r = threadIdx.x % N;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
@@ -438,14 +456,20 @@ struct Select {
     }
     sync();
   }
-  DEVI static uint32_t pick(DrawSmem& sm, bool by_count, u64* need, u64* n) {
+  DEVI static uint32_t pick(bool by_count, u64* need, u64* n) {
     const int r = threadIdx.x % N;
     sync();
-    u64 sum = 0, all, before;
-    for (int i = 0; i < PER; ++i)
-      sum += by_count ? sm.sub_cnt[i * N + r] : sm.sub_mass[i * N + r];
+    u64 v[PER], sum = 0, all, before;
+    uint32_t cnt[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      cnt[i] = sm.sub_cnt[i * N + r];
+      if (!by_count) v[i] = sm.sub_mass[i * N + r];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += by_count ? v[i] = cnt[i] : v[i];
     if constexpr (N > 64) {
-      before = block_scan(sum, sm.tmp, &all);
+      before = block_scan(sum, &all);
     } else {
       const u64 inc = wave_scan(sum);
       before = inc - sum;
@@ -453,16 +477,19 @@ struct Select {
     }
     const u64 want = min(*need, all);  // (a merged bin's sum may have been rounded up)
     if (before < want && want <= before + sum) {  // one thread: find it among its own
-      for (int i = 0; i < PER; ++i) {
-        const uint32_t cnt = sm.sub_cnt[i * N + r];
-        const u64 v = by_count ? cnt : sm.sub_mass[i * N + r];
-        if (before < want && want <= before + v) {
-          sm.i = r * PER + i;
-          sm.a = want - before;
-          sm.b = cnt;
-        }
-        before += v;
+      int at = 0;
+      u64 left = want - before;
+      uint32_t n_at = cnt[0];
+#pragma unroll
+      for (int i = 0; i + 1 < PER; ++i) {  // (once left is within v[at], no more)
+        const bool next = at == i && left > v[i];
+        left -= next ? v[i] : 0;
+        at += next;
+        n_at = next ? cnt[i + 1] : n_at;
       }
+      sm.i = r * PER + at;
+      sm.a = left;
+      sm.b = n_at;
     }
     sync();
     const uint32_t sub = sm.i;
@@ -472,6 +499,9 @@ struct Select {
     return sub;
   }
 };
+
+using BlockSelect = Select<kDraw, 10>;
+using WaveSelect = Select<64, 8>;
 
 // floor(x total) for x in [0, 1), in whole numbers: fp64 would round totals past
 // 2^53, and a border of equal weights would move.
@@ -542,33 +572,50 @@ DEVI void draw_plain(const T* row, int cols, int mis, const Settings& s, float u
 
 // A token's bin below the row's maximum and its weight in the row's scale (0
 // past the bins).
-DEVI u64 row_weight(const DrawSmem& sm, float x, int* b) {
+DEVI u64 row_weight(float x, int* b) {
   u64 w;
   *b = bin_of(x, sm.xr, 4.0 * sm.c, &w);
-  return *b == 0 ? w : *b < kBins ? (u64)((double)w * sm.scale[*b] + 0.5) : 0;
+  const u64 scaled = (u64)((double)w * sm.scale[min(*b, kBins - 1)] + 0.5);
+  return *b == 0 ? w : *b < kBins ? scaled : 0;
 }
 DEVI bool above(uint32_t key, int col, uint32_t cut_key, int cut_col) {
   return key > cut_key || (key == cut_key && col <= cut_col);
 }
-DEVI bool min_p_keeps(const DrawSmem& sm, float x) {
+DEVI bool min_p_keeps(float x) {
   return x == sm.xr || (double)x * sm.c >= sm.lmin || sm.lmin == -INFINITY;
 }
 
 // The least and one past the greatest key of the logits of bins lo .. hi, into
-// sm.ends: a bin falls with the logit, so each end is found by a search over the
-// keys, 64 at a time (wavefronts 0 and 1).
-DEVI void find_ends(int lo, int hi, DrawSmem& sm) {
+// sm.ends: a bin falls with the logit, so each end is the least key of a bin up to
+// a bound (wavefront 0: up to hi; 1: below lo).  It lies next to bound / q4; where
+// it does not (q4 = 0, ends of the range), a search over the keys, 64 at a time.
+DEVI void find_ends(int lo, int hi) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __syncthreads();
   if (wave < 2) {
-    // wave 0: the least key of a bin up to hi; wave 1: the least of a bin below lo
     const int bound = wave == 0 ? hi : lo - 1;
+    const double q4 = 4.0 * sm.c;
     uint32_t first = key_of(-INFINITY) + 1, end = key_of(sm.xr) + 1;  // it lies in [first, end]
+    auto up_to = [&](uint32_t k) __attribute__((always_inline)) {
+      u64 w;
+      return bin_of(of_key(k), sm.xr, q4, &w) <= bound;
+    };
+    if (bound < 0) {
+      first = end;
+    } else {
+      const float guess = (float)((floor((double)sm.xr * q4) - bound) / q4) + 0.0f;
+      const uint32_t k = key_of(guess == guess ? guess : 0.0f) - 32 + lane;
+      const u64 yes = __ballot(k >= first && k < end && up_to(k));
+      const u64 no = __ballot(k >= first && k < end && !up_to(k));
+      if (yes && no) {  // (the noes come first)
+        const int n = __builtin_ctzll(yes);
+        first = end = lane_value(k, n);
+      }
+    }
     while (first < end) {
       const uint32_t step = (end - first) / 64 + 1;
       const uint32_t k = first + (uint32_t)min((u64)step * lane, (u64)(end - first - 1));
-      u64 w;
-      const u64 yes = __ballot(bin_of(of_key(k), sm.xr, 4.0 * sm.c, &w) <= bound);
+      const u64 yes = __ballot(up_to(k));
       // lanes from the first yes on; the answer is that lane's key or before it
       const int n = yes ? __builtin_ctzll(yes) : 64;
       if (n < 64) end = lane_value(k, n);
@@ -586,66 +633,121 @@ DEVI void find_ends(int lo, int hi, DrawSmem& sm) {
 // need them and each place that may is code.
 template <typename T, int MODE>
 __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, int part, int end,
-                                               Pass p, DrawSmem& sm) {
+                                               Pass p) {
   const int lane = threadIdx.x & 63;
   __syncthreads();
   if (MODE == kCollect) {
     if (threadIdx.x == 0) sm.base[64] = 0;
     __syncthreads();
   }
-  constexpr int U = 4;  // loads in flight
+  constexpr int U = 4;                        // vectors of 8 logits in flight
+  constexpr int VW = kTok / Vec16<T>::N;      // loads a vector
   constexpr int KS = sizeof(T) == 2 ? 16 : 0;
   const float x0 = of_key(p.k0), x1 = of_key(p.k1);
-  u64 kept = 0;
-  auto token = [&](float y, int c) __attribute__((always_inline)) {
-    if (!(y >= x0 && y <= x1)) return;
-    const uint32_t key = key_of(y);
-    int b;
-    if (MODE == kCollect) {
-      const uint32_t at = atomicAdd(&sm.base[64], 1u);
-      if (at < (uint32_t)kList) sm.list[at] = (u64)key << 32 | (uint32_t)c;
-    } else if (MODE == kSubs) {
-      if (!above(key, c, p.cut_key, p.cut_col) || (p.step == 2 && (c ^ p.col0) >> 9)) return;
-      const uint32_t sub = sub_at<kDraw>(p.step == 0   ? (p.top - (key >> KS)) >> p.sh
-                                         : p.step == 1 ? c >> 9
-                                                       : c & 511);
-      atomicAdd(&sm.sub_cnt[sub], 1u);
-      if (!p.by_count) atomicAdd(&sm.sub_mass[sub], row_weight(sm, y, &b));
-    } else if (MODE == kBinsOf) {
-      const u64 w = row_weight(sm, y, &b);
-      atomicAdd(&sm.cnt[b], 1u);
-      atomicAdd(&sm.mass[b], w);
-    } else {
-      if (!above(key, c, p.cut_key, p.cut_col) || (p.min_p && !min_p_keeps(sm, y))) return;
-      if (MODE == kKeep) {
-        kept += p.table ? sm.sub_mass[p.top - (key >> KS)] : row_weight(sm, y, &b);
-      } else {  // kCellsOf
-        const u64 w = row_weight(sm, y, &b);
-        if (w > 0) atomicAdd(&sm.cell[(c + mis) % kChunk / kCell], w);
-        else atomicMin(&sm.kmin, (uint32_t)((c + mis) % kChunk));
+  // a thread's vector of 8 logits in columns c ..: of the weights, all are formed
+  // before the first is used
+  auto vec8 = [&](const float* y, int c) __attribute__((always_inline)) {
+    bool in[kTok];
+    uint32_t key[kTok];
+    int b[kTok];
+    u64 w[kTok];
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      in[j] = y[j] >= x0 && y[j] <= x1;
+      key[j] = key_of(y[j]);
+      if (MODE != kBinsOf && MODE != kCollect)
+        in[j] = in[j] && above(key[j], c + j, p.cut_key, p.cut_col);
+      if (MODE == kSubs) in[j] = in[j] && !p.digit.skips(c + j);
+      if (MODE == kKeep || MODE == kCellsOf) in[j] = in[j] && (!p.min_p || min_p_keeps(y[j]));
+    }
+    if (MODE == kCollect) {  // one place in the list for all of a wavefront's tokens
+      uint32_t n = 0;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) n += in[j];
+      const uint32_t inc = wave_scan(n), all = lane_value(inc, 63);
+      if (all == 0) return;
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&sm.base[64], all);
+      at = lane_value(at, 0) + inc - n;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        if (in[j] && at < (uint32_t)kList) sm.list[at] = (u64)key[j] << 32 | (uint32_t)(c + j);
+        at += in[j];
       }
+      return;
+    }
+    if (MODE == kKeep && p.table) {
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) w[j] = sm.sub_mass[in[j] ? p.digit.top - (key[j] >> KS) : 0];
+    } else if (MODE != kSubs || !p.by_count) {
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) w[j] = row_weight(in[j] ? y[j] : sm.xr, &b[j]);
+    }
+    u64 sum = 0;
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      if (MODE == kSubs && in[j]) {
+        const uint32_t at =
+            BlockSelect::at(p.digit.sub(key[j] >> KS, c + j, BlockSelect::SUBS));
+        atomicAdd(&sm.sub_cnt[at], 1u);
+        if (!p.by_count) atomicAdd(&sm.sub_mass[at], w[j]);
+      }
+      if (MODE == kBinsOf && in[j]) {
+        atomicAdd(&sm.cnt[b[j]], 1u);
+        atomicAdd(&sm.mass[b[j]], w[j]);
+      }
+      if (MODE == kKeep || MODE == kCellsOf) sum += in[j] ? w[j] : 0;
+      if (MODE == kCellsOf && in[j] && w[j] == 0)
+        atomicMin(&sm.kmin, (uint32_t)((c + j + mis) % kChunk));
+    }
+    if (MODE == kKeep) {  // (a wavefront's 512 columns lie in one chunk)
+      sum = wave_total(sum);
+      if (lane == 0 && sum > 0) atomicAdd(&sm.kept[(c + mis) / kChunk], sum);
+    }
+    // (a thread's 8 columns lie in one cell)
+    if (MODE == kCellsOf && sum > 0) atomicAdd(&sm.cell[(c + mis) % kChunk / kCell], sum);
+  };
+  // A vector of 8 logits at a time, the next U - 1 in flight.  (One body, looped:
+  // code that a row runs through once is fetched from memory as it goes, and a body
+  // for each of 32 logits took longer to arrive than its data.)
+  const int s0 = part * (kThreads / 2), s1 = end * (kThreads / 2);
+  // (a call's pointer argument may be to LDS for all that the compiler knows: loads
+  // through it would be waited for with every LDS operation)
+  typedef __attribute__((address_space(1))) u32x4 GlobalVec;
+  u32x4 raw[U][VW];
+  auto load = [&](int slot, u32x4* to) __attribute__((always_inline)) {
+    // whole vectors inside the row; elsewhere one of the row's, not used
+    const int col = slot * kTok - mis;
+    const int at = slot < s1 && col >= 0 && col + kTok <= cols ? col : mis ? kTok - mis : 0;
+    if (at + kTok <= cols) {
+#pragma unroll
+      for (int v = 0; v < VW; ++v)
+        to[v] = *(const GlobalVec*)(uintptr_t)(row + at + v * (kTok / VW));
     }
   };
-  const int slots = end * (kThreads / 2);
-  for (int s0 = part * (kThreads / 2) + threadIdx.x; s0 < slots; s0 += U * kDraw) {
-    float x[U][kTok];
-    int col[U];
+  int slot = s0 + threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      // (past the end, and past the row: no column)
-      const int slot = s0 + i * kDraw < slots ? s0 + i * kDraw : kMaxChunks * kThreads + 1;
-      col[i] = load8(row, cols, mis, 0, slot, x[i]);
-    }
+  for (int i = 0; i < U; ++i) load(slot + i * kDraw, raw[i]);
+  for (; slot - (int)threadIdx.x < s1; slot += kDraw) {  // (uniform)
+    float x[kTok];
+    const int col = slot * kTok - mis;
+    if (slot < s1 && col >= 0 && col + kTok <= cols) {
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) token(x[i][j], col[i] + j);
-      if (MODE == kKeep) {  // (a wavefront's 512 columns lie in one chunk)
-        kept = wave_total(kept);
-        if (lane == 0 && kept > 0) atomicAdd(&sm.kept[(s0 + i * kDraw) / kThreads], kept);
-        kept = 0;
+      for (int j = 0; j < kTok; ++j) {
+        const uint32_t w = raw[0][j / (kTok / VW)][KS ? j / 2 : j % 4];
+        const float y = !KS ? __builtin_bit_cast(float, w) : j & 1 ? bf16hi(w) : bf16lo(w);
+        x[j] = y + 0.0f;  // (NaN: outside every interval)
       }
+    } else {
+      load8(row, slot < s1 ? cols : 0, mis, 0, slot, x);
     }
+#pragma unroll
+    for (int i = 0; i + 1 < U; ++i)
+#pragma unroll
+      for (int v = 0; v < VW; ++v) raw[i][v] = raw[i + 1][v];
+    load(slot + U * kDraw, raw[U - 1]);
+    if (MODE == kCollect && sm.base[64] > (uint32_t)kList) break;  // they do not fit
+    vec8(x, col);
   }
   __syncthreads();
 }
@@ -655,7 +757,6 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
                             const float* __restrict__ us, const Chunk* __restrict__ rec,
                             const Bins* __restrict__ bins, int n_ch, long long* __restrict__ out,
                             int* __restrict__ advance) {
-  __shared__ DrawSmem sm;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row_i = blockIdx.x;
   if (advance && row_i == 0 && tid == 0) *advance += 1;
   const T* row = logits + row_i * ld;
@@ -741,64 +842,67 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
   // The border among the tokens between keys k0 and k1 that are above the present
   // cut: the one at which their running count (by_count) or weight, in the order,
   // reaches need.  Sets the cut.  A round finds a sub-bin: by key, until one is
-  // left (step 0), then among its equals by column / 512 (1) and column (2).
-  // N threads; subs(k0, k1, sh, step, col0, by_count): adds the tokens' sub-bins;
-  // narrowed(k0, k1, n): called when n tokens are left between two new keys.
-  constexpr int KS = sizeof(T) == 2 ? 16 : 0;  // low bits that every key shares
+  // left, then by column among its equals.
+  // subs(k0, k1, digit, by_count): adds the tokens between k0 and k1 (without the
+  // low bits that every key shares); narrowed(k0, k1, n): n of them are left.
+  constexpr int KS = sizeof(T) == 2 ? 16 : 0;
   // (bf16: the low half of a key is all zeros, of a negative logit's all ones)
   auto key_back = [](uint32_t k) __attribute__((always_inline)) {
     return KS ? k << 16 | (k & 0x8000u ? 0u : 0xffffu) : k;
   };
-  auto border = [&](auto select, auto weighs, uint32_t k0, uint32_t k1, u64 need, bool by_count, auto&& subs,
-                    auto&& narrowed) __attribute__((always_inline)) {
+  auto border = [&](auto select, auto weighs, uint32_t k0, uint32_t k1, u64 need, bool by_count,
+                    auto&& subs, auto&& narrowed) __attribute__((always_inline)) {
     constexpr bool WEIGH = decltype(weighs)::value;
+    constexpr int SUBS = decltype(select)::SUBS, BITS = __builtin_ctz(SUBS);
     k0 >>= KS;
     k1 >>= KS;
-    int col0 = 0;
+    Digit dg{0, 0, -1, kColBits, 0};
     bool all_equals = true;
-    for (int step = 0; step < 3;) {
+    for (;;) {
       const uint32_t span = k1 - k0;
-      const int sh = span < (uint32_t)kSub ? 0 : 22 - __builtin_clz(span);
-      select.clear(sm);
+      dg.sh = span < (uint32_t)SUBS ? 0 : 32 - BITS - __builtin_clz(span);
+      dg.top = k1;
+      select.clear();
       // a key per sub-bin: counted, and weighed once for all its tokens
-      const bool weigh = WEIGH && !by_count && sh == 0;
-      subs(k0, k1, sh, step, col0, by_count || weigh);
+      const bool weigh = WEIGH && !by_count && dg.sh == 0;
+      subs(k0, k1, dg, by_count || weigh);
       if (weigh) {
         __syncthreads();
         for (uint32_t i = tid; i <= k1 - k0; i += kDraw) {
           int b;
-          const uint32_t cnt = sm.sub_cnt[sub_at<kDraw>(i)];
-          if (cnt > 0)
-            sm.sub_mass[sub_at<kDraw>(i)] = cnt * row_weight(sm, of_key(key_back(k1 - i)), &b);
+          const uint32_t cnt = sm.sub_cnt[select.at(i)];
+          if (cnt > 0) sm.sub_mass[select.at(i)] = cnt * row_weight(of_key(key_back(k1 - i)), &b);
         }
       }
       u64 n = 0;
-      const uint32_t sub = select.pick(sm, by_count, &need, &n);
+      const uint32_t sub = select.pick(by_count, &need, &n);
       if (need == 0) break;  // every weight here rounds to zero: all are kept
-      if (step == 0) {
-        const uint32_t top = k1 - (sub << sh);
-        k0 = top - k0 < (1u << sh) ? k0 : top - (1u << sh) + 1;
+      if (dg.cs < 0) {
+        const uint32_t top = k1 - (sub << dg.sh);
+        k0 = top - k0 < (1u << dg.sh) ? k0 : top - (1u << dg.sh) + 1;
         k1 = top;
         narrowed(KS ? k0 << 16 : k0, KS ? k1 << 16 | 0xffffu : k1, n);
         if (k0 < k1) continue;
         if (!by_count) {  // as many of the equal tokens as their weight needs
           int b;
-          const u64 w = row_weight(sm, of_key(key_back(k0)), &b);
+          const u64 w = row_weight(of_key(key_back(k0)), &b);
           need = (need + w - 1) / w;
           by_count = true;
         }
         if (need >= n) break;  // all of them
-        step = 1;
+        dg.cs = kColBits - BITS;
+        all_equals = false;
       } else {
-        if (step == 1) col0 = sub << 9;
-        else col0 |= sub;
-        all_equals = ++step < 3;
+        dg.col0 = dg.col0 >> (dg.cs + BITS) << (dg.cs + BITS) | (int)(sub << dg.cs);
+        if (dg.cs == 0) break;
+        dg.prev = dg.cs;
+        dg.cs = max(dg.cs - BITS, 0);
       }
     }
     k0 = key_back(k0);
     if (!all_equals) {
       cut_key = k0;
-      cut_col = col0;
+      cut_col = dg.col0;
     } else if (k0 > cut_key) {  // (of equals of the cut those up to its column stay)
       cut_key = k0;
       cut_col = 0x7fffffff;
@@ -825,18 +929,16 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     const uint32_t key0 = ~sm.kmin, key1 = sm.kmax;
     if (n_all > (uint32_t)s.k)
       border(
-          Select<kDraw>{}, std::false_type{}, key0, key1, s.k, true,
-          [&](uint32_t k0, uint32_t k1, int sh, int step, int col0, bool)
-              __attribute__((always_inline)) {
-                for (uint32_t i = tid; i < n_all; i += kDraw) {
-                  const u64 e = sm.list[i];
-                  const uint32_t k = (uint32_t)(e >> 32) >> KS;
-                  const int col = (int)(uint32_t)e;
-                  if (k < k0 || k > k1 || (step == 2 && (col ^ col0) >> 9)) continue;
-                  const uint32_t sub = step == 0 ? (k1 - k) >> sh : step == 1 ? col >> 9 : col & 511;
-                  atomicAdd(&sm.sub_cnt[sub_at<kDraw>(sub)], 1u);
-                }
-              },
+          BlockSelect{}, std::false_type{}, key0, key1, s.k, true,
+          [&](uint32_t k0, uint32_t k1, Digit dg, bool) __attribute__((always_inline)) {
+            for (uint32_t i = tid; i < n_all; i += kDraw) {
+              const u64 e = sm.list[i];
+              const uint32_t k = (uint32_t)(e >> 32) >> KS;
+              const int col = (int)(uint32_t)e;
+              if (k >= k0 && k <= k1 && !dg.skips(col))
+                atomicAdd(&sm.sub_cnt[BlockSelect::at(dg.sub(k, col, BlockSelect::SUBS))], 1u);
+            }
+          },
           [](uint32_t, uint32_t, u64) {});
     __syncthreads();
     for (uint32_t i = tid; i < n_all; i += kDraw) {
@@ -845,7 +947,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       const uint32_t at = atomicAdd(&sm.n_few, 1u);
       int b;
       sm.list[kMost + at] = e;
-      sm.few_w[at] = row_weight(sm, of_key((uint32_t)(e >> 32)), &b);
+      sm.few_w[at] = row_weight(of_key((uint32_t)(e >> 32)), &b);
     }
     __syncthreads();
     // the rest by one wavefront, without barriers
@@ -867,44 +969,47 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     if (s.fp) {
       const u64 total = wave_total(mine);
       border(
-          Select<64>{}, std::false_type{}, max(key0, cut_key), key1,
+          WaveSelect{}, std::false_type{}, max(key0, cut_key), key1,
           max(1ull, min(part_of(s.p, total), total)), false,
-          [&](uint32_t k0, uint32_t k1, int sh, int step, int col0, bool by_count)
-              __attribute__((always_inline)) {
+          [&](uint32_t k0, uint32_t k1, Digit dg, bool by_count) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < E; ++i) {
-                  const uint32_t k = key[i] >> KS;
-                  if (lane + 64 * i >= n || k < k0 || k > k1 || (step == 2 && (col[i] ^ col0) >> 9))
-                    continue;
-                  const uint32_t sub = sub_at<64>(step == 0   ? (k1 - k) >> sh
-                                                  : step == 1 ? col[i] >> 9
-                                                              : col[i] & 511);
-                  atomicAdd(&sm.sub_cnt[sub], 1u);
-                  if (!by_count) atomicAdd(&sm.sub_mass[sub], w[i]);
-                }
-              },
+            for (int i = 0; i < E; ++i) {
+              if (64 * i >= n) break;
+              const uint32_t k = key[i] >> KS;
+              if (lane + 64 * i >= n || k < k0 || k > k1 || dg.skips(col[i])) continue;
+              const uint32_t at = WaveSelect::at(dg.sub(k, col[i], WaveSelect::SUBS));
+              atomicAdd(&sm.sub_cnt[at], 1u);
+              if (!by_count) atomicAdd(&sm.sub_mass[at], w[i]);
+            }
+          },
           [](uint32_t, uint32_t, u64) {});
     }
     mine = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      if (lane + 64 * i < n && !(above_cut(key[i], col[i]) && min_p_keeps(sm, of_key(key[i]))))
+      if (lane + 64 * i < n && !(above_cut(key[i], col[i]) && min_p_keeps(of_key(key[i]))))
         w[i] = 0;
       mine += w[i];
     }
-    // the token, in index order: by columns of 512, then by column
+    // the token, in index order
     u64 t = target_of(u, wave_total(mine)) + 1, unused;
-    int col0 = 0;
-    for (int step = 1; step < 3; ++step) {
-      Select<64>::clear(sm);
+    constexpr int SUBS = WaveSelect::SUBS, BITS = __builtin_ctz(SUBS);
+    Digit dg{0, 0, kColBits - BITS, kColBits, 0};
+    for (;;) {
+      WaveSelect::clear();
 #pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (w[i] > 0 && (step == 1 || (col[i] ^ col0) >> 9 == 0))
-          atomicAdd(&sm.sub_mass[sub_at<64>(step == 1 ? col[i] >> 9 : col[i] & 511)], w[i]);
-      const int sub = Select<64>::pick(sm, false, &t, &unused);
-      col0 = step == 1 ? sub << 9 : col0 | sub;
+      for (int i = 0; i < E; ++i) {
+        if (64 * i >= n) break;
+        if (w[i] > 0 && !dg.skips(col[i]))
+          atomicAdd(&sm.sub_mass[WaveSelect::at(dg.sub(0, col[i], SUBS))], w[i]);
+      }
+      const int sub = WaveSelect::pick(false, &t, &unused);
+      dg.col0 = dg.col0 >> (dg.cs + BITS) << (dg.cs + BITS) | sub << dg.cs;
+      if (dg.cs == 0) break;
+      dg.prev = dg.cs;
+      dg.cs = max(dg.cs - BITS, 0);
     }
-    if (lane == 0) *out = col0;
+    if (lane == 0) *out = dg.col0;
     return;
   }
 
@@ -915,10 +1020,10 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
   Pass p{};
   if (s.few) {  // too many for what the chunks wrote out: by passing over the row
     if (tid < kMaxChunks) sm.last[tid] = -1;
-    find_ends(0, kBins - 1, sm);
+    find_ends(0, kBins - 1);
     p.k0 = sm.ends[0];
     p.k1 = sm.ends[1] - 1;
-    pass<T, kBinsOf>(row, cols, mis, 0, 2 * n_ch, p, sm);
+    pass<T, kBinsOf>(row, cols, mis, 0, 2 * n_ch, p);
   } else {
     const int counted = s.fk ? kBins : 0, all = n_ch * kBins;
     for (int i0 = tid; i0 < all; i0 += 4 * kDraw) {
@@ -946,8 +1051,8 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     m_here = sm.mass[tid];
     n_here = sm.cnt[tid];
   }
-  m_before = block_scan(m_here, sm.tmp, &total_m);
-  if (s.fk) n_before = block_scan(n_here, sm.tmp, &total_n);
+  m_before = block_scan(m_here, &total_m);
+  if (s.fk) n_before = block_scan(n_here, &total_n);
 
   // The list holds the tokens between keys list0 and list1 (none: list0 > list1).
   uint32_t list0 = 1, list1 = 0;
@@ -955,7 +1060,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
   // else from the row, if they fit; k0, k1: the bin's keys
   uint32_t bin0 = 0, bin1 = 0;
   auto collect = [&](int j) __attribute__((always_inline)) {
-    find_ends(j, j, sm);
+    find_ends(j, j);
     bin0 = sm.ends[0];
     bin1 = sm.ends[1] - 1;
     if (bin0 >= list0 && bin1 <= list1) return;
@@ -982,7 +1087,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     } else {
       p.k0 = bin0;
       p.k1 = bin1;
-      pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p, sm);
+      pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p);
       if (sm.base[64] > (uint32_t)kList) return;
     }
     list0 = bin0;
@@ -1004,8 +1109,8 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       listed(bin0, bin1, [&](uint32_t key, int col) __attribute__((always_inline)) {
         int b;
         const float x = of_key(key);
-        if (above_cut(key, col) && (!min_p || min_p_keeps(sm, x)))
-          atomicAdd(&sm.kept[(col + mis) / kChunk], row_weight(sm, x, &b));
+        if (above_cut(key, col) && (!min_p || min_p_keeps(x)))
+          atomicAdd(&sm.kept[(col + mis) / kChunk], row_weight(x, &b));
       });
     } else {
       p.k0 = max(bin0, cut_key);
@@ -1014,13 +1119,14 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       p.cut_col = cut_col;
       p.min_p = min_p;
       // few keys: their weights in a table (of them, not of thousands of tokens)
-      p.top = bin1 >> KS;
-      p.table = p.top - (p.k0 >> KS) < (uint32_t)kSub;
-      for (uint32_t i = tid; p.table && i <= p.top - (p.k0 >> KS); i += kDraw) {
+      p.digit.top = bin1 >> KS;
+      const uint32_t keys = p.digit.top - (p.k0 >> KS);
+      p.table = keys < (uint32_t)kSub;
+      for (uint32_t i = tid; p.table && i <= keys; i += kDraw) {
         int b;
-        sm.sub_mass[i] = row_weight(sm, of_key(key_back(p.top - i)), &b);
+        sm.sub_mass[i] = row_weight(of_key(key_back(p.digit.top - i)), &b);
       }
-      pass<T, kKeep>(row, cols, mis, 0, 2 * n_ch, p, sm);
+      pass<T, kKeep>(row, cols, mis, 0, 2 * n_ch, p);
     }
     __syncthreads();
   };
@@ -1035,7 +1141,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
         keep_bin(false);
         u64 mine = tid < kMaxChunks ? sm.kept[tid] : 0;
         if (tid == jc) mine += m_before;  // and the bins above
-        block_scan(mine, sm.tmp, &left);
+        block_scan(mine, &left);
         if (tid < kMaxChunks) sm.kept[tid] = 0;
       }
       need = max(1ull, min(part_of(s.p, left), min(left, total_m)));
@@ -1053,35 +1159,28 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     if (j > jc) break;  // (by rounding) past top-k's border: that one holds
     collect(j);
     border(
-        Select<kDraw>{}, std::true_type{}, bin0, bin1, need, stage == 0,
-        [&](uint32_t k0, uint32_t k1, int sh, int step, int col0, bool by_count)
-            __attribute__((always_inline)) {
-              const uint32_t a0 = k0 << KS, a1 = KS ? k1 << 16 | 0xffffu : k1;
-              // (a bin's first key may lie above the first of its low half)
-              if (max(a0, bin0) >= list0 && min(a1, bin1) <= list1) {
-                listed(a0, a1, [&](uint32_t key, int col) __attribute__((always_inline)) {
-                  if (!above_cut(key, col) || (step == 2 && (col ^ col0) >> 9)) return;
-                  const uint32_t sub = sub_at<kDraw>(step == 0   ? (k1 - (key >> KS)) >> sh
-                                                     : step == 1 ? col >> 9
-                                                                 : col & 511);
-                  int b;
-                  atomicAdd(&sm.sub_cnt[sub], 1u);
-                  if (!by_count)
-                    atomicAdd(&sm.sub_mass[sub], row_weight(sm, of_key(key), &b));
-                });
-              } else {
-                p.step = step;
-                p.sh = sh;
-                p.by_count = by_count;
-                p.k0 = max(a0, bin0);
-                p.k1 = min(a1, bin1);
-                p.top = k1;
-                p.col0 = col0;
-                p.cut_key = cut_key;
-                p.cut_col = cut_col;
-                pass<T, kSubs>(row, cols, mis, 0, 2 * n_ch, p, sm);
-              }
-            },
+        BlockSelect{}, std::true_type{}, bin0, bin1, need, stage == 0,
+        [&](uint32_t k0, uint32_t k1, Digit dg, bool by_count) __attribute__((always_inline)) {
+          const uint32_t a0 = k0 << KS, a1 = KS ? k1 << 16 | 0xffffu : k1;
+          // (a bin's first key may lie above the first of its low half)
+          if (max(a0, bin0) >= list0 && min(a1, bin1) <= list1) {
+            listed(a0, a1, [&](uint32_t key, int col) __attribute__((always_inline)) {
+              if (!above_cut(key, col) || dg.skips(col)) return;
+              const uint32_t at = BlockSelect::at(dg.sub(key >> KS, col, BlockSelect::SUBS));
+              int b;
+              atomicAdd(&sm.sub_cnt[at], 1u);
+              if (!by_count) atomicAdd(&sm.sub_mass[at], row_weight(of_key(key), &b));
+            });
+          } else {
+            p.by_count = by_count;
+            p.k0 = max(a0, bin0);
+            p.k1 = min(a1, bin1);
+            p.digit = dg;
+            p.cut_key = cut_key;
+            p.cut_col = cut_col;
+            pass<T, kSubs>(row, cols, mis, 0, 2 * n_ch, p);
+          }
+        },
         [&](uint32_t k0, uint32_t k1, u64 n) __attribute__((always_inline)) {
           k0 = max(k0, bin0);
           k1 = min(k1, bin1);
@@ -1089,7 +1188,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
           if ((k0 >= list0 && k1 <= list1) || n > (u64)kList) return;
           p.k0 = k0;
           p.k1 = k1;
-          pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p, sm);
+          pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p);
           const bool fits = sm.base[64] <= (uint32_t)kList;
           list0 = fits ? k0 : 1;
           list1 = fits ? k1 : 0;
@@ -1115,7 +1214,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     }
   }
   if (s.few) {  // (its chunks left no weights: every token up to the border)
-    find_ends(0, min(jc, kBins - 1), sm);
+    find_ends(0, min(jc, kBins - 1));
     bin0 = sm.ends[0];
     bin1 = sm.ends[1] - 1;
     list0 = 1;
@@ -1146,19 +1245,19 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       const int col = (int)(uint32_t)e, at = col + mis - ch * kChunk;
       const float x = of_key(key);
       int b;
-      const u64 w = row_weight(sm, x, &b);
-      if (b >= kBins || !above_cut(key, col) || !min_p_keeps(sm, x)) continue;
+      const u64 w = row_weight(x, &b);
+      if (b >= kBins || !above_cut(key, col) || !min_p_keeps(x)) continue;
       if (w > 0) atomicAdd(&sm.cell[at / kCell], w);
       else atomicMin(&sm.kmin, (uint32_t)at);
     }
   } else {
-    find_ends(0, min(jc, kBins - 1), sm);
+    find_ends(0, min(jc, kBins - 1));
     p.k0 = sm.ends[0];
     p.k1 = sm.ends[1] - 1;
     p.cut_key = cut_key;
     p.cut_col = cut_col;
     p.min_p = 1;
-    pass<T, kCellsOf>(row, cols, mis, 2 * ch, 2 * ch + 2, p, sm);
+    pass<T, kCellsOf>(row, cols, mis, 2 * ch, 2 * ch + 2, p);
   }
   __syncthreads();
   // ---- the columns and the token, by one wavefront -------------------------------
@@ -1179,8 +1278,8 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
   float x = col >= 0 && col < cols ? (float)row[col] : -INFINITY;
   x = x == x ? x + 0.0f : -INFINITY;
   int b;
-  u64 w = row_weight(sm, x, &b);
-  if (b >= kBins || !above_cut(key_of(x), col) || !min_p_keeps(sm, x)) w = 0;
+  u64 w = row_weight(x, &b);
+  if (b >= kBins || !above_cut(key_of(x), col) || !min_p_keeps(x)) w = 0;
   const u64 run = wave_scan(w);
   if (run - w <= t && t < run) *out = col;
 }
@@ -1192,7 +1291,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       const T* logits, long ld, int cols, Args a, Chunk* rec, Bins* bins) {                       \
     sample_scan<T>(logits, ld, cols, a, rec, bins);                                               \
   }                                                                                               \
-  extern "C" __global__ __launch_bounds__(256) void teeny_sample_draw_##TN(                      \
+  extern "C" __global__ __launch_bounds__(512) void teeny_sample_draw_##TN(                      \
       const T* logits, long ld, int cols, Args a, const float* u, const Chunk* rec,               \
       const Bins* bins, int n_ch, long long* out, int* advance) {                                 \
     sample_draw<T>(logits, ld, cols, a, u, rec, bins, n_ch, out, advance);                        \
