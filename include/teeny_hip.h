@@ -390,7 +390,8 @@ int teeny_decode_attention_dev(const void* q, const void* k_cache, const void* v
  * 16-byte aligned.  bf16, n_new > 1: the rows n_past[b] .. n_past[b] + n_new - 1
  * must be finite, as the causal forward's; cache rows past them and prefix rows
  * past n_prefix are never read.  workspace:
- * teeny_shared_prefix_attention_workspace_bytes bytes, 16-byte aligned.  No
+ * teeny_shared_prefix_attention_workspace_bytes bytes (0 where many new tokens
+ * fill the device without sharing a row's keys out), 16-byte aligned.  No
  * reference counterpart (it has no KV cache). */
 size_t teeny_shared_prefix_attention_workspace_bytes(int batch, int n_heads_q, int n_heads_kv,
                                                      int n_new, int n_prefix, int cache_len,

@@ -1327,7 +1327,14 @@ struct PrefixShape {  // Shape in prefix_attn.hip
 struct PrefixParts {  // Parts in prefix_attn.hip
   float *m, *l, *o;
 };
+struct FwdPrefix {  // in fa2_fwd_bf16.hip
+  const void *k, *v;
+  int n, len, batch, s;
+  const int32_t* past;
+  int past_stride, past_imm;
+};
 struct PrefixPlan {
+  bool fwd;      // the forward kernel, without shares
   int nw, rows;  // wavefronts per workgroup, rows per row tile
   int row_tiles, p_splits, p_keys, o_splits;
   long groups;   // of 32 (fp32: 16) rows of a sequence and kv head
@@ -1337,6 +1344,9 @@ PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_new, int n_prefix, int 
   PrefixPlan p{};
   const long gs = (long)(hq / hkv) * n_new, rows = batch * gs, cus = device_cus();
   const bool f32 = dtype == TEENY_F32;
+  const long blocks = (gs + 127) / 128 * batch * hkv;
+  p.fwd = !f32 && gs >= 64 && 2 * blocks >= cus;
+  if (p.fwd) return p;
   p.nw = f32 ? 1 : rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
   p.rows = f32 ? 16 : 32 * p.nw;
   p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
@@ -1362,6 +1372,7 @@ size_t teeny_shared_prefix_attention_workspace_bytes(int batch, int n_heads_q, i
       n_new <= 0 || n_prefix < 0 || cache_len <= 0 || head_dim <= 0 || !dtype_ok(dtype))
     return 0;
   const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
+  if (p.fwd) return 0;
   const size_t rows = (size_t)batch * n_heads_q * n_new * (p.p_splits + p.o_splits);
   return 2 * align256(rows * sizeof(float)) + align256(rows * head_dim * sizeof(float));
 }
@@ -1388,12 +1399,25 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
   const uintptr_t at = (uintptr_t)q | (uintptr_t)o | (uintptr_t)k_cache | (uintptr_t)v_cache |
                        (n_prefix > 0 ? (uintptr_t)k_prefix | (uintptr_t)v_prefix : 0);
   if (at % (dtype == TEENY_BF16 ? 16 : 4) != 0) return TEENY_ERR_INVALID_VALUE;
+  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
+  char name[64];
+  if (p.fwd) {
+    int nq = n_heads_q / n_heads_kv * n_new, nmb = (nq + 127) / 128;
+    const long total = (long)nmb * batch * n_heads_kv;
+    if (total >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+    int tot = (int)total;
+    FwdPrefix pre{k_prefix, v_prefix, n_prefix, prefix_len, batch, n_new, n_past, n_past_stride,
+                  n_past_host};
+    snprintf(name, sizeof name, "teeny_fa2_fwd_bf16_d%d_prefix", head_dim);
+    void* args[] = {&q, &k_cache, &v_cache, &o, &nq, &cache_len, &softmax_scale, &n_heads_q,
+                    &n_heads_kv, &nmb, &tot, &merged, &pre};
+    return launch(name, dim3((unsigned)tot), dim3(256), 0, stream, args);
+  }
   if (!workspace || workspace_bytes < teeny_shared_prefix_attention_workspace_bytes(
                                           batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len,
                                           head_dim, dtype))
     return TEENY_ERR_WORKSPACE;
   if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
-  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
   const int shares = p.p_splits + p.o_splits;
   const size_t rows = (size_t)batch * n_heads_q * n_new;
   PrefixParts parts{(float*)workspace,
@@ -1405,7 +1429,6 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
   const long wgs = (long)p.p_splits * p.row_tiles * n_heads_kv +
                    (long)p.o_splits * batch * n_heads_kv * p.groups;
   if (wgs >= (1L << 31) || (long)rows >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
-  char name[64];
   if (dtype == TEENY_BF16)
     snprintf(name, sizeof name, "teeny_prefix_attn_bf16_d%d_w%d", head_dim, p.nw);
   else

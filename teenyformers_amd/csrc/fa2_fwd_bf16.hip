@@ -70,12 +70,27 @@ struct __attribute__((aligned(16))) FwdSmem {
 // subtiles (2: 64 keys, two workgroups per CU; 1: 32 keys, whose smaller
 // register set and LDS footprint let three workgroups share a CU).  With
 // NSUB = 1 the second subtile's statements below are compiled out.
-template <int D, bool CAUSAL, int NW = 4, bool PACK = false, int NSUB = 2>
+//
+// PREFIX (teeny_shared_prefix_attention's rows in numbers): the keys are the
+// prefix's, which all sequences share, and then each sequence's own (k, v: caches
+// of nk rows).  The rows of a (b, kv head) are its nq = G S (q head, new token)
+// pairs, 32 NW consecutive ones a workgroup, whatever G is: they read the same
+// keys.  Row r is token r % S and sees own keys 0 .. past + r % S.  A tile holds
+// keys of one part.  Workgroups go kv head by kv head, so an XCD's L2 keeps few
+// prefix heads.  No LSE.
+struct FwdPrefix {
+  const bf16 *k, *v;        // [Hkv, len, D], rows 0 .. n - 1
+  int n, len, batch, s;     // s: new tokens of a sequence
+  const int* past;          // as Shape in prefix_attn.hip
+  int past_stride, past_imm;
+};
+
+template <int D, bool CAUSAL, int NW = 4, bool PACK = false, int NSUB = 2, bool PREFIX = false>
 __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const bf16* __restrict__ k,
                              const bf16* __restrict__ v, bf16* __restrict__ o,
                              float* __restrict__ lse, int nq, int nk, float scale, int hq, int hkv,
                              int num_m_blocks, int total_blocks, int o_merged,
-                             const float2* __restrict__ rope_cs) {
+                             const float2* __restrict__ rope_cs, const FwdPrefix pre = {}) {
   constexpr int BN = SUBN * NSUB;      // keys per tile
   constexpr int BM = 32 * NW;          // query rows per workgroup
   constexpr int NT = 64 * NW;          // threads
@@ -97,7 +112,8 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // causal blocks: heads in groups of 4 (measured 1.02-1.06x at B16 Hq32 Hkv8
   // S512 and B4 S2048 against pairs; equal blocks gain nothing from it)
   pair_order<CAUSAL ? 4 : 2>(id, num_m_blocks, total_blocks / num_m_blocks, bh, rank);
-  const int mb = num_m_blocks - 1 - rank;  // the last query block is the heaviest
+  // the last query block is the heaviest (PREFIX: the lightest, its rows may end)
+  const int mb = PREFIX ? rank : num_m_blocks - 1 - rank;
   // bhq: this wavefront's (b, q head); wrow0: its first query row; blk_end:
   // one past the workgroup's last row.  GQA-packed (PACK, NW = hq / hkv): bh
   // is a (b, kv head), every wavefront takes the same 32 rows of its own q
@@ -105,7 +121,13 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // rows 32 w of the block's BM.
   int bhq, wrow0, blk_end;
   long kvh;
-  if constexpr (PACK) {
+  if constexpr (PREFIX) {
+    const int hk = bh / pre.batch, b = bh - hk * pre.batch;
+    kvh = (long)b * hkv + hk;
+    bhq = (int)kvh;
+    wrow0 = mb * BM + wave * 32;
+    blk_end = mb * BM + BM;
+  } else if constexpr (PACK) {
     const int b = bh / hkv;
     kvh = bh;
     bhq = b * hq + (bh - b * hkv) * NW + wave;
@@ -175,10 +197,42 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
 
   int kend = nk;
   if (CAUSAL) kend = min(nk, blk_end);
-  const int n_iter = (kend + BN - 1) / BN;
+  int n_iter = (kend + BN - 1) / BN;
+  // PREFIX: own keys of this lane's row (lim) and of the wavefront's first tokens
+  // that every row of it sees (lim_all); prefix tiles
+  int lim = 0, lim_all = 0, n_pre = 0, own_rows = 0;
+  int own_live = 0;  // PREFIX: own tiles of this wavefront
+  if constexpr (PREFIX) {
+    const int b = (int)(kvh / hkv);
+    int past = pre.past ? pre.past[(long)b * pre.past_stride] : pre.past_imm;
+    past = __builtin_amdgcn_readfirstlane(min(max(past, -pre.s), nk));
+    // least and greatest token of rows r0 .. r1 - 1
+    auto tokens = [&](int r0, int r1, int& t0, int& t1) {
+      t0 = r0 % pre.s;
+      t1 = (r1 - 1) % pre.s;
+      if (r1 - r0 >= pre.s || t0 > t1) {
+        t0 = 0;
+        t1 = pre.s - 1;
+      }
+    };
+    int t0, t1;
+    tokens(mb * BM, min(blk_end, nq), t0, t1);
+    const int own_end = min(past + t1 + 1, nk);
+    own_rows = max(0, min(past + pre.s, nk));
+    n_pre = (pre.n + BN - 1) / BN;
+    n_iter = n_pre + (own_end + BN - 1) / BN;
+    if (wrow0 < nq) {
+      tokens(wrow0, min(wrow0 + 32, nq), t0, t1);
+      own_live = n_pre + (min(past + t1 + 1, nk) + BN - 1) / BN;
+      lim_all = min(past + t0 + 1, nk);
+    }
+    lim = min(past + min(qrow, nq - 1) % pre.s + 1, nk);
+  }
   // causal: the workgroup's tiles past this wavefront's last row are fully
   // masked for it; it computes only the first n_live (wave-uniform)
-  const int n_live = CAUSAL ? min(n_iter, wave_qmax / BN + 1) : n_iter;
+  const int n_live = PREFIX   ? max(1, own_live)
+                     : CAUSAL ? min(n_iter, wave_qmax / BN + 1)
+                              : n_iter;
 
   // ---- direct global -> LDS tile loads --------------------------------------
   // buffer_load ... lds (MUBUF, not FLAT: LDS waits elsewhere in the loop keep
@@ -189,15 +243,28 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // swizzles unchanged, so a lane's chunks are one byte offset plus i * LSTEP.
   const uint32_t k_src = swz<SWZ_ROW, D>(wave * 64 + lane) * 16;
   const uint32_t v_src = swz<SWZ_DUAL, D>(wave * 64 + lane) * 16;
-  const auto krsrc = make_rsrc(kb, nk * D * 2);
-  const auto vrsrc = make_rsrc(vb, nk * D * 2);
+  // (PREFIX: own rows past the new tokens' last are not read either)
+  const auto krsrc = make_rsrc(kb, (PREFIX ? own_rows : nk) * D * 2);
+  const auto vrsrc = make_rsrc(vb, (PREFIX ? own_rows : nk) * D * 2);
+  const long pbase = PREFIX ? (kvh % hkv) * (long)pre.len * D : 0;
+  const auto kprsrc = make_rsrc(PREFIX ? pre.k + pbase : kb, pre.n * D * 2);
+  const auto vprsrc = make_rsrc(PREFIX ? pre.v + pbase : vb, pre.n * D * 2);
   // it: tile index; koff / voff: byte offsets of its K and V buffers.  Rows
   // past the sequence lie outside the descriptors' ranges and load as zeros:
   // their scores are masked, and P = 0 times V = 0 adds nothing.
   auto load_tile = [&](int it, int koff, int voff) {
     char* kdst = sm.k[0] + koff + wave * 64 * 16;
     char* vdst = sm.v[0] + voff + wave * 64 * 16;
-    const int sbase = it * BN * D * 2;
+    if (PREFIX && it < n_pre) {
+      const int pbytes = it * BN * D * 2;
+#pragma unroll
+      for (int i = 0; i < TCH; ++i) {
+        dma16(kprsrc, kdst + i * LSTEP, k_src, pbytes + i * LSTEP);
+        dma16(vprsrc, vdst + i * LSTEP, v_src, pbytes + i * LSTEP);
+      }
+      return;
+    }
+    const int sbase = (it - n_pre) * BN * D * 2;
 #pragma unroll
     for (int i = 0; i < TCH; ++i) {
       dma16(krsrc, kdst + i * LSTEP, k_src, sbase + i * LSTEP);
@@ -296,6 +363,21 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // raw scores of keys past the sequence or (causal) past the row -> -inf;
   // only tiles that reach past nk or past the wave's first row need it
   auto mask = [&](int kbase, f32x16& s0, f32x16& s1) {
+    if constexpr (PREFIX) {
+      const bool own = kbase >= n_pre * BN;
+      const int t0 = own ? kbase - n_pre * BN : kbase;
+      if (t0 + BN <= (own ? lim_all : pre.n)) return;
+      const int end = own ? lim : pre.n;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = t0 + 8 * (r >> 2) + 4 * g + (r & 3);
+        if (key >= end) s0[r] = -INFINITY;
+        if constexpr (NSUB == 2) {
+          if (key + 32 >= end) s1[r] = -INFINITY;
+        }
+      }
+      return;
+    }
     if ((kbase + BN > nk) || (CAUSAL && kbase + BN - 1 > wrow0)) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -510,7 +592,8 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // ---- epilogue ----
   l_run += l_run2;
   const float l_tot = l_run + other_half(l_run);
-  const float inv = 1.0f / l_tot;  // rows past nq: never stored
+  // rows past nq: never stored; PREFIX: zeros for a row without a key
+  const float inv = PREFIX && l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
   // O goes through LDS (the K/V buffers, free once every wavefront's last PV
   // product has read its tile): each wavefront writes its 32 x D tile, the
   // 16-byte chunk c of row r at chunk c ^ (r % CPR) of that row, and reads it
@@ -546,6 +629,20 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
                        pack_bf16x2(acc_o[t][4 * j + 2] * inv, acc_o[t][4 * j + 3] * inv)};
       *reinterpret_cast<u32x2*>(ot + (wa ^ ((4 * t + j) << 4))) = w;
     }
+  }
+  if constexpr (PREFIX) {
+    const int b = (int)(kvh / hkv), hk = (int)(kvh - (long)b * hkv);
+#pragma unroll
+    for (int kk = 0; kk < 32 / RPI; ++kk) {
+      const u32x4 val = *reinterpret_cast<const u32x4*>(
+          ot + (ra ^ (((kk % (CPR / RPI)) * RPI) << 4)) + kk * RPI * 2 * D);
+      const int r = wrow0 + kk * RPI + ln / CPR;
+      const int hr = r / pre.s, t = r - hr * pre.s;  // the row's q head in the group, token
+      const long row = o_merged ? ((long)b * pre.s + t) * hq + hk * (hq / hkv) + hr
+                                : kvh * (long)nq + r;
+      if (r < nq) *reinterpret_cast<u32x4*>(o + row * D + 8 * (ln % CPR)) = val;
+    }
+    return;
   }
   const int hd = bhq % hq;  // this wavefront's q head within its batch row
   bf16* ob = o + (long)(bhq - hd) * nq * D + (long)wrow0 * rs + (long)hd * (o_merged ? D : nq * D);
@@ -595,3 +692,15 @@ TEENY_FA2_FWD_BF16_K(n_w8, 128, false, 8, false, 2, 2)
 TEENY_FA2_FWD_BF16_K(c_g4, 64, true, 4, true, 2, 3)
 TEENY_FA2_FWD_BF16_K(c_g4, 128, true, 4, true, 1, 3)
 TEENY_FA2_FWD_BF16_K(c_g8, 128, true, 8, true, 2, 2)
+
+// A shared prefix: the causal forms' tiles, three workgroups per CU
+#define TEENY_FA2_FWD_PREFIX_K(D, NSUB)                                                          \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3)))        \
+  void teeny_fa2_fwd_bf16_d##D##_prefix(const bf16* q, const bf16* k, const bf16* v, bf16* o,    \
+                                        int nq, int nk, float scale, int hq, int hkv, int nmb,   \
+                                        int total, int o_merged, FwdPrefix pre) {                \
+    fa2_fwd_bf16<D, false, 4, false, NSUB, true>(q, k, v, o, nullptr, nq, nk, scale, hq, hkv,    \
+                                                 nmb, total, o_merged, nullptr, pre);            \
+  }
+TEENY_FA2_FWD_PREFIX_K(64, 2)
+TEENY_FA2_FWD_PREFIX_K(128, 1)

@@ -99,6 +99,12 @@ SHAPES = [
     (2, 8, 2, 33, 128, 65, 80, [0, 47]),
     (1, 4, 2, 130, 64, 259, 131, [1]),
     (9, 6, 2, 7, 64, 0, 50, [0, 1, 2, 3, 30, 31, 32, 33, 43]),
+    # rows enough for the forward kernel (bf16): 128 workgroups of 128 rows and more
+    (16, 32, 8, 17, 128, 70, 40, [i for i in range(16)]),
+    (33, 16, 4, 33, 64, 0, 70, [i for i in range(33)]),
+    (8, 64, 8, 40, 64, 129, 45, [5, 0, 1, 2, 3, 4, 5, 5]),
+    (24, 24, 8, 50, 128, 33, 114, [0, 64] * 12),
+    (4, 16, 16, 300, 64, 31, 364, [0, 64, 1, 31]),
 ]
 
 
@@ -135,33 +141,38 @@ def test_past_lengths(cuda, dtype, past):
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 def test_rows_that_see_nothing_and_past_the_cache(cuda, dtype):
     """Device lengths that leave no key (zeros), some rows without a key, and rows
-    past the cache's end (the whole cache)."""
-    q, kp, vp, k, v = make(cuda, dtype, 4, 4, 2, 3, 64, 1, 35)
-    past = [-3, -2, 35, -100]
-    want, tol = reference(q, kp, vp, k, v, 0, past, 0.125)
-    n = torch.tensor(past, dtype=torch.int32, device="cuda")
-    got = ops.shared_prefix_attention(q, kp[:, :0], vp[:, :0], k, v, 0, n, 0.125)
-    assert ((got.double() - want).abs() <= tol).all()
-    assert (got[0] == 0).all() and (got[1, :, 0] == 0).all() and (got[3] == 0).all()
-    assert (got[1, :, 1:] != 0).any()
+    past the cache's end (the whole cache); few rows, and as many as the forward
+    kernel takes."""
+    for B, Hkv, S, D in ((4, 2, 3, 64), (4, 32, 64, 64), (8, 16, 64, 128)):
+        q, kp, vp, k, v = make(cuda, dtype, B, 2 * Hkv, Hkv, S, D, 1, S + 32)
+        past = [-S, 1 - S, S + 32, -100] * (B // 4)
+        want, tol = reference(q, kp, vp, k, v, 0, past, 0.125)
+        n = torch.tensor(past, dtype=torch.int32, device="cuda")
+        got = ops.shared_prefix_attention(q, kp[:, :0], vp[:, :0], k, v, 0, n, 0.125)
+        assert ((got.double() - want).abs() <= tol).all()
+        assert (got[0] == 0).all() and (got[1, :, :-1] == 0).all() and (got[3] == 0).all()
+        assert (got[1, :, -1] != 0).any()
 
 
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 def test_large_scores_and_offsets(cuda, dtype):
-    """Scores far from zero, the largest in either part: one softmax over both."""
-    ts = make(cuda, dtype, 3, 4, 2, 1, 64, 90, 50)
-    q, kp, vp, k, v = ts
-    q.mul_(8.0)
-    k[1] *= 3.0
-    kp[0] *= 3.0
-    check(ts, 90, [10, 49, 30], 1)
+    """Scores far from zero, the largest in either part: one softmax over both
+    (exponents past the forward kernel's 2^31 above its first tile among them)."""
+    for B, Hkv, S in ((3, 2, 1), (16, 16, 32)):
+        ts = make(cuda, dtype, B, 2 * Hkv, Hkv, S, 64, 90, 49 + S)
+        q, kp, vp, k, v = ts
+        q.mul_(8.0)
+        k[1] *= 3.0
+        kp[0] *= 3.0
+        check(ts, 90, [10, 49, 30, 3] * (B // 4) if B > 3 else [10, 49, 30], S)
 
 
-@pytest.mark.parametrize("S", [1, 3, 40])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,S", [(3, 1), (3, 3), (3, 40), (66, 40)])
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-def test_merged_layout(cuda, dtype, S):
-    ts = make(cuda, dtype, 3, 8, 2, S, 64, 77, 60)
-    past = torch.tensor([0, 5, 60 - S], dtype=torch.int32, device="cuda")
+def test_merged_layout(cuda, dtype, B, S, D):
+    ts = make(cuda, dtype, B, 8, 2, S, D, 77, 60)
+    past = torch.tensor([0, 5, 60 - S] * (B // 3), dtype=torch.int32, device="cuda")
     a = ops.shared_prefix_attention(*ts, 77, past)
     b = ops.shared_prefix_attention(*ts, 77, past, merged=True)
     assert torch.equal(ops.merge_heads(a), b)
