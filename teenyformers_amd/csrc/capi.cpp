@@ -1321,7 +1321,7 @@ struct PrefixShape {  // Shape in prefix_attn.hip
   int n_prefix, prefix_len, cache_len;
   const int32_t* past;
   int past_stride, past_imm;
-  int p_splits, p_keys, row_tiles, o_splits;
+  int p_splits, p_keys, row_tiles, tile_rows, o_splits;
   float scale;
 };
 struct PrefixParts {  // Parts in prefix_attn.hip
@@ -1347,10 +1347,12 @@ PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_new, int n_prefix, int 
   const long blocks = (gs + 127) / 128 * batch * hkv;
   p.fwd = !f32 && gs >= 64 && 2 * blocks >= cus;
   if (p.fwd) return p;
-  p.nw = f32 ? 1 : rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8;
-  p.rows = f32 ? 16 : 32 * p.nw;
-  p.row_tiles = (int)((rows + p.rows - 1) / p.rows);
-  const long slots = cus * (f32 ? 4 : p.nw == 8 ? 1 : p.nw == 4 ? 2 : 3);
+  const int unit = f32 ? 16 : 32;  // rows of a wavefront
+  const long units = (rows + unit - 1) / unit;
+  p.nw = f32 || units == 1 ? 1 : units == 2 ? 2 : 4;
+  p.row_tiles = (int)((units + p.nw - 1) / p.nw);
+  p.rows = (int)((units + p.row_tiles - 1) / p.row_tiles) * unit;  // even tiles
+  const long slots = cus * (f32 ? 4 : p.nw == 4 ? 2 : 3);
   if (n_prefix > 0) {
     const long want = std::max(1L, slots / ((long)p.row_tiles * hkv));
     const long per = ((n_prefix + want - 1) / want + 31) / 32 * 32;
@@ -1425,7 +1427,7 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
                     (float*)((char*)workspace + 2 * align256(rows * shares * sizeof(float)))};
   PrefixShape a{batch,      n_heads_kv, n_heads_q / n_heads_kv * n_new, n_new, n_prefix, prefix_len,
                 cache_len,  n_past,     n_past_stride, n_past_host,
-                p.p_splits, p.p_keys,   p.row_tiles,   p.o_splits,  softmax_scale};
+                p.p_splits, p.p_keys,   p.row_tiles,   p.rows,      p.o_splits, softmax_scale};
   const long wgs = (long)p.p_splits * p.row_tiles * n_heads_kv +
                    (long)p.o_splits * batch * n_heads_kv * p.groups;
   if (wgs >= (1L << 31) || (long)rows >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
@@ -1436,10 +1438,13 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
   void* a0[] = {&q, &k_prefix, &v_prefix, &k_cache, &v_cache, &a, &parts};
   int rc = launch(name, dim3((unsigned)wgs), dim3(64 * p.nw), 0, stream, a0);
   if (rc) return rc;
-  snprintf(name, sizeof name, "teeny_prefix_merge_%s", dtype_tag(dtype));
+  // (a wavefront a row where that fills the device)
+  const bool wave = (long)rows >= 16L * device_cus();
+  const unsigned rpw = wave ? 4 : 1;
+  snprintf(name, sizeof name, "teeny_prefix_merge_%s%s", dtype_tag(dtype), wave ? "_wave" : "");
   void* a1[] = {&parts, &o, &a, &head_dim, &merged};
-  const unsigned lds = ((unsigned)(shares + 3) / 4 * 4 + 1024) * 4;
-  return launch(name, dim3((unsigned)rows), dim3(256), lds, stream, a1);
+  const unsigned lds = (rpw * ((unsigned)(shares + 3) / 4 * 4) + 1024) * 4;
+  return launch(name, dim3((unsigned)((rows + rpw - 1) / rpw)), dim3(256), lds, stream, a1);
 }
 
 int teeny_argmax_rows(const void* x, int64_t* out, int rows, int cols, int dtype,

@@ -31,7 +31,7 @@ struct Shape {
   const int* past;                // keys in the caches before the call: past[b past_stride]
   int past_stride, past_imm;      // past null: past_imm
   int p_splits, p_keys;           // shares of the prefix, keys per share (a multiple of TK)
-  int row_tiles;                  // row tiles of a kv head over the prefix
+  int row_tiles, tile_rows;       // row tiles of a kv head over the prefix, rows of each
   int o_splits;                   // shares of a sequence's own keys
   float scale;
 };
@@ -190,10 +190,11 @@ __device__ void prefix_attn(const bf16* __restrict__ q, const bf16* __restrict__
     id /= a.row_tiles;
     const int hk = id % a.hkv, split = id / a.hkv;
     const int rows = a.batch * a.gs;
-    const int r = (rt * NW + wave) * 32 + l32;
+    const int first = rt * a.tile_rows + wave * 32;  // the wavefront's rows
+    const int r_end = min(rows, (rt + 1) * a.tile_rows), r = first + l32;
     {
       const int rc = min(r, rows - 1), b = rc / a.gs;
-      st.load_q(q + ((long)(b * a.hkv + hk) * a.gs + (rc - b * a.gs)) * D, r < rows);
+      st.load_q(q + ((long)(b * a.hkv + hk) * a.gs + (rc - b * a.gs)) * D, r < r_end);
     }
     const int k0 = split * a.p_keys, keys = min(a.p_keys, a.n_prefix - k0);
     const int n_tiles = (keys + TK - 1) / TK;
@@ -229,6 +230,7 @@ __device__ void prefix_attn(const bf16* __restrict__ q, const bf16* __restrict__
       else __builtin_amdgcn_s_waitcnt(kVmcnt0);
       barrier_only();
       if (it + 2 < n_tiles) load(it + 2);
+      if (first >= r_end) continue;  // (uniform: a wavefront without rows only loads)
       const char* kt = sm.u.ring[it % kRing][0];
       const char* vt = sm.u.ring[it % kRing][1];
       f32x16 s = st.scores(kt);
@@ -240,14 +242,13 @@ __device__ void prefix_attn(const bf16* __restrict__ q, const bf16* __restrict__
     }
     barrier_only();  // the ring becomes the rows' way out
     const float l_tot = st.l + other_half(st.l);
-    const int first = (rt * NW + wave) * 32;  // the wavefront's rows
     const long row0 = split * n_rows + (long)hk * rows + first;
-    if (g == 0 && r < rows) {
+    if (g == 0 && r < r_end) {
       out.m[row0 + l32] = st.m;
       out.l[row0 + l32] = l_tot;
     }
-    if (first < rows)
-      store_tile_rows<D>(sm.u.out[wave], out.o + row0 * D, rows - first,
+    if (first < r_end)
+      store_tile_rows<D>(sm.u.out[wave], out.o + row0 * D, r_end - first,
                          [&](int t, int j) {
                            return f32x4{st.acc[t][4 * j], st.acc[t][4 * j + 1],
                                         st.acc[t][4 * j + 2], st.acc[t][4 * j + 3]};
@@ -310,20 +311,22 @@ __device__ void prefix_attn(const bf16* __restrict__ q, const bf16* __restrict__
     st.product(va, pb);
   }
   const float l_tot = st.l + other_half(st.l);
-  __syncthreads();  // every wavefront is done with its tiles
-  if (g == 0) {
-    sm.u.c.m[wave][l32] = st.m;
-    sm.u.c.l[wave][l32] = l_tot;
-  }
-  float* orow = sm.u.c.o[wave] + l32 * D;
-#pragma unroll
-  for (int t = 0; t < Rows<D>::DT; ++t)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<f32x4*>(orow + 32 * t + 8 * j + 4 * g) =
-          f32x4{st.acc[t][4 * j], st.acc[t][4 * j + 1], st.acc[t][4 * j + 2], st.acc[t][4 * j + 3]};
-  __syncthreads();
   const int n_here = min(32, a.gs - rg * 32);
+  __syncthreads();  // every wavefront is done with its tiles
+  if (l32 < n_here) {  // (of 32 rows a group of 4 has 4: all were 5 us of 16 at 64 sequences)
+    if (g == 0) {
+      sm.u.c.m[wave][l32] = st.m;
+      sm.u.c.l[wave][l32] = l_tot;
+    }
+    float* orow = sm.u.c.o[wave] + l32 * D;
+#pragma unroll
+    for (int t = 0; t < Rows<D>::DT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(orow + 32 * t + 8 * j + 4 * g) = f32x4{
+            st.acc[t][4 * j], st.acc[t][4 * j + 1], st.acc[t][4 * j + 2], st.acc[t][4 * j + 3]};
+  }
+  __syncthreads();
   const long p0 = (a.p_splits + split) * n_rows + row0 + rg * 32;
   for (int i = tid; i < n_here * D; i += NW * 64) {
     const int rr = i / D, d = i - rr * D;
@@ -487,62 +490,80 @@ __device__ void prefix_attn_f32(const float* __restrict__ q, const float* __rest
   store_col<D>(out.o + prow * D, acc, g, [](float x) { return x; });
 }
 
-// The shares of one row, weighed and summed: grid B Hkv GS rows, 256 threads:
-// D / 4 lanes of four d, 1024 / D groups of them on every so many shares.
-template <typename T>
+// The shares of a row, weighed and summed.  A row takes TPR threads: D / 4 lanes of
+// four d each in groups that go over the shares side by side.  A workgroup (256
+// threads) a row where rows are few, so that the loads of many shares fly at once; a
+// wavefront a row where they are many.
+template <typename T, int TPR>
 __device__ void prefix_merge(const Parts in, T* __restrict__ o, const Shape a, int head_dim,
                              int merged) {
-  constexpr int NT = 256;
-  extern __shared__ __attribute__((aligned(16))) float wt[];  // a weight per share, then the groups' sums [groups][D]
+  constexpr int NT = 256, RPW = NT / TPR;
+  // per row a weight per share (padded to 4), then the groups' sums
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   __shared__ float red[2][NT / 64];
-  const int tid = threadIdx.x, shares = a.p_splits + a.o_splits;
-  const long n_rows = (long)a.batch * a.hkv * a.gs, row = blockIdx.x;
+  const int row_i = threadIdx.x / TPR, tid = threadIdx.x % TPR, shares = a.p_splits + a.o_splits;
+  const long n_rows = (long)a.batch * a.hkv * a.gs;
+  const long want = (long)blockIdx.x * RPW + row_i, row = min(want, n_rows - 1);
   const int bh = (int)(row / a.gs), rem = (int)(row - (long)bh * a.gs);
   const int b = bh / a.hkv, hk = bh - b * a.hkv;
   const long prow = ((long)hk * a.batch + b) * a.gs + rem;  // among the prefix's rows
+  const int padded = (shares + 3) / 4 * 4;
+  float* wt = lds + row_i * padded;
+  float* sums = lds + RPW * padded + row_i * 4 * TPR;
   auto at = [&](int i) { return i * n_rows + (i < a.p_splits ? prow : row); };
+  // the largest of the shares' maxima, and of the sums
+  auto across = [&](float v, int slot, bool sum) {
+    v = sum ? wave_sum(v) : wave_max(v);
+    if (TPR == 64) return v;
+    if ((threadIdx.x & 63) == 0) red[slot][threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[slot][0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) v = sum ? v + red[slot][w] : fmaxf(v, red[slot][w]);
+    return v;
+  };
   float mx = -INFINITY;
-  for (int i = tid; i < shares; i += NT) {
+  for (int i = tid; i < shares; i += TPR) {
     wt[i] = in.m[at(i)];
     mx = fmaxf(mx, wt[i]);
   }
-  mx = wave_max(mx);
-  if ((tid & 63) == 0) red[0][tid >> 6] = mx;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) mx = fmaxf(mx, red[0][w]);
+  mx = across(mx, 0, false);
   const float ref = mx == -INFINITY ? 0.0f : mx;  // no key at all: zeros
   float den = 0.0f;
-  for (int i = tid; i < shares; i += NT) {
+  for (int i = tid; i < shares; i += TPR) {
     const float e = fast_exp2(wt[i] - ref);
     wt[i] = e;
     den += e * in.l[at(i)];
   }
-  den = wave_sum(den);
-  if ((tid & 63) == 0) red[1][tid >> 6] = den;
+  den = across(den, 1, true);
   __syncthreads();
-  den = 0.0f;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) den += red[1][w];
-  const int lanes = head_dim / 4, groups = NT / lanes;
+  const int lanes = head_dim / 4, groups = TPR / lanes;
   const int grp = tid / lanes, d = (tid - grp * lanes) * 4;
   f32x4 acc = {};
-  for (int i = grp; i < shares; i += groups) {
-    const float e = wt[i];
-    if (e > 0.0f) acc += e * *reinterpret_cast<const f32x4*>(in.o + at(i) * head_dim + d);
+  constexpr int U = 4;  // shares of a group in flight
+  for (int i0 = grp; i0 < shares; i0 += U * groups) {
+    f32x4 v[U];
+    float e[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (past the end: the last one, unweighed)
+      const int i = min(i0 + u * groups, shares - 1);
+      e[u] = i0 + u * groups < shares ? wt[i] : 0.0f;
+      v[u] = *reinterpret_cast<const f32x4*>(in.o + at(i) * head_dim + d);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc += e[u] * v[u];
   }
-  float* sums = wt + (shares + 3) / 4 * 4;
   *reinterpret_cast<f32x4*>(sums + grp * head_dim + d) = acc;
   __syncthreads();
-  if (tid < head_dim) {
+  long to = row * head_dim;
+  if (merged) {
+    const int h = hk * (a.gs / a.s) + rem / a.s, s = rem % a.s;
+    to = (((long)b * a.s + s) * a.hkv * (a.gs / a.s) + h) * head_dim;
+  }
+  for (int dd = tid; dd < head_dim && want < n_rows; dd += TPR) {
     float v = 0.0f;
-    for (int i = 0; i < groups; ++i) v += sums[i * head_dim + tid];
-    long to = row * head_dim;
-    if (merged) {
-      const int h = hk * (a.gs / a.s) + rem / a.s, s = rem % a.s;
-      to = (((long)b * a.s + s) * a.hkv * (a.gs / a.s) + h) * head_dim;
-    }
-    o[to + tid] = (T)(den > 0.0f ? v / den : 0.0f);
+    for (int i = 0; i < groups; ++i) v += sums[i * head_dim + dd];
+    o[to + dd] = (T)(den > 0.0f ? v / den : 0.0f);
   }
 }
 
@@ -557,11 +578,9 @@ __device__ void prefix_merge(const Parts in, T* __restrict__ o, const Shape a, i
 TEENY_PREFIX_BF16_INST(64, 1)
 TEENY_PREFIX_BF16_INST(64, 2)
 TEENY_PREFIX_BF16_INST(64, 4)
-TEENY_PREFIX_BF16_INST(64, 8)
 TEENY_PREFIX_BF16_INST(128, 1)
 TEENY_PREFIX_BF16_INST(128, 2)
 TEENY_PREFIX_BF16_INST(128, 4)
-TEENY_PREFIX_BF16_INST(128, 8)
 
 #define TEENY_PREFIX_F32_INST(D)                                                               \
   extern "C" __global__ __launch_bounds__(64) void teeny_prefix_attn_f32_d##D(                 \
@@ -575,12 +594,12 @@ TEENY_PREFIX_F32_INST(32)
 TEENY_PREFIX_F32_INST(64)
 TEENY_PREFIX_F32_INST(128)
 
-extern "C" __global__ __launch_bounds__(256) void teeny_prefix_merge_bf16(Parts p, bf16* o, Shape a,
-                                                                          int head_dim,
-                                                                          int merged) {
-  prefix_merge<bf16>(p, o, a, head_dim, merged);
-}
-extern "C" __global__ __launch_bounds__(256) void teeny_prefix_merge_f32(Parts p, float* o, Shape a,
-                                                                         int head_dim, int merged) {
-  prefix_merge<float>(p, o, a, head_dim, merged);
-}
+#define TEENY_PREFIX_MERGE_INST(TN, T, SFX, TPR)                                               \
+  extern "C" __global__ __launch_bounds__(256) void teeny_prefix_merge_##TN##SFX(              \
+      Parts p, T* o, Shape a, int head_dim, int merged) {                                       \
+    prefix_merge<T, TPR>(p, o, a, head_dim, merged);                                            \
+  }
+TEENY_PREFIX_MERGE_INST(bf16, bf16, , 256)
+TEENY_PREFIX_MERGE_INST(bf16, bf16, _wave, 64)
+TEENY_PREFIX_MERGE_INST(f32, float, , 256)
+TEENY_PREFIX_MERGE_INST(f32, float, _wave, 64)
