@@ -1340,19 +1340,36 @@ struct PrefixPlan {
   long groups;   // of 32 (fp32: 16) rows of a sequence and kv head
 };
 PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_new, int n_prefix, int cache_len,
-                       int dtype) {
+                       int head_dim, int dtype) {
   PrefixPlan p{};
   const long gs = (long)(hq / hkv) * n_new, rows = batch * gs, cus = device_cus();
   const bool f32 = dtype == TEENY_F32;
-  const long blocks = (gs + 127) / 128 * batch * hkv;
-  p.fwd = !f32 && gs >= 64 && 2 * blocks >= cus;
+  // bf16: the forward kernel's walk over all keys by each 128-row block, or shares
+  // of the keys and a merge; estimated times in us (256 CUs), heads of 128:
+  //   forward  5 + 17.5 per 1000 keys, times the blocks per CU where over one
+  //   shares   10 + 0.9 per million (row, key) pairs + 1.2 per 1000 rows merged
+  // Measured, forward and shares, Hkv8 G4 D128, sequences x tokens behind keys:
+  // 1 x 512 behind 1000 33, 49, behind 16000 320, 264; 4 x 64 behind 1000 25, 28,
+  // behind 16000 308, 140; 8 x 32 behind 4000 74, 49; 8 x 64 76, 83; 8 x 128 89,
+  // 149; 16 x 16 70, 49; 32 x 4 71, 33; 16 x 32 behind 500 15, 39.
+  const double keys = (double)n_prefix + cache_len, per_d = head_dim / 128.0;
+  const double blocks = (double)((gs + 127) / 128) * batch * hkv;
+  const double fwd_us = 5 + 0.0175 * keys * per_d * std::max(1.0, 1.1 * blocks / cus);
+  const double shares_us = 10 + (0.9e-6 * keys * per_d + 1.2e-3) * rows * hkv * 256.0 / cus;
+  p.fwd = !f32 && fwd_us < shares_us;
   if (p.fwd) return p;
   const int unit = f32 ? 16 : 32;  // rows of a wavefront
   const long units = (rows + unit - 1) / unit;
   p.nw = f32 || units == 1 ? 1 : units == 2 ? 2 : 4;
   p.row_tiles = (int)((units + p.nw - 1) / p.nw);
   p.rows = (int)((units + p.row_tiles - 1) / p.row_tiles) * unit;  // even tiles
-  const long slots = cus * (f32 ? 4 : p.nw == 4 ? 2 : 3);
+  // Workgroups over the prefix.  More would be resident, but each leaves a share of
+  // its rows to write and merge, and the own keys' workgroups need room beside them.
+  // us of attention and merge at 3 (4 wavefronts: 2), 1.5 (1) and 0.75 (0.5) a CU,
+  // Hkv8 D128: 64 sequences behind 8191 47.7, 36.1, 47.9; 16 behind 2048 (2
+  // wavefronts) 15.4, 15.4, 14.5; 4 behind 32000 (1) 31.3, 31.4, 48.1; 5 tokens of 8
+  // behind 3001 27.3, 21.9, 23.6.
+  const long slots = f32 ? 4 * cus : p.nw == 4 ? cus : p.nw == 2 ? cus * 3 / 4 : cus * 3 / 2;
   if (n_prefix > 0) {
     const long want = std::max(1L, slots / ((long)p.row_tiles * hkv));
     const long per = ((n_prefix + want - 1) / want + 31) / 32 * 32;
@@ -1361,8 +1378,11 @@ PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_new, int n_prefix, int 
   }
   p.groups = (gs + (f32 ? 15 : 31)) / (f32 ? 16 : 32);
   const long items = (long)batch * hkv * p.groups;
-  const long most = (cache_len + 128L * p.nw - 1) / (128L * p.nw);
-  p.o_splits = (int)std::max(1L, std::min(std::min(most, 16L), slots / std::max(1L, items)));
+  // own keys: 64 a wavefront, until two workgroups a CU share them (us with 1, 2 and
+  // 4 a CU: 8 sequences of 4000 own keys 31.3, 27.2, 30.0; 2 of 2000, 16 heads of 64,
+  // 11.2, 9.6, 9.5; 128 keys a wavefront: 2 of 200 10.9, with 64 9.5)
+  const long most = (cache_len + 64L * p.nw - 1) / (64L * p.nw);
+  p.o_splits = (int)std::max(1L, std::min(std::min(most, 16L), 2 * cus / std::max(1L, items)));
   return p;
 }
 }  // namespace
@@ -1373,7 +1393,8 @@ size_t teeny_shared_prefix_attention_workspace_bytes(int batch, int n_heads_q, i
   if (batch <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0 ||
       n_new <= 0 || n_prefix < 0 || cache_len <= 0 || head_dim <= 0 || !dtype_ok(dtype))
     return 0;
-  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
+  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len,
+                                   head_dim, dtype);
   if (p.fwd) return 0;
   const size_t rows = (size_t)batch * n_heads_q * n_new * (p.p_splits + p.o_splits);
   return 2 * align256(rows * sizeof(float)) + align256(rows * head_dim * sizeof(float));
@@ -1401,7 +1422,8 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
   const uintptr_t at = (uintptr_t)q | (uintptr_t)o | (uintptr_t)k_cache | (uintptr_t)v_cache |
                        (n_prefix > 0 ? (uintptr_t)k_prefix | (uintptr_t)v_prefix : 0);
   if (at % (dtype == TEENY_BF16 ? 16 : 4) != 0) return TEENY_ERR_INVALID_VALUE;
-  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len, dtype);
+  const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len,
+                                   head_dim, dtype);
   char name[64];
   if (p.fwd) {
     int nq = n_heads_q / n_heads_kv * n_new, nmb = (nq + 127) / 128;

@@ -442,11 +442,15 @@ def test_shared_prefix_attention_validation(L):
                dict(s=65), dict(L=1 << 24), dict(lp=1 << 24), dict(b=1 << 25)):
         assert f(**kw) == SHAPE, kw
     for kw in (dict(host=-1), dict(host=64), dict(past=P, st=2), dict(scale=0.0), dict(q=P + 2),
-               dict(o=P + 8), dict(kp=P + 4), dict(ws=P + 8), dict(scale=float("inf"))):
+               dict(o=P + 8), dict(kp=P + 4), dict(scale=float("inf"))):
         assert f(**kw) == VALUE, kw
     assert f(q=P + 2, dtype=F32) == VALUE
-    need = L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 100, 64, 64, BF16)
-    assert need > 0 and f(wsb=need - 1) == WS and f(ws=None) == WS
+    # (few keys need none)
+    assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 100, 64, 64, BF16) == 0
+    need = L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 100, 3000, 64, BF16)
+    assert need > 0 and f(L=3000, wsb=need - 1) == WS and f(L=3000, ws=None) == WS
+    assert f(L=3000, ws=P + 8) == VALUE
+    assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 100, 64, 64, F32) > 0
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 3, 2, 1, 100, 64, 64, BF16) == 0
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, -1, 64, 64, BF16) == 0
 

@@ -108,11 +108,25 @@ SHAPES = [
 ]
 
 
+# A longer cache (never read past its used rows) is what makes bf16 share few rows'
+# keys out; short ones run the forward kernel over them.
+LONGER = pytest.mark.parametrize("longer", [0, 3000], ids=["", "long"])
+
+
+@LONGER
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("shape", SHAPES, ids=[str(s[:7]) for s in SHAPES])
-def test_against_definition(cuda, dtype, shape):
+def test_against_definition(cuda, dtype, shape, longer):
     B, Hq, Hkv, S, D, P, L, past = shape
-    check(make(cuda, dtype, B, Hq, Hkv, S, D, P, L, prefix_len=P + 3), P, past, S)
+    check(make(cuda, dtype, B, Hq, Hkv, S, D, P, L + longer, prefix_len=P + 3), P, past, S)
+
+
+def test_both_ways_are_tested(cuda):
+    """Of the shapes above, in bf16, some run the forward kernel and some share keys."""
+    need = ops._lib.lib().teeny_shared_prefix_attention_workspace_bytes
+    kinds = {(longer, need(B, Hq, Hkv, S, P, L + longer, D, 1) > 0)
+             for B, Hq, Hkv, S, D, P, L, _ in SHAPES for longer in (0, 3000)}
+    assert {(0, False), (3000, True), (3000, False)} <= kinds
 
 
 @pytest.mark.parametrize("D", [8, 16, 32])
@@ -121,17 +135,19 @@ def test_f32_small_heads(cuda, D, S):
     check(make(cuda, F32, 3, 6, 3, S, D, 45, 60), 45, [0, 7, 60 - S], S)
 
 
+@LONGER
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("P", [31, 32, 33, 63, 64, 65, 95, 127, 128, 129, 1000])
-def test_prefix_lengths(cuda, dtype, P):
-    check(make(cuda, dtype, 2, 8, 2, 1, 64, P, 34, seed=P), P, [0, 33], 1)
+def test_prefix_lengths(cuda, dtype, P, longer):
+    check(make(cuda, dtype, 2, 8, 2, 1, 64, P, 34 + longer, seed=P), P, [0, 33], 1)
 
 
+@LONGER
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("past", [0, 30, 31, 32, 62, 63, 64, 400, 2000])
-def test_past_lengths(cuda, dtype, past):
+def test_past_lengths(cuda, dtype, past, longer):
     """One length for all, given by the host and by one device value."""
-    ts = make(cuda, dtype, 3, 8, 2, 1, 128, 40, past + 1, seed=past)
+    ts = make(cuda, dtype, 3, 8, 2, 1, 128, 40, past + 1 + longer, seed=past)
     a = check(ts, 40, [past] * 3, 1, as_tensor=False)
     one = torch.tensor([past], dtype=torch.int32, device="cuda")
     b = ops.shared_prefix_attention(*ts, 40, one)
@@ -143,9 +159,10 @@ def test_rows_that_see_nothing_and_past_the_cache(cuda, dtype):
     """Device lengths that leave no key (zeros), some rows without a key, and rows
     past the cache's end (the whole cache); few rows, and as many as the forward
     kernel takes."""
-    for B, Hkv, S, D in ((4, 2, 3, 64), (4, 32, 64, 64), (8, 16, 64, 128)):
-        q, kp, vp, k, v = make(cuda, dtype, B, 2 * Hkv, Hkv, S, D, 1, S + 32)
-        past = [-S, 1 - S, S + 32, -100] * (B // 4)
+    for B, Hkv, S, D, L in ((4, 2, 3, 64, 35), (4, 2, 3, 128, 3000), (4, 2, 40, 64, 3000),
+                            (8, 16, 64, 128, 96)):
+        q, kp, vp, k, v = make(cuda, dtype, B, 2 * Hkv, Hkv, S, D, 1, L)
+        past = [-S, 1 - S, L, -100] * (B // 4)
         want, tol = reference(q, kp, vp, k, v, 0, past, 0.125)
         n = torch.tensor(past, dtype=torch.int32, device="cuda")
         got = ops.shared_prefix_attention(q, kp[:, :0], vp[:, :0], k, v, 0, n, 0.125)
@@ -158,8 +175,8 @@ def test_rows_that_see_nothing_and_past_the_cache(cuda, dtype):
 def test_large_scores_and_offsets(cuda, dtype):
     """Scores far from zero, the largest in either part: one softmax over both
     (exponents past the forward kernel's 2^31 above its first tile among them)."""
-    for B, Hkv, S in ((3, 2, 1), (16, 16, 32)):
-        ts = make(cuda, dtype, B, 2 * Hkv, Hkv, S, 64, 90, 49 + S)
+    for B, Hkv, S, longer in ((3, 2, 1, 0), (3, 2, 1, 3000), (16, 16, 32, 0)):
+        ts = make(cuda, dtype, B, 2 * Hkv, Hkv, S, 64, 90, 49 + S + longer)
         q, kp, vp, k, v = ts
         q.mul_(8.0)
         k[1] *= 3.0
@@ -168,10 +185,11 @@ def test_large_scores_and_offsets(cuda, dtype):
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@LONGER
 @pytest.mark.parametrize("B,S", [(3, 1), (3, 3), (3, 40), (66, 40)])
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-def test_merged_layout(cuda, dtype, B, S, D):
-    ts = make(cuda, dtype, B, 8, 2, S, D, 77, 60)
+def test_merged_layout(cuda, dtype, B, S, D, longer):
+    ts = make(cuda, dtype, B, 8, 2, S, D, 77, 60 + longer)
     past = torch.tensor([0, 5, 60 - S] * (B // 3), dtype=torch.int32, device="cuda")
     a = ops.shared_prefix_attention(*ts, 77, past)
     b = ops.shared_prefix_attention(*ts, 77, past, merged=True)
@@ -231,10 +249,11 @@ def test_offsets_past_32_bits(cuda):
     assert ((got[0, :, 0].double() - want).abs() <= A * (4 * 2.0 ** -8 + 2.0 ** -8)).all()
 
 
+@LONGER
 @pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
-def test_captured_and_replayed(cuda, dtype):
+def test_captured_and_replayed(cuda, dtype, longer):
     """The lengths are read at replay."""
-    ts = make(cuda, dtype, 4, 8, 2, 1, 64, 300, 90)
+    ts = make(cuda, dtype, 4, 8, 2, 1, 64, 300, 90 + longer)
     n = torch.zeros(4, dtype=torch.int32, device="cuda")
     out = torch.zeros_like(ts[0])
     ops.shared_prefix_attention(*ts, 300, n, out=out)
@@ -279,10 +298,12 @@ def test_refusals(cuda):
             f(*args)
     with pytest.raises(ValueError):
         f(*ts, 10, 0, out=torch.empty_like(q).float())
-    for kw, text in [(dict(softmax_scale=0.0), "value|domain|-7"), (dict(softmax_scale=NAN), "-7"),
-                     (dict(workspace=torch.empty(8, dtype=torch.uint8, device="cuda")), "workspace")]:
-        with pytest.raises(Exception, match=text):
+    for kw in (dict(softmax_scale=0.0), dict(softmax_scale=NAN)):
+        with pytest.raises(Exception, match="-7"):
             f(*ts, 10, 0, **kw)
+    with pytest.raises(Exception, match="workspace"):
+        f(*make(cuda, BF, 2, 4, 2, 2, 64, 10, 3000), 10, 0,
+          workspace=torch.empty(8, dtype=torch.uint8, device="cuda"))
     odd = torch.empty(q.numel() + 1, dtype=BF, device="cuda")[1:].view(q.shape)
     with pytest.raises(Exception, match="-7"):
         f(odd, kp, vp, k, v, 10, 0)
