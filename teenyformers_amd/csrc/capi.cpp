@@ -1334,7 +1334,7 @@ struct FwdPrefix {  // in fa2_fwd_bf16.hip
   int past_stride, past_imm;
 };
 struct PrefixPlan {
-  bool fwd;      // the forward kernel, without shares
+  bool fwd;      // without shares: the forward kernel, or (fp32) whole walks
   int nw, rows;  // wavefronts per workgroup, rows per row tile
   int row_tiles, p_splits, p_keys, o_splits;
   long groups;   // of 32 (fp32: 16) rows of a sequence and kv head
@@ -1356,9 +1356,15 @@ PrefixPlan prefix_plan(int batch, int hq, int hkv, int n_new, int n_prefix, int 
   const double blocks = (double)((gs + 127) / 128) * batch * hkv;
   const double fwd_us = 5 + 0.0175 * keys * per_d * std::max(1.0, 1.1 * blocks / cus);
   const double shares_us = 10 + (0.9e-6 * keys * per_d + 1.2e-3) * rows * hkv * 256.0 / cus;
-  p.fwd = !f32 && fwd_us < shares_us;
-  if (p.fwd) return p;
   const int unit = f32 ? 16 : 32;  // rows of a wavefront
+  // fp32: a walk over all keys takes 1.7 us per 32 of them but no second launch; with
+  // four wavefronts a CU of whole 16-row tiles it also saves the shares' traffic.
+  // us, whole and shares: 4 sequences of 4 heads of 64 behind 61 + 9 keys 7.8, 8.3,
+  // behind 200 15.4, 8.4; 8 x 128 tokens, Hq16 Hkv8 D64, behind 500 42, 66 (1024
+  // wavefronts); 2 x 512, 8 heads, behind 2000 134, 77 (512).
+  const long walks = (gs + unit - 1) / unit * batch * hkv;
+  p.fwd = f32 ? keys <= 128 || (gs >= unit && walks >= 4 * cus) : fwd_us < shares_us;
+  if (p.fwd) return p;
   const long units = (rows + unit - 1) / unit;
   p.nw = f32 || units == 1 ? 1 : units == 2 ? 2 : 4;
   p.row_tiles = (int)((units + p.nw - 1) / p.nw);
@@ -1425,6 +1431,17 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
   const PrefixPlan p = prefix_plan(batch, n_heads_q, n_heads_kv, n_new, n_prefix, cache_len,
                                    head_dim, dtype);
   char name[64];
+  if (p.fwd && dtype == TEENY_F32) {
+    const int gs = n_heads_q / n_heads_kv * n_new;
+    const long wgs = (long)(gs + 15) / 16 * batch * n_heads_kv;
+    if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+    PrefixShape a{batch,     n_heads_kv, gs,            n_new,       n_prefix, prefix_len,
+                  cache_len, n_past,     n_past_stride, n_past_host, 0,        0,
+                  0,         0,          1,             softmax_scale};
+    snprintf(name, sizeof name, "teeny_prefix_attn_f32_d%d_whole", head_dim);
+    void* args[] = {&q, &k_prefix, &v_prefix, &k_cache, &v_cache, &a, &o, &merged};
+    return launch(name, dim3((unsigned)wgs), dim3(64), 0, stream, args);
+  }
   if (p.fwd) {
     int nq = n_heads_q / n_heads_kv * n_new, nmb = (nq + 127) / 128;
     const long total = (long)nmb * batch * n_heads_kv;

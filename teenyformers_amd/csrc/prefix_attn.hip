@@ -350,29 +350,36 @@ __device__ void prefix_attn(const bf16* __restrict__ q, const bf16* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// fp32: a wavefront per 16 rows and share of the keys, on the fp32 matrix cores,
-// K and V read straight from memory in operand order (as the fp32 decode kernel
-// does); grid: p_splits * row_tiles * hkv, then o_splits * batch * hkv * ceil(gs / 16).
+// fp32: a wavefront per 16 rows, on the fp32 matrix cores, K and V read straight
+// from memory in operand order (as the fp32 decode kernel does).
+//   shares  grid p_splits * row_tiles * hkv, then o_splits * batch * hkv *
+//           ceil(gs / 16): a share of one part's keys, to the merge
+//   whole   grid batch * hkv * ceil(gs / 16): all keys of a sequence's rows, both
+//           parts one after the other, to the output: few keys, or many rows
 // ---------------------------------------------------------------------------
-template <int D>
+template <int D, bool WHOLE>
 __device__ void prefix_attn_f32(const float* __restrict__ q, const float* __restrict__ kp,
                                 const float* __restrict__ vp, const float* __restrict__ kc,
-                                const float* __restrict__ vc, const Shape a, const Parts out) {
+                                const float* __restrict__ vc, const Shape a, const Parts out,
+                                float* __restrict__ o, int merged) {
   constexpr int NC = Geo<D>::NC, VW = Geo<D>::VW, NH = Geo<D>::NH;
   const int lane = threadIdx.x, j = lane & 15, g = lane >> 4;
   const long n_rows = (long)a.batch * a.hkv * a.gs;
-  const int n_pre = a.p_splits * a.row_tiles * a.hkv;
+  const int n_share = WHOLE ? 0 : a.p_splits * a.row_tiles * a.hkv;
   const float *kb, *vb, *qrow;
   long prow;           // the lane's row among the partials
   bool valid;
-  int k0, k1, lim;     // the share's keys; the lane's end
-  if ((int)blockIdx.x < n_pre) {
-    int id = xcd_remap(blockIdx.x, n_pre);
+  int k0, k1, lim;     // the keys of the walk; the lane's end
+  int hk, b = 0, rem = 0, past = 0;
+  if ((int)blockIdx.x < n_share) {
+    int id = xcd_remap(blockIdx.x, n_share);
     const int rt = id % a.row_tiles;
     id /= a.row_tiles;
-    const int hk = id % a.hkv, split = id / a.hkv;
+    hk = id % a.hkv;
+    const int split = id / a.hkv;
     const int rows = a.batch * a.gs, r = rt * 16 + j;
-    const int rc = min(r, rows - 1), b = rc / a.gs;
+    const int rc = min(r, rows - 1);
+    b = rc / a.gs;
     valid = r < rows;
     qrow = q + ((long)(b * a.hkv + hk) * a.gs + (rc - b * a.gs)) * D;
     kb = kp + (long)hk * a.prefix_len * D;
@@ -382,22 +389,24 @@ __device__ void prefix_attn_f32(const float* __restrict__ q, const float* __rest
     lim = k1;
     prow = split * n_rows + (long)hk * rows + rc;
   } else {
-    const int groups = (a.gs + 15) / 16;
-    int id = blockIdx.x - n_pre;
-    const int split = id % a.o_splits;
-    id /= a.o_splits;
+    const int groups = (a.gs + 15) / 16, splits = WHOLE ? 1 : a.o_splits;
+    int id = blockIdx.x - n_share;
+    const int split = id % splits;
+    id /= splits;
     const int rg = id % groups;
     id /= groups;
-    const int hk = id % a.hkv, b = id / a.hkv;
-    const int past = past_of(a, b);
-    const int rem = min(rg * 16 + j, a.gs - 1);
+    // (whole: kv head by kv head, for the prefix in an XCD's L2)
+    hk = WHOLE ? id / a.batch : id % a.hkv;
+    b = WHOLE ? id - hk * a.batch : id / a.hkv;
+    past = past_of(a, b);
+    rem = min(rg * 16 + j, a.gs - 1);
     valid = rg * 16 + j < a.gs;
     const long row0 = (long)(b * a.hkv + hk) * a.gs;
     qrow = q + (row0 + rem) * D;
     kb = kc + (long)(b * a.hkv + hk) * a.cache_len * D;
     vb = vc + (long)(b * a.hkv + hk) * a.cache_len * D;
     const int n_keys = min(past + a.s, a.cache_len);
-    const int per = ((n_keys + a.o_splits - 1) / a.o_splits + TK - 1) / TK * TK;
+    const int per = ((n_keys + splits - 1) / splits + TK - 1) / TK * TK;
     k0 = split * per;
     k1 = min(k0 + per, n_keys);
     lim = min(past + rem % a.s + 1, k1);
@@ -408,81 +417,99 @@ __device__ void prefix_attn_f32(const float* __restrict__ q, const float* __rest
   f32x4 acc[NH][VW];
   zero_acc<D>(acc);
   float m = -INFINITY, l = 0.0f;
-  for (int t0 = k0; t0 < k1; t0 += 32) {
-    // rows at or past k1 re-read row k1 - 1; their P is zero, and so is their V
-    f32x4 kf[2][NC];
-    float vf[8][NH][VW];
+  // whole: the prefix first, then (kb, vb, k0, k1, lim)
+  for (int part = WHOLE && a.n_prefix > 0 ? 0 : 1; part < 2; ++part) {
+    const bool pre = WHOLE && part == 0;
+    const float* ks = pre ? kp + (long)hk * a.prefix_len * D : kb;
+    const float* vs = pre ? vp + (long)hk * a.prefix_len * D : vb;
+    const int end = pre ? a.n_prefix : k1, stop = pre ? end : lim;
+    for (int t0 = pre ? 0 : k0; t0 < end; t0 += 32) {
+      // rows at or past the end re-read the last; their P is zero, and so is their V
+      f32x4 kf[2][NC];
+      float vf[8][NH][VW];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) row_regs<D>(kb + (long)min(t0 + 16 * u + j, k1 - 1) * D, g, kf[u]);
+      for (int u = 0; u < 2; ++u)
+        row_regs<D>(ks + (long)min(t0 + 16 * u + j, end - 1) * D, g, kf[u]);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const float* row = vb + (long)min(t0 + 16 * (s >> 2) + 4 * g + (s & 3), k1 - 1) * D;
+      for (int s = 0; s < 8; ++s) {
+        const float* row = vs + (long)min(t0 + 16 * (s >> 2) + 4 * g + (s & 3), end - 1) * D;
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        if constexpr (VW == 4) {
-          const f32x4 x = *reinterpret_cast<const f32x4g*>(row + 64 * h + 4 * j);
+        for (int h = 0; h < NH; ++h) {
+          if constexpr (VW == 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4g*>(row + 64 * h + 4 * j);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) vf[s][h][e] = x[e];
-        } else if constexpr (VW == 2) {
-          const f32x2 x = *reinterpret_cast<const f32x2g*>(row + 2 * j);
-          vf[s][h][0] = x[0];
-          vf[s][h][1] = x[1];
-        } else {
-          vf[s][h][0] = D == 8 && j >= 8 ? 0.0f : row[j];
+            for (int e = 0; e < 4; ++e) vf[s][h][e] = x[e];
+          } else if constexpr (VW == 2) {
+            const f32x2 x = *reinterpret_cast<const f32x2g*>(row + 2 * j);
+            vf[s][h][0] = x[0];
+            vf[s][h][1] = x[1];
+          } else {
+            vf[s][h][0] = D == 8 && j >= 8 ? 0.0f : row[j];
+          }
         }
       }
-    }
-    __builtin_amdgcn_sched_barrier(0);  // every load is issued first
-    f32x4 s[2] = {};
+      __builtin_amdgcn_sched_barrier(0);  // every load is issued first
+      f32x4 s[2] = {};
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s[u] = mfma4(kf[u][c][e], qf[c][e], s[u]);
-    float mx = -INFINITY;
-    const float m_old = m;
+          for (int u = 0; u < 2; ++u) s[u] = mfma4(kf[u][c][e], qf[c][e], s[u]);
+      float mx = -INFINITY;
+      const float m_old = m;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[u][r] = t0 + 16 * u + 4 * g + r < lim ? s[u][r] * a.scale : -INFINITY;
-        mx = fmaxf(mx, s[u][r]);
-      }
-    m = fmaxf(m, max_g(mx));
-    const float ref = m == -INFINITY ? 0.0f : m;  // no key of the row so far
-    const float alpha = expf(m_old - ref);
-    l *= alpha;
+        for (int r = 0; r < 4; ++r) {
+          s[u][r] = t0 + 16 * u + 4 * g + r < stop ? s[u][r] * a.scale : -INFINITY;
+          mx = fmaxf(mx, s[u][r]);
+        }
+      m = fmaxf(m, max_g(mx));
+      const float ref = m == -INFINITY ? 0.0f : m;  // no key of the row so far
+      const float alpha = expf(m_old - ref);
+      l *= alpha;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[u][r] = expf(s[u][r] - ref);
-        l += s[u][r];
-      }
-#pragma unroll
-    for (int h = 0; h < NH; ++h)
-#pragma unroll
-      for (int e = 0; e < VW; ++e) acc[h][e] *= alpha;
-    if (t0 + 32 > k1) {
-#pragma unroll
-      for (int x = 0; x < 8; ++x)
-        if (t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= k1)
-#pragma unroll
-          for (int h = 0; h < NH; ++h)
-#pragma unroll
-            for (int e = 0; e < VW; ++e) vf[x][h][e] = 0.0f;
-    }
-#pragma unroll
-    for (int x = 0; x < 8; ++x)
+        for (int r = 0; r < 4; ++r) {
+          s[u][r] = expf(s[u][r] - ref);
+          l += s[u][r];
+        }
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
-        for (int e = 0; e < VW; ++e)
-          acc[h][e] = mfma4(vf[x][h][e], s[x >> 2][x & 3], acc[h][e]);
+        for (int e = 0; e < VW; ++e) acc[h][e] *= alpha;
+      if (t0 + 32 > end) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if (t0 + 16 * (x >> 2) + 4 * g + (x & 3) >= end)
+#pragma unroll
+            for (int h = 0; h < NH; ++h)
+#pragma unroll
+              for (int e = 0; e < VW; ++e) vf[x][h][e] = 0.0f;
+      }
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int e = 0; e < VW; ++e)
+            acc[h][e] = mfma4(vf[x][h][e], s[x >> 2][x & 3], acc[h][e]);
+    }
   }
   l = sum_g(l);
   if (!valid) return;
+  if constexpr (WHOLE) {
+    long to = ((long)(b * a.hkv + hk) * a.gs + rem) * D;
+    if (merged) {
+      const int group = a.gs / a.s, h = hk * group + rem / a.s, t = rem % a.s;
+      to = (((long)b * a.s + t) * a.hkv * group + h) * D;
+    }
+    // a row without a key: zeros (l NaN: NaN)
+    store_col<D>(o + to, acc, g, [l](float x) { return l == 0.0f ? 0.0f : x / l; });
+    return;
+  }
   if (g == 0) {
     out.m[prow] = m * kLog2e;
     out.l[prow] = l;
@@ -563,7 +590,7 @@ __device__ void prefix_merge(const Parts in, T* __restrict__ o, const Shape a, i
   for (int dd = tid; dd < head_dim && want < n_rows; dd += TPR) {
     float v = 0.0f;
     for (int i = 0; i < groups; ++i) v += sums[i * head_dim + dd];
-    o[to + dd] = (T)(den > 0.0f ? v / den : 0.0f);
+    o[to + dd] = (T)(den == 0.0f ? 0.0f : v / den);
   }
 }
 
@@ -586,7 +613,12 @@ TEENY_PREFIX_BF16_INST(128, 4)
   extern "C" __global__ __launch_bounds__(64) void teeny_prefix_attn_f32_d##D(                 \
       const float* q, const float* kp, const float* vp, const float* kc, const float* vc,      \
       Shape a, Parts p) {                                                                       \
-    prefix_attn_f32<D>(q, kp, vp, kc, vc, a, p);                                               \
+    prefix_attn_f32<D, false>(q, kp, vp, kc, vc, a, p, nullptr, 0);                            \
+  }                                                                                             \
+  extern "C" __global__ __launch_bounds__(64) void teeny_prefix_attn_f32_d##D##_whole(         \
+      const float* q, const float* kp, const float* vp, const float* kc, const float* vc,      \
+      Shape a, float* o, int merged) {                                                          \
+    prefix_attn_f32<D, true>(q, kp, vp, kc, vc, a, {}, o, merged);                             \
   }
 TEENY_PREFIX_F32_INST(8)
 TEENY_PREFIX_F32_INST(16)

@@ -620,9 +620,11 @@ def decode_qkv_attention(qkv: "Partials", k_cache, v_cache, n_past, n_heads_q: i
 def _on_device_of(t: torch.Tensor):
     """The context in which a call on t runs: t's device current (its current
     stream then is the one that _stream gives)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    here = torch.cuda.current_device() if _current_device is None else _current_device()
+    return _no_context if t.get_device() == here else torch.cuda.device(t.device)
+
+
+_no_context = contextlib.nullcontext()
 
 
 def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: int, n_past,
@@ -639,32 +641,34 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: i
     graphs).  Returns o in q's shape, or with merged [B, S, Hq*D].  No gradients.
     workspace: uint8, teeny_shared_prefix_attention_workspace_bytes, that no call
     on another stream uses at the same time; by default a fresh one."""
-    if q.dim() not in (3, 4):
+    shape = q.shape
+    if len(shape) not in (3, 4):
         raise ValueError("shared_prefix_attention: q is [B, Hq, D] or [B, Hq, S, D]")
     if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4:
         k_prefix, v_prefix = k_prefix[0], v_prefix[0]
-    _dev(q, k_prefix, v_prefix, k_cache, v_cache, out, workspace)
-    B, Hq, D = q.shape[0], q.shape[1], q.shape[-1]
-    S = q.shape[2] if q.dim() == 4 else 1
-    if (k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[0] != B
-            or k_cache.shape[3] != D):
+    B, Hq, D = shape[0], shape[1], shape[-1]
+    S = shape[2] if len(shape) == 4 else 1
+    dtype, dev = q.dtype, q.get_device()
+    for t in (q, k_prefix, v_prefix, k_cache, v_cache):
+        if t.dtype != dtype:
+            raise TypeError("shared_prefix_attention: q, the prefix and the caches share a dtype")
+        if t.get_device() != dev or dev < 0:
+            raise ValueError("shared_prefix_attention: all tensors are on one device, a GPU")
+        if not t.is_contiguous():
+            raise ValueError("teenyformers_amd ops take contiguous tensors")
+    kc, kp = k_cache.shape, k_prefix.shape
+    if len(kc) != 4 or kc != v_cache.shape or kc[0] != B or kc[3] != D:
         raise ValueError("shared_prefix_attention: the caches are [B, Hkv, L, D] matching q")
-    Hkv, L = k_cache.shape[1], k_cache.shape[2]
-    if (k_prefix.dim() != 3 or k_prefix.shape != v_prefix.shape or k_prefix.shape[0] != Hkv
-            or k_prefix.shape[2] != D):
+    Hkv, L = kc[1], kc[2]
+    if len(kp) != 3 or kp != v_prefix.shape or kp[0] != Hkv or kp[2] != D:
         raise ValueError("shared_prefix_attention: the prefix is [Hkv, Lp, D] matching the caches")
-    ts = (k_prefix, v_prefix, k_cache, v_cache)
-    if any(t.dtype != q.dtype for t in ts):
-        raise TypeError("shared_prefix_attention: q, the prefix and the caches share a dtype")
-    if any(t.device != q.device for t in ts):
-        raise ValueError("shared_prefix_attention: all tensors are on one device")
-    if not 0 <= n_prefix <= k_prefix.shape[1]:
+    if not 0 <= n_prefix <= kp[1]:
         raise ValueError("shared_prefix_attention: n_prefix must lie in the prefix's rows")
     code = _code(q)
     past, stride, past_host = None, 0, 0
     if isinstance(n_past, torch.Tensor):
-        if (n_past.dtype != torch.int32 or n_past.device != q.device or not n_past.is_contiguous()
-                or n_past.numel() not in (1, B)):
+        if (n_past.dtype != torch.int32 or n_past.get_device() != dev
+                or not n_past.is_contiguous() or n_past.numel() not in (1, B)):
             raise TypeError("n_past must be an int, or an int32 tensor of one value or one per "
                             "sequence on q's device")
         past, stride = n_past, int(n_past.numel() == B)
@@ -674,22 +678,24 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: i
             raise ValueError("shared_prefix_attention: rows n_past .. n_past + S - 1 must lie in "
                              "the cache")
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    shape = (B, S, Hq * D) if merged else tuple(q.shape)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
-    elif tuple(out.shape) != shape or out.dtype != q.dtype or out.device != q.device:
-        raise ValueError(f"shared_prefix_attention: out must be {shape} of q's type and device")
+        out = torch.empty((B, S, Hq * D) if merged else shape, dtype=dtype, device=q.device)
+    elif (out.shape != ((B, S, Hq * D) if merged else shape) or out.dtype != dtype
+          or out.get_device() != dev or not out.is_contiguous()):
+        raise ValueError("shared_prefix_attention: out must be contiguous, of the result's shape, "
+                         "type and device")
     if workspace is None:
         need = _lib.lib().teeny_shared_prefix_attention_workspace_bytes(B, Hq, Hkv, S, n_prefix, L, D,
                                                                         code)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.device != q.device:
-        raise ValueError("shared_prefix_attention: workspace must be on q's device")
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("shared_prefix_attention: workspace must be contiguous, on q's device")
+    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
     with _on_device_of(q):
         call("teeny_shared_prefix_attention", _p(q), _p(k_prefix), _p(v_prefix), _p(k_cache),
-             _p(v_cache), _p(out), B, Hq, Hkv, S, n_prefix, k_prefix.shape[1], _p(past), stride,
-             past_host, L, D, scale, int(bool(merged)), code, _p(workspace),
-             workspace.numel() * workspace.element_size(), _stream())
+             _p(v_cache), _p(out), B, Hq, Hkv, S, n_prefix, kp[1], _p(past), stride, past_host, L, D,
+             scale, int(bool(merged)), code, _p(workspace), size, _stream())
     return out
 
 
@@ -711,11 +717,11 @@ def argmax_rows(x, out=None, advance=None):
     return out
 
 
-def _per_row(name: str, value, rows: int, dtype, like: torch.Tensor):
+def _per_row(name: str, value, rows: int, dtype, device: int):
     """A sampling setting as (number, device tensor or None)."""
     if not isinstance(value, torch.Tensor):
         return value, None
-    if (value.dtype != dtype or value.numel() != rows or value.device != like.device
+    if (value.dtype != dtype or value.numel() != rows or value.get_device() != device
             or not value.is_contiguous()):
         raise ValueError(f"sample_rows: {name} is a number or a contiguous {dtype} tensor with a "
                          "value per row, on the logits' device")
@@ -743,30 +749,36 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
     apart (a slice of padded columns) or be one row (expand).  advance: as
     argmax_rows.  workspace: teeny_sample_rows_workspace_bytes bytes (uint8) that
     no call on another stream uses at the same time; by default a fresh one."""
-    if not logits.is_cuda:
+    dev = logits.get_device()
+    if dev < 0:
         raise ValueError("teenyformers_amd ops take device tensors (no CPU fallback)")
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("sample_rows: logits are [..., V] with V >= 1")
     code = _code(logits)
-    shape, V = logits.shape[:-1], logits.shape[-1]
+    V = logits.shape[-1]
     x = logits if logits.dim() == 2 else logits.reshape(-1, V)
-    if x.stride(1) != 1 and V > 1 or 0 < x.stride(0) < V:
+    ld = x.stride(0)
+    if x.stride(1) != 1 and V > 1 or 0 < ld < V:
         x = x.contiguous()
+        ld = V
     rows = x.shape[0]
-    _dev(u, out, advance, workspace)
-    if u.dtype != torch.float32 or u.numel() != rows or u.device != x.device:
-        raise ValueError("sample_rows: u is fp32 with a value per row, on the logits' device")
+    if (u.dtype != torch.float32 or u.numel() != rows or u.get_device() != dev
+            or not u.is_contiguous()):
+        raise ValueError("sample_rows: u is fp32 with a value per row, contiguous on the logits' "
+                         "device")
     if out is None:
-        out = torch.empty(shape, dtype=torch.int64, device=x.device)
-    elif out.dtype != torch.int64 or out.numel() != rows or out.device != x.device:
-        raise ValueError("sample_rows: out is int64 with a value per row, on the logits' device")
+        out = torch.empty(logits.shape[:-1], dtype=torch.int64, device=x.device)
+    elif (out.dtype != torch.int64 or out.numel() != rows or out.get_device() != dev
+          or not out.is_contiguous()):
+        raise ValueError("sample_rows: out is int64 with a value per row, contiguous on the logits' "
+                         "device")
     if advance is not None and (advance.dtype != torch.int32 or advance.numel() != 1
-                                or advance.device != x.device):
+                                or advance.get_device() != dev):
         raise ValueError("sample_rows: advance is one int32 on the logits' device")
-    t, ts = _per_row("temperature", temperature, rows, torch.float32, x)
-    k, ks = _per_row("top_k", top_k, rows, torch.int32, x)
-    p, ps = _per_row("top_p", top_p, rows, torch.float32, x)
-    m, ms = _per_row("min_p", min_p, rows, torch.float32, x)
+    t, ts = _per_row("temperature", temperature, rows, torch.float32, dev)
+    k, ks = _per_row("top_k", top_k, rows, torch.int32, dev)
+    p, ps = _per_row("top_p", top_p, rows, torch.float32, dev)
+    m, ms = _per_row("min_p", min_p, rows, torch.float32, dev)
     if ts is None and not t >= 0.0:
         raise ValueError("sample_rows: temperature must be at least 0")
     if ks is None and k < 0:
@@ -777,16 +789,17 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
         raise ValueError("sample_rows: min_p must be in [0, 1]")
     if rows == 0:
         return out
-    need = _lib.lib().teeny_sample_rows_workspace_bytes(rows, V)
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    elif workspace.device != x.device:
-        raise ValueError("sample_rows: workspace must be on the logits' device")
+        size = _lib.lib().teeny_sample_rows_workspace_bytes(rows, V)
+        workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("sample_rows: workspace must be contiguous, on the logits' device")
+    else:
+        size = workspace.numel() * workspace.element_size()
     with _on_device_of(x):
-        call("teeny_sample_rows", _p(x), x.stride(0) if rows > 1 else V, _p(u), rows, V, float(t),
+        call("teeny_sample_rows", _p(x), ld if rows > 1 else V, _p(u), rows, V, float(t),
              _p(ts), min(int(k), 2 ** 31 - 1), _p(ks), float(p), _p(ps), float(m), _p(ms), _p(out),
-             code, _p(advance), _p(workspace), workspace.numel() * workspace.element_size(),
-             _stream())
+             code, _p(advance), _p(workspace), size, _stream())
     return out
 
 

@@ -451,6 +451,7 @@ def test_shared_prefix_attention_validation(L):
     assert need > 0 and f(L=3000, wsb=need - 1) == WS and f(L=3000, ws=None) == WS
     assert f(L=3000, ws=P + 8) == VALUE
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 100, 64, 64, F32) > 0
+    assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, 30, 64, 64, F32) == 0
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 3, 2, 1, 100, 64, 64, BF16) == 0
     assert L.teeny_shared_prefix_attention_workspace_bytes(2, 4, 2, 1, -1, 64, 64, BF16) == 0
 

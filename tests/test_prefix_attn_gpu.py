@@ -129,10 +129,19 @@ def test_both_ways_are_tested(cuda):
     assert {(0, False), (3000, True), (3000, False)} <= kinds
 
 
-@pytest.mark.parametrize("D", [8, 16, 32])
+@pytest.mark.parametrize("D", [8, 16, 32, 64, 128])
+@pytest.mark.parametrize("P,L", [(45, 300), (20, 60), (0, 21)])
 @pytest.mark.parametrize("S", [1, 4, 21])
-def test_f32_small_heads(cuda, D, S):
-    check(make(cuda, F32, 3, 6, 3, S, D, 45, 60), 45, [0, 7, 60 - S], S)
+def test_f32_head_dims(cuda, D, S, P, L):
+    """Shares of the keys, and whole walks over few of them."""
+    check(make(cuda, F32, 3, 6, 3, S, D, P, L), P, [0, 7 if L > 40 else 0, L - S], S)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_f32_many_rows(cuda, D):
+    """Whole walks because rows fill the device, over many keys."""
+    past = [0, 3, 50, 31] * 8
+    check(make(cuda, F32, 32, 16, 16, 32, D, 150, 90), 150, past, 32)
 
 
 @LONGER
