@@ -296,17 +296,29 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
   const int counted = s.fk && !s.few ? kBins : kFirstBins;
   int bin[kTok];
   uint32_t rank[kTok];
+  // Most tokens of a small top-k, or of min-p alone, lie below any that counts: those
+  // under `floor_x` are left by one fp32 comparison (a margin of 1e-6 below the
+  // border that fp64 decides).
+  const double top = floor((double)mx * q4);
+  const float edge = (float)(s.few ? (top - (kFirstBins - 1)) / q4 : least / s.c);
+  const float floor_x = fabsf(edge) < 1e37f ? edge - 1e-6f * fabsf(edge) - 1e-37f : -INFINITY;
+  auto place = [&](int j, u64* w) __attribute__((always_inline)) {
+    int b = bin_of(x[j], mx, q4, w);
+    if (mx == -INFINITY || ((double)x[j] * s.c < least && x[j] != mx)) b = kBins;
+    return b;
+  };
   auto tokens = [&](auto weighs) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
+      bin[j] = kBins;
+      if (!decltype(weighs)::value && !(x[j] >= floor_x)) continue;
       u64 w;
-      bin[j] = bin_of(x[j], mx, q4, &w);
-      if (mx == -INFINITY || ((double)x[j] * s.c < least && x[j] != mx)) bin[j] = kBins;
-      if (decltype(weighs)::value && bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
+      bin[j] = place(j, &w);
+      if ((decltype(weighs)::value || !s.few) && bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
       if (bin[j] < counted) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
     }
   };
-  if (s.few) tokens(std::false_type{});
+  if (s.few || least > -INFINITY) tokens(std::false_type{});
   else tokens(std::true_type{});
   __syncthreads();
   uint32_t have = 0;
@@ -315,8 +327,12 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
     if (have < (uint32_t)s.k) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < kTok; ++j)
+      for (int j = 0; j < kTok; ++j) {
+        u64 unused;
+        if (bin[j] < counted) continue;
+        bin[j] = place(j, &unused);
         if (bin[j] >= counted && bin[j] < kBins) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
+      }
       __syncthreads();
     }
   }
@@ -370,7 +386,7 @@ constexpr int kCell = 64, kCells = kChunk / kCell;  // columns of a chunk's cell
 
 // A pass over (a part of) the row, by the workgroup, for its tokens between two
 // keys: what bins with too many tokens for the list are worked on with.
-enum PassMode { kCollect, kSubs, kKeep, kBinsOf, kCellsOf };
+enum PassMode { kCollect, kSubs, kKeys, kKeep, kBinsOf, kCellsOf };
 struct DrawSmem {
   u64 list[kList];              // key << 32 | column of the collected tokens
   u64 few_w[kSmallK];           // weights of what a small top-k leaves
@@ -393,9 +409,15 @@ struct DrawSmem {
   int i, j;
 };
 
+// A bin with too many tokens for the list, of up to kKeysMax keys (bf16 logits):
+// their counts by chunk and key take the list's place.
+constexpr int kKeysMax = kList * 2 / kMaxChunks;
 // (of the module, not the kernel: the calls below reach it as LDS, not through
 // generic pointers, whose accesses made a pass over a row 15 times as long)
 static __shared__ DrawSmem sm;
+DEVI uint32_t& key_count(int ch, uint32_t below_top) {
+  return reinterpret_cast<uint32_t*>(sm.list)[ch * kKeysMax + below_top];
+}
 
 // Exclusive prefix sum over the workgroup; total in *total.
 DEVI u64 block_scan(u64 v, u64* total) {
@@ -429,9 +451,9 @@ constexpr int kColBits = 19;
 struct Pass {
   uint32_t k0, k1;               // the keys
   Digit digit;                   // kSubs
-  int by_count, table, min_p;    // kSubs; kKeep: weights from a table, of keys to digit.top
+  int by_count, min_p;           // kSubs; kKeep, kCellsOf: and those that min-p keeps
   uint32_t cut_key;              // kSubs, kKeep, kCellsOf: tokens above this cut
-  int cut_col;                   // ... and, with min_p, that min-p keeps
+  int cut_col;
 };
 // One round of a radix select by N threads (a wavefront, or the workgroup): clear
 // the sub-bins, add the tokens to sm.sub_cnt and sm.sub_mass at at(sub-bin),
@@ -628,9 +650,8 @@ DEVI void find_ends(int lo, int hi) {
 }
 
 // The pass over columns of parts [part, end) (half chunks).  kCollect: into the
-// list, sm.base[64] counting them, past what fits too.  kKeep with p.table: the
-// weight of key k is sm.sub_mass[p.top - k].  Calls of their own, because few rows
-// need them and each place that may is code.
+// list, sm.base[64] counting them, past what fits too.  Calls of their own, because
+// few rows need them and each place that may is code.
 template <typename T, int MODE>
 __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, int part, int end,
                                                Pass p) {
@@ -655,7 +676,7 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
     for (int j = 0; j < kTok; ++j) {
       in[j] = y[j] >= x0 && y[j] <= x1;
       key[j] = key_of(y[j]);
-      if (MODE != kBinsOf && MODE != kCollect)
+      if (MODE != kBinsOf && MODE != kCollect && MODE != kKeys)
         in[j] = in[j] && above(key[j], c + j, p.cut_key, p.cut_col);
       if (MODE == kSubs) in[j] = in[j] && !p.digit.skips(c + j);
       if (MODE == kKeep || MODE == kCellsOf) in[j] = in[j] && (!p.min_p || min_p_keeps(y[j]));
@@ -676,10 +697,7 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
       }
       return;
     }
-    if (MODE == kKeep && p.table) {
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) w[j] = sm.sub_mass[in[j] ? p.digit.top - (key[j] >> KS) : 0];
-    } else if (MODE != kSubs || !p.by_count) {
+    if (MODE != kKeys && (MODE != kSubs || !p.by_count)) {
 #pragma unroll
       for (int j = 0; j < kTok; ++j) w[j] = row_weight(in[j] ? y[j] : sm.xr, &b[j]);
     }
@@ -692,6 +710,8 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
         atomicAdd(&sm.sub_cnt[at], 1u);
         if (!p.by_count) atomicAdd(&sm.sub_mass[at], w[j]);
       }
+      if (MODE == kKeys && in[j])
+        atomicAdd(&key_count((c + mis) / kChunk, p.digit.top - (key[j] >> KS)), 1u);
       if (MODE == kBinsOf && in[j]) {
         atomicAdd(&sm.cnt[b[j]], 1u);
         atomicAdd(&sm.mass[b[j]], w[j]);
@@ -1059,11 +1079,13 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
   // collects the tokens of bin j in the list, from what the chunks wrote out or
   // else from the row, if they fit; k0, k1: the bin's keys
   uint32_t bin0 = 0, bin1 = 0;
+  int dense = -1;  // the bin whose tokens are held as counts by chunk and key
   auto collect = [&](int j) __attribute__((always_inline)) {
     find_ends(j, j);
     bin0 = sm.ends[0];
     bin1 = sm.ends[1] - 1;
-    if (bin0 >= list0 && bin1 <= list1) return;
+    if ((bin0 >= list0 && bin1 <= list1) || dense == j) return;
+    dense = -1;
     __syncthreads();
     if (wave == 0) {
       uint32_t f0 = 0, n = 0;
@@ -1088,7 +1110,17 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       p.k0 = bin0;
       p.k1 = bin1;
       pass<T, kCollect>(row, cols, mis, 0, 2 * n_ch, p);
-      if (sm.base[64] > (uint32_t)kList) return;
+      if (sm.base[64] > (uint32_t)kList) {
+        p.digit.top = bin1 >> KS;
+        if (p.digit.top - (bin0 >> KS) < (uint32_t)kKeysMax) {
+          __syncthreads();
+          for (int i = tid; i < kMaxChunks * kKeysMax; i += kDraw)
+            reinterpret_cast<uint32_t*>(sm.list)[i] = 0;
+          pass<T, kKeys>(row, cols, mis, 0, 2 * n_ch, p);
+          dense = j;
+        }
+        return;
+      }
     }
     list0 = bin0;
     list1 = bin1;
@@ -1102,6 +1134,61 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       if (key >= k0 && key <= k1) f(key, (int)(uint32_t)e);
     }
   };
+  // The border in the dense bin; what is past it leaves the counts.
+  auto dense_border = [&](u64 need, bool by_count) __attribute__((always_inline)) {
+    const uint32_t top = bin1 >> KS;
+    u64 cnt = 0, w = 0, all;
+    int b;
+    if (tid < kKeysMax) {
+      for (int ch = 0; ch < n_ch; ++ch) cnt += key_count(ch, tid);
+      if (cnt > 0) w = row_weight(of_key(key_back(top - tid)), &b);
+    }
+    const u64 v = by_count ? cnt : cnt * w, before = block_scan(v, &all);
+    need = min(need, all);
+    if (v > 0 && before < need && need <= before + v) {
+      sm.i = tid;
+      sm.a = by_count ? need - before : (need - before + w - 1) / w;  // of the equal tokens
+    }
+    __syncthreads();
+    if (need == 0) return;  // every weight here rounds to zero: all are kept
+    const int below = sm.i;
+    const u64 ties = sm.a;
+    __syncthreads();
+    // the chunk of the last of them, and how many it has before
+    if (wave == 0) {
+      const u64 n = lane < n_ch ? key_count(lane, below) : 0, sum = wave_scan(n) - n;
+      if (sum < ties && ties <= sum + n) {
+        sm.i = lane;
+        sm.a = ties - sum;
+      }
+    }
+    __syncthreads();
+    const int last_ch = sm.i;
+    const u64 left = sm.a;
+    // its column: 16 a thread
+    const float x = of_key(key_back(top - below));
+    float y[2][kTok];
+    const int col = load8(row, cols, mis, last_ch, 2 * tid, y[0]);
+    load8(row, cols, mis, last_ch, 2 * tid + 1, y[1]);
+    u64 here = 0;
+#pragma unroll
+    for (int t = 0; t < 2 * kTok; ++t) here += y[t / kTok][t % kTok] == x;
+    u64 n = block_scan(here, &all);
+    if (n < left && left <= n + here) {
+#pragma unroll
+      for (int t = 0; t < 2 * kTok; ++t)
+        if (y[t / kTok][t % kTok] == x && ++n == left) sm.j = col + t;
+    }
+    for (int i = tid; i < n_ch * kKeysMax; i += kDraw) {
+      const int ch = i / kKeysMax, k = i - ch * kKeysMax;
+      if (k > below || (k == below && ch > last_ch)) key_count(ch, k) = 0;
+      else if (k == below && ch == last_ch) key_count(ch, k) = (uint32_t)left;
+    }
+    __syncthreads();
+    cut_key = key_back(top - below);
+    cut_col = sm.j;
+  };
+  static_assert(kKeysMax <= kDraw && 2 * kDraw * kTok == kChunk, "a key, 16 columns a thread");
   // sm.kept[chunk] += the kept weight of bin jc's tokens (min_p: and that it keeps)
   auto keep_bin = [&](bool min_p) __attribute__((always_inline)) {
     __syncthreads();
@@ -1112,20 +1199,21 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
         if (above_cut(key, col) && (!min_p || min_p_keeps(x)))
           atomicAdd(&sm.kept[(col + mis) / kChunk], row_weight(x, &b));
       });
+    } else if (dense == jc) {
+      for (int i = tid; i < n_ch * kKeysMax; i += kDraw) {
+        const int ch = i / kKeysMax, k = i - ch * kKeysMax;
+        const uint32_t n = key_count(ch, k);
+        if (n == 0) continue;
+        int b;
+        const float x = of_key(key_back((bin1 >> KS) - k));
+        if (!min_p || min_p_keeps(x)) atomicAdd(&sm.kept[ch], n * row_weight(x, &b));
+      }
     } else {
       p.k0 = max(bin0, cut_key);
       p.k1 = bin1;
       p.cut_key = cut_key;
       p.cut_col = cut_col;
       p.min_p = min_p;
-      // few keys: their weights in a table (of them, not of thousands of tokens)
-      p.digit.top = bin1 >> KS;
-      const uint32_t keys = p.digit.top - (p.k0 >> KS);
-      p.table = keys < (uint32_t)kSub;
-      for (uint32_t i = tid; p.table && i <= keys; i += kDraw) {
-        int b;
-        sm.sub_mass[i] = row_weight(of_key(key_back(p.digit.top - i)), &b);
-      }
       pass<T, kKeep>(row, cols, mis, 0, 2 * n_ch, p);
     }
     __syncthreads();
@@ -1158,6 +1246,11 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     need = sm.a;
     if (j > jc) break;  // (by rounding) past top-k's border: that one holds
     collect(j);
+    jc = j;
+    if (dense == j) {
+      dense_border(need, stage == 0);
+      continue;
+    }
     border(
         BlockSelect{}, std::true_type{}, bin0, bin1, need, stage == 0,
         [&](uint32_t k0, uint32_t k1, Digit dg, bool by_count) __attribute__((always_inline)) {
@@ -1193,7 +1286,6 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
           list0 = fits ? k0 : 1;
           list1 = fits ? k1 : 0;
         });
-    jc = j;
   }
   if (s.lmin > -INFINITY) {
     const double r = floor((double)xr * q4) - floor(4.0 * sm.lmin);
@@ -1219,6 +1311,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     bin1 = sm.ends[1] - 1;
     list0 = 1;
     list1 = 0;
+    dense = -1;
   }
   if (s.few || jc < kBins) keep_bin(true);
   __syncthreads();
