@@ -58,6 +58,20 @@ DEVI void zero_acc(f32x4 (*acc)[Geo<D>::VW]) {
     for (int e = 0; e < Geo<D>::VW; ++e) acc[h][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
+// the lane's column of acc += w row
+template <int D>
+DEVI void add_row(const float* row, float w, int g, f32x4 (*acc)[Geo<D>::VW]) {
+  constexpr int VW = Geo<D>::VW;
+  if (D == 8 && g >= 2) return;
+#pragma unroll
+  for (int h = 0; h < Geo<D>::NH; ++h)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < VW; ++e)
+        acc[h][e][r] += w * row[16 * VW * h + VW * (4 * g + r) + e];
+}
+
 // the lane's column of acc, each value through f, to row [D]: output tile e
 // of group h holds d = 16 VW h + VW (4 g + r) + e
 template <int D, typename F>

@@ -215,18 +215,6 @@ DEVI float row_dot(const float* row, const f32x4* col, int g) {
     for (int t = 0; t < 4; ++t) s += x[c][t] * col[c][t];
   return sum_g(s);
 }
-template <int D>
-DEVI void add_row(const float* row, float w, int g, f32x4 (*acc)[Geo<D>::VW]) {
-  constexpr int VW = Geo<D>::VW;
-  if (D == 8 && g >= 2) return;
-#pragma unroll
-  for (int h = 0; h < Geo<D>::NH; ++h)
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int e = 0; e < VW; ++e)
-        acc[h][e][r] += w * row[16 * VW * h + VW * (4 * g + r) + e];
-}
 
 // Work item of a workgroup: (rank, head), rank 0 a head's longest walk, all
 // heads' rank 0 first.  With a multiple of 8 heads one XCD (ids deal round

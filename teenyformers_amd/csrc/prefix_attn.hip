@@ -489,6 +489,29 @@ __device__ void prefix_attn_f32(const float* __restrict__ q, const float* __rest
 #pragma unroll
               for (int e = 0; e < VW; ++e) vf[x][h][e] = 0.0f;
       }
+      // new tokens' own rows that some row must not see: 0 * Inf of a masked value is
+      // NaN in a sum over keys, so a tile that is not finite goes key by key to the
+      // rows that see it (tested where S > 1, on a walk's last tiles alone)
+      if (!pre && a.s > 1 && min(t0 + 32, end) > past + 1) {
+        float bad = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+#pragma unroll
+          for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) bad += 0.0f * vf[x][h][e];
+        if (__any(bad != bad)) {
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+#pragma unroll 1
+            for (int kg = 0; kg < 4; ++kg) {
+              const int key = t0 + 16 * (x >> 2) + 4 * kg + (x & 3);
+              const float p = __shfl(s[x >> 2][x & 3], 16 * kg + j);
+              if (key < stop) add_row<D>(vs + (long)key * D, p, g, acc);
+            }
+          continue;
+        }
+      }
 #pragma unroll
       for (int x = 0; x < 8; ++x)
 #pragma unroll

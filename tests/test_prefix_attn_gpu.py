@@ -316,3 +316,44 @@ def test_refusals(cuda):
     odd = torch.empty(q.numel() + 1, dtype=BF, device="cuda")[1:].view(q.shape)
     with pytest.raises(Exception, match="-7"):
         f(odd, kp, vp, k, v, 10, 0)
+
+
+@pytest.mark.parametrize("S,P,L", [(5, 45, 300), (5, 20, 60), (40, 45, 300), (40, 0, 90)])
+@pytest.mark.parametrize("D", [8, 32, 64, 128])
+@pytest.mark.parametrize("G", [1, 3])
+def test_f32_new_tokens_that_are_not_finite(cuda, G, D, S, P, L):
+    """A new token's V of Inf, or K of NaN, reaches that token's row and later ones;
+    earlier ones keep their values."""
+    past = [17, 3]
+    ts = make(cuda, F32, 2, 2 * G, 2, S, D, P, L)
+    q, kp, vp, k, v = ts
+    want, tol = reference(q, kp, vp, k, v, P, past, 0.25)
+    t0, t1 = 2, S - 1
+    v[0, :, past[0] + t0, 3] = float("inf")
+    k[1, :, past[1] + t1] = NAN
+    v[1, :, past[1] + t1] = NAN
+    n = torch.tensor(past, dtype=torch.int32, device="cuda")
+    got = ops.shared_prefix_attention(q, kp, vp, k, v, P, n, 0.25).double()
+    others = [d for d in range(D) if d != 3]
+    ok = (got - want).abs() <= tol
+    assert ok[0, :, :t0].all() and ok[0][:, :, others].all() and ok[1, :, :t1].all()
+    assert not torch.isfinite(got[0, :, t0, 3]).any() and torch.isnan(got[1, :, t1]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_two_streams_at_once(cuda, dtype):
+    """Calls in flight together, each with a workspace of its own."""
+    shapes = [(8, 8, 2, 1, 64, 700, 3000), (4, 8, 2, 3, 128, 900, 3000)]
+    ts = [make(cuda, dtype, *s, seed=i) for i, s in enumerate(shapes)]
+    run = lambda i: ops.shared_prefix_attention(*ts[i], shapes[i][5], 900 + i)  # noqa: E731
+    want = [run(0), run(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
