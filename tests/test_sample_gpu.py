@@ -292,3 +292,44 @@ def test_refusals(cuda):
         ops.sample_rows(x, u, workspace=torch.empty(8, dtype=torch.uint8, device="cuda"))
     with pytest.raises(Exception, match="shape"):
         ops.sample_rows(torch.zeros((1, 524281), dtype=torch.bfloat16, device="cuda"), u[:1])
+
+
+DENSE = {
+    "minp": dict(m=0.985), "topp_low": dict(p=0.3), "k_topp": dict(k=20000, p=0.9),
+    "few": dict(k=300, p=0.5), "few_minp": dict(k=500, m=0.99),
+    "all": dict(k=30000, p=0.5, m=0.985), "k_minp": dict(k=60001, m=0.99),
+}
+
+
+@pytest.mark.parametrize("how", sorted(DENSE))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,spread", [(70000, 0.01), (128256, 0.002), (128256, 0.3)])
+def test_borders_of_flat_rows(cuda, V, spread, dtype, how):
+    """Each border in a bin of thousands of tokens: of few keys and of many, with
+    one border after another in the same bin and in different ones."""
+    x, u = make(3, V, dtype, 23, cuda, zipf=False)
+    check(x * spread, u, **DENSE[how])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_flat_rows_apart_and_unaligned(cuda, dtype):
+    x, u = make(4, 50003, dtype, 29, cuda, zipf=False)
+    for first in (0, 3, 5):
+        check((x * 0.01)[:, first:49999], u, k=9000, p=0.7)
+
+
+def test_two_streams_at_once(cuda):
+    """Calls in flight together, each with a workspace of its own."""
+    xs = [make(32, 40000, torch.bfloat16, 31 + i, cuda) for i in range(2)]
+    how = [dict(top_p=0.9), dict(top_k=700, top_p=0.95, min_p=0.001)]
+    want = [ops.sample_rows(x, u, **h) for (x, u), h in zip(xs, how)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(ops.sample_rows(*xs[i], **how[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
