@@ -255,6 +255,7 @@ template <typename V> DEVI V wave_total(V v) { return lane_value(wave_scan(v), 6
 struct ScanSmem {
   u64 mass[kBins];
   uint32_t cnt[192];
+  uint32_t tops[192];   // threads whose largest token is in each bin
   uint32_t first[192];  // tokens before each bin
   float red[kWaves];
   u64 sums[kWaves];
@@ -272,12 +273,13 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
   const int col = load8(row, cols, misaligned(row), ch, tid, x);
   const Settings s = settings(a, row_i, cols);
   if (tid < 192) {
-    sm.cnt[tid] = 0;
+    sm.cnt[tid] = sm.tops[tid] = 0;
     if (tid < kBins) sm.mass[tid] = 0;
   }
   float mx = x[0];
 #pragma unroll
   for (int j = 1; j < kTok; ++j) mx = fmaxf(mx, x[j]);
+  const float mine = mx;
   mx = wave_max(mx);
   if (lane == 0) sm.red[tid >> 6] = mx;
   __syncthreads();
@@ -304,51 +306,70 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
   // Without top-p, tokens that min-p drops even by the chunk's own maximum do not
   // count.
   const double q4 = 4.0 * s.c, least = s.fp ? -INFINITY : (double)mx * s.c + s.lmin;
-  const int counted = s.fk && !s.few ? kBins : kFirstBins;
-  int bin[kTok];
-  uint32_t rank[kTok];
-  // Most tokens of a small top-k, or of min-p alone, lie below any that counts: those
-  // under `floor_x` are left by one fp32 comparison (a margin of 1e-6 below the
-  // border that fp64 decides).
-  const double top = floor((double)mx * q4);
-  const float edge = (float)(s.few ? (top - (kFirstBins - 1)) / q4 : least / s.c);
-  const float floor_x = fabsf(edge) < 1e37f ? edge - 1e-6f * fabsf(edge) - 1e-37f : -INFINITY;
   Series series;
   series.hold();
-  auto place = [&](int j, auto limited, u64* w) __attribute__((always_inline)) {
-    const int b = bin_of(x[j], mx, q4, w, series);
-    return decltype(limited)::value && (double)x[j] * s.c < least && x[j] != mx ? kBins : b;
+  auto place = [&](float y, auto limited, u64* w) __attribute__((always_inline)) {
+    const int b = bin_of(y, mx, q4, w, series);
+    return decltype(limited)::value && (double)y * s.c < least && y != mx ? kBins : b;
   };
-  auto tokens = [&](auto limited) __attribute__((always_inline)) {
+  int counted = s.fk ? kBins : kFirstBins;
+  if (s.few) {
+    // the first bins in which k threads have their largest token hold the chunk's
+    // first k (no such: all bins)
+    u64 unused;
+    const int b = place(mine, std::true_type{}, &unused);
+    if (b < kBins) atomicAdd(&sm.tops[b], 1u);
+    __syncthreads();
+    uint32_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) sum += sm.tops[3 * lane + i];
+    const uint32_t inc = wave_scan(sum);
+    const u64 enough = __ballot(inc >= (uint32_t)s.k);
+    counted = enough ? min(3 * (int)__builtin_ctzll(enough) + 3, kBins) : kBins;
+  }
+  int bin[kTok];
+  uint32_t rank[kTok];
+#pragma unroll
+  for (int j = 0; j < kTok; ++j) bin[j] = kBins;
+  uint32_t nth = 0x76543210;  // a digit each: the token that x[j], bin[j], rank[j] is of
+  if (s.few || least > -INFINITY) {
+    // Few tokens count: those under `floor_x` are left by one fp32 comparison (a
+    // margin of 1e-6 below the border that fp64 decides), and a wavefront goes over
+    // the others, not over its columns.
+    const double top = floor((double)mx * q4);
+    const float edge = (float)(s.few ? (top - (counted - 1)) / q4 : least / s.c);
+    const float floor_x = fabsf(edge) < 1e37f ? edge - 1e-6f * fabsf(edge) - 1e-37f : -INFINITY;
+    uint32_t left = 0;
+    nth = 0;
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) left |= (uint32_t)(x[j] >= floor_x) << j;
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      if (!__any(left != 0)) break;
+      if (left != 0) {
+        const int j = __builtin_ctz(left);
+        left &= left - 1;
+        const float a0 = j & 1 ? x[1] : x[0], a1 = j & 1 ? x[3] : x[2];
+        const float a2 = j & 1 ? x[5] : x[4], a3 = j & 1 ? x[7] : x[6];
+        const float b0 = j & 2 ? a1 : a0, b1 = j & 2 ? a3 : a2, y = j & 4 ? b1 : b0;
+        u64 w;
+        bin[i] = place(y, std::true_type{}, &w);
+        if (!s.few && bin[i] < kBins) atomicAdd(&sm.mass[bin[i]], w);
+        if (bin[i] < counted) rank[i] = atomicAdd(&sm.cnt[bin[i]], 1u);
+        x[i] = y;  // (j >= i, and no later token of this thread is x[i])
+        nth |= (uint32_t)j << 4 * i;
+      }
+    }
+  } else {
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
-      bin[j] = kBins;
-      if (decltype(limited)::value && !(x[j] >= floor_x)) continue;
       u64 w;
-      bin[j] = place(j, limited, &w);
-      if ((!decltype(limited)::value || !s.few) && bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
+      bin[j] = place(x[j], std::false_type{}, &w);
+      if (bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
       if (bin[j] < counted) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
     }
-  };
-  if (s.few || least > -INFINITY) tokens(std::true_type{});
-  else tokens(std::false_type{});
-  __syncthreads();
-  uint32_t have = 0;
-  if (s.few) {  // too few in the first bins: the others too
-    have = wave_total(lane < kFirstBins ? sm.cnt[lane] : 0);
-    if (have < (uint32_t)s.k) {
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) {
-        u64 unused;
-        if (bin[j] < counted) continue;
-        bin[j] = place(j, std::true_type{}, &unused);
-        if (bin[j] >= counted && bin[j] < kBins) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
-      }
-      __syncthreads();
-    }
   }
-  const int known = s.few && have < (uint32_t)s.k ? kBins : counted;  // bins counted
+  __syncthreads();
   if (tid < 64) {  // three bins a lane
     uint32_t n[3], sum = 0;
 #pragma unroll
@@ -362,7 +383,7 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
     for (int i = 0; i < 3; ++i) {
       const int b = 3 * lane + i;
       sm.first[b] = before;
-      last += b < known && before + n[i] <= (uint32_t)kCand &&
+      last += b < counted && before + n[i] <= (uint32_t)kCand &&
               !(s.few && before >= (uint32_t)s.k);
       before += n[i];
     }
@@ -381,7 +402,8 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
 #pragma unroll
   for (int j = 0; j < kTok; ++j)
     if (bin[j] <= last)
-      to.list[sm.first[bin[j]] + rank[j]] = (u64)key_of(x[j]) << 32 | (uint32_t)(col + j);
+      to.list[sm.first[bin[j]] + rank[j]] =
+          (u64)key_of(x[j]) << 32 | (uint32_t)(col + (int)(nth >> 4 * j & 15));
   if (s.few) return;
   if (tid <= kBins) to.first[tid] = sm.first[tid];
   if (tid < kBins) to.mass[tid] = sm.mass[tid];
