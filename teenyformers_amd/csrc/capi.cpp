@@ -1553,9 +1553,15 @@ int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int
   SampleArgs a{temperature, top_p, min_p, temperature_rows, top_p_rows, min_p_rows, top_k_rows,
                top_k};
   char name[48];
-  snprintf(name, sizeof name, "teeny_sample_scan_%s", dtype_tag(dtype));
+  // A workgroup's threads: 16 wavefronts of one load each where no more workgroups
+  // than CUs run, else 8 of two, whose loads wait side by side.  us with 16 and 8, bf16
+  // x 128256: 1 row 6.0, 6.5; 16 rows with top-k 5.5, 5.8; 64 with top-p 18.4, 16.9;
+  // 512 of mixed settings 99, 82.
+  const bool wide = n <= (size_t)device_cus();
+  snprintf(name, sizeof name, "teeny_sample_scan_%s%s", dtype_tag(dtype), wide ? "_w16" : "");
   void* a0[] = {&logits, &ld, &cols, &a, &rec, &bins};
-  int rc = launch(name, dim3((unsigned)n_ch, (unsigned)rows), dim3(1024), 0, stream, a0);
+  int rc = launch(name, dim3((unsigned)n_ch, (unsigned)rows), dim3(wide ? 1024 : 512), 0, stream,
+                  a0);
   if (rc) return rc;
   snprintf(name, sizeof name, "teeny_sample_draw_%s", dtype_tag(dtype));
   void* a1[] = {&logits, &ld, &cols, &a, &u, &rec, &bins, &n_ch, &out, &advance};

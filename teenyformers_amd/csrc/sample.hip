@@ -49,9 +49,10 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64;  // of the scan
-constexpr int kTok = 8;                   // tokens per thread and chunk
-constexpr int kChunk = kThreads * kTok;   // columns per chunk
+constexpr int kTok = 8;                   // tokens of a thread's vector
+constexpr int kChunk = 8192;              // columns per chunk
+constexpr int kSlots = kChunk / kTok;     // vectors of a chunk
+constexpr int kParts = kSlots / 64;       // parts of 512 columns: a wavefront's vectors
 constexpr int kMaxChunks = 64;            // a lane each
 constexpr int kBins = 180;                // quarter octaves below the row's maximum: 45 octaves
 constexpr int kFirstBins = 48;            // of them those that are counted first: 12 octaves
@@ -252,53 +253,67 @@ template <typename V> DEVI V wave_total(V v) { return lane_value(wave_scan(v), 6
 // ---------------------------------------------------------------------------
 // scan: grid (chunks, rows)
 // ---------------------------------------------------------------------------
-struct ScanSmem {
+template <int VEC> struct ScanSmem {
   u64 mass[kBins];
   uint32_t cnt[192];
   uint32_t tops[192];   // threads whose largest token is in each bin
   uint32_t first[192];  // tokens before each bin
-  float red[kWaves];
-  u64 sums[kWaves];
+  float red[kParts / VEC];
+  u64 sums[kParts];
   int last;
 };
 
-template <typename T>
+// VEC: vectors of 8 tokens a thread.
+template <typename T, int VEC>
 __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, const Args a,
                             Chunk* __restrict__ rec, Bins* __restrict__ bins) {
-  __shared__ ScanSmem sm;
+  constexpr int kScan = kSlots / VEC, kScanWaves = kScan / 64;
+  __shared__ ScanSmem<VEC> sm;
   const int tid = threadIdx.x, lane = tid & 63, ch = blockIdx.x, row_i = blockIdx.y;
   const long slot = (long)row_i * gridDim.x + ch;
   const T* row = logits + row_i * ld;
-  float x[kTok];
-  const int col = load8(row, cols, misaligned(row), ch, tid, x);
+  float x[VEC][kTok];
+  int col[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v)
+    col[v] = load8(row, cols, misaligned(row), ch, v * kScan + tid, x[v]);
   const Settings s = settings(a, row_i, cols);
   if (tid < 192) {
     sm.cnt[tid] = sm.tops[tid] = 0;
     if (tid < kBins) sm.mass[tid] = 0;
   }
-  float mx = x[0];
+  float mine[VEC], mx = -INFINITY;  // the largest of each vector
 #pragma unroll
-  for (int j = 1; j < kTok; ++j) mx = fmaxf(mx, x[j]);
-  const float mine = mx;
+  for (int v = 0; v < VEC; ++v) {
+    mine[v] = x[v][0];
+#pragma unroll
+    for (int j = 1; j < kTok; ++j) mine[v] = fmaxf(mine[v], x[v][j]);
+    mx = fmaxf(mx, mine[v]);
+  }
   mx = wave_max(mx);
   if (lane == 0) sm.red[tid >> 6] = mx;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, sm.red[w]);
+  for (int w = 0; w < kScanWaves; ++w) mx = fmaxf(mx, sm.red[w]);
   mx = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, mx)));
   Bins& to = bins[slot];
   if (!s.filters) {
     const double lref = (double)mx * s.c;
-    u64 sum = 0;
 #pragma unroll
-    for (int j = 0; j < kTok; ++j)
-      if (x[j] > -INFINITY) sum += weight(x[j] == mx ? 0.0 : lref - (double)x[j] * s.c);
-    sum = wave_total(sum);
-    if (lane == 0) sm.sums[tid >> 6] = sum;
+    for (int v = 0; v < VEC; ++v) {
+      u64 sum = 0;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        const float y = x[v][j];
+        if (y > -INFINITY) sum += weight(y == mx ? 0.0 : lref - (double)y * s.c);
+      }
+      sum = wave_total(sum);
+      if (lane == 0) sm.sums[v * kScanWaves + (tid >> 6)] = sum;
+    }
     __syncthreads();
     if (tid < 64) {
-      const u64 w = lane < kWaves ? sm.sums[lane] : 0, all = wave_total(w);
-      if (lane < kWaves) to.mass[lane] = w;
+      const u64 w = lane < kParts ? sm.sums[lane] : 0, all = wave_total(w);
+      if (lane < kParts) to.mass[lane] = w;
       if (lane == 0) rec[slot] = Chunk{lref, all, mx, 0, 0, 0};
     }
     return;
@@ -314,11 +329,14 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
   };
   int counted = s.fk ? kBins : kFirstBins;
   if (s.few) {
-    // the first bins in which k threads have their largest token hold the chunk's
+    // the first bins in which k vectors have their largest token hold the chunk's
     // first k (no such: all bins)
-    u64 unused;
-    const int b = place(mine, std::true_type{}, &unused);
-    if (b < kBins) atomicAdd(&sm.tops[b], 1u);
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+      u64 unused;
+      const int b = place(mine[v], std::true_type{}, &unused);
+      if (b < kBins) atomicAdd(&sm.tops[b], 1u);
+    }
     __syncthreads();
     uint32_t sum = 0;
 #pragma unroll
@@ -327,11 +345,9 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
     const u64 enough = __ballot(inc >= (uint32_t)s.k);
     counted = enough ? min(3 * (int)__builtin_ctzll(enough) + 3, kBins) : kBins;
   }
-  int bin[kTok];
-  uint32_t rank[kTok];
-#pragma unroll
-  for (int j = 0; j < kTok; ++j) bin[j] = kBins;
-  uint32_t nth = 0x76543210;  // a digit each: the token that x[j], bin[j], rank[j] is of
+  int bin[VEC][kTok];
+  uint32_t rank[VEC][kTok];
+  uint32_t nth[VEC];  // a digit each: the token that x[v][i], bin[v][i], rank[v][i] is of
   if (s.few || least > -INFINITY) {
     // Few tokens count: those under `floor_x` are left by one fp32 comparison (a
     // margin of 1e-6 below the border that fp64 decides), and a wavefront goes over
@@ -339,34 +355,48 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
     const double top = floor((double)mx * q4);
     const float edge = (float)(s.few ? (top - (counted - 1)) / q4 : least / s.c);
     const float floor_x = fabsf(edge) < 1e37f ? edge - 1e-6f * fabsf(edge) - 1e-37f : -INFINITY;
-    uint32_t left = 0;
-    nth = 0;
+    auto few = [&](auto vector) __attribute__((always_inline)) {
+      constexpr int v = decltype(vector)::value;
+      uint32_t left = 0;
+      nth[v] = 0;
 #pragma unroll
-    for (int j = 0; j < kTok; ++j) left |= (uint32_t)(x[j] >= floor_x) << j;
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      if (!__any(left != 0)) break;
-      if (left != 0) {
-        const int j = __builtin_ctz(left);
-        left &= left - 1;
-        const float a0 = j & 1 ? x[1] : x[0], a1 = j & 1 ? x[3] : x[2];
-        const float a2 = j & 1 ? x[5] : x[4], a3 = j & 1 ? x[7] : x[6];
-        const float b0 = j & 2 ? a1 : a0, b1 = j & 2 ? a3 : a2, y = j & 4 ? b1 : b0;
-        u64 w;
-        bin[i] = place(y, std::true_type{}, &w);
-        if (!s.few && bin[i] < kBins) atomicAdd(&sm.mass[bin[i]], w);
-        if (bin[i] < counted) rank[i] = atomicAdd(&sm.cnt[bin[i]], 1u);
-        x[i] = y;  // (j >= i, and no later token of this thread is x[i])
-        nth |= (uint32_t)j << 4 * i;
+      for (int j = 0; j < kTok; ++j) {
+        left |= (uint32_t)(x[v][j] >= floor_x) << j;
+        bin[v][j] = kBins;
       }
-    }
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        if (!__any(left != 0)) break;
+        if (left != 0) {
+          const int j = __builtin_ctz(left);
+          left &= left - 1;
+          const float a0 = j & 1 ? x[v][1] : x[v][0], a1 = j & 1 ? x[v][3] : x[v][2];
+          const float a2 = j & 1 ? x[v][5] : x[v][4], a3 = j & 1 ? x[v][7] : x[v][6];
+          const float b0 = j & 2 ? a1 : a0, b1 = j & 2 ? a3 : a2, y = j & 4 ? b1 : b0;
+          u64 w;
+          const int b = bin[v][i] = place(y, std::true_type{}, &w);
+          if (!s.few && b < kBins) atomicAdd(&sm.mass[b], w);
+          if (b < counted) rank[v][i] = atomicAdd(&sm.cnt[b], 1u);
+          x[v][i] = y;  // (j >= i, and no later token of this vector is x[v][i])
+          nth[v] |= (uint32_t)j << 4 * i;
+        }
+      }
+    };
+    // (as a loop its body's arrays are not held in registers)
+    static_assert(VEC <= 2, "");
+    few(std::integral_constant<int, 0>{});
+    if constexpr (VEC == 2) few(std::integral_constant<int, 1>{});
   } else {
 #pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      u64 w;
-      bin[j] = place(x[j], std::false_type{}, &w);
-      if (bin[j] < kBins) atomicAdd(&sm.mass[bin[j]], w);
-      if (bin[j] < counted) rank[j] = atomicAdd(&sm.cnt[bin[j]], 1u);
+    for (int v = 0; v < VEC; ++v) {
+      nth[v] = 0x76543210;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        u64 w;
+        const int b = bin[v][j] = place(x[v][j], std::false_type{}, &w);
+        if (b < kBins) atomicAdd(&sm.mass[b], w);
+        if (b < counted) rank[v][j] = atomicAdd(&sm.cnt[b], 1u);
+      }
     }
   }
   __syncthreads();
@@ -400,10 +430,12 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
   __syncthreads();
   const int last = sm.last;
 #pragma unroll
-  for (int j = 0; j < kTok; ++j)
-    if (bin[j] <= last)
-      to.list[sm.first[bin[j]] + rank[j]] =
-          (u64)key_of(x[j]) << 32 | (uint32_t)(col + (int)(nth >> 4 * j & 15));
+  for (int v = 0; v < VEC; ++v)
+#pragma unroll
+    for (int j = 0; j < kTok; ++j)
+      if (bin[v][j] <= last)
+        to.list[sm.first[bin[v][j]] + rank[v][j]] =
+            (u64)key_of(x[v][j]) << 32 | (uint32_t)(col[v] + (int)(nth[v] >> 4 * j & 15));
   if (s.few) return;
   if (tid <= kBins) to.first[tid] = sm.first[tid];
   if (tid < kBins) to.mass[tid] = sm.mass[tid];
@@ -603,7 +635,7 @@ DEVI void draw_plain(const T* row, int cols, int mis, const Settings& s, float u
   t = min(t, lane_value(r.mass, ch) - 1);
   const double lref = __builtin_bit_cast(double, lane_value(__builtin_bit_cast(u64, r.lref), ch));
   const float xmax = __builtin_bit_cast(float, lane_value(__builtin_bit_cast(uint32_t, r.xmax), ch));
-  const u64 part = lane < kWaves ? bins[ch].mass[lane] : 0, pinc = wave_scan(part);
+  const u64 part = lane < kParts ? bins[ch].mass[lane] : 0, pinc = wave_scan(part);
   const int sub = __builtin_ctzll(__ballot(pinc - part <= t && t < pinc));
   t -= lane_value(pinc - part, sub);
   float x[kTok];
@@ -764,7 +796,7 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
   // A vector of 8 logits at a time, the next U - 1 in flight.  (One body, looped:
   // code that a row runs through once is fetched from memory as it goes, and a body
   // for each of 32 logits took longer to arrive than its data.)
-  const int s0 = part * (kThreads / 2), s1 = end * (kThreads / 2);
+  const int s0 = part * (kSlots / 2), s1 = end * (kSlots / 2);
   // (a call's pointer argument may be to LDS for all that the compiler knows: loads
   // through it would be waited for with every LDS operation)
   typedef __attribute__((address_space(1))) u32x4 GlobalVec;
@@ -1414,9 +1446,13 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
 }  // namespace
 
 #define TEENY_SAMPLE_INST(TN, T)                                                                  \
-  extern "C" __global__ __launch_bounds__(1024) void teeny_sample_scan_##TN(                     \
+  extern "C" __global__ __launch_bounds__(512) void teeny_sample_scan_##TN(                       \
       const T* logits, long ld, int cols, Args a, Chunk* rec, Bins* bins) {                       \
-    sample_scan<T>(logits, ld, cols, a, rec, bins);                                               \
+    sample_scan<T, 2>(logits, ld, cols, a, rec, bins);                                            \
+  }                                                                                               \
+  extern "C" __global__ __launch_bounds__(1024) void teeny_sample_scan_##TN##_w16(                \
+      const T* logits, long ld, int cols, Args a, Chunk* rec, Bins* bins) {                       \
+    sample_scan<T, 1>(logits, ld, cols, a, rec, bins);                                            \
   }                                                                                               \
   extern "C" __global__ __launch_bounds__(512) void teeny_sample_draw_##TN(                      \
       const T* logits, long ld, int cols, Args a, const float* u, const Chunk* rec,               \

@@ -333,3 +333,31 @@ def test_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+@pytest.mark.parametrize("how", sorted(HOW))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,V", [(300, 1), (270, 61), (270, 8185), (150, 8193), (60, 40001)])
+def test_more_chunks_than_workgroups_at_once(cuda, rows, V, dtype, how):
+    """Rows enough for the scan's other workgroup size, and its rows' ends."""
+    x, u = make(rows, V, dtype, 300 + V, cuda)
+    check(x, u, **HOW[how])
+
+
+@pytest.mark.parametrize("how", sorted(DENSE))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_flat_rows(cuda, dtype, how):
+    x, u = make(40, 60000, dtype, 37, cuda, zipf=False)
+    check(x * 0.01, u, **DENSE[how])
+
+
+def test_results_do_not_depend_on_the_workgroups(cuda):
+    """One row alone and among many: the same token."""
+    x, u = make(300, 20000, torch.bfloat16, 41, cuda)
+    x[7, 100:9000] = -INF
+    x[8] = -INF
+    x[9, 5] = INF
+    for how in (dict(), dict(top_k=50, top_p=0.9), dict(top_k=600), dict(top_p=0.95), dict(min_p=0.05)):
+        got = ops.sample_rows(x, u, 0.9, **how)
+        for i in (0, 7, 8, 9, 299):
+            assert torch.equal(got[i:i + 1], ops.sample_rows(x[i:i + 1], u[i:i + 1], 0.9, **how))
