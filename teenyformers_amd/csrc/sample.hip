@@ -51,8 +51,9 @@
 // 78; fp32, 24 x 32001 with min-p 5.5, 9.5.  Few rows are bound by their chains
 // (load, maximum, weights, borders), a workgroup each.  Rows by the hundred are bound
 // in the scan by vector instructions (57 a token and wavefront with top-p) and by
-// workgroups that wait for their loads: 512 rows are read at 1.6 TB/s.  Their draws,
-// all resident at once, take the time of the rows with the fullest border bins.
+// workgroups that wait for their loads: 512 rows are read at 1.6 TB/s.  Their draws
+// (a workgroup a CU: 200 registers; in 128 the compiler spills, and 64 rows took 25
+// us) take the time of the rows with the fullest border bins.
 #include "common.h"
 
 #include <type_traits>
@@ -227,6 +228,13 @@ DEVI int load8(const T* row, int cols, int mis, int ch, int slot, float* x) {
   for (int j = 0; j < kTok; ++j) x[j] = fmaxf(x[j] + 0.0f, -INFINITY);
   return col;
 }
+// x[j] of a vector in registers
+DEVI float nth_of(const float* x, int j) {
+  const float a0 = j & 1 ? x[1] : x[0], a1 = j & 1 ? x[3] : x[2];
+  const float a2 = j & 1 ? x[5] : x[4], a3 = j & 1 ? x[7] : x[6];
+  const float b0 = j & 2 ? a1 : a0, b1 = j & 2 ? a3 : a2;
+  return j & 4 ? b1 : b0;
+}
 template <typename T> DEVI int misaligned(const T* row) {
   return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
 }
@@ -383,9 +391,7 @@ __device__ void sample_scan(const T* __restrict__ logits, long ld, int cols, con
         if (left != 0) {
           const int j = __builtin_ctz(left);
           left &= left - 1;
-          const float a0 = j & 1 ? x[v][1] : x[v][0], a1 = j & 1 ? x[v][3] : x[v][2];
-          const float a2 = j & 1 ? x[v][5] : x[v][4], a3 = j & 1 ? x[v][7] : x[v][6];
-          const float b0 = j & 2 ? a1 : a0, b1 = j & 2 ? a3 : a2, y = j & 4 ? b1 : b0;
+          const float y = nth_of(x[v], j);
           u64 w;
           const int b = bin[v][i] = place(y, std::true_type{}, &w);
           if (!s.few && b < kBins) atomicAdd(&sm.mass[b], w);
@@ -740,13 +746,31 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
     if (threadIdx.x == 0) sm.base[64] = 0;
     __syncthreads();
   }
-  constexpr int U = 4;                        // vectors of 8 logits in flight
+  constexpr int U = 2;                        // vectors of 8 logits: one in use, one loading
   constexpr int VW = kTok / Vec16<T>::N;      // loads a vector
   constexpr int KS = sizeof(T) == 2 ? 16 : 0;
   const float x0 = of_key(p.k0), x1 = of_key(p.k1);
   // a thread's vector of 8 logits in columns c ..: of the weights, all are formed
   // before the first is used
   auto vec8 = [&](const float* y, int c) __attribute__((always_inline)) {
+    if (MODE == kCollect) {  // one place in the list for all of a wavefront's tokens
+      uint32_t left = 0;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) left |= (uint32_t)(y[j] >= x0 && y[j] <= x1) << j;
+      const uint32_t n = __builtin_popcount(left), inc = wave_scan(n), all = lane_value(inc, 63);
+      if (all == 0) return;
+      uint32_t at = 0;
+      if (lane == 0) at = atomicAdd(&sm.base[64], all);
+      at = lane_value(at, 0) + inc - n;
+      while (left != 0) {
+        const int j = __builtin_ctz(left);
+        left &= left - 1;
+        if (at < (uint32_t)kList)
+          sm.list[at] = (u64)key_of(nth_of(y, j)) << 32 | (uint32_t)(c + j);
+        ++at;
+      }
+      return;
+    }
     bool in[kTok];
     uint32_t key[kTok];
     int b[kTok];
@@ -755,26 +779,10 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
     for (int j = 0; j < kTok; ++j) {
       in[j] = y[j] >= x0 && y[j] <= x1;
       key[j] = key_of(y[j]);
-      if (MODE != kBinsOf && MODE != kCollect && MODE != kKeys)
+      if (MODE != kBinsOf && MODE != kKeys)
         in[j] = in[j] && above(key[j], c + j, p.cut_key, p.cut_col);
       if (MODE == kSubs) in[j] = in[j] && !p.digit.skips(c + j);
       if (MODE == kKeep || MODE == kCellsOf) in[j] = in[j] && (!p.min_p || min_p_keeps(y[j]));
-    }
-    if (MODE == kCollect) {  // one place in the list for all of a wavefront's tokens
-      uint32_t n = 0;
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) n += in[j];
-      const uint32_t inc = wave_scan(n), all = lane_value(inc, 63);
-      if (all == 0) return;
-      uint32_t at = 0;
-      if (lane == 0) at = atomicAdd(&sm.base[64], all);
-      at = lane_value(at, 0) + inc - n;
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) {
-        if (in[j] && at < (uint32_t)kList) sm.list[at] = (u64)key[j] << 32 | (uint32_t)(c + j);
-        at += in[j];
-      }
-      return;
     }
     if (MODE != kKeys && (MODE != kSubs || !p.by_count)) {
 #pragma unroll
@@ -806,9 +814,10 @@ __device__ __attribute__((noinline)) void pass(const T* row, int cols, int mis, 
     // (a thread's 8 columns lie in one cell)
     if (MODE == kCellsOf && sum > 0) atomicAdd(&sm.cell[(c + mis) % kChunk / kCell], sum);
   };
-  // A vector of 8 logits at a time, the next U - 1 in flight.  (One body, looped:
-  // code that a row runs through once is fetched from memory as it goes, and a body
-  // for each of 32 logits took longer to arrive than its data.)
+  // A vector of 8 logits at a time, the next one in flight (four or eight at a time
+  // are no faster: one CU issues the instructions of a row of 128256 in about 26 us).
+  // (One body, looped: code that a row runs through once is fetched from memory as
+  // it goes, and a body for each of 32 logits took longer to arrive than its data.)
   const int s0 = part * (kSlots / 2), s1 = end * (kSlots / 2);
   // (a call's pointer argument may be to LDS for all that the compiler knows: loads
   // through it would be waited for with every LDS operation)
