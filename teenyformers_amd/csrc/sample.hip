@@ -47,8 +47,8 @@
 //          keys (bf16: 512 mixed rows 184 -> 78 us), else read from the row again.
 //
 // Measured, bf16 x 128256, us of scan and draw: 1 row without filters 6.0, 4.2; 16
-// with top-k 50 and top-p 5.6, 13; 64 with top-p 17, 16; 512 of mixed settings 82,
-// 78; fp32, 24 x 32001 with min-p 5.5, 9.5.  Few rows are bound by their chains
+// with top-k 50 and top-p 5.6, 11; 64 with top-p 17, 14; 512 of mixed settings 82,
+// 75; fp32, 24 x 32001 with min-p 5.5, 9.5.  Few rows are bound by their chains
 // (load, maximum, weights, borders), a workgroup each.  Rows by the hundred are bound
 // in the scan by vector instructions (57 a token and wavefront with top-p) and by
 // workgroups that wait for their loads: 512 rows are read at 1.6 TB/s.  Their draws
@@ -488,6 +488,8 @@ struct DrawSmem {
   u64 tmp[kDrawWaves];
   uint32_t ends[2];             // keys of the first and last logit of some bins
   uint32_t kmin, kmax, n_few;
+  int ties[64];                 // columns of a border's equal tokens
+  uint32_t n_ties;
   u64 a, b;                     // a value that one thread hands to all
   float xr;
   double c, lmin;               // log2(e) / T; min-p in terms of L = x c, -inf without
@@ -902,7 +904,7 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
       sm.c = c;
       sm.lmin = s.lmin > -INFINITY ? (double)m * c + s.lmin : -INFINITY;
       sm.i = all;
-      sm.kmin = sm.kmax = sm.n_few = 0;
+      sm.kmin = sm.kmax = sm.n_few = sm.n_ties = 0;
     }
   }
   for (int i = tid; i < kBins; i += kDraw) {
@@ -952,14 +954,15 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
   // reaches need.  Sets the cut.  A round finds a sub-bin: by key, until one is
   // left, then by column among its equals.
   // subs(k0, k1, digit, by_count): adds the tokens between k0 and k1 (without the
-  // low bits that every key shares); narrowed(k0, k1, n): n of them are left.
+  // low bits that every key shares); narrowed(k0, k1, n): n of them are left;
+  // equals(k, f): f(column) of those with key k, if they are at hand.
   constexpr int KS = sizeof(T) == 2 ? 16 : 0;
   // (bf16: the low half of a key is all zeros, of a negative logit's all ones)
   auto key_back = [](uint32_t k) __attribute__((always_inline)) {
     return KS ? k << 16 | (k & 0x8000u ? 0u : 0xffffu) : k;
   };
   auto border = [&](auto select, auto weighs, uint32_t k0, uint32_t k1, u64 need, bool by_count,
-                    auto&& subs, auto&& narrowed) __attribute__((always_inline)) {
+                    auto&& subs, auto&& narrowed, auto&& equals) __attribute__((always_inline)) {
     constexpr bool WEIGH = decltype(weighs)::value;
     constexpr int SUBS = decltype(select)::SUBS, BITS = __builtin_ctz(SUBS);
     k0 >>= KS;
@@ -998,8 +1001,25 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
           by_count = true;
         }
         if (need >= n) break;  // all of them
-        dg.cs = kColBits - BITS;
         all_equals = false;
+        // up to 64: a lane each, which counts the columns before its own (64 rows
+        // with top-p 13.9 us, by two more rounds 15.9)
+        if (n <= 64 && equals(k0, [&](int col) __attribute__((always_inline)) {
+              const uint32_t i = atomicAdd(&sm.n_ties, 1u);
+              if (i < 64) sm.ties[i] = col;
+            })) {
+          select.sync();
+          const int ties = __builtin_amdgcn_readfirstlane((int)n);
+          const int col = lane < ties ? sm.ties[lane] : 0x7fffffff;
+          u64 before = 0;
+          for (int i = 0; i < ties; ++i) before += (int)lane_value((uint32_t)col, i) < col;
+          const u64 at = __ballot(lane < ties && before == need - 1);
+          dg.col0 = (int)lane_value((uint32_t)col, __builtin_ctzll(at));
+          select.sync();
+          if (tid == 0) sm.n_ties = 0;
+          break;
+        }
+        dg.cs = kColBits - BITS;
       } else {
         dg.col0 = dg.col0 >> (dg.cs + BITS) << (dg.cs + BITS) | (int)(sub << dg.cs);
         if (dg.cs == 0) break;
@@ -1047,7 +1067,14 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
                 atomicAdd(&sm.sub_cnt[BlockSelect::at(dg.sub(k, col, BlockSelect::SUBS))], 1u);
             }
           },
-          [](uint32_t, uint32_t, u64) {});
+          [](uint32_t, uint32_t, u64) {},
+          [&](uint32_t k, auto&& f) __attribute__((always_inline)) {
+            for (uint32_t i = tid; i < n_all; i += kDraw) {
+              const u64 e = sm.list[i];
+              if ((uint32_t)(e >> 32) >> KS == k) f((int)(uint32_t)e);
+            }
+            return true;
+          });
     __syncthreads();
     for (uint32_t i = tid; i < n_all; i += kDraw) {
       const u64 e = sm.list[i];
@@ -1060,6 +1087,8 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
     __syncthreads();
     // the rest by one wavefront, without barriers
     if (wave > 0) return;
+    // (up to 64 tokens a lane each, which sums the weights of those before it, instead
+    // of rounds of a radix select: 16 rows with 50 tokens 11.5 -> 14.9 us)
     constexpr int E = kSmallK / 64;  // tokens a lane
     const uint32_t n = sm.n_few;
     uint32_t key[E];
@@ -1090,7 +1119,15 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
               if (!by_count) atomicAdd(&sm.sub_mass[at], w[i]);
             }
           },
-          [](uint32_t, uint32_t, u64) {});
+          [](uint32_t, uint32_t, u64) {},
+          [&](uint32_t k, auto&& f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+              if (64 * i >= n) break;
+              if (lane + 64 * i < n && key[i] >> KS == k) f(col[i]);
+            }
+            return true;
+          });
     }
     mine = 0;
 #pragma unroll
@@ -1373,6 +1410,14 @@ __device__ void sample_draw(const T* __restrict__ logits, long ld, int cols, con
           const bool fits = sm.base[64] <= (uint32_t)kList;
           list0 = fits ? k0 : 1;
           list1 = fits ? k1 : 0;
+        },
+        [&](uint32_t k, auto&& f) __attribute__((always_inline)) {
+          const uint32_t a0 = max(k << KS, bin0), a1 = min(KS ? k << 16 | 0xffffu : k, bin1);
+          if (a0 < list0 || a1 > list1) return false;
+          listed(a0, a1, [&](uint32_t key, int col) __attribute__((always_inline)) {
+            if (above_cut(key, col)) f(col);
+          });
+          return true;
         });
   }
   if (s.lmin > -INFINITY) {

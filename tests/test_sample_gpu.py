@@ -361,3 +361,25 @@ def test_results_do_not_depend_on_the_workgroups(cuda):
         got = ops.sample_rows(x, u, 0.9, **how)
         for i in (0, 7, 8, 9, 299):
             assert torch.equal(got[i:i + 1], ops.sample_rows(x[i:i + 1], u[i:i + 1], 0.9, **how))
+
+
+@pytest.mark.parametrize("n", [2, 63, 64, 65, 130])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_borders_among_a_few_equal_tokens(cuda, dtype, n):
+    """n equal tokens spread over the row, and the border at each kind of place
+    among them: by count, by weight, one after the other."""
+    V = 20011
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.rand((6, V), generator=g, device="cuda") * 4 - 12
+    at = torch.randperm(V, generator=g, device="cuda")[:n + 9]
+    x[:, at[:n]] = 2.0
+    x[:, at[n:]] = 3.0 + torch.rand((6, 9), generator=g, device="cuda")
+    x = x.to(dtype)
+    u = torch.tensor([0.0, 0.2, 0.5, 0.7, 0.9, 0.9999], device="cuda")
+    for k in (8, 9, 10, 9 + n // 2, 8 + n, 9 + n, 10 + n, 600):
+        check(x, u, k=k)
+        check(x, u, k=k, p=0.95)
+        check(x, u, T=2.0, k=k + 513, p=0.9)
+    for p in (0.3, 0.8, 0.9, 0.97):
+        check(x, u, p=p)
+        check(x, u, T=0.5, p=p)
