@@ -220,13 +220,14 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     };
     int t0, t1;
     tokens(mb * BM, min(blk_end, nq), t0, t1);
-    const int own_end = min(past + t1 + 1, nk);
+    // own tiles of the rows up to token t (a negative length: none, and every prefix tile)
+    auto own_tiles = [&](int t) { return (max(0, min(past + t + 1, nk)) + BN - 1) / BN; };
     own_rows = max(0, min(past + pre.s, nk));
     n_pre = (pre.n + BN - 1) / BN;
-    n_iter = n_pre + (own_end + BN - 1) / BN;
+    n_iter = n_pre + own_tiles(t1);
     if (wrow0 < nq) {
       tokens(wrow0, min(wrow0 + 32, nq), t0, t1);
-      own_live = n_pre + (min(past + t1 + 1, nk) + BN - 1) / BN;
+      own_live = n_pre + own_tiles(t1);
       lim_all = min(past + t0 + 1, nk);
     }
     lim = min(past + min(qrow, nq - 1) % pre.s + 1, nk);

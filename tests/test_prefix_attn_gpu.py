@@ -357,3 +357,27 @@ def test_two_streams_at_once(cuda, dtype):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+# (type, new tokens, q heads, kv heads, D, cache rows past the new tokens, by shares)
+NEGATIVE = [
+    (BF, 300, 8, 2, 64, 0, False), (BF, 512, 4, 2, 128, 0, False),
+    (BF, 300, 8, 2, 64, 9000, True), (BF, 512, 4, 2, 128, 9000, True), (BF, 1, 8, 2, 128, 3000, True),
+    (F32, 300, 4, 2, 64, 0, True), (F32, 300, 16, 4, 64, 0, False), (F32, 1, 8, 2, 128, 0, True),
+]
+
+
+@pytest.mark.parametrize("P", [33, 1000])
+@pytest.mark.parametrize("dtype,S,Hq,Hkv,D,more,shares", NEGATIVE, ids=[
+    f"{'bf16' if c[0] == BF else 'f32'}-{c[1:]}" for c in NEGATIVE])
+def test_negative_lengths_behind_a_prefix(cuda, dtype, S, Hq, Hkv, D, more, shares, P):
+    """Device lengths below zero: rows that see the prefix alone, all of it, in each
+    way that the call may run."""
+    past = [-S, 1 - S, -100, -1, 0]
+    L = S + more + (60 if S == 1 else 0)
+    need = ops._lib.lib().teeny_shared_prefix_attention_workspace_bytes(
+        len(past), Hq, Hkv, S, P, L, D, 1 if dtype == BF else 0)
+    # (fp32: up to 128 keys are walked whole)
+    assert (need > 0) == (shares and not (dtype == F32 and P + L <= 128))
+    got = check(make(cuda, dtype, len(past), Hq, Hkv, S, D, P, L, prefix_len=P + 2), P, past, S)
+    assert (got != 0).any(3).all()
