@@ -19,8 +19,9 @@ timings, and is the workload of the decode kernel profiles:
 --num-samples N draws N continuations of the prompt, which runs and is stored
 once (Llama.generate_samples); --top-k, --top-p and --min-p cut the
 distribution.  Any of them draws on the device (ops.sample_rows, random
-numbers from torch's generator with --seed); without them, --temperature keeps
-the reference's sampler on the host.
+numbers from torch's generator with --seed), at temperature 1 unless
+--temperature says otherwise; without them, --temperature keeps the reference's
+sampler on the host, and its default is 0 (greedy).
 """
 from __future__ import annotations
 
@@ -210,7 +211,9 @@ def main(argv=None) -> int:
     ap.add_argument("--model-dir", help="config.json, tokenizer.json and *.safetensors")
     ap.add_argument("--prompt", default="The quick brown fox")
     ap.add_argument("--max-new-tokens", type=int, default=128)
-    ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--temperature", type=float, default=None,
+                    help="0 is greedy, whatever the filters; default 1 with --num-samples above 1 "
+                         "or a filter, else 0")
     ap.add_argument("--num-samples", type=int, default=1,
                     help="continuations of the prompt, drawn on the device")
     ap.add_argument("--top-k", type=int, default=0, help="0: off")
@@ -226,12 +229,14 @@ def main(argv=None) -> int:
     args = ap.parse_args(argv)
     if args.max_new_tokens < 1:
         ap.error("--max-new-tokens must be at least 1")
+    args.on_device = (args.num_samples > 1 or args.top_k > 0 or args.top_p < 1.0
+                      or args.min_p > 0.0)
+    if args.temperature is None:
+        args.temperature = 1.0 if args.on_device else 0.0
     if not (args.temperature >= 0.0 and args.num_samples >= 1 and 0 <= args.top_k < 2 ** 31
             and 0.0 < args.top_p <= 1.0 and 0.0 <= args.min_p <= 1.0):
         ap.error("--temperature and --top-k are at least 0, --num-samples at least 1, --top-p in "
                  "(0, 1], --min-p in [0, 1]")
-    args.on_device = (args.num_samples > 1 or args.top_k > 0 or args.top_p < 1.0
-                      or args.min_p > 0.0)
     if args.preset:
         return bench_preset(args)
     if not args.model_dir:

@@ -180,3 +180,16 @@ def test_config_d_ff_default_rounding():
     for d in range(1, 8193):
         want = _m.ceil(Fraction(_m.ceil(Fraction(8 * d, 3)), 64)) * 64
         assert llama.LlamaConfig(d_model=d).d_ff() == want, d
+
+
+@pytest.mark.parametrize("given,temperature", [
+    ([], 0.0), (["--num-samples", "8", "--top-k", "50", "--top-p", "0.9", "--min-p", "0.02"], 1.0),
+    (["--num-samples", "2"], 1.0), (["--top-k", "5"], 1.0), (["--top-p", "0.9"], 1.0), (["--min-p", "0.1"], 1.0),
+    (["--top-k", "5", "--temperature", "0.5"], 0.5), (["--num-samples", "2", "--temperature", "0"], 0.0),
+    (["--temperature", "0.7"], 0.7)])
+def test_default_temperature(monkeypatch, given, temperature):
+    """Samples and filters draw unless --temperature 0 asks for greedy tokens."""
+    seen = []
+    monkeypatch.setattr(generate, "generate_text", lambda args: seen.append(args.temperature) or 0)
+    assert generate.main(["--model-dir", "unread", *given]) == 0
+    assert seen == [temperature]
