@@ -99,7 +99,6 @@ def generate_text(args) -> int:
     print(args.prompt, end="", flush=True)
     prompt = torch.tensor([ids], dtype=torch.int64, device="cuda")
     if args.on_device:
-        print()
         return print_samples(args, model, prompt, tok, eos)
     cache, logits = model.prefill(prompt, len(ids) + args.max_new_tokens)
     if not args.no_stream_layout:
@@ -137,16 +136,35 @@ def random_numbers(args) -> torch.Tensor:
 
 
 def print_samples(args, model, prompt, tok, eos: int) -> int:
-    """--num-samples continuations, each up to its end-of-sequence token."""
+    """--num-samples continuations, each up to its end-of-sequence token.  One is
+    printed token by token, several each as soon as it and those before it have
+    ended; the steps stop with the last of them."""
     if not args.no_stream_layout:
         model.stream_layout()
-    out = model.generate_samples(prompt, random_numbers(args), args.temperature, args.top_k,
-                                 args.top_p, args.min_p).tolist()
-    for i, row in enumerate(out):
-        row = row[:row.index(eos)] if eos in row else row
-        if args.num_samples > 1:
-            print(f"--- {i + 1}")
-        print(tok.decode(row, skip_special_tokens=True))
+    n = args.num_samples
+    rows, running, shown = [[] for _ in range(n)], set(range(n)), 0
+    print(end="" if n == 1 else "\n")
+    steps = model.sample_steps(prompt, random_numbers(args), args.temperature, args.top_k,
+                               args.top_p, args.min_p)
+    for step, ids in enumerate(steps):
+        for i, token in enumerate(ids.view(-1).tolist()):
+            if i not in running:
+                continue
+            if token == eos or token < 0:  # (-1: a row without a token to draw)
+                running.remove(i)
+                continue
+            rows[i].append(token)
+            if n == 1:
+                print(tok.decode([token], skip_special_tokens=True), end="", flush=True)
+        if step + 1 == args.max_new_tokens:
+            running.clear()
+        while n > 1 and shown < n and shown not in running:
+            print(f"--- {shown + 1}\n{tok.decode(rows[shown], skip_special_tokens=True)}", flush=True)
+            shown += 1
+        if not running:
+            break
+    if n == 1:
+        print()
     return 0
 
 

@@ -458,6 +458,15 @@ class Llama:
         keys are stored once.  ids [B, S] (with lengths, as extend): each sequence's
         own text behind the prompt.  Settings as ops.sample_rows.  graph: the step
         is captured once and replayed (the same tokens)."""
+        return torch.cat(list(self.sample_steps(prompt, u, temperature, top_k, top_p, min_p, ids,
+                                                lengths, graph)), dim=1)
+
+    def sample_steps(self, prompt: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
+                     top_p=1.0, min_p=0.0, ids: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, graph: bool = True):
+        """generate_samples step by step: an iterator over the steps' tokens [B, 1].
+        A step runs when its tokens are asked for, so a caller that has seen enough
+        (every sequence ended) leaves the rest undone."""
         n_new, B = u.shape
         if n_new < 1 or u.dtype != torch.float32:
             raise ValueError("generate_samples: u is fp32 [n_new, B]")
@@ -466,18 +475,17 @@ class Llama:
         logits = logits.expand(B, -1) if ids is None else self.extend(cache, ids, lengths)
         how = (temperature, top_k, top_p, min_p)
         nxt = ops.sample_rows(logits, u[0].contiguous(), *how).view(B, 1)
-        out = [nxt]
+        yield nxt
         if n_new > 1 and graph:
             sg = SampleGraph(self, cache, nxt, u[1].contiguous(), *how)
-            out.append(sg.ids.clone())
+            yield sg.ids.clone()
             for i in range(2, n_new):
                 sg.replay(u[i])
-                out.append(sg.ids.clone())
+                yield sg.ids.clone()
         for i in range(1, n_new if not graph else 0):
             logits = self.decode_step(cache, nxt)
             nxt = ops.sample_rows(logits, u[i].contiguous(), *how).view(B, 1)
-            out.append(nxt)
-        return torch.cat(out, dim=1)
+            yield nxt
 
     def generate(self, prompt: torch.Tensor, n_new: int) -> torch.Tensor:
         """Greedy decoding with the KV cache -> generated ids [B, n_new]."""

@@ -193,3 +193,46 @@ def test_default_temperature(monkeypatch, given, temperature):
     monkeypatch.setattr(generate, "generate_text", lambda args: seen.append(args.temperature) or 0)
     assert generate.main(["--model-dir", "unread", *given]) == 0
     assert seen == [temperature]
+
+
+class _Words:
+    def decode(self, ids, skip_special_tokens=True):
+        return " ".join(f"w{i}" for i in ids)
+
+
+class _Steps:
+    """A model of given tokens: what a step's tokens found printed, and how many ran."""
+
+    def __init__(self, steps, out):
+        self.steps, self.out, self.printed = steps, out, []
+
+    def stream_layout(self):
+        pass
+
+    def sample_steps(self, *a):
+        for row in self.steps:
+            self.printed.append(self.out.getvalue())
+            yield torch.tensor(row).view(-1, 1)
+
+
+@pytest.mark.parametrize("steps,text,printed", [
+    # one: printed as it is drawn, up to the end of sequence
+    ([[5], [7], [2], [9]], "w5w7\n", ["", "w5", "w5w7"]),
+    ([[5], [7]], "w5w7\n", ["", "w5"]),
+    ([[2], [7]], "\n", [""]),
+    ([[-1], [7]], "\n", [""]),  # no token to draw
+    # several: in their order, each once it has ended
+    ([[5, 6, 2], [2, 7, 9], [8, 2, 9], [1, 1, 1]], "\n--- 1\nw5\n--- 2\nw6 w7\n--- 3\n\n",
+     ["\n", "\n", "\n--- 1\nw5\n"]),
+    ([[5, 6], [2, 7], [8, 8]], "\n--- 1\nw5\n--- 2\nw6 w7 w8\n", ["\n", "\n", "\n--- 1\nw5\n"]),
+])
+def test_print_samples(monkeypatch, steps, text, printed):
+    """Output while it runs, and no step after the last sequence's end."""
+    monkeypatch.setattr(generate, "random_numbers", lambda args: None)
+    args = generate.argparse.Namespace(no_stream_layout=True, num_samples=len(steps[0]), temperature=1.0,
+                                       top_k=0, top_p=1.0, min_p=0.0, max_new_tokens=len(steps))
+    buf = io.StringIO()
+    model = _Steps(steps, buf)
+    with redirect_stdout(buf):
+        assert generate.print_samples(args, model, None, _Words(), 2) == 0
+    assert buf.getvalue() == text and model.printed == printed

@@ -276,3 +276,21 @@ def test_preset_with_samples(cuda, monkeypatch):
                               "4", "--max-new-tokens", "5", "--temperature", "1.0"]) == 0
     line = json.loads(buf.getvalue())
     assert line["num_samples"] == 4 and line["decode_ms_per_step"] > 0
+
+
+def test_sample_steps_stop_with_the_caller(cuda, monkeypatch):
+    """The steps of generate_samples, run as their tokens are asked for."""
+    m = model_of(BF)
+    u = u_of(9, 3)
+    want = m.generate_samples(ids_of(1, 12), u, 0.9)
+    replays = []
+    replay = llama.SampleGraph.replay
+    monkeypatch.setattr(llama.SampleGraph, "replay", lambda self, u: replays.append(1) or replay(self, u))
+    for graph in (True, False):
+        got = []
+        for ids in m.sample_steps(ids_of(1, 12), u, 0.9, graph=graph):
+            got.append(ids)
+            if len(got) == 5:
+                break
+        assert torch.equal(torch.cat(got, 1), want[:, :5])
+    assert len(replays) == 3
