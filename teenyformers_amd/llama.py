@@ -576,6 +576,9 @@ class DecodeGraph:
 
     def __init__(self, model: Llama, cache: KVCache, ids: torch.Tensor,
                  trace: list | None = None):
+        if cache.length >= cache.capacity:
+            # (the position is the device's: no kernel of the first step refuses it)
+            raise RuntimeError("KV cache is full")
         self.model, self.cache = model, cache
         self.ids = ids.to(torch.int64).clone()
         lengths = getattr(cache, "lengths", None)  # (a copy: replays move it on)

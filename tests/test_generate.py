@@ -236,3 +236,15 @@ def test_print_samples(monkeypatch, steps, text, printed):
     with redirect_stdout(buf):
         assert generate.print_samples(args, model, None, _Words(), 2) == 0
     assert buf.getvalue() == text and model.printed == printed
+
+
+@pytest.mark.parametrize("graph", [llama.DecodeGraph, llama.SampleGraph])
+@pytest.mark.parametrize("lengths", [None, torch.tensor([3, 8], dtype=torch.int32)], ids=["one", "each"])
+def test_no_captured_step_over_a_full_cache(graph, lengths):
+    """Refused before the first step runs, as replay() refuses the next."""
+    from types import SimpleNamespace
+    cache = SimpleNamespace(length=8, capacity=8, lengths=lengths, k=[torch.zeros(2, 1, 8, 64)])
+    u = () if graph is llama.DecodeGraph else (torch.zeros(2),)
+    with pytest.raises(RuntimeError, match="full"):
+        graph(None, cache, torch.zeros((2, 1), dtype=torch.int64), *u)
+    assert cache.length == 8

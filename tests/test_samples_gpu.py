@@ -294,3 +294,20 @@ def test_sample_steps_stop_with_the_caller(cuda, monkeypatch):
                 break
         assert torch.equal(torch.cat(got, 1), want[:, :5])
     assert len(replays) == 3
+
+
+@pytest.mark.parametrize("lengths", [None, torch.tensor([1, 4])], ids=["one", "each"])
+def test_a_full_cache_takes_no_captured_step(cuda, lengths):
+    """Prompts that fill the sequences' rows: no step draws from keys without its own."""
+    m = model_of(BF)
+    cache, _ = m.share_prefix(ids_of(1, 5), 2, 4)
+    m.extend(cache, ids_of(2, 4), lengths)
+    nxt, u = ids_of(2, 1), u_of(1, 2)[0]
+    with pytest.raises(RuntimeError, match="full"):
+        llama.SampleGraph(m, cache, nxt, u)
+    with pytest.raises(RuntimeError, match="full"):
+        llama.DecodeGraph(m, cache, nxt)
+    assert cache.length == 4
+    plain, _ = m.prefill(ids_of(2, 6), 6)
+    with pytest.raises(RuntimeError, match="full"):
+        llama.DecodeGraph(m, plain, nxt)
