@@ -176,18 +176,18 @@ def bench_samples(args, model, ids) -> int:
         model.stream_layout()
     how = (args.temperature, args.top_k, args.top_p, args.min_p)
     first = ops.sample_rows(logits.expand(args.num_samples, -1), u[0], *how).view(-1, 1)
-    ms = 0.0
-    if args.max_new_tokens > 1:
+    ms = None  # of a replayed step, if there is one
+    if args.max_new_tokens > 2:
         sg = llama.SampleGraph(model, cache, first, u[1], *how)
         torch.cuda.synchronize()
         t0 = time.perf_counter()
         for i in range(2, args.max_new_tokens):
             sg.replay(u[i])
         torch.cuda.synchronize()
-        ms = (time.perf_counter() - t0) * 1e3 / max(1, args.max_new_tokens - 2)
+        ms = (time.perf_counter() - t0) * 1e3 / (args.max_new_tokens - 2)
     print(json.dumps({"preset": args.preset, "num_samples": args.num_samples,
                       "prompt_len": args.prompt_len, "new_tokens": args.max_new_tokens,
-                      "decode_ms_per_step": round(ms, 3),
+                      "decode_ms_per_step": round(ms, 3) if ms else None,
                       "decode_tokens_per_s": round(args.num_samples / ms * 1e3, 1) if ms else None}),
           flush=True)
     return 0

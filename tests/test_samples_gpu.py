@@ -311,3 +311,18 @@ def test_a_full_cache_takes_no_captured_step(cuda, lengths):
     plain, _ = m.prefill(ids_of(2, 6), 6)
     with pytest.raises(RuntimeError, match="full"):
         llama.DecodeGraph(m, plain, nxt)
+
+
+@pytest.mark.parametrize("n_new", [1, 2, 3])
+def test_preset_rates_are_of_steps_that_ran(cuda, monkeypatch, n_new):
+    """The first two tokens come before the first replay, whose time is printed."""
+    monkeypatch.setitem(generate.PRESETS, "tiny", dict(TINY))
+    buf = io.StringIO()
+    with redirect_stdout(buf):
+        assert generate.main(["--preset", "tiny", "--batch", "1", "--prompt-len", "20", "--num-samples",
+                              "4", "--max-new-tokens", str(n_new)]) == 0
+    line = json.loads(buf.getvalue())
+    if n_new < 3:
+        assert line["decode_ms_per_step"] is None and line["decode_tokens_per_s"] is None
+    else:
+        assert line["decode_ms_per_step"] > 0 and line["decode_tokens_per_s"] > 0
