@@ -497,7 +497,7 @@ def qkv_rope_split(qkv, q_out, k_cache, v_cache, pos0, n_heads_q: int, n_heads_k
     captured graphs).  q_out None (a dense qkv only): the caches only.
     Behind a shared prefix (shared_prefix_attention): rope_offset, the prefix's
     length, is added to the rotary positions (not to the rows), and pos0 may hold
-    a value per sequence."""
+    a value per sequence; q_out is required there."""
     if rope_offset or isinstance(pos0, torch.Tensor) and pos0.numel() > 1:
         return _qkv_rope_split_rows(qkv, q_out, k_cache, v_cache, pos0, n_heads_q, n_heads_kv,
                                     rope_base, rope_offset)
@@ -531,7 +531,13 @@ def _qkv_rope_split_rows(qkv, q_out, k_cache, v_cache, pos0, n_heads_q: int, n_h
                          rope_base: float, rope_offset: int):
     parts = isinstance(qkv, Partials)
     src = qkv.slabs if parts else qkv
+    if q_out is None:
+        raise ValueError("qkv_rope_split: behind a prefix, or with a position per sequence, q_out is "
+                         "required")
     _dev(src, q_out, k_cache, v_cache)
+    dev = q_out.get_device()
+    if any(t.get_device() != dev for t in (src, k_cache, v_cache)):
+        raise ValueError("qkv_rope_split: all tensors are on one device")
     B, S, W = qkv.shape
     D, L = k_cache.shape[3], k_cache.shape[2]
     if (W != (n_heads_q + 2 * n_heads_kv) * D or q_out.shape != (B, n_heads_q, S, D)
@@ -541,10 +547,10 @@ def _qkv_rope_split_rows(qkv, q_out, k_cache, v_cache, pos0, n_heads_q: int, n_h
     if qkv.dtype != q_out.dtype or k_cache.dtype != q_out.dtype or v_cache.dtype != q_out.dtype:
         raise TypeError("qkv_rope_split: qkv, q_out and the caches share a dtype")
     row0, host = (pos0, 0) if isinstance(pos0, torch.Tensor) else (None, int(pos0))
-    if row0 is not None and (row0.dtype != torch.int32 or not row0.is_cuda
+    if row0 is not None and (row0.dtype != torch.int32 or row0.get_device() != dev
                              or row0.numel() not in (1, B) or not row0.is_contiguous()):
         raise TypeError("a device position must be an int32 CUDA tensor of one value or one per "
-                        "sequence")
+                        "sequence, on q_out's device")
     with _on_device_of(q_out):
         call("teeny_qkv_rope_split_rows", None if parts else _p(src), _p(src) if parts else None,
              qkv.n if parts else 0, _p(q_out), _p(k_cache), _p(v_cache), B, S, _p(row0),

@@ -481,3 +481,17 @@ def test_generate_command_refuses(capsys):
                 ["--min-p", "-0.1"], ["--min-p", "2"], ["--temperature", "-1"], ["--temperature", "nan"]):
         with pytest.raises(SystemExit):
             generate.main(["--preset", "llama3-8b", *bad])
+
+
+def test_qkv_split_behind_a_prefix_needs_q():
+    """ops.qkv_rope_split without q_out is the prompt's form: refused by name elsewhere."""
+    import torch
+
+    from teenyformers_amd import ops
+    qkv, cache = torch.zeros(2, 1, 512), torch.zeros(2, 2, 4, 64)
+    for kw in (dict(pos0=0, rope_offset=5), dict(pos0=torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="q_out is required"):
+            ops.qkv_rope_split(qkv, None, cache, cache, n_heads_q=4, n_heads_kv=2, rope_base=1e4, **kw)
+    # (a tensor elsewhere than on a GPU is refused as before)
+    with pytest.raises(ValueError, match="device"):
+        ops.qkv_rope_split(qkv, torch.zeros(2, 4, 1, 64), cache, cache, 0, 4, 2, 1e4, rope_offset=5)
