@@ -650,7 +650,9 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: i
     shape = q.shape
     if len(shape) not in (3, 4):
         raise ValueError("shared_prefix_attention: q is [B, Hq, D] or [B, Hq, S, D]")
-    if k_prefix.dim() == 4 and k_prefix.shape[0] == 1 and v_prefix.dim() == 4:
+    if k_prefix.shape != v_prefix.shape:
+        raise ValueError("shared_prefix_attention: k_prefix and v_prefix are of one shape")
+    if k_prefix.dim() == 4 and k_prefix.shape[0] == 1:
         k_prefix, v_prefix = k_prefix[0], v_prefix[0]
     B, Hq, D = shape[0], shape[1], shape[-1]
     S = shape[2] if len(shape) == 4 else 1
@@ -666,7 +668,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: i
     if len(kc) != 4 or kc != v_cache.shape or kc[0] != B or kc[3] != D:
         raise ValueError("shared_prefix_attention: the caches are [B, Hkv, L, D] matching q")
     Hkv, L = kc[1], kc[2]
-    if len(kp) != 3 or kp != v_prefix.shape or kp[0] != Hkv or kp[2] != D:
+    if len(kp) != 3 or kp[0] != Hkv or kp[2] != D:
         raise ValueError("shared_prefix_attention: the prefix is [Hkv, Lp, D] matching the caches")
     if not 0 <= n_prefix <= kp[1]:
         raise ValueError("shared_prefix_attention: n_prefix must lie in the prefix's rows")

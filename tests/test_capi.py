@@ -495,3 +495,15 @@ def test_qkv_split_behind_a_prefix_needs_q():
     # (a tensor elsewhere than on a GPU is refused as before)
     with pytest.raises(ValueError, match="device"):
         ops.qkv_rope_split(qkv, torch.zeros(2, 4, 1, 64), cache, cache, 0, 4, 2, 1e4, rope_offset=5)
+
+
+def test_shared_prefix_of_two_shapes():
+    """A prefix's K and V are one cache's: V of two sequences is refused, not cut."""
+    import torch
+
+    from teenyformers_amd import ops
+    q, c = torch.zeros(2, 4, 64), torch.zeros(2, 2, 8, 64)
+    k, v = torch.zeros(1, 2, 5, 64), torch.zeros(2, 2, 5, 64)
+    for a, b in ((k, v), (v, k), (k, k[0]), (k[0], k), (k, k[:, :, :4])):
+        with pytest.raises(ValueError, match="of one shape"):
+            ops.shared_prefix_attention(q, a, b, c, c, 5, 0)
