@@ -445,7 +445,7 @@ class Llama:
         h = self.hidden(ids, cache, 0)
         if lengths is None:
             return self.logits(h[:, -1])
-        lengths = lengths.to(device=ids.device, dtype=torch.int32)
+        lengths = lengths.to(device=ids.device, dtype=torch.int32, copy=True)  # (the cache's own)
         cache.lengths, cache.length = lengths, int(lengths.max())
         rows = (lengths.to(torch.int64) - 1).view(B, 1, 1).expand(B, 1, h.shape[2])
         return self.logits(h.gather(1, rows)[:, 0])

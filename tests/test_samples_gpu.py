@@ -326,3 +326,18 @@ def test_preset_rates_are_of_steps_that_ran(cuda, monkeypatch, n_new):
         assert line["decode_ms_per_step"] is None and line["decode_tokens_per_s"] is None
     else:
         assert line["decode_ms_per_step"] > 0 and line["decode_tokens_per_s"] > 0
+
+
+def test_extend_keeps_lengths_of_its_own(cuda):
+    """The caller's int32 lengths may change after the call."""
+    m = model_of(F32)
+    own, lengths = ids_of(3, 6, seed=3), torch.tensor([6, 2, 4], dtype=torch.int32, device="cuda")
+    nxt, out = ids_of(3, 1, seed=4), []
+    for change in (0, 1):
+        cache, _ = m.share_prefix(ids_of(1, 9), 3, 8)
+        given = lengths.clone()
+        m.extend(cache, own, given)
+        given += change
+        out.append(m.decode_step(cache, nxt))
+        assert cache.lengths.tolist() == [7, 3, 5]
+    assert torch.equal(*out)
