@@ -796,6 +796,8 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
     if ms is None and not 0.0 <= m <= 1.0:
         raise ValueError("sample_rows: min_p must be in [0, 1]")
     if rows == 0:
+        if advance is not None:
+            advance.add_(1)
         return out
     if workspace is None:
         size = _lib.lib().teeny_sample_rows_workspace_bytes(rows, V)

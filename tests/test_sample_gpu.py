@@ -383,3 +383,10 @@ def test_borders_among_a_few_equal_tokens(cuda, dtype, n):
     for p in (0.3, 0.8, 0.9, 0.97):
         check(x, u, p=p)
         check(x, u, T=0.5, p=p)
+
+
+def test_a_batch_without_rows_moves_the_position_on(cuda):
+    x, u = make(2, 10, torch.float32, 1, cuda)
+    pos = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert ops.sample_rows(x[:0], u[:0], advance=pos).shape == (0,) and int(pos) == 1
+    assert ops.sample_rows(x, u, advance=pos).shape == (2,) and int(pos) == 2
