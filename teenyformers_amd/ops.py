@@ -692,15 +692,15 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: i
           or out.get_device() != dev or not out.is_contiguous()):
         raise ValueError("shared_prefix_attention: out must be contiguous, of the result's shape, "
                          "type and device")
-    if workspace is None:
-        need = _lib.lib().teeny_shared_prefix_attention_workspace_bytes(B, Hq, Hkv, S, n_prefix, L, D,
-                                                                        code)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.get_device() != dev or not workspace.is_contiguous():
+    if workspace is not None and (workspace.get_device() != dev or not workspace.is_contiguous()):
         raise ValueError("shared_prefix_attention: workspace must be contiguous, on q's device")
-    size = 0 if workspace is None else workspace.numel() * workspace.element_size()
     with _on_device_of(q):
+        if workspace is None:  # (asked on q's device: the shares go by its CUs)
+            need = _lib.lib().teeny_shared_prefix_attention_workspace_bytes(B, Hq, Hkv, S, n_prefix, L,
+                                                                            D, code)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        size = 0 if workspace is None else workspace.numel() * workspace.element_size()
         call("teeny_shared_prefix_attention", _p(q), _p(k_prefix), _p(v_prefix), _p(k_cache),
              _p(v_cache), _p(out), B, Hq, Hkv, S, n_prefix, kp[1], _p(past), stride, past_host, L, D,
              scale, int(bool(merged)), code, _p(workspace), size, _stream())

@@ -381,3 +381,26 @@ def test_negative_lengths_behind_a_prefix(cuda, dtype, S, Hq, Hkv, D, more, shar
     assert (need > 0) == (shares and not (dtype == F32 and P + L <= 128))
     got = check(make(cuda, dtype, len(past), Hq, Hkv, S, D, P, L, prefix_len=P + 2), P, past, S)
     assert (got != 0).any(3).all()
+
+
+def test_workspace_is_sized_on_the_device_of_the_launch(cuda, monkeypatch):
+    """The shares go by the device's CUs, so both are asked of q's device."""
+    from types import SimpleNamespace
+    ts = make(cuda, BF, 2, 8, 2, 1, 64, 700, 3000)
+    want = ops.shared_prefix_attention(*ts, 700, 50)
+    on = []
+
+    class Device:
+        def __enter__(self):
+            on.append(True)
+
+        def __exit__(self, *a):
+            on.clear()
+
+    need, here = ops._lib.lib().teeny_shared_prefix_attention_workspace_bytes, []
+    lib = SimpleNamespace(
+        teeny_shared_prefix_attention_workspace_bytes=lambda *a: here.append(bool(on)) or need(*a))
+    monkeypatch.setattr(ops, "_on_device_of", lambda t: Device())
+    monkeypatch.setattr(ops, "_lib", SimpleNamespace(lib=lambda: lib))
+    assert torch.equal(ops.shared_prefix_attention(*ts, 700, 50), want)
+    assert here == [True]
