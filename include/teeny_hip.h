@@ -430,9 +430,13 @@ int teeny_argmax_rows_advance(const void* x, int64_t* out, int rows, int cols, i
  * temperature 0 takes the first of the order (the lowest index of the maximum,
  * where teeny_argmax_rows takes the last).  -inf and NaN logits are never drawn;
  * a row with no other gives -1; +inf logits share a row among themselves.
- * Probabilities are held as whole numbers of 2^-44 of the row's largest and
- * summed exactly: the result does not depend on timing or on the other rows, and
- * a token below 2^-45 of the most probable one is not drawn.
+ * Probabilities are held as whole numbers of 2^-44 of a reference and summed
+ * exactly: the result does not depend on timing or on the other rows, and a token
+ * below 2^-45 of its reference is not drawn.  The reference is the row's largest
+ * probability where a filter is set.  Without any it is the largest of the token's
+ * chunk, 8192 columns counted from the 16-byte boundary at or before the row; a
+ * chunk's sum is then a whole number of 2^-44 of the row's largest, so that a chunk
+ * whose sum is below 2^-45 of it is not drawn from.
  * Each setting is a value for every row, or (temperature_rows, ... not null) one
  * per row in device memory, read when the kernel runs: there a temperature that
  * is not above 0 counts as 0, a top_k below 1 as off, a top_p not below 1 as

@@ -404,3 +404,18 @@ def test_workspace_is_sized_on_the_device_of_the_launch(cuda, monkeypatch):
     monkeypatch.setattr(ops, "_lib", SimpleNamespace(lib=lambda: lib))
     assert torch.equal(ops.shared_prefix_attention(*ts, 700, 50), want)
     assert here == [True]
+
+
+# of each size: one token, a few, prompts; the keys' shares or a walk without them
+REPEATED = [(BF, 16, 32, 8, 1, 128, 2048, 128, 101), (BF, 4, 32, 8, 1, 128, 32000, 320, 257),
+            (BF, 32, 16, 16, 1, 64, 1021, 320, 300), (BF, 8, 32, 8, 5, 128, 3001, 128, 90),
+            (BF, 8, 32, 8, 257, 128, 4096, 320, 0), (F32, 4, 4, 4, 1, 64, 61, 64, 8),
+            (F32, 4, 8, 8, 3, 64, 700, 300, 200)]
+
+
+@pytest.mark.parametrize("dtype,B,Hq,Hkv,S,D,P,L,past", REPEATED, ids=[str(c[1:]) for c in REPEATED])
+def test_calls_repeat_themselves(cuda, dtype, B, Hq, Hkv, S, D, P, L, past):
+    """The same bits each time: shares are merged in one order, without atomics."""
+    ts = make(cuda, dtype, B, Hq, Hkv, S, D, P, L)
+    want = ops.shared_prefix_attention(*ts, P, past)
+    assert all(torch.equal(ops.shared_prefix_attention(*ts, P, past), want) for _ in range(10))

@@ -390,3 +390,38 @@ def test_a_batch_without_rows_moves_the_position_on(cuda):
     pos = torch.zeros(1, dtype=torch.int32, device="cuda")
     assert ops.sample_rows(x[:0], u[:0], advance=pos).shape == (0,) and int(pos) == 1
     assert ops.sample_rows(x, u, advance=pos).shape == (2,) and int(pos) == 2
+
+
+@pytest.mark.parametrize("k", [200, 215, 230, 300, 512, 513])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_top_k_around_what_the_chunks_write_out(cuda, dtype, k):
+    """16 chunks of 128256 columns write out k tokens each and more: what the draw
+    takes in at k = 200, not at 300 (it passes over the row), and weighs by bins
+    from 513 on."""
+    x, u = make(4, 128256, dtype, 43, cuda)
+    for how in (dict(), dict(p=0.9), dict(T=0.5, m=0.01), dict(T=1.3, p=0.95, m=0.002)):
+        check(x, u, k=k, **how)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_least_weight_that_is_drawn(cuda, dtype):
+    """Without filters down to 2^-45 of the largest of the token's 8192 columns, with
+    them to 2^-45 of the row's."""
+    x = torch.full((3, 20000), -100.0, device="cuda")
+    x[:, 9000] = 0.0
+    x[:, 5] = -30.0
+    x[:, 0] = torch.tensor([-70.0, -77.0, -44.0], device="cuda")
+    u = torch.zeros(3, device="cuda")
+    for scale in (1.0, 0.5):  # the logits in octaves
+        T = scale / np.log(2.0)
+        y = (x * scale).to(dtype)
+        assert ops.sample_rows(y, u, T).tolist() == [0, 5, 0]
+        assert ops.sample_rows(y, u, T, top_k=19999).tolist() == [5, 5, 0]
+
+
+@pytest.mark.parametrize("rows", [1, 16, 300])
+def test_calls_repeat_themselves(cuda, rows):
+    x, u = make(rows, 128256, torch.bfloat16, 47, cuda)
+    for how in (dict(), dict(top_k=50, top_p=0.9), dict(top_k=300), dict(top_p=0.95), dict(min_p=0.01)):
+        want = ops.sample_rows(x, u, 1.3, **how)
+        assert all(torch.equal(ops.sample_rows(x, u, 1.3, **how), want) for _ in range(5))
