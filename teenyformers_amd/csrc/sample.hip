@@ -32,7 +32,7 @@
 //          The chunk's maximum, and its weight by 512 columns.  With filters: its
 //          tokens weighed and counted by bins below the chunk's maximum, in LDS,
 //          and the tokens of its first bins, up to 1024, written out bin by bin,
-//          so that the draw reads those alone.  A top-k of up to 512 needs no more
+//          so that the draw reads those alone.  A small top-k needs no more
 //          than the chunk's own first k and no weight: the largest token of each
 //          vector of 8 says from which bin on none of them lies, and a wavefront
 //          goes over the others only (16 rows 7.1 -> 5.5 us).
@@ -70,7 +70,8 @@ constexpr int kMaxChunks = 64;            // a lane each
 constexpr int kBins = 180;                // quarter octaves below the row's maximum: 45 octaves
 constexpr int kFirstBins = 48;            // of them those that are counted first: 12 octaves
 constexpr int kCand = 1024;               // tokens that a chunk writes out
-constexpr int kSmallK = 512;              // a top-k that the chunk's own first k settle
+constexpr int kSmallK = 512;              // a top-k that the chunk's own first k settle ...
+constexpr int kFewTokens = 3200;          // ... k times the chunks
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr int kFrac = 44;                 // fraction bits of a weight
 constexpr u64 kLow52 = (1ull << 52) - 1;
@@ -96,7 +97,7 @@ struct Settings {
   double p, lmin;  // top-p; log2(min_p), -inf without
   int k;
   bool fk, fp, filters;
-  bool few;        // a top-k of up to kSmallK: the chunks' first tokens alone
+  bool few;        // a small top-k: the chunks' first tokens alone
 };
 
 // One row's settings: a value for all rows, or a device array of one per row.
@@ -122,7 +123,13 @@ DEVI Settings settings(const Args& a, int row, int cols) {
   s.p = p > 0.0 ? p : 0.0;
   s.lmin = m > 0.0 && !greedy ? (m < 1.0 ? log2(m) : 0.0) : -INFINITY;
   s.filters = s.fk || s.fp || s.lmin > -INFINITY;
-  s.few = s.fk && k <= kSmallK;
+  // Small: up to kSmallK, and the draw's list takes the first k of all chunks and the
+  // rest of the bin that completes each chunk's.  us by this way and by bins, bf16 (fp32)
+  // x 128256, 16 chunks: 16 rows with k = 50 14.7, 21.9 (16.6, 22.8), 165 19.7, 22.1, 200
+  // 20.5, 22.4 (22.6, 24.3); 64 rows with 200 26.7, 32.9; 16 x 32001 with 512 22.9, 19.9.
+  // Where they do not fit this way passes over the row: with 225 and more of 16 chunks
+  // 172, by bins 22.6.
+  s.few = s.fk && k <= kSmallK && k * ((cols + 7 + kChunk - 1) / kChunk) <= kFewTokens;
   return s;
 }
 
@@ -467,6 +474,7 @@ constexpr int kDraw = 512, kDrawWaves = kDraw / 64;
 constexpr int kSub = 1024;      // sub-bins of the radix select
 constexpr int kList = 4096;     // tokens collected in LDS
 constexpr int kMost = kList - kSmallK;  // ... for a small top-k, what it leaves behind them
+static_assert(kFewTokens < kMost, "");
 constexpr int kCell = 64, kCells = kChunk / kCell;  // columns of a chunk's cells
 
 // A pass over (a part of) the row, by the workgroup, for its tokens between two

@@ -395,9 +395,8 @@ def test_a_batch_without_rows_moves_the_position_on(cuda):
 @pytest.mark.parametrize("k", [200, 215, 230, 300, 512, 513])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_top_k_around_what_the_chunks_write_out(cuda, dtype, k):
-    """16 chunks of 128256 columns write out k tokens each and more: what the draw
-    takes in at k = 200, not at 300 (it passes over the row), and weighs by bins
-    from 513 on."""
+    """16 chunks of 128256 columns: the draw takes in what they write out for a k of
+    200, and weighs larger ones by bins."""
     x, u = make(4, 128256, dtype, 43, cuda)
     for how in (dict(), dict(p=0.9), dict(T=0.5, m=0.01), dict(T=1.3, p=0.95, m=0.002)):
         check(x, u, k=k, **how)
@@ -425,3 +424,12 @@ def test_calls_repeat_themselves(cuda, rows):
     for how in (dict(), dict(top_k=50, top_p=0.9), dict(top_k=300), dict(top_p=0.95), dict(min_p=0.01)):
         want = ops.sample_rows(x, u, 1.3, **how)
         assert all(torch.equal(ops.sample_rows(x, u, 1.3, **how), want) for _ in range(5))
+
+
+@pytest.mark.parametrize("how", [dict(k=1), dict(k=300, p=0.5), dict(k=500, m=0.99), dict(k=500, p=0.7, m=0.985)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,spread", [(8000, 0.01), (40000, 0.01), (49000, 0.3), (49000, 0.002)])
+def test_small_top_k_of_flat_rows(cuda, V, spread, dtype, how):
+    """Chunks whose first bins hold more than they write out: passes over the row."""
+    x, u = make(3, V, dtype, 53, cuda, zipf=False)
+    check(x * spread, u, **how)
