@@ -137,13 +137,18 @@ def random_numbers(args) -> torch.Tensor:
 
 def print_samples(args, model, prompt, tok, eos: int) -> int:
     """--num-samples continuations, each up to its end-of-sequence token.  One is
-    printed token by token, several each as soon as it and those before it have
+    printed as it is drawn, several each as soon as it and those before it have
     ended; the steps stop with the last of them."""
     if not args.no_stream_layout:
         model.stream_layout()
     n = args.num_samples
     rows, running, shown = [[] for _ in range(n)], set(range(n)), 0
+    begin = 0  # (one: tokens up to shown are printed, those from begin on are context)
     print(end="" if n == 1 else "\n")
+
+    def text(tokens):
+        return tok.decode(tokens, skip_special_tokens=True)
+
     steps = model.sample_steps(prompt, random_numbers(args), args.temperature, args.top_k,
                                args.top_p, args.min_p)
     for step, ids in enumerate(steps):
@@ -154,13 +159,18 @@ def print_samples(args, model, prompt, tok, eos: int) -> int:
                 running.remove(i)
                 continue
             rows[i].append(token)
-            if n == 1:
-                print(tok.decode([token], skip_special_tokens=True), end="", flush=True)
         if step + 1 == args.max_new_tokens:
             running.clear()
         while n > 1 and shown < n and shown not in running:
-            print(f"--- {shown + 1}\n{tok.decode(rows[shown], skip_special_tokens=True)}", flush=True)
+            print(f"--- {shown + 1}\n{text(rows[shown])}", flush=True)
             shown += 1
+        if n == 1:
+            # what the new tokens add to the text of the last ones (a token's own text
+            # may lack a space, or hold a part of a character)
+            now = text(rows[0][begin:])
+            if not (running and now.endswith("\ufffd")):
+                print(now[len(text(rows[0][begin:shown])):], end="", flush=True)
+                begin, shown = shown, len(rows[0])
         if not running:
             break
     if n == 1:

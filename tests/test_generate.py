@@ -217,8 +217,8 @@ class _Steps:
 
 @pytest.mark.parametrize("steps,text,printed", [
     # one: printed as it is drawn, up to the end of sequence
-    ([[5], [7], [2], [9]], "w5w7\n", ["", "w5", "w5w7"]),
-    ([[5], [7]], "w5w7\n", ["", "w5"]),
+    ([[5], [7], [8], [2], [9]], "w5 w7 w8\n", ["", "w5", "w5 w7", "w5 w7 w8"]),
+    ([[5], [7]], "w5 w7\n", ["", "w5"]),
     ([[2], [7]], "\n", [""]),
     ([[-1], [7]], "\n", [""]),  # no token to draw
     # several: in their order, each once it has ended
@@ -248,3 +248,27 @@ def test_no_captured_step_over_a_full_cache(graph, lengths):
     with pytest.raises(RuntimeError, match="full"):
         graph(None, cache, torch.zeros((2, 1), dtype=torch.int64), *u)
     assert cache.length == 8
+
+
+class _Bytes:
+    """Tokens that are bytes of UTF-8."""
+
+    def decode(self, ids, skip_special_tokens=True):
+        return bytes(ids).decode("utf-8", errors="replace")
+
+
+@pytest.mark.parametrize("data", ["a\u00e9b", "\u20ac\u20ac x", "\u00e9"])
+@pytest.mark.parametrize("cut", [0, 1])
+def test_print_one_sample_of_parts_of_characters(monkeypatch, data, cut):
+    """Characters of several tokens come whole; a part is printed at the end alone."""
+    monkeypatch.setattr(generate, "random_numbers", lambda args: None)
+    ids = list(data.encode())
+    ids = ids[:len(ids) - cut]
+    args = generate.argparse.Namespace(no_stream_layout=True, num_samples=1, temperature=1.0, top_k=0,
+                                       top_p=1.0, min_p=0.0, max_new_tokens=len(ids))
+    buf = io.StringIO()
+    model = _Steps([[i] for i in ids], buf)
+    with redirect_stdout(buf):
+        assert generate.print_samples(args, model, None, _Bytes(), -5) == 0
+    assert buf.getvalue() == _Bytes().decode(ids) + "\n"
+    assert not any("\ufffd" in p for p in model.printed)

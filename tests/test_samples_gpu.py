@@ -341,3 +341,30 @@ def test_extend_keeps_lengths_of_its_own(cuda):
         out.append(m.decode_step(cache, nxt))
         assert cache.lengths.tolist() == [7, 3, 5]
     assert torch.equal(*out)
+
+
+def test_command_draws_one_sample(cuda, tmp_path, monkeypatch):
+    """One sample behind its prompt's text, up to its end; no step follows it."""
+    from tokenizers import Tokenizer, models, pre_tokenizers
+
+    from tests.test_generate import _hf_tensors, _write_checkpoint
+    cfg = llama.LlamaConfig(**TINY)
+    _write_checkpoint(str(tmp_path), cfg, _hf_tensors(cfg, seed=3))
+    tok = Tokenizer(models.WordLevel({f"w{i}": i for i in range(cfg.vocab_size)}, unk_token="w0"))
+    tok.pre_tokenizer = pre_tokenizers.Whitespace()
+    tok.save(str(tmp_path / "tokenizer.json"))
+    m = llama.Llama(cfg, llama.load_hf_weights(cfg, str(tmp_path)))
+    row = m.generate_samples(torch.tensor([[5, 17, 3]], device="cuda"), u_of(9, 1, seed=7), 1.0, 40).tolist()[0]
+    replays = []
+    replay = llama.SampleGraph.replay
+    monkeypatch.setattr(llama.SampleGraph, "replay", lambda self, u: replays.append(1) or replay(self, u))
+    for eos in (None, row[4]):
+        replays.clear()
+        monkeypatch.setattr(generate, "eos_id", lambda t: -5 if eos is None else eos)
+        buf = io.StringIO()
+        with redirect_stdout(buf):
+            assert generate.main(["--model-dir", str(tmp_path), "--prompt", "w5 w17 w3", "--max-new-tokens",
+                                  "9", "--top-k", "40", "--seed", "7"]) == 0
+        end = 9 if eos is None else row.index(eos)
+        assert buf.getvalue() == "w5 w17 w3" + tok.decode(row[:end]) + "\n"
+        assert len(replays) == (7 if eos is None else max(0, end - 1))
