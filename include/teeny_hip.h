@@ -569,6 +569,61 @@ int teeny_qkv_rope_split_rows(const void* qkv, const float* parts, int n_parts, 
                               int rope_offset, int cache_len, int n_heads_q, int n_heads_kv,
                               int head_dim, float ln_rope_base, int dtype, hipStream_t stream);
 
+/* A cache in pages, which sequences take as they grow and share by reference:
+ * k/v_pages [n_pages, n_heads_kv, page_size, head_dim] (page_size a power of two,
+ * 16 to 1024), key j of sequence b in row j % page_size of page page_table[b
+ * table_ld + j / page_size] (int32 device memory, [batch, table_width] with rows
+ * table_ld apart, read when the kernels run).  Entries outside 0 .. n_pages-1 are
+ * absent pages: nothing is written to them, and their keys do not count (a
+ * table's unused entries; pages given back behind a window).
+ * The new tokens of all sequences are packed: tokens starts[b] .. starts[b+1]-1
+ * are sequence b's (int32 device memory, batch+1 values that do not fall; none
+ * for a sequence is allowed), or with starts null tokens / batch each.  Token i
+ * of sequence b is at position n_past[b] + i (int32 device memory, one value per
+ * sequence; null: n_past_host for all).  Tokens behind starts[batch] are nobody's:
+ * their rows of the outputs are left as they were.  All tensors are 16-byte
+ * aligned; head_dim: fp32 8, 16, 32, 64, 128; bf16 64, 128.
+ *
+ * teeny_paged_qkv_rope_split: the QKV projection's rows (qkv [tokens, (Hq + 2 Hkv)
+ * D], or qkv null and parts, K-split fp32 slabs as teeny_qkv_rope_split_partials_dev
+ * takes them) to q_out [tokens, Hq, D] (rotated) and the rows of their pages (k
+ * rotated, v).  Positions outside the table are not written.  Angles are formed in
+ * 64 bits (ln_rope_base too); the other splits form them in 32, as the reference
+ * does, so far positions differ by up to p 2^-24 radians.
+ *
+ * teeny_paged_attention: o [tokens, Hq, D] = the attention of q [tokens, Hq, D];
+ * token i of sequence b attends to keys 0 .. n_past[b] + i (its own is in its page
+ * already) of the pages that are present, rows without a key give zeros.  Rows of
+ * the pages behind the last key are never read, and a key has no influence on
+ * tokens before it, whatever its values.  max_new: the most new tokens of a
+ * sequence (with more, their rows may be left as they were); max_keys: n_past plus
+ * the new tokens at most, which only picks the number of shares.  workspace:
+ * teeny_paged_attention_workspace_bytes bytes (for max_keys up to table_width *
+ * page_size), 16-byte aligned, that no call on another stream uses meanwhile.
+ * softmax_scale as the forwards'.
+ *
+ * teeny_copy_pages: page to[i] = page from[i] for i < n (host arrays), in each of
+ * `planes` pools plane_bytes apart (a layer's K, a layer's V): what a fork does
+ * with its last page and a compaction with its pages.  Every index lies in the
+ * pool; a page is written by one pair at most, and not read by another. */
+int teeny_paged_qkv_rope_split(const void* qkv, const float* parts, int n_parts, void* q_out,
+                               void* k_pages, void* v_pages, const int32_t* page_table,
+                               int table_ld, int table_width, const int32_t* starts,
+                               const int32_t* n_past, int n_past_host, int batch, int tokens,
+                               int n_pages, int page_size, int n_heads_q, int n_heads_kv,
+                               int head_dim, double ln_rope_base, int dtype, hipStream_t stream);
+size_t teeny_paged_attention_workspace_bytes(int batch, int tokens, int max_new, int max_keys,
+                                             int n_heads_q, int n_heads_kv, int head_dim,
+                                             int dtype);
+int teeny_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o,
+                          const int32_t* page_table, int table_ld, int table_width,
+                          const int32_t* starts, const int32_t* n_past, int n_past_host, int batch,
+                          int tokens, int max_new, int max_keys, int n_pages, int page_size,
+                          int n_heads_q, int n_heads_kv, int head_dim, float softmax_scale,
+                          int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream);
+int teeny_copy_pages(void* pages, int planes, long plane_bytes, long page_bytes, int n_pages,
+                     const int32_t* from, const int32_t* to, int n, hipStream_t stream);
+
 /* teeny_decode_qkv_attention_dev: a one-token decode step's attention in
  * one launch, for position p = *n_past (read when the kernel runs): the
  * QKV projection's K-split slabs parts[n_parts][batch][(Hq + 2 Hkv) D] are

@@ -93,6 +93,11 @@ _SIGNATURES = {
     "teeny_shared_prefix_attention_workspace_bytes": ([_i] * 8, _sz),
     "teeny_shared_prefix_attention": ([_p] * 6 + [_i] * 6 + [_p] + [_i] * 4 + [_f, _i, _i, _p, _sz,
                                                                            _p], _i),
+    "teeny_paged_qkv_rope_split": ([_p, _p, _i] + [_p] * 4 + [_i, _i, _p, _p] + [_i] * 8
+                                   + [_d, _i, _p], _i),
+    "teeny_paged_attention_workspace_bytes": ([_i] * 8, _sz),
+    "teeny_paged_attention": ([_p] * 5 + [_i, _i, _p, _p] + [_i] * 10 + [_f, _i, _p, _sz, _p], _i),
+    "teeny_copy_pages": ([_p, _i, _l, _l, _i, _p, _p, _i, _p], _i),
     "teeny_sample_rows_workspace_bytes": ([_i, _i], _sz),
     "teeny_sample_rows": ([_p, _l, _p, _i, _i, _d, _p, _i, _p, _d, _p, _d, _p, _p, _i, _p, _p, _sz,
                            _p], _i),

@@ -17,7 +17,9 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -37,6 +39,7 @@
   X(llama)               \
   X(decode_bf16)         \
   X(prefix_attn)         \
+  X(paged)               \
   X(sample)              \
   X(linear_bf16)         \
   X(gemm_bf16)           \
@@ -1487,6 +1490,206 @@ int teeny_shared_prefix_attention(const void* q, const void* k_prefix, const voi
   void* a1[] = {&parts, &o, &a, &head_dim, &merged};
   const unsigned lds = (rpw * ((unsigned)(shares + 3) / 4 * 4) + 1024) * 4;
   return launch(name, dim3((unsigned)((rows + rpw - 1) / rpw)), dim3(256), lds, stream, a1);
+}
+
+// A cache in pages (paged.hip).
+namespace {
+struct Paged {  // in paged.h
+  const int32_t *table, *starts, *past;
+  int batch, tokens, each, past_all;
+  int ld, width, n_pages, lg;
+  int hq, hkv;
+};
+struct PagedPlan {  // Plan in paged.hip
+  float scale;
+  int keys, splits, keys_many, splits_many, few, groups;
+};
+struct PagedParts {  // Parts in paged.hip
+  float *m, *l, *o;
+};
+constexpr int kPageMoves = 448;  // kMoves in paged.hip
+struct PageMoves {               // Moves in paged.hip
+  int n;
+  int from[kPageMoves], to[kPageMoves];
+};
+int log2_of(int x) { return 31 - __builtin_clz((unsigned)x); }
+
+int paged_args(Paged* a, const int32_t* table, int table_ld, int table_width, const int32_t* starts,
+               const int32_t* n_past, int n_past_host, int batch, int tokens, int n_pages,
+               int page_size, int hq, int hkv, int head_dim) {
+  if (!table) return TEENY_ERR_NULL_POINTER;
+  if (batch <= 0 || tokens < 0 || table_width <= 0 || table_ld < table_width || n_pages <= 0 ||
+      hq <= 0 || hkv <= 0 || hq % hkv != 0 || page_size < 16 || page_size > 1024 ||
+      (page_size & (page_size - 1)) != 0 || (long)table_width * page_size > (1L << 30) ||
+      (long)tokens * (hq + 2 * hkv) >= kMaxElems / head_dim || (long)batch * table_ld >= kMaxElems)
+    return TEENY_ERR_INVALID_SHAPE;
+  if (!starts && tokens % batch != 0) return TEENY_ERR_INVALID_SHAPE;
+  if (!n_past && (n_past_host < 0 || n_past_host > (1 << 30))) return TEENY_ERR_INVALID_VALUE;
+  *a = Paged{table,       starts,  n_past, batch, tokens, starts ? 0 : tokens / batch, n_past_host,
+             table_ld,    table_width, n_pages, log2_of(page_size), hq, hkv};
+  return TEENY_OK;
+}
+
+// Shares of the keys: see the entry point.
+PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, int hkv, int head_dim,
+                     int dtype) {
+  (void)tokens;
+  (void)head_dim;
+  PagedPlan p{};
+  const bool f32 = dtype == TEENY_F32;
+  const int unit = f32 ? 16 : 32, waves = f32 ? 1 : 4;
+  const long rows = (long)(hq / hkv) * max_new;
+  p.few = 0x7fffffff;
+  p.groups = (int)((rows + unit - 1) / unit);
+  const long items = (long)batch * hkv * p.groups, want = 2L * device_cus();
+  const long most = std::max(1L, want / std::max(1L, items));
+  const long step = 32L * waves;
+  p.keys = (int)(((max_keys + most - 1) / most + step - 1) / step * step);
+  p.splits = std::max(1, (max_keys + p.keys - 1) / p.keys);
+  p.keys_many = p.keys;
+  p.splits_many = 1;
+  return p;
+}
+}  // namespace
+
+int teeny_paged_qkv_rope_split(const void* qkv, const float* parts, int n_parts, void* q_out,
+                               void* k_pages, void* v_pages, const int32_t* page_table,
+                               int table_ld, int table_width, const int32_t* starts,
+                               const int32_t* n_past, int n_past_host, int batch, int tokens,
+                               int n_pages, int page_size, int n_heads_q, int n_heads_kv,
+                               int head_dim, double ln_rope_base, int dtype, hipStream_t stream) {
+  if (!q_out || !k_pages || !v_pages || (qkv == nullptr) == (parts == nullptr))
+    return TEENY_ERR_NULL_POINTER;
+  if (!dtype_ok(dtype) || !fa2_head_dim_ok(head_dim, dtype)) return TEENY_ERR_UNSUPPORTED;
+  Paged a;
+  int rc = paged_args(&a, page_table, table_ld, table_width, starts, n_past, n_past_host, batch,
+                      tokens, n_pages, page_size, n_heads_q, n_heads_kv, head_dim);
+  if (rc) return rc;
+  if (!std::isfinite(ln_rope_base)) return TEENY_ERR_INVALID_VALUE;
+  const uintptr_t at = (uintptr_t)qkv | (uintptr_t)parts | (uintptr_t)q_out | (uintptr_t)k_pages |
+                       (uintptr_t)v_pages;
+  if (at % 16 != 0) return TEENY_ERR_INVALID_VALUE;
+  if (tokens == 0) return TEENY_OK;
+  int lg_d = log2_of(head_dim);
+  char name[48];
+  if (parts) {
+    long part_stride = (long)tokens * (n_heads_q + 2 * n_heads_kv) * head_dim;
+    if (n_parts <= 0 || part_stride >= kMaxElems / n_parts) return TEENY_ERR_INVALID_SHAPE;
+    snprintf(name, sizeof name, "teeny_paged_split_parts_%s", dtype_tag(dtype));
+    void* args[] = {&parts, &n_parts, &part_stride, &q_out, &k_pages, &v_pages, &a, &lg_d,
+                    &ln_rope_base};
+    return launch(name, dim3((unsigned)tokens), dim3(256), 0, stream, args);
+  }
+  const bool one = tokens <= 4 * device_cus();
+  snprintf(name, sizeof name, "teeny_paged_split_%s%s", dtype_tag(dtype), one ? "_one" : "");
+  void* args[] = {&qkv, &q_out, &k_pages, &v_pages, &a, &lg_d, &ln_rope_base};
+  return launch(name, dim3((unsigned)(one ? tokens : (tokens + 3) / 4)), dim3(256), 0, stream, args);
+}
+
+size_t teeny_paged_attention_workspace_bytes(int batch, int tokens, int max_new, int max_keys,
+                                             int n_heads_q, int n_heads_kv, int head_dim,
+                                             int dtype) {
+  if (batch <= 0 || tokens <= 0 || max_new <= 0 || max_keys <= 0 || n_heads_q <= 0 ||
+      n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0 || head_dim <= 0 || !dtype_ok(dtype))
+    return 0;
+  const PagedPlan p = paged_plan(batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv, head_dim,
+                                 dtype);
+  const int most = std::max(p.splits, p.splits_many);
+  if (most <= 1) return 0;
+  const size_t rows = (size_t)tokens * n_heads_q * most;
+  return 2 * align256(rows * sizeof(float)) + align256(rows * head_dim * sizeof(float));
+}
+
+int teeny_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o,
+                          const int32_t* page_table, int table_ld, int table_width,
+                          const int32_t* starts, const int32_t* n_past, int n_past_host, int batch,
+                          int tokens, int max_new, int max_keys, int n_pages, int page_size,
+                          int n_heads_q, int n_heads_kv, int head_dim, float softmax_scale,
+                          int dtype, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (!q || !k_pages || !v_pages || !o) return TEENY_ERR_NULL_POINTER;
+  if (!dtype_ok(dtype) || !fa2_head_dim_ok(head_dim, dtype)) return TEENY_ERR_UNSUPPORTED;
+  Paged a;
+  int rc = paged_args(&a, page_table, table_ld, table_width, starts, n_past, n_past_host, batch,
+                      tokens, n_pages, page_size, n_heads_q, n_heads_kv, head_dim);
+  if (rc) return rc;
+  if (max_new < 0 || max_keys < 0) return TEENY_ERR_INVALID_VALUE;
+  if (!scale_ok(softmax_scale, dtype)) return TEENY_ERR_INVALID_VALUE;
+  const uintptr_t at = (uintptr_t)q | (uintptr_t)o | (uintptr_t)k_pages | (uintptr_t)v_pages;
+  if (at % 16 != 0) return TEENY_ERR_INVALID_VALUE;
+  if (tokens == 0 || max_new == 0) return TEENY_OK;
+  max_new = starts ? std::min(max_new, tokens) : a.each;
+  max_keys = std::max(1, std::min(max_keys, table_width * page_size));
+  PagedPlan p = paged_plan(batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv, head_dim, dtype);
+  p.scale = softmax_scale;
+  const int shares = std::max(p.splits, p.splits_many);
+  const size_t rows = (size_t)tokens * n_heads_q;
+  if (rows * shares >= (size_t)kMaxElems) return TEENY_ERR_INVALID_SHAPE;
+  PagedParts parts{};
+  if (shares > 1) {
+    if (!workspace || workspace_bytes < teeny_paged_attention_workspace_bytes(
+                                            batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv,
+                                            head_dim, dtype))
+      return TEENY_ERR_WORKSPACE;
+    if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
+    const size_t each = align256(rows * shares * sizeof(float));
+    parts = {(float*)workspace, (float*)((char*)workspace + each),
+             (float*)((char*)workspace + 2 * each)};
+  }
+  const long wgs = (long)p.splits * p.groups * batch * n_heads_kv;
+  if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+  char name[64];
+  if (dtype == TEENY_BF16)
+    snprintf(name, sizeof name, "teeny_paged_attn_bf16_d%d_w4", head_dim);
+  else
+    snprintf(name, sizeof name, "teeny_paged_attn_f32_d%d", head_dim);
+  void* a0[] = {&q, &k_pages, &v_pages, &o, &a, &p, &parts};
+  rc = launch(name, dim3((unsigned)wgs), dim3(dtype == TEENY_BF16 ? 256 : 64), 0, stream, a0);
+  if (rc || shares == 1) return rc;
+  int lg_d = log2_of(head_dim);
+  snprintf(name, sizeof name, "teeny_paged_merge_%s", dtype_tag(dtype));
+  void* a1[] = {&parts, &o, &a, &p, &lg_d};
+  return launch(name, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a1);
+}
+
+int teeny_copy_pages(void* pages, int planes, long plane_bytes, long page_bytes, int n_pages,
+                     const int32_t* from, const int32_t* to, int n, hipStream_t stream) {
+  if (!pages || (n > 0 && (!from || !to))) return TEENY_ERR_NULL_POINTER;
+  if (planes <= 0 || planes > 65535 || n_pages <= 0 || n < 0 || page_bytes <= 0 ||
+      page_bytes > (1L << 30) || plane_bytes < page_bytes * n_pages)
+    return TEENY_ERR_INVALID_SHAPE;
+  if ((uintptr_t)pages % 16 != 0 || page_bytes % 16 != 0 || plane_bytes % 16 != 0)
+    return TEENY_ERR_INVALID_VALUE;
+  // every pair before the first copy: a page is written once, and by no pair both
+  // read and written
+  if (n > 0) {
+    std::unique_ptr<int32_t[]> sorted(new (std::nothrow) int32_t[2 * (size_t)n]);
+    if (!sorted) return TEENY_ERR_WORKSPACE;
+    int32_t *f = sorted.get(), *t = f + n;
+    std::copy(from, from + n, f);
+    std::copy(to, to + n, t);
+    std::sort(f, f + n);
+    std::sort(t, t + n);
+    if (f[0] < 0 || f[n - 1] >= n_pages || t[0] < 0 || t[n - 1] >= n_pages)
+      return TEENY_ERR_INVALID_VALUE;
+    for (int i = 0, j = 0; i < n; ++i) {
+      if (i > 0 && t[i] == t[i - 1]) return TEENY_ERR_INVALID_VALUE;
+      while (j < n && f[j] < t[i]) ++j;
+      if (j < n && f[j] == t[i]) return TEENY_ERR_INVALID_VALUE;
+    }
+  }
+  int chunks = (int)((page_bytes + 16383) / 16384);
+  PageMoves m;
+  for (int i = 0; i < n; i += m.n) {
+    m.n = std::min(n - i, kPageMoves);
+    std::memcpy(m.from, from + i, m.n * sizeof(int));
+    std::memcpy(m.to, to + i, m.n * sizeof(int));
+    if ((long)chunks * m.n >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+    void* args[] = {&pages, &plane_bytes, &page_bytes, &chunks, &m};
+    int rc = launch("teeny_copy_pages", dim3((unsigned)(chunks * m.n), (unsigned)planes), dim3(256),
+                    0, stream, args);
+    if (rc) return rc;
+  }
+  return TEENY_OK;
 }
 
 int teeny_argmax_rows(const void* x, int64_t* out, int rows, int cols, int dtype,

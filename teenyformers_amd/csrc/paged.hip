@@ -1,0 +1,635 @@
+// A cache in pages: what writes it, attends to it and moves its pages (the layout:
+// paged.h).
+//
+//   split    the QKV projection's rows: q rotated to [T, Hq, D], k (rotated) and v to
+//            the rows of their pages
+//   attn     attention of a sequence's new tokens over its pages, few rows a kv head
+//            (many: the forward kernel, fa2_fwd_bf16.hip), in shares of the keys
+//   merge    the shares of a row, weighed and summed
+//   copy     pages of all layers copied within the pool
+//
+// Reference: no counterpart (no KV cache, examples/llama_generate.rs:373-381); a row
+// is the reference's attention (flash_attn2.rs:61-126) over the sequence's keys.
+#include "attn_rows.h"
+#include "f32_mfma.h"
+#include "paged.h"
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// split: TOK tokens a workgroup.  Their rows of the projection are one run of
+// memory; a thread's first loads are in flight while each wavefront finds a token's
+// sequence, position and page and its (cos, sin), once for all heads.
+//
+// Angles are formed and reduced in 64 bits: of position p the fp32 product p base^
+// (-2k/D) is off by up to p 2^-24 radians (2e-3 at 32768), as much as a bf16 rounds.
+// ---------------------------------------------------------------------------
+template <typename T, bool PARTS, int TOK>
+__device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__ parts, int n_parts,
+                            long part_stride, T* __restrict__ q_out, T* __restrict__ kp,
+                            T* __restrict__ vp, const Paged a, int lg_d, double ln_base) {
+  constexpr int NT = 256, VN = Vec16<T>::N, U = PARTS ? 1 : TOK == 1 ? 3 : 6;
+  static_assert(TOK <= NT / 64, "a wavefront a token");
+  __shared__ float2 cs[TOK][64];
+  __shared__ long at[TOK];  // element of the token's row in its page, head 0; -1: none
+  __shared__ int live[TOK];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int head_dim = 1 << lg_d, lg_v = lg_d - __builtin_ctz(VN);  // vectors of a head
+  const int vecs = (a.hq + 2 * a.hkv) << lg_v;                      // ... of a token
+  const int tok0 = blockIdx.x * TOK, total = min(TOK, a.tokens - tok0) * vecs;
+  const long src = (long)tok0 * vecs * VN;
+  u32x4 raw[U];
+  float sum[VN];
+  auto load = [&](int i0) __attribute__((always_inline)) {
+    if constexpr (PARTS) {
+      if (i0 < total) ld_parts<T, VN>(parts + src + (long)i0 * VN, part_stride, n_parts, sum);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        raw[u] = *reinterpret_cast<const u32x4*>(qkv + src + (long)min(i0 + u * NT, total - 1) * VN);
+    }
+  };
+  load(tid);
+  if (wave < TOK) {
+    const int t = tok0 + wave;
+    const int b = t < a.tokens ? seq_at(a, t) : -1;
+    long row = -1;
+    int pos = 0, in = 0;
+    if (b >= 0) {
+      const Seq s = seq_of(a, b);
+      const int i = t - s.t0;
+      in = i >= 0 && i < s.n;
+      pos = s.past + i;
+      if (in && pos >= 0 && pos < s.cap) {
+        const int page = a.table[(long)b * a.ld + (pos >> a.lg)];
+        if ((unsigned)page < (unsigned)a.n_pages)
+          row = (((long)page * a.hkv << a.lg) + (pos & ((1 << a.lg) - 1))) << lg_d;
+      }
+    }
+    if (lane == 0) {
+      at[wave] = row;
+      live[wave] = in;
+    }
+    if (lane < head_dim / 2) {
+      // turns, less whole ones: in [-1/2, 1/2]
+      double turn = pos * (exp(-2.0 * lane * ln_base / head_dim) * 0.15915494309189533577);
+      turn -= rint(turn);
+      double sn, cn;
+      sincospi(2.0 * turn, &sn, &cn);
+      cs[wave][lane] = make_float2((float)cn, (float)sn);
+    }
+  }
+  __syncthreads();
+  const long head_k = (long)1 << (a.lg + lg_d);  // elements between a page's kv heads
+  for (int i0 = tid; i0 < total; i0 += U * NT) {
+    if (i0 != tid) load(i0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * NT;
+      if (i >= total) break;
+      int tk = 0;
+#pragma unroll
+      for (int x = 1; x < TOK; ++x) tk += i >= x * vecs;
+      const int col = i - tk * vecs, head = col >> lg_v, v = col & ((1 << lg_v) - 1);
+      T* dst;
+      if (head < a.hq) {
+        if (!live[tk]) continue;
+        dst = q_out + (((long)(tok0 + tk) * a.hq + head) << lg_d);
+      } else {
+        if (at[tk] < 0) continue;
+        const bool is_k = head < a.hq + a.hkv;
+        dst = (is_k ? kp : vp) + at[tk] + (head - a.hq - (is_k ? 0 : a.hkv)) * head_k;
+      }
+      float in[VN], out[VN];
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const uint32_t w = raw[u][VN == 4 ? j : j / 2];
+        if constexpr (PARTS) in[j] = sum[j];
+        else if constexpr (VN == 4) in[j] = __builtin_bit_cast(float, w);
+        else in[j] = j & 1 ? bf16hi(w) : bf16lo(w);
+      }
+      if (head < a.hq + a.hkv) {
+        const float2* c = cs[tk] + v * (VN / 2);
+#pragma unroll
+        for (int j = 0; j < VN / 2; ++j)
+          rope_rotate(in[2 * j], in[2 * j + 1], c[j].x, c[j].y, out[2 * j], out[2 * j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VN; ++j) out[j] = in[j];
+      }
+      Vec16<T>::store(dst + v * VN, out);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// copy: page `to` of a plane becomes page `from` of it, for every pair and plane; no
+// page is read by one pair and written by another.  A workgroup moves 16 KiB.
+// ---------------------------------------------------------------------------
+constexpr int kMoves = 448;  // pairs in a launch's arguments
+struct Moves {
+  int n;
+  int from[kMoves], to[kMoves];
+};
+__device__ void copy_pages(char* pages, long plane_bytes, long page_bytes, int chunks, const Moves& m) {
+  const int pair = blockIdx.x / chunks, ch = blockIdx.x - pair * chunks;
+  char* plane = pages + blockIdx.y * plane_bytes;
+  const u32x4* src = reinterpret_cast<const u32x4*>(plane + m.from[pair] * page_bytes);
+  u32x4* dst = reinterpret_cast<u32x4*>(plane + m.to[pair] * page_bytes);
+  const long n = page_bytes / 16;
+  constexpr int U = 4;
+  const long i0 = (long)ch * (U * 256) + threadIdx.x;
+  u32x4 v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = src[min(i0 + u * 256, n - 1)];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (i0 + u * 256 < n) dst[i0 + u * 256] = v[u];
+}
+
+// ---------------------------------------------------------------------------
+// attn
+// ---------------------------------------------------------------------------
+// How a launch shares the work out.  The rows of a sequence and kv head are r = i G
+// + g: token i, q head g of the group.
+struct Plan {
+  float scale;
+  int keys, splits;            // of sequences with up to `few` rows: keys of a share, shares
+  int keys_many, splits_many;  // of the others
+  int few;
+  int groups;                  // row tiles of a sequence in the grid
+};
+// Partials [share][T Hq rows]; m in the log2 domain, -inf: no key.  Sequences of one
+// share write their output instead.
+struct Parts {
+  float *m, *l, *o;
+};
+// (the last share of the grid takes all that is left)
+DEVI int shares(const Seq& s, int keys, int most) {
+  return min(max(1, (s.keys(s.n - 1) + keys - 1) / keys), most);
+}
+
+template <int D, int NW>
+struct __attribute__((aligned(16))) AttnSmem {
+  static constexpr int TILE = TK * D * 2;
+  union {
+    char tile[NW][2][TILE];  // a K and a V tile of each wavefront
+    struct {
+      float o[NW][32 * D];
+      float m[NW][32], l[NW][32];
+    } c;                     // the wavefronts' shares
+  } u;
+};
+
+// Rows whose values in V are not finite and that some query must not see: 0 times
+// such a value would be NaN, so their tile is added key by key to the rows that see
+// it.  vt: the tile; pb: its P; lim: the lane's keys, relative to the tile.
+template <int D>
+DEVI void add_keys(Rows<D>& st, const char* vt, const uint32_t* pb, int lim) {
+  const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float mine = r & 1 ? bf16hi(pb[r >> 1]) : bf16lo(pb[r >> 1]), other = other_half(mine);
+#pragma unroll 1
+    for (int gg = 0; gg < 2; ++gg) {
+      const int key = 8 * (r >> 2) + 4 * gg + (r & 3);
+      const float p = gg == g ? mine : other;
+      if (key >= lim) continue;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(
+              vt + swz<SWZ_DUAL, D>(key * (D / 8) + 4 * t + j) * 16 + 8 * g);
+          st.acc[t][4 * j] += p * bf16lo(w[0]);
+          st.acc[t][4 * j + 1] += p * bf16hi(w[0]);
+          st.acc[t][4 * j + 2] += p * bf16lo(w[1]);
+          st.acc[t][4 * j + 3] += p * bf16hi(w[1]);
+        }
+    }
+  }
+}
+template <int DT>
+DEVI bool any_bad(const u32x4 (*va)[DT]) {
+  uint32_t bad = 0;
+#pragma unroll
+  for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = va[hh][t][i] & 0x7f807f80u;
+        bad |= (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+      }
+  return __any(bad != 0);
+}
+
+// grid: splits * groups * batch * hkv; a workgroup: a share of the keys of 32 rows,
+// of which each wavefront takes a run through tiles of its own.
+template <int D, int NW>
+__device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ kp,
+                           const bf16* __restrict__ vp, bf16* __restrict__ o, const Paged a,
+                           const Plan pl, const Parts out) {
+  constexpr int TILE = TK * D * 2, NLD = TILE / 1024;
+  __shared__ AttnSmem<D, NW> sm;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int id = blockIdx.x;
+  const int rg = id % pl.groups;
+  id /= pl.groups;
+  const int hk = id % a.hkv;
+  id /= a.hkv;
+  const int split = id % pl.splits, b = id / pl.splits;
+  const Seq s = seq_of(a, b);
+  const int G = a.hq / a.hkv;
+  const long all = (long)s.n * G;
+  if (all > pl.few || rg * 32 >= all) return;
+  const int rows = (int)all, n_sh = shares(s, pl.keys, pl.splits);
+  if (split >= n_sh) return;
+  const int r = rg * 32 + l32, rc = min(r, rows - 1), tok = rc / G;
+  const long row = (long)(s.t0 + tok) * a.hq + hk * G + (rc - tok * G);
+  const float sl2 = pl.scale * kLog2e;
+  Rows<D> st;
+  st.init();
+  st.load_q(q + row * D, r < rows);
+  // keys: of the lane's row; of the rows' first and last token
+  const int lim = s.keys(tok), lim0 = s.keys(rg * 32 / G);
+  const int last = s.keys((min(rows, rg * 32 + 32) - 1) / G);
+  const int s0 = split * pl.keys, s1 = split + 1 < pl.splits ? min(s0 + pl.keys, last) : last;
+  const int kpw = ((max(0, s1 - s0) + NW - 1) / NW + TK - 1) / TK * TK;
+  const int k0 = s0 + wave * kpw, end = min(k0 + kpw, s1);
+  const int n_tiles = max(0, end - k0 + TK - 1) / TK;
+  PageWalk walk(a, b);
+  // loads of a tile: 16 rows lie in one page (its rows at or past `end`, and absent
+  // pages, lie outside the descriptor and load as zeros); returns the absent halves
+  auto load = [&](const bf16* pool, char* to, int it, auto sw) __attribute__((always_inline)) {
+    int absent = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int key = k0 + it * TK + 16 * h, page = walk.at(key >> a.lg);
+      const int n = page < 0 ? 0 : min(max(end - key, 0), 16);
+      const long at = (((long)max(page, 0) * a.hkv + hk) << a.lg) + (key & ((1 << a.lg) - 1));
+      const auto rs = make_rsrc(pool + at * D, n * D * 2);
+      absent |= (page < 0) << h;
+#pragma unroll
+      for (int i = h * NLD / 2; i < (h + 1) * NLD / 2; ++i)
+        dma16(rs, to + i * 1024, swz<decltype(sw)::value, D>(i * 64 + lane) * 16 - h * 16 * D * 2, 0);
+    }
+    return absent;
+  };
+  using RowSwz = std::integral_constant<Swz, SWZ_ROW>;
+  using DualSwz = std::integral_constant<Swz, SWZ_DUAL>;
+  char *kt = sm.u.tile[wave][0], *vt = sm.u.tile[wave][1];
+  uint32_t pb[8];
+  u32x4 va[2][Rows<D>::DT];
+  int absent = 0;
+  if (n_tiles > 0) {
+    absent = load(kp, kt, 0, RowSwz{});
+    load(vp, vt, 0, DualSwz{});
+  }
+  for (int it = 0; it < n_tiles; ++it) {
+    // K of a tile before its V, each refilled as soon as it has been read
+    __builtin_amdgcn_s_waitcnt(kVmWait<NLD>());
+    f32x16 sc = st.scores(kt);
+    __builtin_amdgcn_s_waitcnt(kLgkmcnt0);
+    int next = 0;
+    if (it + 1 < n_tiles) next = load(kp, kt, it + 1, RowSwz{});
+    const int t0 = k0 + it * TK;
+    const bool edge = t0 + TK > min(lim0, end);
+    if (edge) st.mask(sc, min(lim, end) - t0);
+    if (absent) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x)
+        if (absent >> (x >> 3) & 1) sc[x] = -INFINITY;
+    }
+    st.softmax(sc, sl2, pb);
+    if (it + 1 < n_tiles) __builtin_amdgcn_s_waitcnt(kVmWait<NLD>());
+    else __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    st.read_v(vt, va);
+    __builtin_amdgcn_s_waitcnt(kLgkmcnt0);
+    const bool bad = edge && lim0 < last && any_bad<Rows<D>::DT>(va);
+    if (bad) {
+      add_keys<D>(st, vt, pb, min(lim, end) - t0);
+      __builtin_amdgcn_s_waitcnt(kLgkmcnt0);
+    }
+    if (it + 1 < n_tiles) load(vp, vt, it + 1, DualSwz{});
+    if (!bad) st.product(va, pb);
+    absent = next;
+  }
+  const float l_tot = st.l + other_half(st.l);
+  const int n_here = min(32, rows - rg * 32);
+  __syncthreads();  // every wavefront is done with its tiles
+  if (l32 < n_here) {
+    if (g == 0) {
+      sm.u.c.m[wave][l32] = st.m;
+      sm.u.c.l[wave][l32] = l_tot;
+    }
+    float* orow = sm.u.c.o[wave] + l32 * D;
+#pragma unroll
+    for (int t = 0; t < Rows<D>::DT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4*>(orow + 32 * t + 8 * j + 4 * g) = f32x4{
+            st.acc[t][4 * j], st.acc[t][4 * j + 1], st.acc[t][4 * j + 2], st.acc[t][4 * j + 3]};
+  }
+  __syncthreads();
+  const long n_rows = (long)a.tokens * a.hq;
+  for (int i = tid; i < n_here * (D / 4); i += NW * 64) {
+    const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, sm.u.c.m[w][rr]);
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    f32x4 num = {};
+    float den = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float e = fast_exp2(sm.u.c.m[w][rr] - ref);
+      num += e * *reinterpret_cast<const f32x4*>(sm.u.c.o[w] + rr * D + d);
+      den += e * sm.u.c.l[w][rr];
+    }
+    const int ri = rg * 32 + rr, ti = ri / G;
+    const long to = (long)(s.t0 + ti) * a.hq + hk * G + (ri - ti * G);
+    if (n_sh == 1) {
+      const float inv = den == 0.0f ? 0.0f : 1.0f / den;  // a row without a key: zeros
+      *reinterpret_cast<u32x2*>(o + to * D + d) =
+          u32x2{pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv)};
+      continue;
+    }
+    *reinterpret_cast<f32x4*>(out.o + (split * n_rows + to) * D + d) = num;
+    if (d == 0) {
+      out.m[split * n_rows + to] = mm;
+      out.l[split * n_rows + to] = den;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// fp32: a wavefront per 16 rows and share, on the fp32 matrix cores, K and V read
+// straight from the pages in operand order.  The same grid, groups of 16 rows.
+// ---------------------------------------------------------------------------
+template <int D>
+__device__ void paged_attn_f32(const float* __restrict__ q, const float* __restrict__ kp,
+                               const float* __restrict__ vp, float* __restrict__ o, const Paged a,
+                               const Plan pl, const Parts out) {
+  constexpr int NC = Geo<D>::NC, VW = Geo<D>::VW, NH = Geo<D>::NH;
+  const int lane = threadIdx.x, j = lane & 15, g = lane >> 4;
+  int id = blockIdx.x;
+  const int rg = id % pl.groups;
+  id /= pl.groups;
+  const int hk = id % a.hkv;
+  id /= a.hkv;
+  const int split = id % pl.splits, b = id / pl.splits;
+  const Seq s = seq_of(a, b);
+  const int G = a.hq / a.hkv;
+  const long rows = (long)s.n * G;
+  if ((long)rg * 16 >= rows) return;
+  const int n_sh = shares(s, pl.keys, pl.splits);
+  if (split >= n_sh) return;
+  const long rc = min((long)rg * 16 + j, rows - 1);
+  const int tok = (int)(rc / G);
+  const bool valid = (long)rg * 16 + j < rows;
+  const long row = (long)(s.t0 + tok) * a.hq + hk * G + (int)(rc - (long)tok * G);
+  const int last = s.keys((int)((min(rows, (long)rg * 16 + 16) - 1) / G));
+  const int lim0 = s.keys((int)((long)rg * 16 / G));
+  const int k0 = split * pl.keys, end = split + 1 < pl.splits ? min(k0 + pl.keys, last) : last;
+  const int stop = min(s.keys(tok), end);
+  f32x4 qf[NC];
+  row_regs<D>(q + row * D, g, qf);
+  f32x4 acc[NH][VW];
+  zero_acc<D>(acc);
+  float m = -INFINITY, l = 0.0f;
+  PageWalk walk(a, b);
+  for (int t0 = k0; t0 < end; t0 += 32) {
+    f32x4 kf[2][NC];
+    float vf[8][NH][VW];
+    // 16 rows lie in one page; rows at or past the end re-read the last one before it
+    // (where there is none, the pool's first): their P is zero, and so is their V
+    long base[2];
+    int n[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = t0 + 16 * u, page = walk.at(key >> a.lg);
+      n[u] = page < 0 ? 0 : min(max(end - key, 0), 16);
+      base[u] = n[u] == 0 ? 0 : (((long)page * a.hkv + hk) << a.lg) + (key & ((1 << a.lg) - 1));
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      row_regs<D>(kp + (base[u] + max(0, min(j, n[u] - 1))) * D, g, kf[u]);
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int u = x >> 2;
+      const float* vr = vp + (base[u] + max(0, min(4 * g + (x & 3), n[u] - 1))) * D;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        if constexpr (VW == 4) {
+          const f32x4 y = *reinterpret_cast<const f32x4g*>(vr + 64 * h + 4 * j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vf[x][h][e] = y[e];
+        } else if constexpr (VW == 2) {
+          const f32x2 y = *reinterpret_cast<const f32x2g*>(vr + 2 * j);
+          vf[x][h][0] = y[0];
+          vf[x][h][1] = y[1];
+        } else {
+          vf[x][h][0] = D == 8 && j >= 8 ? 0.0f : vr[j];
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // every load is issued first
+    f32x4 sc[2] = {};
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) sc[u] = mfma4(kf[u][c][e], qf[c][e], sc[u]);
+    float mx = -INFINITY;
+    const float m_old = m;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const bool seen = t0 + 16 * u + 4 * g + r < stop && 4 * g + r < n[u];
+        sc[u][r] = seen ? sc[u][r] * pl.scale : -INFINITY;
+        mx = fmaxf(mx, sc[u][r]);
+      }
+    m = fmaxf(m, max_g(mx));
+    const float ref = m == -INFINITY ? 0.0f : m;  // no key of the row so far
+    const float alpha = expf(m_old - ref);
+    l *= alpha;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sc[u][r] = expf(sc[u][r] - ref);
+        l += sc[u][r];
+      }
+#pragma unroll
+    for (int h = 0; h < NH; ++h)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) acc[h][e] *= alpha;
+    if (n[0] < 16 || n[1] < 16) {
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+        if (4 * g + (x & 3) >= n[x >> 2])
+#pragma unroll
+          for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int e = 0; e < VW; ++e) vf[x][h][e] = 0.0f;
+    }
+    // rows that some query of the 16 must not see: as add_keys
+    if (lim0 < last && min(t0 + 32, end) > lim0) {
+      float bad = 0.0f;
+#pragma unroll
+      for (int x = 0; x < 8; ++x)
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int e = 0; e < VW; ++e) bad += 0.0f * vf[x][h][e];
+      if (__any(bad != bad)) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+#pragma unroll 1
+          for (int kg = 0; kg < 4; ++kg) {
+            const int in = 4 * kg + (x & 3);
+            const float p = __shfl(sc[x >> 2][x & 3], 16 * kg + j);
+            if (t0 + 16 * (x >> 2) + in < stop && in < n[x >> 2])
+              add_row<D>(vp + (base[x >> 2] + in) * D, p, g, acc);
+          }
+        continue;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int e = 0; e < VW; ++e) acc[h][e] = mfma4(vf[x][h][e], sc[x >> 2][x & 3], acc[h][e]);
+  }
+  l = sum_g(l);
+  if (!valid) return;
+  if (n_sh == 1) {
+    store_col<D>(o + row * D, acc, g, [l](float x) { return l == 0.0f ? 0.0f : x / l; });
+    return;
+  }
+  const long to = (long)split * a.tokens * a.hq + row;
+  if (g == 0) {
+    out.m[to] = m * kLog2e;
+    out.l[to] = l;
+  }
+  store_col<D>(out.o + to * D, acc, g, [](float x) { return x; });
+}
+
+// The shares of a row, weighed by 2^(m - max m) and summed: a wavefront a row, whose
+// lanes hold four d each in groups that go over the shares side by side.
+template <typename T>
+__device__ void paged_merge(const Parts in, T* __restrict__ o, const Paged a, const Plan pl, int lg_d) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long n_rows = (long)a.tokens * a.hq, row = (long)blockIdx.x * 4 + wave;
+  if (row >= n_rows) return;
+  const int t = (int)(row / a.hq), b = seq_at(a, t);
+  if (b < 0) return;
+  const Seq s = seq_of(a, b);
+  if (t < s.t0 || t >= s.t0 + s.n) return;
+  const bool many = (long)s.n * (a.hq / a.hkv) > pl.few;
+  const int n = many ? shares(s, pl.keys_many, pl.splits_many) : shares(s, pl.keys, pl.splits);
+  if (n <= 1) return;
+  float mx = -INFINITY;
+  for (int i = lane; i < n; i += 64) mx = fmaxf(mx, in.m[i * n_rows + row]);
+  mx = wave_max(mx);
+  const float ref = mx == -INFINITY ? 0.0f : mx;  // no key at all: zeros
+  const int lanes = 1 << (lg_d - 2), grp = lane >> (lg_d - 2), groups = 64 >> (lg_d - 2);
+  const int d = (lane & (lanes - 1)) * 4;
+  f32x4 acc = {};
+  float den = 0.0f;
+  constexpr int U = 4;  // shares of a group in flight
+  for (int i0 = grp; i0 - grp < n; i0 += U * groups) {
+    f32x4 v[U];
+    float mi[U], li[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (past the end: the last one, unweighed)
+      const long at = min(i0 + u * groups, n - 1) * n_rows + row;
+      v[u] = *reinterpret_cast<const f32x4*>(in.o + (at << lg_d) + d);
+      mi[u] = in.m[at];
+      li[u] = in.l[at];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float e = i0 + u * groups < n ? fast_exp2(mi[u] - ref) : 0.0f;
+      if (e == 0.0f) continue;  // (a share without a key, or without weight)
+      acc += e * v[u];
+      den += e * li[u];
+    }
+  }
+  for (int off = lanes; off < 64; off <<= 1) {
+    den += __shfl_xor(den, off);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += __shfl_xor(acc[i], off);
+  }
+  if (grp > 0) return;
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] *= inv;
+  T* to = o + (row << lg_d) + d;
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+  else
+    *reinterpret_cast<f32x4g*>(to) = acc;
+}
+
+}  // namespace
+
+#define TEENY_PAGED_SPLIT_INST(TN, T, SFX, TOK)                                                  \
+  extern "C" __global__ __launch_bounds__(256) void teeny_paged_split_##TN##SFX(                  \
+      const T* qkv, T* q_out, T* kp, T* vp, Paged a, int lg_d, double ln_base) {                  \
+    paged_split<T, false, TOK>(qkv, nullptr, 0, 0, q_out, kp, vp, a, lg_d, ln_base);              \
+  }
+TEENY_PAGED_SPLIT_INST(bf16, bf16, , 4)
+TEENY_PAGED_SPLIT_INST(bf16, bf16, _one, 1)
+TEENY_PAGED_SPLIT_INST(f32, float, , 4)
+TEENY_PAGED_SPLIT_INST(f32, float, _one, 1)
+#define TEENY_PAGED_SPLIT_PARTS_INST(TN, T)                                                      \
+  extern "C" __global__ __launch_bounds__(256) void teeny_paged_split_parts_##TN(                 \
+      const float* parts, int n_parts, long part_stride, T* q_out, T* kp, T* vp, Paged a,         \
+      int lg_d, double ln_base) {                                                                 \
+    paged_split<T, true, 1>(nullptr, parts, n_parts, part_stride, q_out, kp, vp, a, lg_d,         \
+                            ln_base);                                                             \
+  }
+TEENY_PAGED_SPLIT_PARTS_INST(bf16, bf16)
+TEENY_PAGED_SPLIT_PARTS_INST(f32, float)
+
+extern "C" __global__ __launch_bounds__(256) void teeny_copy_pages(char* pages, long plane_bytes,
+                                                                    long page_bytes, int chunks,
+                                                                    Moves m) {
+  copy_pages(pages, plane_bytes, page_bytes, chunks, m);
+}
+
+#define TEENY_PAGED_ATTN_BF16_INST(D, NW)                                                        \
+  extern "C" __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))       \
+  void teeny_paged_attn_bf16_d##D##_w##NW(const bf16* q, const bf16* kp, const bf16* vp, bf16* o, \
+                                          Paged a, Plan pl, Parts p) {                           \
+    paged_attn<D, NW>(q, kp, vp, o, a, pl, p);                                                   \
+  }
+TEENY_PAGED_ATTN_BF16_INST(64, 4)
+TEENY_PAGED_ATTN_BF16_INST(128, 4)
+
+#define TEENY_PAGED_ATTN_F32_INST(D)                                                             \
+  extern "C" __global__ __launch_bounds__(64) void teeny_paged_attn_f32_d##D(                    \
+      const float* q, const float* kp, const float* vp, float* o, Paged a, Plan pl, Parts p) {    \
+    paged_attn_f32<D>(q, kp, vp, o, a, pl, p);                                                   \
+  }
+TEENY_PAGED_ATTN_F32_INST(8)
+TEENY_PAGED_ATTN_F32_INST(16)
+TEENY_PAGED_ATTN_F32_INST(32)
+TEENY_PAGED_ATTN_F32_INST(64)
+TEENY_PAGED_ATTN_F32_INST(128)
+
+#define TEENY_PAGED_MERGE_INST(TN, T)                                                            \
+  extern "C" __global__ __launch_bounds__(256) void teeny_paged_merge_##TN(Parts p, T* o, Paged a, \
+                                                                           Plan pl, int lg_d) {   \
+    paged_merge<T>(p, o, a, pl, lg_d);                                                           \
+  }
+TEENY_PAGED_MERGE_INST(bf16, bf16)
+TEENY_PAGED_MERGE_INST(f32, float)

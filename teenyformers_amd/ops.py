@@ -9,6 +9,7 @@ Shapes follow the reference with the batch split out:
 from __future__ import annotations
 
 import contextlib
+import ctypes
 import functools
 import math
 import threading
@@ -705,6 +706,167 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k_cache, v_cache, n_prefix: i
              _p(v_cache), _p(out), B, Hq, Hkv, S, n_prefix, kp[1], _p(past), stride, past_host, L, D,
              scale, int(bool(merged)), code, _p(workspace), size, _stream())
     return out
+
+
+# ---------------------------------------------------------------------------
+# A cache in pages
+# ---------------------------------------------------------------------------
+
+def _paged(what: str, x, k_pages, v_pages, page_table, n_past, starts):
+    """The checked arguments that describe a batch over pages: (batch, n_pages,
+    Hkv, page_size, D, [table, its row stride, width, starts, n_past, its host value])."""
+    dev, dtype = k_pages.get_device(), k_pages.dtype
+    for t in (x, k_pages, v_pages):
+        if t.get_device() != dev or dev < 0:
+            raise ValueError(f"{what}: all tensors are on one device, a GPU")
+        if not t.is_contiguous():
+            raise ValueError("teenyformers_amd ops take contiguous tensors")
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"{what}: k_pages and v_pages are [n_pages, Hkv, page_size, D]")
+    if v_pages.dtype != dtype:
+        raise TypeError(f"{what}: the tensors share a dtype")
+    n_pages, hkv, size, D = k_pages.shape
+    if not 16 <= size <= 1024 or size & (size - 1):
+        raise ValueError(f"{what}: the page size is a power of two, 16 to 1024")
+    if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.get_device() != dev
+            or page_table.stride(1) != 1 and page_table.shape[1] > 1):
+        raise ValueError(f"{what}: page_table is int32 [B, P] on the pages' device, its rows "
+                         "contiguous")
+    B, width = page_table.shape
+    if B < 1 or width < 1 or n_pages < 1:
+        raise ValueError(f"{what}: at least one sequence, page and table entry")
+    ld = page_table.stride(0) if B > 1 else width
+    if ld < width:
+        raise ValueError(f"{what}: the rows of page_table do not overlap")
+    if starts is None:
+        if x.shape[0] % B:
+            raise ValueError(f"{what}: without starts every sequence has as many new tokens")
+    elif (starts.dtype != torch.int32 or starts.get_device() != dev or starts.shape != (B + 1,)
+          or not starts.is_contiguous()):
+        raise ValueError(f"{what}: starts is int32 [B + 1] on the pages' device")
+    past, host = None, 0
+    if isinstance(n_past, torch.Tensor):
+        if (n_past.dtype != torch.int32 or n_past.get_device() != dev or n_past.shape != (B,)
+                or not n_past.is_contiguous()):
+            raise ValueError(f"{what}: n_past is an int, or int32 [B] on the pages' device")
+        past = n_past
+    else:
+        host = int(n_past)
+        if not 0 <= host <= width * size:
+            raise ValueError(f"{what}: n_past lies in the table's pages")
+    return B, n_pages, hkv, size, D, (_p(page_table), ld, width, _p(starts), _p(past), host)
+
+
+def paged_qkv_rope_split(qkv, k_pages, v_pages, page_table, n_past, n_heads_q: int,
+                         rope_base: float, starts=None, q_out=None):
+    """The QKV projection's rows qkv [T, (Hq+2Hkv)*D] (or Partials) of the new
+    tokens of B sequences -> q [T, Hq, D] (RoPE), with k (RoPE) and v written to
+    their pages (teeny_paged_qkv_rope_split).
+
+    k/v_pages [n_pages, Hkv, page_size, D]; page_table int32 [B, P] (entries
+    outside the pool: absent pages); the tokens are packed, starts int32 [B+1]
+    (without: T/B each), token i of sequence b at position n_past[b] + i; n_past:
+    an int, or int32 [B] on the device.  All device tensors are read when the
+    kernel runs (for captured graphs).  Positions without a page are not written;
+    tokens behind starts[B] are nobody's, their rows of q_out are left as they were."""
+    parts = isinstance(qkv, Partials)
+    src = qkv.slabs if parts else qkv
+    T = math.prod(qkv.shape[:-1])
+    x = src if parts else src.reshape(T, qkv.shape[-1])
+    B, n_pages, hkv, size, D, where = _paged("paged_qkv_rope_split", x[0] if parts else x, k_pages,
+                                             v_pages, page_table, n_past, starts)
+    if qkv.dtype != k_pages.dtype:
+        raise TypeError("paged_qkv_rope_split: the tensors share a dtype")
+    if n_heads_q < 1 or n_heads_q % hkv or qkv.shape[-1] != (n_heads_q + 2 * hkv) * D:
+        raise ValueError("paged_qkv_rope_split: qkv is [T, (Hq+2Hkv)*D] matching the pages")
+    if q_out is None:
+        q_out = torch.empty((T, n_heads_q, D), dtype=k_pages.dtype, device=k_pages.device)
+    elif (q_out.shape != (T, n_heads_q, D) or q_out.dtype != k_pages.dtype
+          or q_out.get_device() != k_pages.get_device() or not q_out.is_contiguous()):
+        raise ValueError("paged_qkv_rope_split: q_out is contiguous [T, Hq, D] on the pages' device")
+    with _on_device_of(k_pages):
+        call("teeny_paged_qkv_rope_split", None if parts else _p(x), _p(src) if parts else None,
+             qkv.n if parts else 0, _p(q_out), _p(k_pages), _p(v_pages), *where, B, T, n_pages, size,
+             n_heads_q, hkv, D, math.log(float(rope_base)), _code(k_pages), _stream())
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, n_past, softmax_scale: float | None = None,
+                    starts=None, max_new: int | None = None, max_keys: int | None = None, out=None,
+                    workspace=None):
+    """Attention of the new tokens q [T, Hq, D] of B sequences over their pages ->
+    o [T, Hq, D] (teeny_paged_attention; the arguments as paged_qkv_rope_split's, which
+    wrote the new tokens' keys): token i of sequence b attends to keys 0 .. n_past[b] + i
+    of the pages that are present; zeros where there is none.  One call serves one-token
+    steps, drafted tokens, chunks of prompts and batches that mix them.
+
+    max_new: the most new tokens of a sequence where the host knows it (with starts, by
+    default T); max_keys: the most keys (by default the table's), which only picks how many
+    workgroups share them.  No gradients.  workspace: uint8,
+    teeny_paged_attention_workspace_bytes, that no call on another stream uses at the
+    same time; by default a fresh one."""
+    B, n_pages, hkv, size, D, where = _paged("paged_attention", q, k_pages, v_pages, page_table,
+                                             n_past, starts)
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] < 1 or q.shape[1] % hkv:
+        raise ValueError("paged_attention: q is [T, Hq, D] matching the pages")
+    if q.dtype != k_pages.dtype:
+        raise TypeError("paged_attention: the tensors share a dtype")
+    T, Hq = q.shape[0], q.shape[1]
+    if max_new is not None and max_new < 0 or max_keys is not None and max_keys < 0:
+        raise ValueError("paged_attention: max_new and max_keys are at least 0")
+    new = T // B if starts is None else T if max_new is None else min(int(max_new), T)
+    most = where[2] * size
+    keys = most if max_keys is None else min(int(max_keys), most)
+    code = _code(q)
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    if out is None:
+        out = torch.empty_like(q)
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.get_device() != q.get_device()
+          or not out.is_contiguous()):
+        raise ValueError("paged_attention: out is contiguous, of q's shape, type and device")
+    if workspace is not None and (workspace.get_device() != q.get_device()
+                                  or not workspace.is_contiguous()):
+        raise ValueError("paged_attention: workspace must be contiguous, on q's device")
+    with _on_device_of(q):
+        if workspace is None:  # (asked on q's device: the shares go by its CUs)
+            need = _lib.lib().teeny_paged_attention_workspace_bytes(B, T, new, max(1, keys), Hq, hkv,
+                                                                    D, code)
+            if need:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        size_ws = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        call("teeny_paged_attention", _p(q), _p(k_pages), _p(v_pages), _p(out), *where, B, T, new,
+             keys, n_pages, size, Hq, hkv, D, scale, code, _p(workspace), size_ws, _stream())
+    return out
+
+
+def copy_pages(pages: torch.Tensor, src, dst) -> torch.Tensor:
+    """pages[..., dst[i], :, :, :] = pages[..., src[i], :, :, :] for all i, in place and in
+    one launch for all leading dimensions (teeny_copy_pages): pages [..., n_pages, Hkv,
+    page_size, D], the K and V pools of every layer.  src, dst: page numbers on the host;
+    a page is written once at most, and not both read and written (refused, before anything
+    is copied)."""
+    if pages.dim() < 4:
+        raise ValueError("copy_pages: pages is [..., n_pages, Hkv, page_size, D]")
+    _dev(pages)
+    src, dst = [int(i) for i in src], [int(i) for i in dst]
+    if len(src) != len(dst):
+        raise ValueError("copy_pages: as many sources as destinations")
+    if not src or pages.numel() == 0:
+        if src:
+            raise ValueError("copy_pages: the pool has no pages")
+        return pages
+    n_pages = pages.shape[-4]
+    if min(src) < 0 or min(dst) < 0 or max(src) >= n_pages or max(dst) >= n_pages:
+        raise ValueError("copy_pages: page numbers lie in the pool")
+    if len(set(dst)) != len(dst) or not set(src).isdisjoint(dst):
+        raise ValueError("copy_pages: a page is written once, and not both read and written")
+    size = pages.element_size() * math.prod(pages.shape[-3:])
+    planes = math.prod(pages.shape[:-4])
+    ints = ctypes.c_int32 * len(src)
+    with _on_device_of(pages):
+        call("teeny_copy_pages", _p(pages), planes, size * n_pages, size, n_pages, ints(*src),
+             ints(*dst), len(src), _stream())
+    return pages
 
 
 def argmax_rows(x, out=None, advance=None):

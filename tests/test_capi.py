@@ -507,3 +507,72 @@ def test_shared_prefix_of_two_shapes():
     for a, b in ((k, v), (v, k), (k, k[0]), (k[0], k), (k, k[:, :, :4])):
         with pytest.raises(ValueError, match="of one shape"):
             ops.shared_prefix_attention(q, a, b, c, c, 5, 0)
+
+
+def test_paged_validation(L):
+    def split(**kw):
+        a = dict(qkv=P, parts=None, n_parts=0, q=P, k=P, v=P, table=P, ld=8, width=8, starts=None, past=P,
+                 host=0, b=2, t=2, n_pages=9, page=16, hq=8, hkv=2, d=128, ln=9.2, dtype=BF16)
+        a.update(kw)
+        return L.teeny_paged_qkv_rope_split(*a.values(), None)
+
+    def att(**kw):
+        a = dict(q=P, k=P, v=P, o=P, table=P, ld=8, width=8, starts=None, past=P, host=0, b=2, t=2, new=1,
+                 keys=128, n_pages=9, page=16, hq=8, hkv=2, d=128, scale=0.1, dtype=BF16, ws=P, size=1 << 30)
+        a.update(kw)
+        return L.teeny_paged_attention(*a.values(), None)
+
+    for f in (split, att):
+        for name in ("q", "k", "v", "table"):
+            assert f(**{name: None}) == NULLP, name
+        for kw in (dict(b=0), dict(t=-1), dict(t=3), dict(width=0), dict(ld=7), dict(n_pages=0), dict(page=8),
+                   dict(page=24), dict(page=2048), dict(hkv=3), dict(hq=0), dict(t=1 << 24),
+                   dict(width=1 << 27, ld=1 << 27)):
+            assert f(**kw) == SHAPE, kw
+        assert f(d=32) == UNSUP and f(dtype=7) == UNSUP
+        assert f(past=None, host=-1) == VALUE
+        assert f(k=P + 8) == VALUE
+    assert split(qkv=None) == NULLP and split(parts=P) == NULLP
+    assert split(qkv=None, parts=P, n_parts=0) == SHAPE
+    assert split(ln=float("nan")) == VALUE
+    assert att(o=None) == NULLP
+    for kw in (dict(new=-1), dict(keys=-1), dict(scale=0.0), dict(scale=float("inf"))):
+        assert att(**kw) == VALUE, kw
+    # no GPU work without tokens
+    assert att(t=0) == OK and split(t=0) == OK and att(new=0) == OK
+
+    ws = L.teeny_paged_attention_workspace_bytes
+    assert ws(1, 1, 1, 4000, 8, 2, 128, BF16) > 0
+    assert ws(0, 1, 1, 4000, 8, 2, 128, BF16) == 0 and ws(1, 1, 1, 4000, 8, 3, 128, BF16) == 0
+    assert att(b=1, t=1, keys=4000, width=300, ld=300, ws=None) == WS
+    assert att(b=1, t=1, keys=4000, width=300, ld=300, size=16) == WS
+    assert att(b=1, t=1, keys=4000, width=300, ld=300, ws=P + 8) == VALUE
+
+    def copy(src, dst, n=None, **kw):
+        a = dict(pages=P, planes=2, plane=16 * 512, page=512, n_pages=16)
+        a.update(kw)
+        ints = ctypes.c_int32 * len(src)
+        return L.teeny_copy_pages(*a.values(), ints(*src), ints(*dst), len(src) if n is None else n, None)
+
+    assert copy([], []) == OK
+    assert copy([1], [2], pages=None) == NULLP
+    assert L.teeny_copy_pages(P, 2, 16 * 512, 512, 16, None, None, 1, None) == NULLP
+    for kw in (dict(planes=0), dict(planes=1 << 17), dict(n_pages=0), dict(n=-1), dict(page=0), dict(plane=512)):
+        assert copy([1], [2], **kw) == SHAPE, kw
+    assert copy([1], [2], pages=P + 8) == VALUE and copy([1], [2], page=8) == VALUE
+    for src, dst in (([16], [1]), ([-1], [1]), ([1], [16]), ([1], [-1]), ([1, 2], [3, 3]), ([1, 2], [2, 3]), ([4], [4])):
+        assert copy(src, dst) == VALUE, (src, dst)
+
+
+def test_paged_ops_refuse_host_tensors():
+    import torch
+
+    from teenyformers_amd import ops
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    table = torch.zeros((1, 2), dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.paged_attention(torch.zeros((1, 4, 64), dtype=torch.bfloat16), k, k, table, 0)
+    with pytest.raises(ValueError):
+        ops.paged_qkv_rope_split(torch.zeros((1, 512), dtype=torch.bfloat16), k, k, table, 0, 4, 1e4)
+    with pytest.raises(ValueError):
+        ops.copy_pages(k, [0], [1])
