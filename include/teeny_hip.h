@@ -624,6 +624,31 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
 int teeny_copy_pages(void* pages, int planes, long plane_bytes, long page_bytes, int n_pages,
                      const int32_t* from, const int32_t* to, int n, hipStream_t stream);
 
+/* Drafted tokens checked against the target's probabilities.  drafts [batch,
+ * n_drafts] (int64); target: logits [batch, n_drafts + 1, cols] (row i of a
+ * sequence: the target's after the first i drafts; sequences target_seq and rows
+ * target_row elements apart), draft: the draft model's logits [batch, n_drafts,
+ * cols] that draft i was drawn from, or null where the drafts come from no
+ * distribution (looked up, or a model's first choices).  With p_i = softmax(target_i
+ * / T) and q_i = softmax(draft_i / T), or all on drafts[i]: drafts are accepted in
+ * order while u[b, i] q_i(d) < p_i(d), and then one token is drawn with u[b, n_drafts]
+ * (the first in index order whose running weight exceeds u times the whole): from
+ * max(p_n - q_n, 0) where draft n was refused, from p_n where all were accepted or
+ * draft n is no token (outside 0 .. cols-1: a sequence with fewer drafts ends there).
+ * The tokens then are distributed as the target's own.  tokens [batch, n_drafts + 1]:
+ * the accepted drafts, the drawn token, -1; accepted [batch]: how many.
+ * u [batch, n_drafts + 1] in [0, 1), fp32.  temperature >= 0, or temperature_rows
+ * (fp32 device memory, one per sequence); 0: p and q one-hot at the lowest index of
+ * the row's maximum.  NaN and -inf logits have no weight; a row without any other
+ * draws -1.  n_drafts 1 .. 64; workspace: teeny_verify_drafts_workspace_bytes bytes,
+ * 16-byte aligned. */
+size_t teeny_verify_drafts_workspace_bytes(int batch, int n_drafts, int cols, int with_draft);
+int teeny_verify_drafts(const void* target, long target_seq, long target_row, const void* draft,
+                        long draft_seq, long draft_row, const int64_t* drafts, const float* u,
+                        int batch, int n_drafts, int cols, double temperature,
+                        const float* temperature_rows, int64_t* tokens, int32_t* accepted, int dtype,
+                        void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* teeny_decode_qkv_attention_dev: a one-token decode step's attention in
  * one launch, for position p = *n_past (read when the kernel runs): the
  * QKV projection's K-split slabs parts[n_parts][batch][(Hq + 2 Hkv) D] are

@@ -101,6 +101,9 @@ _SIGNATURES = {
     "teeny_sample_rows_workspace_bytes": ([_i, _i], _sz),
     "teeny_sample_rows": ([_p, _l, _p, _i, _i, _d, _p, _i, _p, _d, _p, _d, _p, _p, _i, _p, _p, _sz,
                            _p], _i),
+    "teeny_verify_drafts_workspace_bytes": ([_i] * 4, _sz),
+    "teeny_verify_drafts": ([_p, _l, _l, _p, _l, _l, _p, _p, _i, _i, _i, _d, _p, _p, _p, _i, _p, _sz,
+                             _p], _i),
     "teeny_linear_bf16": ([_p, _p, _p, _i, _i, _i, _p], _i),
     "teeny_gemm_bf16": ([_p, _p, _p, _i, _i, _i, _p], _i),
     "teeny_linear_swiglu_bf16": ([_p, _p, _p, _i, _i, _i, _p], _i),

@@ -37,8 +37,8 @@ ARCH = "gfx950"
 # Order matters only for readability; capi.cpp declares the same list.
 KERNEL_SOURCES = [
     "transpose", "rope", "norm", "swiglu", "embed", "fa2_f32", "fa2_fwd_bf16", "fa2_bwd_bf16",
-    "llama", "decode_bf16", "prefix_attn", "paged", "sample", "linear_bf16", "gemm_bf16",
-    "gemm_f32",
+    "llama", "decode_bf16", "prefix_attn", "paged", "sample", "verify", "linear_bf16",
+    "gemm_bf16", "gemm_f32",
 ]
 
 HIPCC_FLAGS = [

@@ -41,6 +41,7 @@
   X(prefix_attn)         \
   X(paged)               \
   X(sample)              \
+  X(verify)              \
   X(linear_bf16)         \
   X(gemm_bf16)           \
   X(gemm_f32)
@@ -1772,6 +1773,63 @@ int teeny_sample_rows(const void* logits, long ld, const float* u, int rows, int
   snprintf(name, sizeof name, "teeny_sample_draw_%s", dtype_tag(dtype));
   void* a1[] = {&logits, &ld, &cols, &a, &u, &rec, &bins, &n_ch, &out, &advance};
   return launch(name, dim3((unsigned)rows), dim3(512), 0, stream, a1);
+}
+
+// Verification of drafted tokens (verify.hip).
+namespace {
+constexpr int kMaxDrafts = 64;
+struct VerifyArgs {  // Args in verify.hip
+  const void *target, *draft;
+  long t_seq, t_row, d_seq, d_row;
+  const int64_t* drafts;
+  const float *u, *ts;
+  double t;
+  int batch, k, cols, n_ch;
+};
+}  // namespace
+
+size_t teeny_verify_drafts_workspace_bytes(int batch, int n_drafts, int cols, int with_draft) {
+  if (batch <= 0 || n_drafts <= 0 || n_drafts > kMaxDrafts || cols <= 0 || cols > kSampleCols)
+    return 0;
+  const long rows = (long)batch * (n_drafts + 1 + (with_draft ? n_drafts : 0));
+  if (rows > 65535) return 0;
+  return align256((size_t)rows * sample_chunks(cols) * 16) + align256((size_t)batch * 64 * 8);
+}
+
+int teeny_verify_drafts(const void* target, long target_seq, long target_row, const void* draft,
+                        long draft_seq, long draft_row, const int64_t* drafts, const float* u,
+                        int batch, int n_drafts, int cols, double temperature,
+                        const float* temperature_rows, int64_t* tokens, int32_t* accepted, int dtype,
+                        void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (!target || !drafts || !u || !tokens || !accepted) return TEENY_ERR_NULL_POINTER;
+  if (!dtype_ok(dtype)) return TEENY_ERR_UNSUPPORTED;
+  const long rows = (long)std::max(batch, 0) * (n_drafts + 1 + (draft ? n_drafts : 0));
+  if (batch <= 0 || n_drafts <= 0 || n_drafts > kMaxDrafts || cols <= 0 || cols > kSampleCols ||
+      rows > 65535 || target_seq < 0 || target_row < cols ||
+      (draft && (draft_seq < 0 || (n_drafts > 1 && draft_row < cols))))
+    return TEENY_ERR_INVALID_SHAPE;
+  if (((uintptr_t)target | (uintptr_t)draft) % dtype_size(dtype) != 0) return TEENY_ERR_INVALID_VALUE;
+  if (!temperature_rows && !(temperature >= 0.0)) return TEENY_ERR_INVALID_VALUE;
+  if (!workspace || workspace_bytes < teeny_verify_drafts_workspace_bytes(batch, n_drafts, cols,
+                                                                          draft != nullptr))
+    return TEENY_ERR_WORKSPACE;
+  if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
+  VerifyArgs a{target, draft, target_seq, target_row, draft_seq, draft_row, drafts, u,
+               temperature_rows, temperature, batch, n_drafts, cols, sample_chunks(cols)};
+  void* rec = workspace;
+  void* part = (char*)workspace + align256((size_t)rows * a.n_ch * 16);
+  char name[48];
+  snprintf(name, sizeof name, "teeny_verify_scan_%s", dtype_tag(dtype));
+  void* a0[] = {&a, &rec};
+  int rc = launch(name, dim3((unsigned)a.n_ch, (unsigned)rows), dim3(512), 0, stream, a0);
+  if (rc) return rc;
+  snprintf(name, sizeof name, "teeny_verify_rest_%s", dtype_tag(dtype));
+  void* a1[] = {&a, &rec, &part};
+  rc = launch(name, dim3((unsigned)a.n_ch, (unsigned)batch), dim3(512), 0, stream, a1);
+  if (rc) return rc;
+  snprintf(name, sizeof name, "teeny_verify_pick_%s", dtype_tag(dtype));
+  void* a2[] = {&a, &rec, &part, &tokens, &accepted};
+  return launch(name, dim3((unsigned)batch), dim3(512), 0, stream, a2);
 }
 
 // Decode-step linear layers (linear_bf16.hip): 512 threads, 128 W rows per

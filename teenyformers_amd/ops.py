@@ -975,6 +975,79 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
     return out
 
 
+def _logit_rows(name: str, x: torch.Tensor):
+    """x [B, n, V] with its columns side by side, and the sequences' and rows' strides."""
+    V = x.shape[2]
+    if x.stride(2) != 1 and V > 1 or x.shape[1] > 1 and x.stride(1) < V or x.shape[0] > 1 and x.stride(0) < 0:
+        x = x.contiguous()
+    return x, x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else V
+
+
+def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor,
+                  draft_logits: torch.Tensor | None = None, temperature=1.0, tokens=None, accepted=None,
+                  workspace: torch.Tensor | None = None):
+    """Drafted tokens checked against the target's probabilities (teeny_verify_drafts):
+    drafts int64 [B, K] and the target's logits [B, K+1, V] after 0 .. K of them ->
+    (tokens int64 [B, K+1], accepted int32 [B]): each sequence's accepted drafts, the
+    token drawn after them, and -1.  The tokens are distributed as the target's own.
+
+    Draft i is accepted while u[:, i] q_i(d) < p_i(d); the token after the last accepted
+    one is drawn with u[:, K] from max(p_n - q_n, 0), or from p_n where no draft was
+    refused.  draft_logits [B, K, V]: what the drafts were drawn from (at the same
+    temperature); without, each draft is taken as certain (looked up, or a model's first
+    choice).  A draft outside the vocabulary (-1) ends its sequence's drafts.  u: fp32 in
+    [0, 1).  temperature: a number, or fp32 [B], read when the kernels run; 0: the
+    target's lowest index of the row's maximum decides.  workspace: uint8,
+    teeny_verify_drafts_workspace_bytes, that no call on another stream uses at the same
+    time; by default a fresh one."""
+    dev = logits.get_device()
+    if dev < 0:
+        raise ValueError("teenyformers_amd ops take device tensors (no CPU fallback)")
+    if logits.dim() != 3 or logits.shape[1] < 2 or logits.shape[2] < 1:
+        raise ValueError("verify_drafts: logits are [B, K + 1, V] with K and V at least 1")
+    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    code = _code(logits)
+
+    def of(name, t, shape, dtype):
+        if t.shape != shape or t.dtype != dtype or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"verify_drafts: {name} is contiguous {dtype} {list(shape)} on the logits' "
+                             "device")
+        return t
+
+    of("drafts", drafts, (B, K), torch.int64)
+    of("u", u, (B, K + 1), torch.float32)
+    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=logits.device) if tokens is None else \
+        of("tokens", tokens, (B, K + 1), torch.int64)
+    accepted = torch.empty(B, dtype=torch.int32, device=logits.device) if accepted is None else \
+        of("accepted", accepted, (B,), torch.int32)
+    ts = None
+    if isinstance(temperature, torch.Tensor):
+        ts, temperature = of("temperature", temperature, (B,), torch.float32), 0.0
+    elif not temperature >= 0.0:
+        raise ValueError("verify_drafts: temperature must be at least 0")
+    x, x_seq, x_row = _logit_rows("logits", logits)
+    q, q_seq, q_row = None, 0, 0
+    if draft_logits is not None:
+        if draft_logits.shape != (B, K, V) or draft_logits.get_device() != dev:
+            raise ValueError("verify_drafts: draft_logits are [B, K, V] on the logits' device")
+        if draft_logits.dtype != logits.dtype:
+            raise TypeError("verify_drafts: both logits share a dtype")
+        q, q_seq, q_row = _logit_rows("draft_logits", draft_logits)
+    if B == 0:
+        return tokens, accepted
+    if workspace is None:
+        size = _lib.lib().teeny_verify_drafts_workspace_bytes(B, K, V, int(q is not None))
+        workspace = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError("verify_drafts: workspace must be contiguous, on the logits' device")
+    else:
+        size = workspace.numel() * workspace.element_size()
+    with _on_device_of(x):
+        call("teeny_verify_drafts", _p(x), x_seq, x_row, _p(q), q_seq, q_row, _p(drafts), _p(u), B, K, V,
+             float(temperature), _p(ts), _p(tokens), _p(accepted), code, _p(workspace), size, _stream())
+    return tokens, accepted
+
+
 def _no_grad(x2: torch.Tensor, w: torch.Tensor) -> bool:
     # the library's linear kernels have no backward: autograd uses torch's GEMM
     return not (torch.is_grad_enabled() and (x2.requires_grad or w.requires_grad))

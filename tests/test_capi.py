@@ -576,3 +576,23 @@ def test_paged_ops_refuse_host_tensors():
         ops.paged_qkv_rope_split(torch.zeros((1, 512), dtype=torch.bfloat16), k, k, table, 0, 4, 1e4)
     with pytest.raises(ValueError):
         ops.copy_pages(k, [0], [1])
+
+
+def test_verify_drafts_validation(L):
+    def verify(**kw):
+        a = dict(target=P, t_seq=400, t_row=100, draft=P, d_seq=300, d_row=100, drafts=P, u=P, b=2, k=3, cols=100,
+                 t=1.0, ts=None, tokens=P, accepted=P, dtype=BF16, ws=P, size=1 << 30)
+        a.update(kw)
+        return L.teeny_verify_drafts(*a.values(), None)
+
+    for name in ("target", "drafts", "u", "tokens", "accepted"):
+        assert verify(**{name: None}) == NULLP, name
+    assert verify(dtype=9) == UNSUP
+    for kw in (dict(b=0), dict(b=-3), dict(k=0), dict(k=65), dict(cols=0), dict(cols=1 << 20), dict(t_row=99),
+               dict(d_row=99), dict(t_seq=-1), dict(d_seq=-1), dict(b=1 << 15)):
+        assert verify(**kw) == SHAPE, kw
+    for kw in (dict(target=P + 1), dict(draft=P + 1), dict(t=-1.0), dict(t=float("nan")), dict(ws=P + 8)):
+        assert verify(**kw) == VALUE, kw
+    assert verify(ws=None) == WS and verify(size=64) == WS
+    ws = L.teeny_verify_drafts_workspace_bytes
+    assert ws(2, 3, 100, 1) > 0 and ws(2, 65, 100, 1) == 0 and ws(0, 3, 100, 0) == 0 and ws(1 << 15, 3, 100, 0) == 0
