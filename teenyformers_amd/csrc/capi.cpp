@@ -1501,12 +1501,17 @@ struct Paged {  // in paged.h
   int ld, width, n_pages, lg;
   int hq, hkv;
 };
-struct PagedPlan {  // Plan in paged.hip
+struct PagedPlan {  // in paged.h
   float scale;
-  int keys, splits, keys_many, splits_many, few, groups;
+  int keys, splits, keys_many, splits_many, few, groups, tiles;
 };
-struct PagedParts {  // Parts in paged.hip
+struct PagedParts {  // in paged.h
   float *m, *l, *o;
+};
+struct FwdPaged {  // in fa2_fwd_bf16.hip
+  Paged a;
+  PagedPlan pl;
+  PagedParts parts;
 };
 constexpr int kPageMoves = 448;  // kMoves in paged.hip
 struct PageMoves {               // Moves in paged.hip
@@ -1531,24 +1536,31 @@ int paged_args(Paged* a, const int32_t* table, int table_ld, int table_width, co
   return TEENY_OK;
 }
 
-// Shares of the keys: see the entry point.
+// Sequences of up to `few` rows a kv head take shares of their keys by workgroups of 32
+// rows, the others the forward kernel's walk by workgroups of 128.
 PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, int hkv, int head_dim,
                      int dtype) {
-  (void)tokens;
   (void)head_dim;
   PagedPlan p{};
   const bool f32 = dtype == TEENY_F32;
   const int unit = f32 ? 16 : 32, waves = f32 ? 1 : 4;
-  const long rows = (long)(hq / hkv) * max_new;
-  p.few = 0x7fffffff;
-  p.groups = (int)((rows + unit - 1) / unit);
-  const long items = (long)batch * hkv * p.groups, want = 2L * device_cus();
+  const long G = hq / hkv, rows = G * max_new, cus = device_cus();
+  p.few = f32 ? 0x7fffffff : 32;
+  p.groups = (int)((std::min(rows, (long)p.few) + unit - 1) / unit);
+  const long items = (long)batch * hkv * p.groups, want = 2 * cus;
   const long most = std::max(1L, want / std::max(1L, items));
   const long step = 32L * waves;
   p.keys = (int)(((max_keys + most - 1) / most + step - 1) / step * step);
   p.splits = std::max(1, (max_keys + p.keys - 1) / p.keys);
-  p.keys_many = p.keys;
   p.splits_many = 1;
+  p.keys_many = max_keys;
+  if (rows > p.few) {
+    p.tiles = (int)(tokens * G / 128 + std::min((long)batch, tokens * G / (p.few + 1)));
+    const long wgs = (long)p.tiles * hkv, slots = 3 * cus;
+    const long n = std::max(1L, std::min(slots / std::max(1L, wgs), (max_keys + 511L) / 512));
+    p.keys_many = (int)(((max_keys + n - 1) / n + 63) / 64 * 64);
+    p.splits_many = std::max(1, (max_keys + p.keys_many - 1) / p.keys_many);
+  }
   return p;
 }
 }  // namespace
@@ -1637,15 +1649,28 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
              (float*)((char*)workspace + 2 * each)};
   }
   const long wgs = (long)p.splits * p.groups * batch * n_heads_kv;
-  if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+  const long many = (long)p.tiles * n_heads_kv * p.splits_many;
+  if (wgs >= (1L << 31) || many >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
   char name[64];
-  if (dtype == TEENY_BF16)
-    snprintf(name, sizeof name, "teeny_paged_attn_bf16_d%d_w4", head_dim);
-  else
-    snprintf(name, sizeof name, "teeny_paged_attn_f32_d%d", head_dim);
-  void* a0[] = {&q, &k_pages, &v_pages, &o, &a, &p, &parts};
-  rc = launch(name, dim3((unsigned)wgs), dim3(dtype == TEENY_BF16 ? 256 : 64), 0, stream, a0);
-  if (rc || shares == 1) return rc;
+  if (many > 0) {
+    FwdPaged f{a, p, parts};
+    int total = (int)many;
+    snprintf(name, sizeof name, "teeny_fa2_fwd_bf16_d%d_paged", head_dim);
+    void* args[] = {&q, &k_pages, &v_pages, &o, &total, &f};
+    rc = launch(name, dim3((unsigned)many), dim3(256), 0, stream, args);
+    if (rc) return rc;
+  }
+  // (all sequences alike: one of the two has work)
+  if (starts || many == 0) {
+    if (dtype == TEENY_BF16)
+      snprintf(name, sizeof name, "teeny_paged_attn_bf16_d%d_w4", head_dim);
+    else
+      snprintf(name, sizeof name, "teeny_paged_attn_f32_d%d", head_dim);
+    void* a0[] = {&q, &k_pages, &v_pages, &o, &a, &p, &parts};
+    rc = launch(name, dim3((unsigned)wgs), dim3(dtype == TEENY_BF16 ? 256 : 64), 0, stream, a0);
+    if (rc) return rc;
+  }
+  if (shares == 1) return TEENY_OK;
   int lg_d = log2_of(head_dim);
   snprintf(name, sizeof name, "teeny_paged_merge_%s", dtype_tag(dtype));
   void* a1[] = {&parts, &o, &a, &p, &lg_d};

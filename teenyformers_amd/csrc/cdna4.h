@@ -45,6 +45,14 @@ constexpr int kMfma = 0x008, kVmemRead = 0x020, kDsRead = 0x100;
 // out of the block they are scheduled in.
 template <typename T> DEVI void pin(T& x) { asm volatile("" : "+v"(x)); }
 
+// The lane's number, formed where it is asked for: what depends on it is not kept in a
+// register through a loop that has none left.
+DEVI int lane_now() {
+  int lane;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(lane));
+  return lane;
+}
+
 // ds_read_b64_tr_b16: within each 16-lane group, output lane i receives
 // element (i % 4) of the 8-byte chunks addressed by lanes i/4, i/4+4, i/4+8
 // and i/4+12 (measured on gfx950): lanes addressing a 4-row x 16-column block

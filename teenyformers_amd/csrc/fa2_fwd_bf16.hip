@@ -48,6 +48,7 @@
 //     apart) instead of [B, Hq, Sq, D]; rope_cs: Q is read from the fused
 //     QKV projection and rotated (RoPE) as it is loaded.
 #include "cdna4.h"
+#include "paged.h"
 
 #include <type_traits>
 
@@ -90,12 +91,92 @@ struct FwdPrefix {
   int past_stride, past_imm;
 };
 
-template <int D, bool CAUSAL, int NW = 4, bool PACK = false, int NSUB = 2, bool PREFIX = false>
+// PAGED (teeny_paged_attention's sequences of many rows): the keys lie in the
+// sequence's pages, the rows of a kv head are its (token, q head of the group) pairs,
+// 32 NW consecutive ones a workgroup, and a workgroup walks a share of their keys.  The
+// page of each 16 keys comes from a register of 64 table entries; a load of a wavefront
+// lies in one page.  Workgroups go kv head by kv head, the last rows of a sequence first.
+struct FwdPaged {
+  Paged a;
+  PagedPlan pl;
+  PagedParts parts;
+};
+
+// 32 rows of a wavefront over the keys k_first .. k_last - 1, one key after the other: where
+// a value of V that is not finite lies behind some row's last key (0 times it would be
+// NaN in a product over a tile).  A lane holds half of a row's d.
+template <int D>
+DEVI void paged_rows(const bf16* q, const bf16* k, const bf16* v, bf16* o, const FwdPaged& pg,
+                     const Seq& seq, int b, int hk, int split, int wrow0, int k_first, int k_last,
+                     bool direct) {
+  constexpr int H = D / 2;
+  const Paged& a = pg.a;
+  const int ln = lane_now(), g = ln >> 5, group = a.hq / a.hkv;
+  const int r = wrow0 + (ln & 31), rc = min(r, seq.n * group - 1), tok = rc / group;
+  const long row = (long)(seq.t0 + tok) * a.hq + hk * group + (rc - tok * group);
+  const int lim = min(seq.keys(tok), k_last);
+  const float sl2 = pg.pl.scale * kLog2e;
+  float acc[H], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < H; ++i) acc[i] = 0.0f;
+#pragma unroll 1
+  for (int key = k_first; key < k_last; ++key) {
+    const int page = a.table[(long)b * a.ld + (key >> a.lg)];
+    if ((unsigned)page >= (unsigned)a.n_pages) continue;
+    const long at = ((((long)page * a.hkv + hk) << a.lg) + (key & ((1 << a.lg) - 1))) * D + g * H;
+    float s = 0.0f;
+#pragma unroll 2
+    for (int c = 0; c < H; c += 8) {
+      float x[8], y[8];
+      Vec16<bf16>::load(q + row * D + g * H + c, x);
+      Vec16<bf16>::load(k + at + c, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = __builtin_fmaf(x[e], y[e], s);
+    }
+    s = (s + other_half(s)) * sl2;
+    if (key >= lim || s == -INFINITY) continue;
+    const float mn = fmaxf(m, s), al = fast_exp2(m - mn), p = fast_exp2(s - mn);
+    m = mn;
+    l = l * al + p;
+#pragma unroll
+    for (int c = 0; c < H; c += 8) {
+      float y[8];
+      Vec16<bf16>::load(v + at + c, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[c + e] = acc[c + e] * al + p * y[e];
+    }
+  }
+  if (r != rc) return;
+  if (direct) {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int c = 0; c < H; c += 8) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = acc[c + e] * inv;
+      Vec16<bf16>::store(o + row * D + g * H + c, y);
+    }
+    return;
+  }
+  const long to = (long)split * a.tokens * a.hq + row;
+  if (g == 0) {
+    pg.parts.m[to] = m;
+    pg.parts.l[to] = l;
+  }
+#pragma unroll
+  for (int c = 0; c < H; c += 4)
+    *reinterpret_cast<f32x4*>(pg.parts.o + to * D + g * H + c) =
+        f32x4{acc[c], acc[c + 1], acc[c + 2], acc[c + 3]};
+}
+
+template <int D, bool CAUSAL, int NW = 4, bool PACK = false, int NSUB = 2, bool PREFIX = false,
+          bool PAGED = false>
 __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const bf16* __restrict__ k,
                              const bf16* __restrict__ v, bf16* __restrict__ o,
                              float* __restrict__ lse, int nq, int nk, float scale, int hq, int hkv,
                              int num_m_blocks, int total_blocks, int o_merged,
-                             const float2* __restrict__ rope_cs, const FwdPrefix pre = {}) {
+                             const float2* __restrict__ rope_cs, const FwdPrefix pre = {},
+                             const FwdPaged pg = {}) {
   constexpr int BN = SUBN * NSUB;      // keys per tile
   constexpr int BM = 32 * NW;          // query rows per workgroup
   constexpr int NT = 64 * NW;          // threads
@@ -116,9 +197,54 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   int bh, rank;
   // causal blocks: heads in groups of 4 (measured 1.02-1.06x at B16 Hq32 Hkv8
   // S512 and B4 S2048 against pairs; equal blocks gain nothing from it)
-  pair_order<CAUSAL ? 4 : 2>(id, num_m_blocks, total_blocks / num_m_blocks, bh, rank);
+  if constexpr (!PAGED)
+    pair_order<CAUSAL ? 4 : 2>(id, num_m_blocks, total_blocks / num_m_blocks, bh, rank);
   // the last query block is the heaviest (PREFIX: the lightest, its rows may end)
-  const int mb = PREFIX ? rank : num_m_blocks - 1 - rank;
+  int mb = PREFIX ? rank : num_m_blocks - 1 - rank;
+  Seq seq{};
+  int group = 1, hk_p = 0, b_p = 0, split_p = 0, k_first = 0, k_last = 0;
+  bool direct = true;
+  if constexpr (PAGED) {
+    group = hq / hkv;
+    hk_p = id / (pg.pl.tiles * pg.pl.splits_many);
+    const int in = id - hk_p * pg.pl.tiles * pg.pl.splits_many;
+    split_p = in / pg.pl.tiles;
+    int left = in - split_p * pg.pl.tiles;
+    // the left-th row tile among those of the sequences of many rows
+    b_p = -1;
+    for (int b0 = 0; b0 < pg.a.batch && b_p < 0; b0 += 64) {
+      int tiles = 0;
+      if (b0 + lane < pg.a.batch) {
+        const long rows = (long)seq_of(pg.a, b0 + lane).n * group;
+        tiles = rows > pg.pl.few ? (int)((rows + BM - 1) / BM) : 0;
+      }
+      int run = tiles;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(run, off, 64);
+        run += lane >= off ? o : 0;
+      }
+      const uint64_t past = __ballot(run > left);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b_p = b0 + l;
+        mb = __builtin_amdgcn_readlane(run, l) - 1 - left;  // the last rows first
+      } else {
+        left -= __builtin_amdgcn_readlane(run, 63);
+      }
+    }
+    if (b_p < 0) return;
+    seq = seq_of(pg.a, b_p);
+    const int n_sh = paged_shares(seq, pg.pl.keys_many, pg.pl.splits_many);
+    if (split_p >= n_sh) return;
+    direct = n_sh == 1;
+    nq = seq.n * group;
+    // the keys of this share that the workgroup's last row sees
+    const int last = seq.keys((min(mb * BM + BM, nq) - 1) / group);
+    k_first = split_p * pg.pl.keys_many;
+    k_last = split_p + 1 < pg.pl.splits_many ? min(k_first + pg.pl.keys_many, last) : last;
+    k_last = max(k_last, k_first);
+  }
   // bhq: this wavefront's (b, q head); wrow0: its first query row; blk_end:
   // one past the workgroup's last row.  GQA-packed (PACK, NW = hq / hkv): bh
   // is a (b, kv head), every wavefront takes the same 32 rows of its own q
@@ -126,7 +252,12 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // rows 32 w of the block's BM.
   int bhq, wrow0, blk_end;
   long kvh;
-  if constexpr (PREFIX) {
+  if constexpr (PAGED) {
+    kvh = 0;
+    bhq = 0;
+    wrow0 = mb * BM + wave * 32;
+    blk_end = mb * BM + BM;
+  } else if constexpr (PREFIX) {
     const int hk = bh / pre.batch, b = bh - hk * pre.batch;
     kvh = (long)b * hkv + hk;
     bhq = (int)kvh;
@@ -147,6 +278,11 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   }
   const int qrow = wrow0 + l32;
   const int wave_qmax = wrow0 + 31;
+  // PAGED: the output row of row r of the kv head
+  auto paged_row = [&](int r) {
+    const int tok = r / group;
+    return (long)(seq.t0 + tok) * hq + hk_p * group + (r - tok * group);
+  };
 
   const bf16* kb = k + kvh * (long)nk * D;
   const bf16* vb = v + kvh * (long)nk * D;
@@ -165,7 +301,9 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   {
     const int qr = min(qrow, nq - 1);
     const bf16* qp;
-    if (rope_cs) {
+    if constexpr (PAGED) {
+      qp = q + paged_row(qr) * D + 8 * g;
+    } else if (rope_cs) {
       const int qb = bhq / hq, qh = bhq - qb * hq;
       qp = q + ((long)qb * nq + qr) * ((hq + 2 * hkv) * D) + qh * D + 8 * g;
     } else {
@@ -202,6 +340,7 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
 
   int kend = nk;
   if (CAUSAL) kend = min(nk, blk_end);
+  if (PAGED) kend = k_last - k_first;
   int n_iter = (kend + BN - 1) / BN;
   // PREFIX: own keys of this lane's row (lim) and of the wavefront's first tokens
   // that every row of it sees (lim_all); prefix tiles
@@ -234,9 +373,18 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     }
     lim = min(past + min(qrow, nq - 1) % pre.s + 1, nk);
   }
+  if constexpr (PAGED) {  // keys relative to the share's first
+    lim_all = min(seq.keys(min(wrow0, nq - 1) / group), k_last) - k_first;
+    const int mine = min(seq.keys(min(wrow0 + 31, nq - 1) / group), k_last) - k_first;
+    own_live = wrow0 < nq ? (max(0, mine) + BN - 1) / BN : 0;
+  }
+  // PAGED: the keys of a lane's row
+  auto paged_lim = [&](int ln) {
+    return min(seq.keys(min(wrow0 + (ln & 31), nq - 1) / group), k_last) - k_first;
+  };
   // causal: the workgroup's tiles past this wavefront's last row are fully
   // masked for it; it computes only the first n_live (wave-uniform)
-  const int n_live = PREFIX   ? max(1, own_live)
+  const int n_live = PREFIX || PAGED ? max(1, own_live)
                      : CAUSAL ? min(n_iter, wave_qmax / BN + 1)
                               : n_iter;
 
@@ -258,9 +406,43 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // it: tile index; koff / voff: byte offsets of its K and V buffers.  Rows
   // past the sequence lie outside the descriptors' ranges and load as zeros:
   // their scores are masked, and P = 0 times V = 0 adds nothing.
+  // PAGED: the pages of the 16-key groups of the tile to load next (-1: absent), read by
+  // scalar loads a tile ahead, and the groups of the tile loaded last without one
+  int pages[BN / 16];
+  int absent = 0;
+  auto fetch_pages = [&](int it) {
+    typedef __attribute__((address_space(4))) const int CInt;
+    const CInt* row = (const CInt*)(uintptr_t)(pg.a.table + (long)b_p * pg.a.ld);
+#pragma unroll
+    for (int h = 0; h < BN / 16; ++h) {
+      const int i = (k_first + it * BN + 16 * h) >> pg.a.lg;
+      pages[h] = row[min(i, pg.a.width - 1)];
+      if (i >= pg.a.width || (unsigned)pages[h] >= (unsigned)pg.a.n_pages) pages[h] = -1;
+    }
+  };
   auto load_tile = [&](int it, int koff, int voff) {
     char* kdst = sm.k[0] + koff + wave * 64 * 16;
     char* vdst = sm.v[0] + voff + wave * 64 * 16;
+    if constexpr (PAGED) {
+      constexpr int RPW = 64 / CPR, RPL = NT / CPR;  // rows of a wavefront's, of a load
+      const int lg = pg.a.lg, tile0 = k_first + it * BN;
+      absent = 0;
+#pragma unroll
+      for (int h = 0; h < BN / 16; ++h) absent |= (pages[h] < 0) << h;
+#pragma unroll
+      for (int i = 0; i < TCH; ++i) {
+        const int row0 = i * RPL + wave * RPW, key = tile0 + (row0 & ~15);
+        // (32 rows a load: two wavefronts' lie in its first 16)
+        const int page = RPL == 16 ? pages[i] : wave < 2 ? pages[2 * i % (BN / 16)] : pages[(2 * i + 1) % (BN / 16)];
+        const int n = page < 0 ? 0 : min(max(k_last - key, 0), 16);
+        const long at = ((((long)max(page, 0) * hkv + hk_p) << lg) + (key & ((1 << lg) - 1))) * D;
+        // the lane's chunk within the 16 rows
+        const int back = RPL == 16 ? 0 : (wave >> 1) * 16 * D * 2;
+        dma16(make_rsrc(k + at, n * D * 2), kdst + i * LSTEP, k_src - back, 0);
+        dma16(make_rsrc(v + at, n * D * 2), vdst + i * LSTEP, v_src - back, 0);
+      }
+      return;
+    }
     if (PREFIX && it < n_pre) {
       const int pbytes = it * BN * D * 2;
 #pragma unroll
@@ -368,7 +550,32 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
 
   // raw scores of keys past the sequence or (causal) past the row -> -inf;
   // only tiles that reach past nk or past the wave's first row need it
-  auto mask = [&](int kbase, f32x16& s0, f32x16& s1) {
+  // (PAGED: those past the row are a wavefront's last two tiles', the tail's alone; gone:
+  // the 16-key groups without a page)
+  auto mask = [&](int kbase, f32x16& s0, f32x16& s1, int gone = 0, bool edge = true) {
+    if constexpr (PAGED) {
+      if (edge && kbase + BN > lim_all) {
+        const int ln = lane_now(), end = paged_lim(ln);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = kbase + 8 * (r >> 2) + 4 * (ln >> 5) + (r & 3);
+          if (key >= end) s0[r] = -INFINITY;
+          if constexpr (NSUB == 2) {
+            if (key + 32 >= end) s1[r] = -INFINITY;
+          }
+        }
+      }
+      if (gone) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (gone >> (r >> 3) & 1) s0[r] = -INFINITY;
+          if constexpr (NSUB == 2) {
+            if (gone >> (2 + (r >> 3)) & 1) s1[r] = -INFINITY;
+          }
+        }
+      }
+      return;
+    }
     if constexpr (PREFIX) {
       const bool own = kbase >= n_pre * BN;
       const int t0 = own ? kbase - n_pre * BN : kbase;
@@ -453,7 +660,9 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // the tile's partial row sums are checked before they join l: a tile with
   // a sum at or above 2^31 (or not finite) is redone with its maximum
   auto check_tile = [&](const f32x16& s0, const f32x16& s1, float& la, float& lb) {
-    if (__any(!(fmaxf(la, lb) < kPmax))) {  // wave-uniform and rare
+    // (PAGED: a row that has met no key yet has no offset either: its first keys may
+    // lie in a later tile, all far below zero)
+    if (__any(!(fmaxf(la, lb) < kPmax) || (PAGED && m_run == -INFINITY))) {  // wave-uniform and rare
 #pragma unroll
       for (int u = 0; u < 4; ++u) max_piece(u, s0, s1);
       la = 0.0f;
@@ -473,13 +682,32 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   };
 
 
+  // PAGED: whether a tile that some row of the wavefront sees only in part holds values
+  // of V that are not finite: such tiles are a wavefront's last two, and its rows are then
+  // formed again key by key (paged_rows).
+  bool bad = false;
+  auto edge_bad = [&](int it, const char* vt) {
+    if (it * BN + BN <= lim_all) return false;
+    uint32_t any = 0;
+#pragma unroll 1
+    for (int i = 0; i < TILE / 1024; ++i) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(vt + i * 1024 + lane_now() * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) any |= bf16_bad(w[j]);
+    }
+    return (bool)__any(any != 0);
+  };
+
   // ---- first tile: scores and P only ----
   if (n_iter > 0) {
     // tile 1 is requested with tile 0, before the first wait: its latency
     // overlaps the first tile's, and the first tile's products wait only for
     // the Q rows and tile 0 (tile 1's 2 TCH loads, issued last, may still fly)
+    if constexpr (PAGED) fetch_pages(0);
     load_tile(0, 0, 0);
+    const int absent0 = absent;
     if (n_iter > 1) {
+      if constexpr (PAGED) fetch_pages(1);
       load_tile(1, TILE, TILE);
       __builtin_amdgcn_s_waitcnt(kVmWaitLgkm0<2 * TCH>());
     } else {
@@ -490,7 +718,8 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     if (rope_cs) rotate_q();
     f32x16 s0, s1;
     qk(sm.k[0], s0, s1);
-    mask(0, s0, s1);
+    mask(0, s0, s1, absent0);
+    if constexpr (PAGED) bad = edge_bad(0, sm.v[0]);
 #pragma unroll
     for (int u = 0; u < 4; ++u) max_piece(u, s0, s1);
     grow = false;  // O is still zero: no scaling due
@@ -501,6 +730,7 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
       pprev[0][i] = pnew[0][i];
       if constexpr (NSUB == 2) pprev[1][i] = pnew[1][i];
     }
+    if constexpr (PAGED) fetch_pages(2);
     __builtin_amdgcn_s_waitcnt(0);  // this thread's loads of tile 1 have landed
     __syncthreads();
   }
@@ -511,13 +741,15 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // unrolled over the 6 tiles after which both rotations repeat, so every LDS
   // address is a lane offset plus a constant (the read's immediate offset)
   // instead of one address add per read.
-  auto tile_step = [&](int it, auto KB, auto VP) {
-    constexpr int kb = decltype(KB)::value;  // K buffer of tile it
-    constexpr int vp = decltype(VP)::value;  // V buffer of tile it - 1
+  auto tile_step = [&](int it, auto KB, auto VP, auto EDGE) {
+    const int kb = KB;  // K buffer of tile it
+    const int vp = VP;  // V buffer of tile it - 1
+    constexpr bool edge = decltype(EDGE)::value;  // PAGED: tiles it - 1 and it may be bad
     const int kbase = it * BN;
     f32x16 s0, s1;
     qk(sm.k[kb], s0, s1);
-    mask(kbase, s0, s1);
+    mask(kbase, s0, s1, absent, edge);
+    if constexpr (edge) bad |= edge_bad(it, sm.v[(vp + 1) % VBUF]);
     // a maximum raised by tile it-1 scales O before tile it-1's product
     if (grow) {
       rescale_o();
@@ -556,6 +788,7 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     }
     pin(l_run);
     pin(l_run2);
+    if constexpr (PAGED) fetch_pages(it + 2);
     __builtin_amdgcn_s_waitcnt(0);  // this thread's loads of tile it+1 have landed
     __syncthreads();
   };
@@ -563,21 +796,28 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
+    using Inner = std::false_type;
     int it = 1;
-    for (; it + 6 <= n_live; it += 6) {
-      tile_step(it, I1{}, I0{});
-      tile_step(it + 1, I0{}, I1{});
-      tile_step(it + 2, I1{}, I2{});
-      tile_step(it + 3, I0{}, I0{});
-      tile_step(it + 4, I1{}, I1{});
-      tile_step(it + 5, I0{}, I2{});
+    // (PAGED: the last two tiles, and the products with them, are the tail's)
+    for (; it + 6 <= (PAGED ? n_live - 2 : n_live); it += 6) {
+      tile_step(it, I1{}, I0{}, Inner{});
+      tile_step(it + 1, I0{}, I1{}, Inner{});
+      tile_step(it + 2, I1{}, I2{}, Inner{});
+      tile_step(it + 3, I0{}, I0{}, Inner{});
+      tile_step(it + 4, I1{}, I1{}, Inner{});
+      tile_step(it + 5, I0{}, I2{}, Inner{});
     }
-    // the last (n_live - 1) % 6 tiles (same buffer sequence)
-    if (it < n_live) tile_step(it, I1{}, I0{});
-    if (it + 1 < n_live) tile_step(it + 1, I0{}, I1{});
-    if (it + 2 < n_live) tile_step(it + 2, I1{}, I2{});
-    if (it + 3 < n_live) tile_step(it + 3, I0{}, I0{});
-    if (it + 4 < n_live) tile_step(it + 4, I1{}, I1{});
+    if constexpr (PAGED) {  // (one body, its buffers found as it goes)
+#pragma unroll 1
+      for (; it < n_live; ++it) tile_step(it, it % KBUF, (it + VBUF - 1) % VBUF, std::true_type{});
+    } else {
+      // the last (n_live - 1) % 6 tiles (same buffer sequence)
+      if (it < n_live) tile_step(it, I1{}, I0{}, Inner{});
+      if (it + 1 < n_live) tile_step(it + 1, I0{}, I1{}, Inner{});
+      if (it + 2 < n_live) tile_step(it + 2, I1{}, I2{}, Inner{});
+      if (it + 3 < n_live) tile_step(it + 3, I0{}, I0{}, Inner{});
+      if (it + 4 < n_live) tile_step(it + 4, I1{}, I1{}, Inner{});
+    }
   }
   if (n_iter > 0) {
     if (grow) rescale_o();
@@ -590,6 +830,7 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     // as in the steps)
     for (int t = n_live; t < n_iter; ++t) {
       if (t + 1 < n_iter) load_tile(t + 1, ((t + 1) % KBUF) * TILE, ((t + 1) % VBUF) * TILE);
+      if constexpr (PAGED) fetch_pages(t + 2);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
     }
@@ -598,8 +839,30 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   // ---- epilogue ----
   l_run += l_run2;
   const float l_tot = l_run + other_half(l_run);
-  // rows past nq: never stored; PREFIX: zeros for a row without a key
-  const float inv = PREFIX && l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+  // rows past nq: never stored; PREFIX, PAGED: zeros for a row without a key
+  const float inv = (PREFIX || PAGED) && l_tot == 0.0f ? 0.0f : 1.0f / l_tot;
+  if constexpr (PAGED) {
+    if (!direct) {
+      const int ln = lane_now(), r = wrow0 + (ln & 31), g = ln >> 5;
+      if (r >= nq) return;
+      if (bad) {
+        paged_rows<D>(q, k, v, o, pg, seq, b_p, hk_p, split_p, wrow0, k_first, k_last, direct);
+        return;
+      }
+      const long row = (long)split_p * pg.a.tokens * hq + paged_row(r);
+      if (g == 0) {
+        pg.parts.m[row] = m_run;
+        pg.parts.l[row] = l_tot;
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4*>(pg.parts.o + row * D + 32 * t + 8 * j + 4 * g) =
+              f32x4{acc_o[t][4 * j], acc_o[t][4 * j + 1], acc_o[t][4 * j + 2], acc_o[t][4 * j + 3]};
+      return;
+    }
+  }
   // O goes through LDS (the K/V buffers, free once every wavefront's last PV
   // product has read its tile): each wavefront writes its 32 x D tile, the
   // 16-byte chunk c of row r at chunk c ^ (r % CPR) of that row, and reads it
@@ -635,6 +898,20 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
                        pack_bf16x2(acc_o[t][4 * j + 2] * inv, acc_o[t][4 * j + 3] * inv)};
       *reinterpret_cast<u32x2*>(ot + (wa ^ ((4 * t + j) << 4))) = w;
     }
+  }
+  if constexpr (PAGED) {
+    if (bad) {
+      paged_rows<D>(q, k, v, o, pg, seq, b_p, hk_p, split_p, wrow0, k_first, k_last, direct);
+      return;
+    }
+#pragma unroll
+    for (int kk = 0; kk < 32 / RPI; ++kk) {
+      const u32x4 val = *reinterpret_cast<const u32x4*>(
+          ot + (ra ^ (((kk % (CPR / RPI)) * RPI) << 4)) + kk * RPI * 2 * D);
+      const int r = wrow0 + kk * RPI + ln / CPR;
+      if (r < nq) *reinterpret_cast<u32x4*>(o + paged_row(r) * D + 8 * (ln % CPR)) = val;
+    }
+    return;
   }
   if constexpr (PREFIX) {
     const int b = (int)(kvh / hkv), hk = (int)(kvh - (long)b * hkv);
@@ -710,3 +987,15 @@ TEENY_FA2_FWD_BF16_K(c_g8, 128, true, 8, true, 2, 2)
   }
 TEENY_FA2_FWD_PREFIX_K(64, 2)
 TEENY_FA2_FWD_PREFIX_K(128, 1)
+
+// A cache in pages
+#define TEENY_FA2_FWD_PAGED_K(D, NSUB)                                                           \
+  extern "C" __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(3, 3)))        \
+  void teeny_fa2_fwd_bf16_d##D##_paged(const bf16* q, const bf16* k, const bf16* v, bf16* o,     \
+                                       int total, FwdPaged pg) {                                 \
+    fa2_fwd_bf16<D, false, 4, false, NSUB, false, true>(q, k, v, o, nullptr, 0, 0, pg.pl.scale,  \
+                                                        pg.a.hq, pg.a.hkv, 1, total, 0, nullptr, \
+                                                        {}, pg);                                 \
+  }
+TEENY_FA2_FWD_PAGED_K(64, 2)
+TEENY_FA2_FWD_PAGED_K(128, 1)

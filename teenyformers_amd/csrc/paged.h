@@ -5,7 +5,7 @@
 // tokens starts[b] .. starts[b + 1] - 1 (starts null: `each` tokens a sequence),
 // token i of them at position past[b] + i (past null: past_all).
 #pragma once
-#include "common.h"
+#include "cdna4.h"
 
 struct Paged {
   const int *table, *starts, *past;
@@ -56,10 +56,65 @@ struct PageWalk {
   DEVI int at(int i) {
     if ((unsigned)(i - first) >= 64u) {
       first = i;
-      const int j = i + (int)(threadIdx.x & 63);
+      const int j = i + lane_now();
       mine = j < width ? row[j] : -1;
       if ((unsigned)mine >= (unsigned)n_pages) mine = -1;
+      pin(mine);  // waited for here: after the branch every use would wait for the tiles in flight
     }
     return __builtin_amdgcn_readlane(mine, i - first);
   }
 };
+
+// How a launch of the attention shares its work out.  The rows of a sequence and kv
+// head are r = i G + g: token i, q head g of the group.
+struct PagedPlan {
+  float scale;
+  int keys, splits;            // of sequences with up to `few` rows: keys of a share, shares
+  int keys_many, splits_many;  // of the others
+  int few;
+  int groups;                  // row tiles of a sequence in the few rows' grid
+  int tiles;                   // row tiles of all others, at most
+};
+// Partials [share][T Hq rows]; m in the log2 domain, -inf: no key.  Sequences of one
+// share write their output instead.
+struct PagedParts {
+  float *m, *l, *o;
+};
+// (the last share of the grid takes all that is left)
+DEVI int paged_shares(const Seq& s, int keys, int most) {
+  return min(max(1, (s.keys(s.n - 1) + keys - 1) / keys), most);
+}
+
+// Values in V that are not finite and that some query must not see: 0 times such a
+// value would be NaN, so their tile is not multiplied but added key by key to the rows
+// that see it.  acc, lane: a wavefront's 32 rows as O^T accumulators; vt: 32 keys of a
+// tile in the SWZ_DUAL order; pb: their P; lim: the lane's keys, relative to vt's first.
+template <int D>
+DEVI void add_keys(f32x16* acc, const char* vt, const uint32_t* pb, int lim) {
+  const int g = lane_now() >> 5;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const float mine = r & 1 ? bf16hi(pb[r >> 1]) : bf16lo(pb[r >> 1]), other = other_half(mine);
+#pragma unroll 1
+    for (int gg = 0; gg < 2; ++gg) {
+      const int key = 8 * (r >> 2) + 4 * gg + (r & 3);
+      const float p = gg == g ? mine : other;
+      if (key >= lim) continue;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(
+              vt + swz<SWZ_DUAL, D>(key * (D / 8) + 4 * t + j) * 16 + 8 * g);
+          acc[t][4 * j] += p * bf16lo(w[0]);
+          acc[t][4 * j + 1] += p * bf16hi(w[0]);
+          acc[t][4 * j + 2] += p * bf16lo(w[1]);
+          acc[t][4 * j + 3] += p * bf16hi(w[1]);
+        }
+    }
+  }
+}
+// whether either bf16 of w is not finite
+DEVI uint32_t bf16_bad(uint32_t w) {
+  return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+}

@@ -151,25 +151,6 @@ __device__ void copy_pages(char* pages, long plane_bytes, long page_bytes, int c
 // ---------------------------------------------------------------------------
 // attn
 // ---------------------------------------------------------------------------
-// How a launch shares the work out.  The rows of a sequence and kv head are r = i G
-// + g: token i, q head g of the group.
-struct Plan {
-  float scale;
-  int keys, splits;            // of sequences with up to `few` rows: keys of a share, shares
-  int keys_many, splits_many;  // of the others
-  int few;
-  int groups;                  // row tiles of a sequence in the grid
-};
-// Partials [share][T Hq rows]; m in the log2 domain, -inf: no key.  Sequences of one
-// share write their output instead.
-struct Parts {
-  float *m, *l, *o;
-};
-// (the last share of the grid takes all that is left)
-DEVI int shares(const Seq& s, int keys, int most) {
-  return min(max(1, (s.keys(s.n - 1) + keys - 1) / keys), most);
-}
-
 template <int D, int NW>
 struct __attribute__((aligned(16))) AttnSmem {
   static constexpr int TILE = TK * D * 2;
@@ -182,34 +163,6 @@ struct __attribute__((aligned(16))) AttnSmem {
   } u;
 };
 
-// Rows whose values in V are not finite and that some query must not see: 0 times
-// such a value would be NaN, so their tile is added key by key to the rows that see
-// it.  vt: the tile; pb: its P; lim: the lane's keys, relative to the tile.
-template <int D>
-DEVI void add_keys(Rows<D>& st, const char* vt, const uint32_t* pb, int lim) {
-  const int g = (threadIdx.x & 63) >> 5;
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const float mine = r & 1 ? bf16hi(pb[r >> 1]) : bf16lo(pb[r >> 1]), other = other_half(mine);
-#pragma unroll 1
-    for (int gg = 0; gg < 2; ++gg) {
-      const int key = 8 * (r >> 2) + 4 * gg + (r & 3);
-      const float p = gg == g ? mine : other;
-      if (key >= lim) continue;
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(
-              vt + swz<SWZ_DUAL, D>(key * (D / 8) + 4 * t + j) * 16 + 8 * g);
-          st.acc[t][4 * j] += p * bf16lo(w[0]);
-          st.acc[t][4 * j + 1] += p * bf16hi(w[0]);
-          st.acc[t][4 * j + 2] += p * bf16lo(w[1]);
-          st.acc[t][4 * j + 3] += p * bf16hi(w[1]);
-        }
-    }
-  }
-}
 template <int DT>
 DEVI bool any_bad(const u32x4 (*va)[DT]) {
   uint32_t bad = 0;
@@ -218,10 +171,7 @@ DEVI bool any_bad(const u32x4 (*va)[DT]) {
 #pragma unroll
     for (int t = 0; t < DT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w = va[hh][t][i] & 0x7f807f80u;
-        bad |= (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
-      }
+      for (int i = 0; i < 4; ++i) bad |= bf16_bad(va[hh][t][i]);
   return __any(bad != 0);
 }
 
@@ -230,7 +180,7 @@ DEVI bool any_bad(const u32x4 (*va)[DT]) {
 template <int D, int NW>
 __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ kp,
                            const bf16* __restrict__ vp, bf16* __restrict__ o, const Paged a,
-                           const Plan pl, const Parts out) {
+                           const PagedPlan pl, const PagedParts out) {
   constexpr int TILE = TK * D * 2, NLD = TILE / 1024;
   __shared__ AttnSmem<D, NW> sm;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
@@ -245,7 +195,7 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
   const int G = a.hq / a.hkv;
   const long all = (long)s.n * G;
   if (all > pl.few || rg * 32 >= all) return;
-  const int rows = (int)all, n_sh = shares(s, pl.keys, pl.splits);
+  const int rows = (int)all, n_sh = paged_shares(s, pl.keys, pl.splits);
   if (split >= n_sh) return;
   const int r = rg * 32 + l32, rc = min(r, rows - 1), tok = rc / G;
   const long row = (long)(s.t0 + tok) * a.hq + hk * G + (rc - tok * G);
@@ -310,7 +260,7 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
     __builtin_amdgcn_s_waitcnt(kLgkmcnt0);
     const bool bad = edge && lim0 < last && any_bad<Rows<D>::DT>(va);
     if (bad) {
-      add_keys<D>(st, vt, pb, min(lim, end) - t0);
+      add_keys<D>(st.acc, vt, pb, min(lim, end) - t0);
       __builtin_amdgcn_s_waitcnt(kLgkmcnt0);
     }
     if (it + 1 < n_tiles) load(vp, vt, it + 1, DualSwz{});
@@ -372,7 +322,7 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
 template <int D>
 __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restrict__ kp,
                                const float* __restrict__ vp, float* __restrict__ o, const Paged a,
-                               const Plan pl, const Parts out) {
+                               const PagedPlan pl, const PagedParts out) {
   constexpr int NC = Geo<D>::NC, VW = Geo<D>::VW, NH = Geo<D>::NH;
   const int lane = threadIdx.x, j = lane & 15, g = lane >> 4;
   int id = blockIdx.x;
@@ -385,7 +335,7 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
   const int G = a.hq / a.hkv;
   const long rows = (long)s.n * G;
   if ((long)rg * 16 >= rows) return;
-  const int n_sh = shares(s, pl.keys, pl.splits);
+  const int n_sh = paged_shares(s, pl.keys, pl.splits);
   if (split >= n_sh) return;
   const long rc = min((long)rg * 16 + j, rows - 1);
   const int tok = (int)(rc / G);
@@ -524,7 +474,7 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
 // The shares of a row, weighed by 2^(m - max m) and summed: a wavefront a row, whose
 // lanes hold four d each in groups that go over the shares side by side.
 template <typename T>
-__device__ void paged_merge(const Parts in, T* __restrict__ o, const Paged a, const Plan pl, int lg_d) {
+__device__ void paged_merge(const PagedParts in, T* __restrict__ o, const Paged a, const PagedPlan pl, int lg_d) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const long n_rows = (long)a.tokens * a.hq, row = (long)blockIdx.x * 4 + wave;
@@ -534,7 +484,7 @@ __device__ void paged_merge(const Parts in, T* __restrict__ o, const Paged a, co
   const Seq s = seq_of(a, b);
   if (t < s.t0 || t >= s.t0 + s.n) return;
   const bool many = (long)s.n * (a.hq / a.hkv) > pl.few;
-  const int n = many ? shares(s, pl.keys_many, pl.splits_many) : shares(s, pl.keys, pl.splits);
+  const int n = many ? paged_shares(s, pl.keys_many, pl.splits_many) : paged_shares(s, pl.keys, pl.splits);
   if (n <= 1) return;
   float mx = -INFINITY;
   for (int i = lane; i < n; i += 64) mx = fmaxf(mx, in.m[i * n_rows + row]);
@@ -609,7 +559,7 @@ extern "C" __global__ __launch_bounds__(256) void teeny_copy_pages(char* pages, 
 #define TEENY_PAGED_ATTN_BF16_INST(D, NW)                                                        \
   extern "C" __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))       \
   void teeny_paged_attn_bf16_d##D##_w##NW(const bf16* q, const bf16* kp, const bf16* vp, bf16* o, \
-                                          Paged a, Plan pl, Parts p) {                           \
+                                          Paged a, PagedPlan pl, PagedParts p) {                           \
     paged_attn<D, NW>(q, kp, vp, o, a, pl, p);                                                   \
   }
 TEENY_PAGED_ATTN_BF16_INST(64, 4)
@@ -617,7 +567,7 @@ TEENY_PAGED_ATTN_BF16_INST(128, 4)
 
 #define TEENY_PAGED_ATTN_F32_INST(D)                                                             \
   extern "C" __global__ __launch_bounds__(64) void teeny_paged_attn_f32_d##D(                    \
-      const float* q, const float* kp, const float* vp, float* o, Paged a, Plan pl, Parts p) {    \
+      const float* q, const float* kp, const float* vp, float* o, Paged a, PagedPlan pl, PagedParts p) {    \
     paged_attn_f32<D>(q, kp, vp, o, a, pl, p);                                                   \
   }
 TEENY_PAGED_ATTN_F32_INST(8)
@@ -627,8 +577,8 @@ TEENY_PAGED_ATTN_F32_INST(64)
 TEENY_PAGED_ATTN_F32_INST(128)
 
 #define TEENY_PAGED_MERGE_INST(TN, T)                                                            \
-  extern "C" __global__ __launch_bounds__(256) void teeny_paged_merge_##TN(Parts p, T* o, Paged a, \
-                                                                           Plan pl, int lg_d) {   \
+  extern "C" __global__ __launch_bounds__(256) void teeny_paged_merge_##TN(PagedParts p, T* o,         \
+                                                           Paged a, PagedPlan pl, int lg_d) {   \
     paged_merge<T>(p, o, a, pl, lg_d);                                                           \
   }
 TEENY_PAGED_MERGE_INST(bf16, bf16)
