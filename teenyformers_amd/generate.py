@@ -22,6 +22,10 @@ distribution.  Any of them draws on the device (ops.sample_rows, random
 numbers from torch's generator with --seed), at temperature 1 unless
 --temperature says otherwise; without them, --temperature keeps the reference's
 sampler on the host, and its default is 0 (greedy).
+
+--draft-len K drafts up to K tokens a step, looked up in the text so far or by a
+smaller model (--draft-dir, the same tokenizer), and checks them in one pass
+(Llama.draft_steps): the same distribution, in fewer passes.
 """
 from __future__ import annotations
 
@@ -135,6 +139,21 @@ def random_numbers(args) -> torch.Tensor:
     return torch.rand((args.max_new_tokens, args.num_samples), generator=g, device="cuda")
 
 
+def drafted(args, model, prompt, eos: int):
+    """--draft-len's steps: lists of each sample's new tokens."""
+    draft = None
+    if args.draft_dir:
+        import os
+        dcfg = llama.LlamaConfig.from_hf_json(os.path.join(args.draft_dir, "config.json"))
+        dtype = model.w["model.norm.weight"].dtype
+        draft = llama.Llama(dcfg, llama.load_hf_weights(dcfg, args.draft_dir, dtype=dtype))
+    g = torch.Generator(device="cuda").manual_seed(args.seed)
+    per = args.draft_len * (2 if draft else 1) + 1
+    u = torch.rand((args.max_new_tokens, args.num_samples, per), generator=g, device="cuda")
+    return model.draft_steps([prompt[0]], u, args.draft_len, args.temperature, args.top_k, args.top_p,
+                             args.min_p, draft, args.num_samples, eos)
+
+
 def print_samples(args, model, prompt, tok, eos: int) -> int:
     """--num-samples continuations, each up to its end-of-sequence token.  One is
     printed as it is drawn, several each as soon as it and those before it have
@@ -149,16 +168,23 @@ def print_samples(args, model, prompt, tok, eos: int) -> int:
     def text(tokens):
         return tok.decode(tokens, skip_special_tokens=True)
 
-    steps = model.sample_steps(prompt, random_numbers(args), args.temperature, args.top_k,
-                               args.top_p, args.min_p)
-    for step, ids in enumerate(steps):
-        for i, token in enumerate(ids.view(-1).tolist()):
-            if i not in running:
-                continue
-            if token == eos or token < 0:  # (-1: a row without a token to draw)
-                running.remove(i)
-                continue
-            rows[i].append(token)
+    if getattr(args, "draft_len", 0):
+        steps = drafted(args, model, prompt, eos)
+    else:
+        steps = ([[t] for t in ids.view(-1).tolist()]
+                 for ids in model.sample_steps(prompt, random_numbers(args), args.temperature,
+                                               args.top_k, args.top_p, args.min_p))
+    for step, new in enumerate(steps):
+        for i, tokens in enumerate(new):
+            for token in tokens:
+                if i not in running:
+                    break
+                if token == eos or token < 0:  # (-1: a row without a token to draw)
+                    running.remove(i)
+                    continue
+                rows[i].append(token)
+                if len(rows[i]) == args.max_new_tokens:
+                    running.remove(i)
         if step + 1 == args.max_new_tokens:
             running.clear()
         while n > 1 and shown < n and shown not in running:
@@ -247,6 +273,9 @@ def main(argv=None) -> int:
     ap.add_argument("--top-k", type=int, default=0, help="0: off")
     ap.add_argument("--top-p", type=float, default=1.0, help="1: off")
     ap.add_argument("--min-p", type=float, default=0.0, help="0: off")
+    ap.add_argument("--draft-len", type=int, default=0,
+                    help="tokens drafted a step (0: none), looked up in the text or by --draft-dir")
+    ap.add_argument("--draft-dir", help="a smaller HF checkpoint of the same tokenizer that drafts")
     ap.add_argument("--seed", type=int, default=42)
     ap.add_argument("--dtype", choices=["bf16", "f32"], default="bf16")
     ap.add_argument("--preset", choices=sorted(PRESETS), help="random weights, timing only")
@@ -261,6 +290,11 @@ def main(argv=None) -> int:
                       or args.min_p > 0.0)
     if args.temperature is None:
         args.temperature = 1.0 if args.on_device else 0.0
+    if not 0 <= args.draft_len <= 64 or args.draft_dir and not args.draft_len:
+        ap.error("--draft-len is 0 to 64, and --draft-dir needs it")
+    if args.draft_len and args.preset:
+        ap.error("--draft-len is for --model-dir")
+    args.on_device = args.on_device or args.draft_len > 0
     if not (args.temperature >= 0.0 and args.num_samples >= 1 and 0 <= args.top_k < 2 ** 31
             and 0.0 < args.top_p <= 1.0 and 0.0 <= args.min_p <= 1.0):
         ap.error("--temperature and --top-k are at least 0, --num-samples at least 1, --top-p in "

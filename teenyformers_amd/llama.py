@@ -36,8 +36,10 @@ MI355X-specific structure (same arithmetic):
 """
 from __future__ import annotations
 
+import contextlib
 import dataclasses
 import functools
+import heapq
 import json
 import math
 
@@ -209,6 +211,155 @@ class SharedPrefixCache:
         self.lengths = None
 
 
+class PagedKVCache:
+    """K/V of many sequences in pages of one pool [n_layers, 2, n_pages, Hkv,
+    page_size, D], taken as sequences grow and given back when they end.  A forked
+    sequence shares its pages with the first one until one of them writes to a
+    shared page, which is then copied (ops.copy_pages, all layers in one launch).
+    The host keeps tables, lengths and uses; nothing here waits for the GPU.  Calls
+    are of one stream: a page given back may be written by the next call on it."""
+
+    def __init__(self, cfg: LlamaConfig, n_pages: int, page_size: int = 64, dtype=torch.bfloat16,
+                 device="cuda"):
+        if n_pages < 1:
+            raise ValueError("PagedKVCache: at least one page")
+        if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
+            raise ValueError("PagedKVCache: the page size is a power of two, 16 to 1024")
+        # rows are written before any query sees them
+        self.pages = torch.empty((cfg.n_layers, 2, n_pages, cfg.n_kv_heads(), page_size, cfg.head_dim()),
+                                 dtype=dtype, device=device)
+        self.k = [layer[0] for layer in self.pages]
+        self.v = [layer[1] for layer in self.pages]
+        self.page_size = page_size
+        self.tables = {}   # by sequence: its pages
+        self.lengths = {}  # ... and its keys
+        self._uses = [0] * n_pages
+        self._free = list(range(n_pages))  # a heap: the lowest page first
+        self._next = 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def add(self) -> int:
+        """A new sequence without keys."""
+        seq, self._next = self._next, self._next + 1
+        self.tables[seq], self.lengths[seq] = [], 0
+        return seq
+
+    def fork(self, seq: int, n: int = 1) -> list:
+        """n sequences that go on from seq's keys, sharing its pages."""
+        table, length = self.tables[seq], self.lengths[seq]
+        new = [self.add() for _ in range(n)]
+        for i in new:
+            self.tables[i], self.lengths[i] = list(table), length
+        for page in table:
+            self._uses[page] += n
+        return new
+
+    def remove(self, seq: int):
+        """The end of a sequence: pages that no other one uses are free again."""
+        self.truncate(seq, 0)
+        del self.tables[seq], self.lengths[seq]
+
+    def truncate(self, seq: int, length: int):
+        """Forget the keys from `length` on (refused drafts)."""
+        if not 0 <= length <= self.lengths[seq]:
+            raise ValueError("truncate: length lies in 0 .. the sequence's keys")
+        table, keep = self.tables[seq], -(-length // self.page_size)
+        for page in table[keep:]:
+            self._uses[page] -= 1
+            if self._uses[page] == 0:
+                heapq.heappush(self._free, page)
+        del table[keep:]
+        self.lengths[seq] = length
+
+    def reserve(self, seqs, counts):
+        """Room for counts[i] more keys of seqs[i]: pages are taken, and those to be
+        written that other sequences share are replaced by copies.  All or nothing:
+        without enough free pages it raises and leaves everything as it was."""
+        if len(set(seqs)) != len(seqs) or len(seqs) != len(counts) or min(counts, default=0) < 0:
+            raise ValueError("reserve: a count for each of different sequences")
+        size, copies, grow, shared = self.page_size, [], 0, {}
+        for seq, n in zip(seqs, counts):
+            table, length = self.tables[seq], self.lengths[seq]
+            grow += -(-(length + n) // size) - len(table)
+            for i in range(length // size, len(table)) if n else ():
+                left = shared.get(table[i], self._uses[table[i]])
+                if left > 1:  # (the last one to write a page keeps it)
+                    shared[table[i]] = left - 1
+                    copies.append((seq, i))
+        if grow + len(copies) > len(self._free):
+            raise RuntimeError("PagedKVCache: no free pages")
+        src, dst = [], []
+        for seq, i in copies:
+            old, new = self.tables[seq][i], heapq.heappop(self._free)
+            self._uses[old] -= 1
+            self._uses[new] = 1
+            self.tables[seq][i] = new
+            src.append(old)
+            dst.append(new)
+        for seq, n in zip(seqs, counts):
+            table = self.tables[seq]
+            for _ in range(-(-(self.lengths[seq] + n) // size) - len(table)):
+                table.append(heapq.heappop(self._free))
+                self._uses[table[-1]] = 1
+        if src:
+            ops.copy_pages(self.pages, src, dst)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool -> how many they are."""
+        used = len(self._uses) - len(self._free)
+        src = [i for i in range(used, len(self._uses)) if self._uses[i]]
+        dst = [i for i in range(used) if not self._uses[i]]
+        to = dict(zip(src, dst))
+        if src:
+            ops.copy_pages(self.pages, src, dst)
+        for table in self.tables.values():
+            table[:] = [to.get(page, page) for page in table]
+        for a, b in to.items():
+            self._uses[b], self._uses[a] = self._uses[a], 0
+        self._free = list(range(used, len(self._uses)))
+        return used
+
+    def batch(self, seqs, counts) -> "PagedBatch":
+        """What a pass over counts[i] new tokens of seqs[i] (in reserved room) reads."""
+        past = [self.lengths[s] for s in seqs]
+        width = max(1, max(len(self.tables[s]) for s in seqs))
+        flat = [x for s in seqs for x in self.tables[s] + [-1] * (width - len(self.tables[s]))]
+        starts = [0]
+        for n in counts:
+            starts.append(starts[-1] + n)
+        # one copy to the device
+        all_ = torch.tensor(flat + starts + past, dtype=torch.int32).to(self.pages.device)
+        table, starts, past_ = all_.split([len(flat), len(starts), len(past)])
+        return PagedBatch(self.k, self.v, table.view(len(seqs), width), starts, past_, max(counts),
+                          max(p + n for p, n in zip(past, counts)))
+
+
+@dataclasses.dataclass
+class PagedBatch:
+    """A pass's new tokens, packed, and where their keys go: as ops.paged_attention."""
+    k: list
+    v: list
+    table: torch.Tensor
+    starts: torch.Tensor
+    n_past: torch.Tensor
+    max_new: int
+    max_keys: int
+
+
+def lookup_drafts(text: list, n: int, longest: int = 3) -> list:
+    """Up to n tokens that followed the last `longest` (or fewer) tokens of the text
+    where they occurred before, latest first; none: []."""
+    for m in range(min(longest, len(text) - 1), 0, -1):
+        end = text[-m:]
+        for i in range(len(text) - m - 1, -1, -1):
+            if text[i:i + m] == end:
+                return text[i + m:i + m + n]
+    return []
+
+
 class Llama:
     """Forward passes of the Llama model (src/llama.rs:40-82) on the HIP ops."""
 
@@ -259,6 +410,13 @@ class Llama:
         rows = ops.split_rows()
         qkv = ops.linear_split(n1, self._lw(p + "qkv_proj.weight"), rows=rows)
         scale = cfg.softmax_scale()
+        if isinstance(cache, PagedBatch):  # packed tokens, B = 1
+            q = ops.paged_qkv_rope_split(qkv, cache.k[i], cache.v[i], cache.table, cache.n_past, Hq,
+                                         cfg.rope_base, starts=cache.starts)
+            att = ops.paged_attention(q, cache.k[i], cache.v[i], cache.table, cache.n_past, scale,
+                                      starts=cache.starts, max_new=cache.max_new,
+                                      max_keys=cache.max_keys)
+            return ops.linear_split(att.view(1, S, Hq * D), self._lw(p + "o_proj.weight"), rows=rows)
         if isinstance(cache, SharedPrefixCache):
             q = torch.empty((B, Hq, S, D), dtype=n1.dtype, device=n1.device)
             ops.qkv_rope_split(qkv, q, cache.k[i], cache.v[i], pos0, Hq, Hkv, cfg.rope_base,
@@ -486,6 +644,161 @@ class Llama:
             logits = self.decode_step(cache, nxt)
             nxt = ops.sample_rows(logits, u[i].contiguous(), *how).view(B, 1)
             yield nxt
+
+    # -- a cache in pages -------------------------------------------------------
+    def run_paged(self, cache: PagedKVCache, seqs: list, ids: list, all_rows: bool = False
+                  ) -> torch.Tensor:
+        """The next tokens of sequences of a paged cache, in one pass: ids[i] (a list or
+        1-D tensor of at least one token) go on after seqs[i]'s keys -> the logits after
+        each sequence's last token [len(seqs), vocab], or with all_rows after each token,
+        packed.  Prompts, chunks of them, single tokens and drafts may be mixed."""
+        if len(ids) != len(seqs) or not seqs:
+            raise ValueError("run_paged: new tokens for each sequence")
+        counts = [len(x) for x in ids]
+        if min(counts) < 1:
+            raise ValueError("run_paged: at least one new token of each sequence")
+        device = cache.pages.device
+        cache.reserve(seqs, counts)
+        batch = cache.batch(seqs, counts)
+        if all(isinstance(x, list) for x in ids):
+            packed = torch.tensor([t for x in ids for t in x], dtype=torch.int64).to(device)
+        else:
+            packed = torch.cat([torch.as_tensor(x, dtype=torch.int64).to(device) for x in ids])
+        # few tokens: the kernels of a decode step
+        with ops.own_gemm() if packed.numel() <= 64 else contextlib.nullcontext():
+            h = self.hidden(packed.view(1, -1), batch, batch.n_past)[0]
+            for seq, n in zip(seqs, counts):
+                cache.lengths[seq] += n
+            if not all_rows and len(seqs) < packed.numel():
+                h = h[(batch.starts[1:] - 1).long()]
+            return self.logits(h)
+
+    def draft_steps(self, prompts: list, u: torch.Tensor, n_draft: int, temperature: float = 1.0,
+                    top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0, draft: "Llama" = None,
+                    samples: int = 1, eos: int | None = None, page_size: int = 64):
+        """Continuations of prompts (1-D ids each), several tokens a step: up to n_draft
+        tokens are drafted for each sequence, by the model `draft` or looked up in its text
+        (lookup_drafts), checked in one pass (run_paged) and accepted or replaced
+        (ops.verify_drafts), so that they are distributed as this model's own; greedy at
+        temperature 0.  With a filter the tokens are drawn row by row (ops.sample_rows) and
+        a draft stays while it is what was drawn.
+
+        samples: continuations of each prompt, which runs once and whose pages they share.
+        u: random numbers fp32 [n_new, B, n_draft + 1], B = len(prompts) * samples, with a
+        draft model [.., 2 n_draft + 1].  An iterator over the steps: for each sequence the
+        list of its new tokens, [] once it has n_new or its last one was eos (or -1, nothing
+        to draw)."""
+        n_new, B, per = u.shape
+        if not prompts or n_new < 1 or n_draft < 1 or samples < 1 or B != len(prompts) * samples:
+            raise ValueError("draft_steps: u is [n_new, len(prompts) * samples, ..], n_draft and samples "
+                             "at least 1")
+        if u.dtype != torch.float32 or per != (2 * n_draft + 1 if draft else n_draft + 1):
+            raise ValueError("draft_steps: u is fp32 with n_draft + 1 numbers a step and sequence, n_draft "
+                             "more with a draft model")
+        if draft is not None and draft.cfg.vocab_size != self.cfg.vocab_size:
+            raise ValueError("draft_steps: both models are of one vocabulary")
+        texts = [p.tolist() if isinstance(p, torch.Tensor) else list(p) for p in prompts]
+        if min(len(t) for t in texts) < 1:
+            raise ValueError("draft_steps: a prompt has at least one token")
+        how = (temperature, top_k, top_p, min_p)
+        filters = top_k > 0 or top_p < 1.0 or min_p > 0.0
+        device = u.device
+
+        def fill(model):
+            """The prompts in a cache of their own, each forked -> cache, sequences, logits."""
+            own = -(-(n_new + n_draft + 1) // page_size) + 2  # of each sample, the prompt's last page too
+            need = sum(-(-len(t) // page_size) + samples * own for t in texts)
+            cache = PagedKVCache(model.cfg, need, page_size, model.w["model.norm.weight"].dtype, device)
+            first = [cache.add() for _ in texts]
+            logits = model.run_paged(cache, first, texts)
+            seqs = [s for f in first for s in [f] + cache.fork(f, samples - 1)]
+            return cache, seqs, logits.repeat_interleave(samples, 0)
+
+        cache, seqs, logits = fill(self)
+        if draft is not None:
+            dcache, dseqs, _ = fill(draft)
+        nxt = ops.sample_rows(logits, u[0, :, n_draft].contiguous(), *how).tolist()
+        texts = [list(t) for t in texts for _ in range(samples)]
+        made = [0] * B
+        live = list(range(B))
+
+        def take(b, tokens):
+            """Adds a sequence's new tokens up to its end."""
+            tokens = tokens[:n_new - made[b]]
+            for i, t in enumerate(tokens):
+                if t < 0 or t == eos:
+                    tokens = tokens[:i + 1]
+                    break
+            texts[b] += tokens
+            made[b] += len(tokens)
+            if made[b] == n_new or tokens[-1] < 0 or tokens[-1] == eos:
+                live.remove(b)
+                cache.remove(seqs[b])
+                if draft is not None:
+                    dcache.remove(dseqs[b])
+            return tokens
+
+        yield [take(b, [nxt[b]]) for b in range(B)]
+        step = 1
+        while live:
+            now = list(live)
+            at = torch.tensor(now).to(device)
+            un = u[step][at]
+            room = [min(n_draft, n_new - made[b] - 1) for b in now]
+            k, q = max(room), None
+            if draft is None:
+                guess = [lookup_drafts(texts[b], r) for b, r in zip(now, room)]
+                k = max(len(x) for x in guess)
+            elif k > 0:
+                feed = [texts[b][dcache.lengths[dseqs[b]]:] for b in now]
+                guess, q = [[] for _ in now], []
+                for j in range(k):
+                    q.append(draft.run_paged(dcache, [dseqs[b] for b in now], feed))
+                    drawn = ops.sample_rows(q[-1], un[:, n_draft + 1 + j].contiguous(), temperature).tolist()
+                    for x, t in zip(guess, drawn):
+                        x.append(t)
+                    feed = [[max(t, 0)] for t in drawn]
+                guess = [x[:r] for x, r in zip(guess, room)]
+            if k == 0:
+                logits = self.run_paged(cache, [seqs[b] for b in now], [texts[b][-1:] for b in now])
+                tokens = ops.sample_rows(logits, un[:, n_draft].contiguous(), *how).view(-1, 1).tolist()
+                accepted = [0] * len(now)
+            else:
+                rows = [x + [-1] * (k - len(x)) for x in guess]
+                ids = [texts[b][-1:] + [max(t, 0) for t in x] for b, x in zip(now, rows)]
+                logits = self.run_paged(cache, [seqs[b] for b in now], ids, all_rows=True)
+                logits = logits.view(len(now), k + 1, -1)
+                pick = torch.cat([un[:, :k], un[:, n_draft:n_draft + 1]], 1)
+                if filters:
+                    tokens = ops.sample_rows(logits, pick.view(-1), *how).tolist()
+                    accepted = []
+                    for t, x in zip(tokens, rows):
+                        n = 0
+                        while n < k and t[n] >= 0 and t[n] == x[n]:
+                            n += 1
+                        accepted.append(n)
+                else:
+                    tokens, accepted = ops.verify_drafts(
+                        logits, torch.tensor(rows).to(device), pick,
+                        None if q is None else torch.stack(q[:k], 1), temperature)
+                    tokens, accepted = tokens.tolist(), accepted.tolist()
+            new = [[] for _ in range(B)]
+            for b, t, n in zip(now, tokens, accepted):
+                held = len(texts[b]) + n  # the text's keys and the accepted drafts'
+                cache.truncate(seqs[b], held)
+                if draft is not None:
+                    dcache.truncate(dseqs[b], min(held, dcache.lengths[dseqs[b]]))
+                new[b] = take(b, t[:n + 1])
+            yield new
+            step += 1
+
+    def generate_drafted(self, prompts: list, u: torch.Tensor, n_draft: int, **how) -> list:
+        """draft_steps to their end: the list of each sequence's new tokens."""
+        out = [[] for _ in range(u.shape[1])]
+        for new in self.draft_steps(prompts, u, n_draft, **how):
+            for x, t in zip(out, new):
+                x += t
+        return out
 
     def generate(self, prompt: torch.Tensor, n_new: int) -> torch.Tensor:
         """Greedy decoding with the KV cache -> generated ids [B, n_new]."""

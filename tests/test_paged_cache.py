@@ -1,0 +1,161 @@
+"""The host side of the cache in pages: tables, shared pages, copies before a write,
+truncation and compaction against a model that keeps each sequence's keys as a list."""
+import random
+
+import pytest
+import torch
+
+from teenyformers_amd import generate, llama, ops
+
+CFG = llama.LlamaConfig(d_model=8, n_heads=1, n_layers=2, vocab_size=16, intermediate_size=8, n_kv_heads_=1)
+
+
+def copy_pages(pages, src, dst):
+    """What ops.copy_pages does, on the host, with its refusals."""
+    assert len(src) == len(dst) and len(set(dst)) == len(dst) and not set(src) & set(dst)
+    pages[..., dst, :, :, :] = pages[..., src, :, :, :]
+    return pages
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    monkeypatch.setattr(ops, "copy_pages", copy_pages)
+    return llama.PagedKVCache(CFG, 40, 16, torch.float32, "cpu")
+
+
+def write(cache, seqs, values):
+    """values[i] as the next keys of seqs[i]: one number a key, in all layers."""
+    counts = [len(v) for v in values]
+    cache.reserve(seqs, counts)
+    b = cache.batch(seqs, counts)
+    assert b.starts.tolist() == [sum(counts[:i]) for i in range(len(counts) + 1)]
+    assert b.n_past.tolist() == [cache.lengths[s] for s in seqs]
+    assert b.max_new == max(counts) and b.max_keys == max(p + n for p, n in zip(b.n_past.tolist(), counts))
+    for i, (s, v) in enumerate(zip(seqs, values)):
+        for j, x in enumerate(v):
+            at = int(b.n_past[i]) + j
+            cache.pages[:, :, int(b.table[i, at // 16]), :, at % 16] = x
+        cache.lengths[s] += len(v)
+
+
+def read(cache, seq):
+    return [float(cache.pages[0, 1, cache.tables[seq][i // 16], 0, i % 16, 0]) for i in range(cache.lengths[seq])]
+
+
+def consistent(cache):
+    uses = [0] * len(cache._uses)
+    for seq, table in cache.tables.items():
+        assert len(table) == -(-cache.lengths[seq] // 16)
+        for page in table:
+            uses[page] += 1
+    assert uses == cache._uses
+    assert sorted(cache._free) == [i for i, n in enumerate(uses) if n == 0]
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_random_use(cache, seed):
+    rng = random.Random(seed)
+    want, counter = {}, iter(range(10 ** 6))
+    for _ in range(150):
+        what = rng.choice(["add", "fork", "write", "write", "write", "write", "truncate", "remove", "compact"])
+        seqs = list(want)
+        if what == "add" and len(seqs) < 8:
+            want[cache.add()] = []
+        elif what == "fork" and seqs and len(seqs) < 8:
+            s = rng.choice(seqs)
+            for f in cache.fork(s, rng.randint(1, 2)):
+                want[f] = list(want[s])
+        elif what == "write" and seqs:
+            some = rng.sample(seqs, rng.randint(1, len(seqs)))
+            values = [[float(next(counter)) for _ in range(rng.choice([0, 1, 1, 3, 17, 40]))] for _ in some]
+            if not any(values):
+                continue
+            state = [list(t) for t in cache.tables.values()], list(cache._uses), sorted(cache._free)
+            try:
+                write(cache, some, values)
+            except RuntimeError:  # full: nothing has changed
+                assert state == ([list(t) for t in cache.tables.values()], list(cache._uses), sorted(cache._free))
+                continue
+            for s, v in zip(some, values):
+                want[s] += v
+        elif what == "truncate" and seqs:
+            s = rng.choice(seqs)
+            n = rng.randint(0, len(want[s]))
+            cache.truncate(s, n)
+            want[s] = want[s][:n]
+        elif what == "remove" and seqs:
+            s = rng.choice(seqs)
+            cache.remove(s)
+            del want[s]
+        elif what == "compact":
+            n = cache.compact()
+            assert all(p < n for t in cache.tables.values() for p in t) and n == len(cache._uses) - cache.free_pages
+        consistent(cache)
+        for s, v in want.items():
+            assert read(cache, s) == v
+
+
+def test_shared_pages_are_stored_once(cache):
+    s = cache.add()
+    write(cache, [s], [[float(i) for i in range(40)]])
+    forks = cache.fork(s, 5)
+    assert cache.free_pages == 37
+    write(cache, forks, [[100.0 + f] for f in forks])  # the last page of each, not the full ones
+    assert cache.free_pages == 32
+    write(cache, [s], [[1.0]])  # its last page is its own by now
+    assert cache.free_pages == 32
+    for f in forks:
+        cache.remove(f)
+    assert cache.free_pages == 37
+
+
+def test_refusals(cache):
+    with pytest.raises(ValueError):
+        llama.PagedKVCache(CFG, 0, 16, device="cpu")
+    for size in (8, 24, 2048):
+        with pytest.raises(ValueError):
+            llama.PagedKVCache(CFG, 4, size, device="cpu")
+    s = cache.add()
+    for seqs, counts in (([s, s], [1, 1]), ([s], [1, 2]), ([s], [-1])):
+        with pytest.raises(ValueError):
+            cache.reserve(seqs, counts)
+    with pytest.raises(ValueError):
+        cache.truncate(s, 1)
+    with pytest.raises(RuntimeError, match="free pages"):
+        cache.reserve([s], [16 * 41])
+    with pytest.raises(KeyError):
+        cache.reserve([99], [1])
+    m = llama.Llama(CFG, {})
+    for seqs, ids in (([], []), ([s], [[1], [2]]), ([s], [[]])):
+        with pytest.raises(ValueError):
+            m.run_paged(cache, seqs, ids)
+    u = torch.zeros((4, 2, 4))
+    for kw in (dict(prompts=[]), dict(prompts=[[1]]), dict(n_draft=2), dict(n_draft=0), dict(samples=2),
+               dict(u=u.double()), dict(prompts=[[1], []]), dict(draft=m),
+               dict(draft=llama.Llama(llama.LlamaConfig(vocab_size=17), {}), u=torch.zeros((4, 2, 7)))):
+        a = dict(prompts=[[1], [2]], u=u, n_draft=3)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            next(m.draft_steps(**a))
+
+
+@pytest.mark.parametrize("text,n,want", [
+    ([1, 2, 3, 9, 1, 2, 3], 2, [9, 1]), ([1, 2, 3, 9, 1, 2, 3], 9, [9, 1, 2, 3]), ([5, 1, 5, 2, 5], 1, [2]),
+    ([1, 2, 3], 4, []), ([7], 3, []), ([7, 7], 3, [7]), ([1, 2, 1], 0, [])])
+def test_lookup_drafts(text, n, want):
+    assert llama.lookup_drafts(text, n) == want
+
+
+def test_command_refuses(capsys):
+    for bad in (["--draft-len", "-1"], ["--draft-len", "65"], ["--draft-dir", "x"],
+                ["--preset", "llama3-8b", "--draft-len", "4"]):
+        with pytest.raises(SystemExit):
+            generate.main(["--model-dir", "unread", *bad])
+
+
+def test_default_temperature_with_drafts(monkeypatch):
+    """Drafts change nothing about what is drawn: greedy unless asked otherwise."""
+    seen = []
+    monkeypatch.setattr(generate, "generate_text", lambda args: seen.append((args.temperature, args.on_device)) or 0)
+    assert generate.main(["--model-dir", "unread", "--draft-len", "4"]) == 0
+    assert seen == [(0.0, True)]
