@@ -1818,7 +1818,8 @@ size_t teeny_verify_drafts_workspace_bytes(int batch, int n_drafts, int cols, in
     return 0;
   const long rows = (long)batch * (n_drafts + 1 + (with_draft ? n_drafts : 0));
   if (rows > 65535) return 0;
-  return align256((size_t)rows * sample_chunks(cols) * 16) + align256((size_t)batch * 64 * 8);
+  return align256((size_t)rows * sample_chunks(cols) * 16) + align256((size_t)batch * 64 * 8) +
+         align256((size_t)batch * 4);
 }
 
 int teeny_verify_drafts(const void* target, long target_seq, long target_row, const void* draft,
@@ -1841,20 +1842,20 @@ int teeny_verify_drafts(const void* target, long target_seq, long target_row, co
   if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
   VerifyArgs a{target, draft, target_seq, target_row, draft_seq, draft_row, drafts, u,
                temperature_rows, temperature, batch, n_drafts, cols, sample_chunks(cols)};
-  void* rec = workspace;
-  void* part = (char*)workspace + align256((size_t)rows * a.n_ch * 16);
+  char* rec = (char*)workspace;
+  char* part = rec + align256((size_t)rows * a.n_ch * 16);
+  char* arrived = part + align256((size_t)batch * 64 * 8);
   char name[48];
+  // as many workgroups as are resident (fewer, so that each takes as many chunks: 144 rows
+  // of 128256 9.6 -> 11.2 us)
+  const unsigned wgs = (unsigned)std::min(rows * a.n_ch, 6L * device_cus());
   snprintf(name, sizeof name, "teeny_verify_scan_%s", dtype_tag(dtype));
-  void* a0[] = {&a, &rec};
-  int rc = launch(name, dim3((unsigned)a.n_ch, (unsigned)rows), dim3(512), 0, stream, a0);
+  void* a0[] = {&a, &rec, &arrived};
+  int rc = launch(name, dim3(wgs), dim3(256), 0, stream, a0);
   if (rc) return rc;
   snprintf(name, sizeof name, "teeny_verify_rest_%s", dtype_tag(dtype));
-  void* a1[] = {&a, &rec, &part};
-  rc = launch(name, dim3((unsigned)a.n_ch, (unsigned)batch), dim3(512), 0, stream, a1);
-  if (rc) return rc;
-  snprintf(name, sizeof name, "teeny_verify_pick_%s", dtype_tag(dtype));
-  void* a2[] = {&a, &rec, &part, &tokens, &accepted};
-  return launch(name, dim3((unsigned)batch), dim3(512), 0, stream, a2);
+  void* a1[] = {&a, &rec, &part, &arrived, &tokens, &accepted};
+  return launch(name, dim3((unsigned)sample_chunks(cols), (unsigned)batch), dim3(512), 0, stream, a1);
 }
 
 // Decode-step linear layers (linear_bf16.hip): 512 threads, 128 W rows per

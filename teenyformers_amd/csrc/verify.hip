@@ -9,18 +9,19 @@
 // whatever the drafts, the tokens are distributed as the target's own.  Temperature
 // 0: one-hot at the lowest index of the row's maximum.
 //
-// Numbers: weights are fp32 (2^((x - max) log2(e) / T), the factor in two parts:
-// 1e-7 relative), sums of eight in fp32 and from there in fp64; what decides
-// (acceptance, the place of u among running sums) is fp64.  A draw from one row sums
-// unscaled weights, exact for equal logits.  No atomics: one order of sums.
+// Numbers: a weight is 2^(x c - K) in fp32, c = log2(e) / T rounded to fp32 and K = c
+// max x rounded (the exponent is one fused product: whatever rounds K is common to all
+// weights, c's rounding moves a weight d octaves down by d 2^-25); sums of eight in fp32
+// and from there in fp64; what decides (acceptance, the place of u among running sums) is
+// fp64.  A draw from one row sums unscaled weights, exact for equal logits.  One order
+// of sums: no atomics on them.
 //
-//   scan   (chunk, row): the maximum of a chunk of 8192 columns and its weights' sum
-//          below it.  Reading the rows bounds it; rows behind a sequence's last real
-//          draft are not read.
-//   rest   (chunk, sequence): each workgroup finds the sequence's accepted drafts from
-//          the chunks' sums (a wavefront a draft, a lane a chunk) and sums its chunk of
-//          what the next token is drawn from.
-//   pick   (sequence): the chunk and the token.
+//   scan   workgroups take chunks of 8192 columns of the rows in turn: their maximum and
+//          the weights' sum below it, each wavefront's below its own first (one barrier a
+//          chunk), the next chunk's loads in flight meanwhile.  Reading the rows bounds it.
+//   rest   (chunk, sequence): each workgroup finds the sequence's accepted drafts from the
+//          scan's sums (a wavefront a draft, a lane a chunk) and sums its chunk of what the
+//          next token is drawn from; the one that ends last finds the chunk and the token.
 #include "sample.h"
 
 namespace {
@@ -46,35 +47,36 @@ struct Args {
   int batch, k, cols, n_ch;
 };
 
-// log2(e) / T (0: greedy) in two parts
+// log2(e) / T (0: greedy)
 struct Factor {
-  double c;
-  float hi, lo;
+  float c;
   bool greedy;
+  DEVI float ref(float xmax) const { return xmax * c; }  // K
 };
-DEVI Factor factor_of(const Args& a, int b) {
-  const double t = a.ts ? (double)a.ts[b] : a.t;
+DEVI Factor factor_of(const Args& a, float ts) {
+  const double t = a.ts ? (double)ts : a.t;
   Factor f;
   f.greedy = !(t > 0.0);  // (NaN too)
-  f.c = f.greedy ? kLog2e : kLog2e / t;
-  f.hi = (float)f.c;
-  f.lo = (float)(f.c - (double)f.hi);
+  f.c = f.greedy ? (float)kLog2e : (float)(kLog2e / t);
   return f;
 }
-// The weight of x below xmax, 0 .. 1
-DEVI float weight(float x, float xmax, const Factor& f) {
-  const float d = x - xmax;
-  const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(d, f.hi, d * f.lo));
-  return !(x > -INFINITY) ? 0.0f : x == xmax ? 1.0f : w == w ? w : 0.0f;
+DEVI Factor factor_of(const Args& a, int b) { return factor_of(a, a.ts ? a.ts[b] : 0.0f); }
+// The weight of x, K = ref; -inf and NaN have none.  (fmaxf takes the number where the
+// exponent is NaN, and 2^-200 is zero.)
+DEVI float weight(float x, float ref, const Factor& f) {
+  return __builtin_amdgcn_exp2f(fmaxf(__builtin_fmaf(x, f.c, -ref), -200.0f));
+}
+// ... where the largest may be infinite: then it and its equals alone
+DEVI float weight(float x, float xmax, float ref, const Factor& f) {
+  return xmax == INFINITY ? (x == INFINITY ? 1.0f : 0.0f) : weight(x, ref, f);
+}
+// 2^(a - b) of two references a <= b, those of maxima xa <= xb
+DEVI float below(float xa, float xb, const Factor& f) {
+  if (!(xa > -INFINITY)) return 0.0f;
+  if (xa == xb) return 1.0f;
+  return __builtin_amdgcn_exp2f(fmaxf(f.ref(xa) - f.ref(xb), -200.0f));
 }
 
-// The drafts of sequence b that are tokens, up to the first that is none.
-DEVI int real_drafts(const Args& a, int b) {
-  const int lane = threadIdx.x & 63;
-  const long long d = lane < a.k ? a.drafts[(long)b * a.k + lane] : -1;
-  const u64 ok = __ballot(d >= 0 && d < a.cols);
-  return ok == ~0ull ? 64 : __builtin_ctzll(~ok);
-}
 template <typename T> DEVI const T* target_row(const Args& a, int b, int i) {
   return (const T*)a.target + b * a.t_seq + i * a.t_row;
 }
@@ -89,74 +91,171 @@ DEVI const Rec* draft_rec(const Args& a, const Rec* rec, int b, int i) {
   return rec + ((long)a.batch * (a.k + 1) + (long)b * a.k + i) * a.n_ch;
 }
 
-DEVI double wave_add(double v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+// Over the wavefront, through DPP: lane 63 has the whole (as wave_scan in sample.h).
+template <int CTRL, int ROWS> DEVI float dpp_f(float v, float none) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+      __builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+}
+DEVI float wave_top(float v) {
+  v = fmaxf(v, dpp_f<0x111, 0xf>(v, -INFINITY));
+  v = fmaxf(v, dpp_f<0x112, 0xf>(v, -INFINITY));
+  v = fmaxf(v, dpp_f<0x114, 0xf>(v, -INFINITY));
+  v = fmaxf(v, dpp_f<0x118, 0xf>(v, -INFINITY));
+  v = fmaxf(v, dpp_f<0x142, 0xa>(v, -INFINITY));
+  v = fmaxf(v, dpp_f<0x143, 0xc>(v, -INFINITY));
+  return __builtin_bit_cast(float, lane_value(__builtin_bit_cast(uint32_t, v), 63));
+}
+template <int CTRL, int ROWS> DEVI double dpp_d(double v) {
+  return __builtin_bit_cast(double, dpp<CTRL, ROWS>(__builtin_bit_cast(u64, v)));
+}
+DEVI double wave_run(double v) {  // inclusive
+  v += dpp_d<0x111, 0xf>(v);
+  v += dpp_d<0x112, 0xf>(v);
+  v += dpp_d<0x114, 0xf>(v);
+  v += dpp_d<0x118, 0xf>(v);
+  v += dpp_d<0x142, 0xa>(v);
+  v += dpp_d<0x143, 0xc>(v);
   return v;
 }
+DEVI double lane_double(double v, int lane) {
+  return __builtin_bit_cast(double, lane_value(__builtin_bit_cast(u64, v), lane));
+}
+DEVI double wave_add(double v) { return lane_double(wave_run(v), 63); }
 
 // ---------------------------------------------------------------------------
+// scan: workgroups of 4 wavefronts take (row, chunk) in turn
+// ---------------------------------------------------------------------------
+constexpr int kScan = 256, kScanWaves = kScan / 64, kVec = kChunk / (kScan * kTok);
+
 template <typename T>
-__device__ void verify_scan(const Args& a, Rec* __restrict__ rec) {
-  __shared__ float red[kWaves];
-  __shared__ double sums[kWaves];
-  __shared__ int firsts[kWaves];
-  const int tid = threadIdx.x, lane = tid & 63, ch = blockIdx.x, row_i = blockIdx.y;
+__device__ void verify_scan(const Args& a, Rec* __restrict__ rec, int* __restrict__ arrived) {
+  constexpr int VW = kTok / Vec16<T>::N;  // loads a vector
+  __shared__ double sums[2][kScanWaves];
+  __shared__ float tops[2][kScanWaves];
+  __shared__ int firsts[2][kScanWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  // (the next launch counts its workgroups here)
+  for (int i = blockIdx.x * kScan + tid; i < a.batch; i += gridDim.x * kScan) arrived[i] = 0;
   const int n_target = a.batch * (a.k + 1);
-  const bool is_target = row_i < n_target;
-  const int per = is_target ? a.k + 1 : a.k, at = is_target ? row_i : row_i - n_target;
-  const int b = at / per, i = at - b * per;
-  const T* row = is_target ? target_row<T>(a, b, i) : draft_row<T>(a, b, i);
-  const int real = real_drafts(a, b);
-  if (i > real || (!is_target && i == real)) return;  // (uniform)
-  const int mis = misaligned(row);
-  float x[2][kTok];
-  int col[2];
+  const int items = (n_target + (a.draft ? a.batch * a.k : 0)) * a.n_ch;
+  struct Place {
+    const T* row;
+    int c0;   // the chunk's first column
+    float t;  // the sequence's temperature, if each has its own
+  };
+  auto place = [&](int i) __attribute__((always_inline)) {
+    const int row_i = i / a.n_ch, ch = i - row_i * a.n_ch;
+    const bool is_target = row_i < n_target;
+    const int per = is_target ? a.k + 1 : a.k, at = is_target ? row_i : row_i - n_target;
+    const int b = at / per;
+    Place p;
+    p.row = is_target ? target_row<T>(a, b, at - b * per) : draft_row<T>(a, b, at - b * per);
+    p.c0 = ch * kChunk - misaligned(p.row);
+    p.t = a.ts ? a.ts[b] : 0.0f;
+    return p;
+  };
+  u32x4 raw[kVec][VW];
+  auto load = [&](const Place& p) __attribute__((always_inline)) {
+    if (a.cols < 2 * kTok) return;
+    const T* some = p.row + (p.c0 < 0 ? p.c0 + kTok : 0);  // a whole vector of the row
 #pragma unroll
-  for (int v = 0; v < 2; ++v) col[v] = load8(row, a.cols, mis, ch, v * kThreads + tid, x[v]);
-  const Factor f = factor_of(a, b);
-  float mx = -INFINITY;
+    for (int v = 0; v < kVec; ++v) {
+      const int c = p.c0 + (v * kScan + tid) * kTok;
+      const T* src = c >= 0 && c + kTok <= a.cols ? p.row + c : some;
 #pragma unroll
-  for (int v = 0; v < 2; ++v)
+      for (int w = 0; w < VW; ++w)
+        raw[v][w] = *reinterpret_cast<const u32x4*>(src + w * Vec16<T>::N);
+    }
+  };
+  int item = blockIdx.x;
+  if (item >= items) return;
+  Place p = place(item);
+  load(p);
+  for (int buf = 0; item < items; item += gridDim.x, buf ^= 1) {
+    float x[kVec][kTok];
 #pragma unroll
-    for (int j = 0; j < kTok; ++j) mx = fmaxf(mx, x[v][j]);
-  mx = wave_max(mx);
-  if (lane == 0) red[tid >> 6] = mx;
-  __syncthreads();
+    for (int v = 0; v < kVec; ++v)
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) mx = fmaxf(mx, red[w]);
-  double sum = 0.0;
-  int first = 0x7fffffff;
+      for (int j = 0; j < kTok; ++j) {
+        const uint32_t w = raw[v][j / (kTok / VW)][VW == 1 ? j / 2 : j % 4];
+        x[v][j] = VW == 2 ? __builtin_bit_cast(float, w) : j & 1 ? bf16hi(w) : bf16lo(w);
+      }
+    if (p.c0 < 0 || p.c0 + kChunk > a.cols) {  // a row's ends one by one
 #pragma unroll
-  for (int v = 0; v < 2; ++v) {
+      for (int v = 0; v < kVec; ++v) {
+        const int c = p.c0 + (v * kScan + tid) * kTok;
+        if (c < 0 || c + kTok > a.cols || a.cols < 2 * kTok)
+#pragma unroll
+          for (int j = 0; j < kTok; ++j)
+            x[v][j] = c + j >= 0 && c + j < a.cols ? (float)p.row[c + j] : -INFINITY;
+      }
+    }
+    const Place q = p;
+    if (item + (int)gridDim.x < items) {
+      p = place(item + gridDim.x);
+      load(p);
+    }
+    const Factor f = factor_of(a, q.t);
+    float mx = -INFINITY;  // (NaN: not the larger one)
+#pragma unroll
+    for (int v = 0; v < kVec; ++v)
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) mx = fmaxf(mx, x[v][j]);
+    mx = wave_top(mx);
+    double sum = 0.0;
+    uint32_t first = 0x7fffffff;
     if (f.greedy) {
 #pragma unroll
-      for (int j = kTok - 1; j >= 0; --j)
-        if (x[v][j] == mx) first = min(first, col[v] + j);
+      for (int v = 0; v < kVec; ++v)
+#pragma unroll
+        for (int j = 0; j < kTok; ++j)
+          if (x[v][j] == mx) first = min(first, (uint32_t)(q.c0 + (v * kScan + tid) * kTok + j));
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) first = min(first, __shfl_xor(first, off, 64));
     } else {
-      float s = 0.0f;
+      const float ref = f.ref(mx);
+      float s[kVec];
+      if (mx == INFINITY) {
 #pragma unroll
-      for (int j = 0; j < kTok; ++j) s += weight(x[v][j], mx, f);
-      sum += (double)s;
-    }
-  }
-  if (f.greedy) {
+        for (int v = 0; v < kVec; ++v) {
+          s[v] = 0.0f;
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) first = min(first, __shfl_xor(first, off, 64));
-  } else {
-    sum = wave_add(sum);
-  }
-  if (lane == 0) {
-    sums[tid >> 6] = sum;
-    firsts[tid >> 6] = first;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWaves; ++w) {
-      sum += sums[w];
-      first = min(first, firsts[w]);
+          for (int j = 0; j < kTok; ++j) s[v] += x[v][j] == INFINITY ? 1.0f : 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          s[v] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < kTok; ++j) s[v] += weight(x[v][j], ref, f);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) sum += (double)s[v];
+      sum = wave_add(sum);
     }
-    rec[(long)row_i * a.n_ch + ch] = Rec{sum, mx, first};
+    if (lane == 0) {
+      sums[buf][wave] = sum;
+      tops[buf][wave] = mx;
+      firsts[buf][wave] = (int)first;
+    }
+    // (the loads in flight are not waited for: the barrier alone, after the LDS writes)
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
+    asm volatile("s_barrier" ::: "memory");
+    // (the buffers alternate: the next barrier comes before this one's next write)
+    if (tid == 0) {
+      float top = tops[buf][0];
+#pragma unroll
+      for (int w = 1; w < kScanWaves; ++w) top = fmaxf(top, tops[buf][w]);
+      Rec r{0.0, top, 0x7fffffff};
+#pragma unroll
+      for (int w = kScanWaves - 1; w >= 0; --w) {
+        r.sum += f.greedy ? 0.0 : sums[buf][w] * (double)below(tops[buf][w], top, f);
+        if (tops[buf][w] == top) r.first = min(r.first, firsts[buf][w]);
+      }
+      rec[item] = r;
+    }
   }
 }
 
@@ -166,12 +265,9 @@ struct Row {
   float xmax;
   int first;  // greedy: the token
 };
-DEVI Row row_of(const Rec* rec, int n_ch, const Factor& f) {
-  const int lane = threadIdx.x & 63;
-  Rec r{0.0, -INFINITY, 0x7fffffff};
-  if (lane < n_ch) r = rec[lane];
+DEVI Row row_of(const Rec& r, const Factor& f) {
   Row o;
-  o.xmax = wave_max(r.xmax);
+  o.xmax = wave_top(r.xmax);
   o.first = 0x7fffffff;
   o.sum = 0.0;
   if (f.greedy) {
@@ -179,17 +275,15 @@ DEVI Row row_of(const Rec* rec, int n_ch, const Factor& f) {
     o.first = (int)lane_value((uint32_t)r.first, __builtin_ctzll(has));  // the first chunk's
     return o;
   }
-  const double d = r.xmax == o.xmax ? 0.0 : ((double)r.xmax - (double)o.xmax) * f.c;
-  o.sum = wave_add(r.xmax > -INFINITY && d == d ? r.sum * exp2(d) : 0.0);
+  o.sum = wave_add(r.sum * (double)below(r.xmax, o.xmax, f));
   return o;
 }
-template <typename T>
-DEVI double prob(const T* row, int col, const Row& r, const Factor& f) {
+// The probability of token `col` with logit x
+DEVI double prob(float x, int col, const Row& r, const Factor& f) {
   if (f.greedy) return r.xmax > -INFINITY && col == r.first ? 1.0 : 0.0;
-  const float x = (float)row[col];
   if (!(x > -INFINITY) || !(r.sum > 0.0)) return 0.0;
-  const double w = x == r.xmax ? 1.0 : exp2(((double)x - (double)r.xmax) * f.c);
-  return w == w ? w / r.sum : 0.0;
+  if (r.xmax == INFINITY) return x == INFINITY ? 1.0 / r.sum : 0.0;
+  return exp2((double)x * f.c - (double)f.ref(r.xmax)) / r.sum;
 }
 
 // What the token after the accepted ones is drawn from: max(p_n - q_n, 0), or p_n.
@@ -199,221 +293,234 @@ struct Rest {
   bool minus_q;  // p_n - q_n, of scaled weights; else p_n's weights without `skip`
   bool greedy;
   int first;     // greedy: the token
-  float pmax, qmax;
-  double ap, aq;
+  float pmax, qmax, pref, qref, ap, aq;
 };
+// Scaled weights' difference, each rounded first: equal ones leave nothing.
+DEVI float surplus(float p, float ap, float q, float aq) {
+#pragma clang fp contract(off)
+  return fmaxf(p * ap - q * aq, 0.0f);
+}
 struct RestSmem {
-  double sum[kMaxDrafts + 1], q_sum[kMaxDrafts];
-  float xmax[kMaxDrafts + 1], q_xmax[kMaxDrafts];
-  int first[kMaxDrafts + 1];
-  int passed[kMaxDrafts + 1];
+  Row row[2 * kMaxDrafts + 1];  // target rows, then the draft model's
 };
 // by all wavefronts of a workgroup
 template <typename T>
 DEVI Rest rest_of(const Args& a, const Rec* rec, int b, const Factor& f, RestSmem& sm) {
+  constexpr int U = 3;  // rows of a wavefront whose records are asked for at once
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-  const int real = real_drafts(a, b);
-  for (int i = wave; i <= real; i += waves) {
-    const Row p = row_of(target_rec(a, rec, b, i), a.n_ch, f);
-    Row q{};
-    int passed = 0;
-    if (i < real) {
-      const int d = (int)a.drafts[(long)b * a.k + i];
-      double qd = 1.0;
-      if (a.draft) {
-        q = row_of(draft_rec(a, rec, b, i), a.n_ch, f);
-        qd = prob(draft_row<T>(a, b, i), d, q, f);
-      }
-      passed = (double)a.u[(long)b * (a.k + 1) + i] * qd < prob(target_row<T>(a, b, i), d, p, f);
-      if (lane == 0) {
-        sm.q_sum[i] = q.sum;
-        sm.q_xmax[i] = q.xmax;
-      }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // a lane a draft: the drafts that are tokens, up to the first that is none, their
+  // logits and random numbers
+  const int mine = min(lane, a.k - 1);
+  const long long d64 = a.drafts[(long)b * a.k + mine];
+  const bool ok = lane < a.k && d64 >= 0 && d64 < a.cols;
+  const u64 all = __ballot(ok);
+  const int real = all == ~0ull ? 64 : __builtin_ctzll(~all);
+  const int d = ok ? (int)d64 : 0;
+  const float u = a.u[(long)b * (a.k + 1) + mine];
+  const float x = (float)target_row<T>(a, b, mine)[d];
+  const float y = a.draft ? (float)draft_row<T>(a, b, mine)[d] : 0.0f;
+  const int rows = real + 1 + (a.draft ? real : 0);
+  for (int r0 = wave; r0 < rows; r0 += U * kWaves) {
+    Rec r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int t = r0 + i * kWaves;
+      r[i] = Rec{0.0, -INFINITY, 0x7fffffff};
+      if (t < rows && lane < a.n_ch)
+        r[i] = (t <= real ? target_rec(a, rec, b, t) : draft_rec(a, rec, b, t - real - 1))[lane];
     }
-    if (lane == 0) {
-      sm.sum[i] = p.sum;
-      sm.xmax[i] = p.xmax;
-      sm.first[i] = p.first;
-      sm.passed[i] = passed;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (r0 + i * kWaves >= rows) break;
+      const Row o = row_of(r[i], f);
+      if (lane == 0) sm.row[r0 + i * kWaves] = o;
     }
   }
   __syncthreads();
+  bool passed = false;
+  if (lane < real) {
+    const double q = a.draft ? prob(y, d, sm.row[real + 1 + lane], f) : 1.0;
+    passed = (double)u * q < prob(x, d, sm.row[lane], f);
+  }
   Rest r;
-  r.n = 0;
-  while (r.n < real && sm.passed[r.n]) ++r.n;
-  r.skip = r.n < real ? (int)a.drafts[(long)b * a.k + r.n] : -1;
+  const u64 yes = __ballot(passed);
+  r.n = yes == ~0ull ? 64 : __builtin_ctzll(~yes);
+  r.skip = r.n < real ? __builtin_amdgcn_readlane(d, r.n) : -1;
+  const Row p = sm.row[r.n];
   r.greedy = f.greedy;
-  r.first = sm.xmax[r.n] > -INFINITY ? sm.first[r.n] : -1;
-  r.pmax = sm.xmax[r.n];
+  r.first = p.xmax > -INFINITY ? p.first : -1;
+  r.pmax = p.xmax;
   r.minus_q = a.draft && r.skip >= 0;
-  r.qmax = r.minus_q ? sm.q_xmax[r.n] : 0.0f;
-  r.ap = sm.sum[r.n] > 0.0 ? 1.0 / sm.sum[r.n] : 0.0;
-  r.aq = r.minus_q && sm.q_sum[r.n] > 0.0 ? 1.0 / sm.q_sum[r.n] : 0.0;
+  r.ap = p.sum > 0.0 ? (float)(1.0 / p.sum) : 0.0f;
+  r.qmax = 0.0f;
+  r.aq = 0.0f;
+  if (r.minus_q) {
+    const Row q = sm.row[real + 1 + r.n];
+    r.qmax = q.xmax;
+    r.aq = q.sum > 0.0 ? (float)(1.0 / q.sum) : 0.0f;
+  }
+  r.pref = f.ref(r.pmax);
+  r.qref = f.ref(r.qmax);
   return r;
 }
-// A thread's 16 columns of a chunk and their weights; their sum
+// The weight of column c
 template <typename T>
-DEVI double weigh(const Args& a, int b, int ch, const Rest& r, const Factor& f, double (*w)[kTok],
-                  int* col) {
-  const T* prow = target_row<T>(a, b, r.n);
-  const T* qrow = r.minus_q ? draft_row<T>(a, b, r.n) : prow;
-  float x[2][kTok], y[2][kTok];
-  // (vectors of the two rows begin at other columns where they are aligned otherwise:
-  // q's columns are then read one by one)
-  const int mis = misaligned(prow), qmis = r.minus_q ? misaligned(qrow) : mis;
+DEVI float weigh_one(const T* prow, const T* qrow, int c, const Rest& r, const Factor& f) {
+  float z = weight((float)prow[c], r.pmax, r.pref, f);
+  if (r.minus_q) z = surplus(z, r.ap, weight((float)qrow[c], r.qmax, r.qref, f), r.aq);
+  return c == r.skip ? 0.0f : z;
+}
+// The sum of a thread's 16 columns of a chunk: those from 16 tid on
+template <typename T>
+DEVI double weigh(const T* prow, const T* qrow, int cols, int ch, const Rest& r, const Factor& f) {
+  constexpr int VW = kTok / Vec16<T>::N;
+  const int c0 = ch * kChunk - misaligned(prow) + 2 * kTok * (int)threadIdx.x;
+  double sum = 0.0;
+  // (vectors of the two rows begin at other columns where they are aligned otherwise)
+  if (c0 >= 0 && c0 + 2 * kTok <= cols && r.pmax < INFINITY && r.qmax < INFINITY &&
+      (!r.minus_q || misaligned(qrow) == misaligned(prow))) {
+    u32x4 x[2 * VW], y[2 * VW];
 #pragma unroll
-  for (int v = 0; v < 2; ++v) col[v] = load8(prow, a.cols, mis, ch, 2 * (int)threadIdx.x + v, x[v]);
-  if (r.minus_q) {
+    for (int v = 0; v < 2 * VW; ++v) x[v] = reinterpret_cast<const u32x4*>(prow + c0)[v];
+    if (r.minus_q)
+#pragma unroll
+      for (int v = 0; v < 2 * VW; ++v) y[v] = reinterpret_cast<const u32x4*>(qrow + c0)[v];
+    auto at = [](const u32x4* z, int j) __attribute__((always_inline)) {
+      const uint32_t w = VW == 2 ? z[j / 4][j % 4] : z[j / 8][j % 8 / 2];
+      return VW == 2 ? __builtin_bit_cast(float, w) : j & 1 ? bf16hi(w) : bf16lo(w);
+    };
+    // sums of eight in fp32
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
-      if (qmis == mis) {
-        load8(qrow, a.cols, mis, ch, 2 * (int)threadIdx.x + v, y[v]);
+      float part = 0.0f;
+      if (r.minus_q) {
+#pragma unroll
+        for (int j = v * kTok; j < (v + 1) * kTok; ++j) {
+          const float z = surplus(weight(at(x, j), r.pref, f), r.ap,
+                                  weight(at(y, j), r.qref, f), r.aq);
+          part += c0 + j == r.skip ? 0.0f : z;
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < kTok; ++j) {
-          const int c = col[v] + j;
-          y[v][j] = c >= 0 && c < a.cols ? fmaxf((float)qrow[c] + 0.0f, -INFINITY) : -INFINITY;
+        for (int j = v * kTok; j < (v + 1) * kTok; ++j) {
+          const float z = weight(at(x, j), r.pref, f);
+          part += c0 + j == r.skip ? 0.0f : z;
         }
       }
+      sum += (double)part;
     }
+  } else {
+#pragma unroll 1
+    for (int j = 0; j < 2 * kTok; ++j)
+      if (c0 + j >= 0 && c0 + j < cols) sum += (double)weigh_one(prow, qrow, c0 + j, r, f);
   }
-  double sum = 0.0;
-#pragma unroll
-  for (int v = 0; v < 2; ++v)
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      double z = (double)weight(x[v][j], r.pmax, f);
-      if (r.minus_q) z = fmax(z * r.ap - (double)weight(y[v][j], r.qmax, f) * r.aq, 0.0);
-      if (col[v] + j == r.skip) z = 0.0;
-      w[v][j] = z;
-      sum += z;
-    }
   return sum;
 }
 
+// grid (chunks, sequences)
 template <typename T>
-__device__ void verify_rest(const Args& a, const Rec* __restrict__ rec, double* __restrict__ part) {
-  __shared__ RestSmem sm;
-  __shared__ double sums[kWaves];
-  const int tid = threadIdx.x, ch = blockIdx.x, b = blockIdx.y;
-  const Factor f = factor_of(a, b);
-  const Rest r = rest_of<T>(a, rec, b, f, sm);
-  if (r.greedy) return;
-  double w[2][kTok];
-  int col[2];
-  const double sum = wave_add(weigh<T>(a, b, ch, r, f, w, col));
-  if ((tid & 63) == 0) sums[tid >> 6] = sum;
-  __syncthreads();
-  if (tid == 0) {
-    double s = 0.0;
-    for (int i = 0; i < kWaves; ++i) s += sums[i];
-    part[(long)b * kMaxChunks + ch] = s;
-  }
-}
-
-// inclusive over the wavefront
-DEVI double wave_run(double v) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const double o = __shfl_up(v, off, 64);
-    v += (int)(threadIdx.x & 63) >= off ? o : 0.0;
-  }
-  return v;
-}
-
-template <typename T>
-__device__ void verify_pick(const Args& a, const Rec* __restrict__ rec,
-                            const double* __restrict__ part, long long* __restrict__ tokens,
+__device__ void verify_rest(const Args& a, const Rec* __restrict__ rec, double* __restrict__ part,
+                            int* __restrict__ arrived, long long* __restrict__ tokens,
                             int* __restrict__ accepted) {
   __shared__ RestSmem sm;
   __shared__ double sums[kWaves];
-  __shared__ int found, last, chunk;
-  __shared__ double target;
-  const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.x;
+  __shared__ int count, has[2][kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, b = blockIdx.y, n_ch = gridDim.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Factor f = factor_of(a, b);
   Rest r = rest_of<T>(a, rec, b, f, sm);
   long long* out = tokens + (long)b * (a.k + 1);
-  if (tid <= a.k && tid != r.n) out[tid] = tid < r.n ? a.drafts[(long)b * a.k + tid] : -1;
-  if (tid == 0) accepted[b] = r.n;
-  if (r.greedy) {
-    if (tid == 0) out[r.n] = r.first;
-    return;
+  if (blockIdx.x == 0) {
+    if (tid <= a.k && (tid != r.n || r.greedy))
+      out[tid] = tid < r.n ? a.drafts[(long)b * a.k + tid] : tid == r.n ? r.first : -1;
+    if (tid == 0) accepted[b] = r.n;
   }
-  if (wave == 0) {
-    double s = lane < a.n_ch ? part[(long)b * kMaxChunks + lane] : 0.0;
-    double run = wave_run(s), all = __shfl(run, 63);
-    const bool none = !(all > 0.0);
-    if (none) {  // p_n lies below q_n everywhere: then p_n itself
-      const Rec* t = target_rec(a, rec, b, r.n);
-      const double d = lane < a.n_ch ? ((double)t[lane].xmax - (double)r.pmax) * f.c : 0.0;
-      s = lane < a.n_ch && t[lane].xmax > -INFINITY
-              ? t[lane].sum * (t[lane].xmax == r.pmax ? 1.0 : d == d ? exp2(d) : 0.0) : 0.0;
-      run = wave_run(s);
-      all = __shfl(run, 63);
+  if (r.greedy) return;
+  const T* prow = target_row<T>(a, b, r.n);
+  const T* qrow = r.minus_q ? draft_row<T>(a, b, r.n) : prow;
+  // Twice through one body (code that runs once is fetched from memory as it goes): the
+  // workgroup's own chunk, then, by the last workgroup of the sequence, the drawn one.
+  int ch = blockIdx.x;
+  double target = 0.0;
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    const double mine = weigh<T>(prow, qrow, a.cols, ch, r, f), run = wave_run(mine);
+    if (lane == 63) sums[wave] = run;
+    __syncthreads();
+    double before = 0.0, all = 0.0;  // of the wavefront; of the chunk
+    for (int i = 0; i < kWaves; ++i) {
+      before += i < wave ? sums[i] : 0.0;
+      all += sums[i];
+    }
+    if (pass == 1) {
+      // the thread that the target falls into (rounding may leave none: the last that has any)
+      const double lo = before + run - mine;
+      const u64 at = __ballot(mine > 0.0 && lo + mine > target), any = __ballot(mine > 0.0);
+      __syncthreads();
+      if (lane == 0) has[0][wave] = at ? 1 : 0, has[1][wave] = any ? 1 : 0;
+      __syncthreads();
+      int w = -1, z = -1;
+      for (int i = kWaves - 1; i >= 0; --i) {
+        if (has[0][i]) w = i;
+        if (has[1][i]) z = max(z, i);
+      }
+      if (wave != (w >= 0 ? w : z)) return;
+      const int l = at ? __builtin_ctzll(at) : 63 - __builtin_clzll(any);
+      const double t = target - lane_double(lo, l);
+      const int c = ch * kChunk - misaligned(prow) + 2 * kTok * (wave * 64 + l) + lane;
+      const double v = lane < 2 * kTok && c >= 0 && c < a.cols ? (double)weigh_one(prow, qrow, c, r, f) : 0.0;
+      const double upto = wave_run(v);
+      const u64 hit = __ballot(v > 0.0 && upto > t), some = __ballot(v > 0.0);
+      if (lane == (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some))) out[r.n] = c;
+      return;
+    }
+    if (tid == 0) {
+      // Store, count and the last one's loads are accesses of device scope, past the L2
+      // caches; the store has been performed before the count is sent.  (Release and
+      // acquire would write back and drop a whole L2 in every workgroup.)
+      __hip_atomic_store(part + (long)b * kMaxChunks + ch, all, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      count = __hip_atomic_fetch_add(arrived + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (count != n_ch - 1) return;
+    // every wavefront finds the chunk for itself
+    double s = lane < n_ch ? __hip_atomic_load(part + (long)b * kMaxChunks + lane, __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    double at = wave_run(s), whole = lane_double(at, 63);
+    if (!(whole > 0.0)) {  // p_n lies below q_n everywhere: then p_n itself
+      const Rec t = target_rec(a, rec, b, r.n)[min(lane, n_ch - 1)];
+      s = lane < n_ch ? t.sum * (double)below(t.xmax, r.pmax, f) : 0.0;
+      at = wave_run(s);
+      whole = lane_double(at, 63);
+      r.minus_q = false;
+      r.skip = -1;
     }
     const float u = a.u[(long)b * (a.k + 1) + a.k];
-    const double t = u > 0.0f ? (double)u * all : 0.0;
-    u64 at = __ballot(s > 0.0 && run > t);  // the first; u of 1: the last that has any
-    const u64 any = __ballot(s > 0.0);
-    const int ch = at ? __builtin_ctzll(at) : any ? 63 - __builtin_clzll(any) : -1;
-    if (lane == 0) {
-      chunk = ch | (none ? 1 << 16 : 0);
-      found = 0x7fffffff;
-      last = -1;
+    const double t = u > 0.0f ? (double)u * whole : 0.0;
+    // the first chunk past it; u of 1: the last that has any
+    const u64 yes = __ballot(s > 0.0 && at > t), any = __ballot(s > 0.0);
+    if (!any) {  // no token to draw
+      if (tid == 0) out[r.n] = -1;
+      return;
     }
-    if (ch >= 0) {
-      const double before = __shfl(run - s, ch);
-      if (lane == 0) target = t - before;
-    }
+    ch = yes ? __builtin_ctzll(yes) : 63 - __builtin_clzll(any);
+    target = t - lane_double(at - s, ch);
   }
-  __syncthreads();
-  if (chunk < 0) {  // no token to draw
-    if (tid == 0) out[r.n] = -1;
-    return;
-  }
-  if (chunk >> 16) {
-    r.minus_q = false;
-    r.skip = -1;
-  }
-  double w[2][kTok];
-  int col[2];
-  const double sum = weigh<T>(a, b, chunk & 0xffff, r, f, w, col), inc = wave_run(sum);
-  if (lane == 63) sums[wave] = inc;
-  __syncthreads();
-  double run = inc - sum;
-  for (int i = 0; i < wave; ++i) run += sums[i];
-  int mine = 0x7fffffff, top = -1;
-#pragma unroll
-  for (int v = 0; v < 2; ++v)
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      run += w[v][j];
-      if (w[v][j] > 0.0) {
-        top = col[v] + j;
-        if (run > target) mine = min(mine, top);
-      }
-    }
-  if (mine < 0x7fffffff) atomicMin(&found, mine);
-  if (top >= 0) atomicMax(&last, top);
-  __syncthreads();
-  if (tid == 0) out[r.n] = found < 0x7fffffff ? found : last;
 }
 
 }  // namespace
 
 #define TEENY_VERIFY_INST(TN, T)                                                                 \
-  extern "C" __global__ __launch_bounds__(512) void teeny_verify_scan_##TN(Args a, Rec* rec) {    \
-    verify_scan<T>(a, rec);                                                                      \
+  extern "C" __global__ __launch_bounds__(256) void teeny_verify_scan_##TN(Args a, Rec* rec,      \
+                                                                           int* arrived) {        \
+    verify_scan<T>(a, rec, arrived);                                                             \
   }                                                                                              \
-  extern "C" __global__ __launch_bounds__(512) void teeny_verify_rest_##TN(Args a, const Rec* rec, \
-                                                                           double* part) {        \
-    verify_rest<T>(a, rec, part);                                                                \
-  }                                                                                              \
-  extern "C" __global__ __launch_bounds__(512) void teeny_verify_pick_##TN(                      \
-      Args a, const Rec* rec, const double* part, long long* tokens, int* accepted) {             \
-    verify_pick<T>(a, rec, part, tokens, accepted);                                              \
+  extern "C" __global__ __launch_bounds__(512) void teeny_verify_rest_##TN(                      \
+      Args a, const Rec* rec, double* part, int* arrived, long long* tokens, int* accepted) {     \
+    verify_rest<T>(a, rec, part, arrived, tokens, accepted);                                     \
   }
 TEENY_VERIFY_INST(f32, float)
 TEENY_VERIFY_INST(bf16, bf16)

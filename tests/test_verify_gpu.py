@@ -1,13 +1,14 @@
 """ops.verify_drafts against its definition in 64 bits (numpy).
 
 The outputs are whole numbers, equal to the definition's wherever that is decided by more
-than the kernels' error.  A weight is fp32: the exponent d c / T of up to 64 octaves (below,
-the weight is under 2^-64) is off by at most 3 2^-24 relative (difference, product, the factor's
-rest), 64 * 3 * 2^-24 ln 2 < 8e-6 relative at a weight of 2^-64, and at weight w by
--log2(w) * 1.3e-7 relative, so by at most 7e-8 of the maximum's weight; exp2 adds 2^-22
-relative, sums of eight 2^-21.  So a probability is within 1e-6 relative plus 1e-7 of the
-largest, running sums of them within 1.2e-6 of the whole, and a difference p - q within 2.4e-6:
-borders nearer than 5e-6 (relative to the sum drawn from) are left out."""
+than the kernels' error.  A weight is fp32, 2^(x c - K): what rounds K is common to a row's
+weights; c is rounded (2^-24 relative, so a weight d octaves down moves by d 2^-24 octaves) and
+so is the fused exponent (|d| 2^-24): below 64 octaves, where a weight is under 2^-64, that is
+2 * 64 * 2^-24 ln 2 < 6e-6 relative, and for a weight w at most 2 -log2(w) w 2^-24 ln 2 < 5e-8 of
+the largest.  exp2 adds 2^-22 relative, sums of eight 2^-21, the scaled difference of two rows
+3 2^-24.  So a probability is within 1e-6 relative plus 1e-7 of the largest, running sums of
+them within 1.2e-6 of the whole, and a difference p - q within 2.4e-6: borders nearer than 5e-6
+(relative to the sum drawn from) are left out."""
 import math
 
 import numpy as np
