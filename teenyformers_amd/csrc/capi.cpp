@@ -1503,10 +1503,11 @@ struct Paged {  // in paged.h
 };
 struct PagedPlan {  // in paged.h
   float scale;
-  int keys, splits, keys_many, splits_many, few, groups, tiles;
+  int keys, splits, keys_many, splits_many, few, groups, tiles, stride;
 };
 struct PagedParts {  // in paged.h
   float *m, *l, *o;
+  float *m_many, *l_many, *o_many;
 };
 struct FwdPaged {  // in fa2_fwd_bf16.hip
   Paged a;
@@ -1536,32 +1537,60 @@ int paged_args(Paged* a, const int32_t* table, int table_ld, int table_width, co
   return TEENY_OK;
 }
 
-// Sequences of up to `few` rows a kv head take shares of their keys by workgroups of 32
-// rows, the others the forward kernel's walk by workgroups of 128.
+// Up to 32 rows a kv head (one-token steps, a few drafts): paged.hip's kernel, workgroups
+// of 32 rows and a share of the keys each.  More: the forward kernel's walk by workgroups
+// of 128 rows, with sequences of few rows (up to 128, or of 32 beside longer ones) in
+// shares beside them.
 PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, int hkv, int head_dim,
                      int dtype) {
   (void)head_dim;
   PagedPlan p{};
   const bool f32 = dtype == TEENY_F32;
-  const int unit = f32 ? 16 : 32, waves = f32 ? 1 : 4;
   const long G = hq / hkv, rows = G * max_new, cus = device_cus();
-  p.few = f32 ? 0x7fffffff : 32;
-  p.groups = (int)((std::min(rows, (long)p.few) + unit - 1) / unit);
-  const long items = (long)batch * hkv * p.groups, want = 2 * cus;
-  const long most = std::max(1L, want / std::max(1L, items));
-  const long step = 32L * waves;
-  p.keys = (int)(((max_keys + most - 1) / most + step - 1) / step * step);
-  p.splits = std::max(1, (max_keys + p.keys - 1) / p.keys);
   p.splits_many = 1;
   p.keys_many = max_keys;
+  auto share = [&](long items, long slots, long least, long step) {
+    const long most = std::max(1L, slots / std::max(1L, items));
+    const long n = std::max((max_keys + most - 1) / most, least);
+    p.keys = (int)((n + step - 1) / step * step);
+    p.splits = std::max(1, (max_keys + p.keys - 1) / p.keys);
+  };
+  if (f32) {
+    p.few = 0x7fffffff;
+    p.groups = (int)((rows + 15) / 16);
+    share((long)batch * hkv * p.groups, 2 * cus, 32, 32);
+    return p;
+  }
+  if (rows <= 32) {
+    p.few = 32;
+    p.groups = 1;
+    p.stride = (int)rows;
+    if (max_keys <= 1024 || (long)batch * hkv >= 2 * cus) p.keys = max_keys, p.splits = 1;
+    else share((long)batch * hkv, 2 * cus, 128, 128);
+    return p;
+  }
+  p.few = rows > 128 ? 32 : 128;
+  p.stride = (int)std::min(rows, (long)p.few);
+  share((long)batch * hkv, 3 * cus, 512, 64);
   if (rows > p.few) {
     p.tiles = (int)(tokens * G / 128 + std::min((long)batch, tokens * G / (p.few + 1)));
-    const long wgs = (long)p.tiles * hkv, slots = 3 * cus;
-    const long n = std::max(1L, std::min(slots / std::max(1L, wgs), (max_keys + 511L) / 512));
+    const long wgs = (long)p.tiles * hkv;
+    const long n = std::max(1L, std::min(3 * cus / std::max(1L, wgs), (max_keys + 511L) / 512));
     p.keys_many = (int)(((max_keys + n - 1) / n + 63) / 64 * 64);
     p.splits_many = std::max(1, (max_keys + p.keys_many - 1) / p.keys_many);
   }
   return p;
+}
+// Rows of partials: of sequences of few rows, of the others (0: none)
+size_t paged_rows_few(const PagedPlan& p, int batch, int tokens, int hq, int hkv) {
+  if (p.splits <= 1) return 0;
+  return (p.stride ? (size_t)batch * hkv * p.stride : (size_t)tokens * hq) * p.splits;
+}
+size_t paged_rows_many(const PagedPlan& p, int tokens, int hq) {
+  return p.splits_many <= 1 ? 0 : (size_t)tokens * hq * p.splits_many;
+}
+size_t paged_part_bytes(size_t rows, int head_dim) {
+  return 2 * align256(rows * sizeof(float)) + align256(rows * head_dim * sizeof(float));
 }
 }  // namespace
 
@@ -1607,10 +1636,8 @@ size_t teeny_paged_attention_workspace_bytes(int batch, int tokens, int max_new,
     return 0;
   const PagedPlan p = paged_plan(batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv, head_dim,
                                  dtype);
-  const int most = std::max(p.splits, p.splits_many);
-  if (most <= 1) return 0;
-  const size_t rows = (size_t)tokens * n_heads_q * most;
-  return 2 * align256(rows * sizeof(float)) + align256(rows * head_dim * sizeof(float));
+  return paged_part_bytes(paged_rows_few(p, batch, tokens, n_heads_q, n_heads_kv), head_dim) +
+         paged_part_bytes(paged_rows_many(p, tokens, n_heads_q), head_dim);
 }
 
 int teeny_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o,
@@ -1634,44 +1661,47 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
   max_keys = std::max(1, std::min(max_keys, table_width * page_size));
   PagedPlan p = paged_plan(batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv, head_dim, dtype);
   p.scale = softmax_scale;
-  const int shares = std::max(p.splits, p.splits_many);
-  const size_t rows = (size_t)tokens * n_heads_q;
-  if (rows * shares >= (size_t)kMaxElems) return TEENY_ERR_INVALID_SHAPE;
+  const size_t few = paged_rows_few(p, batch, tokens, n_heads_q, n_heads_kv);
+  const size_t more = paged_rows_many(p, tokens, n_heads_q);
+  if (few >= (size_t)kMaxElems || more >= (size_t)kMaxElems) return TEENY_ERR_INVALID_SHAPE;
   PagedParts parts{};
-  if (shares > 1) {
-    if (!workspace || workspace_bytes < teeny_paged_attention_workspace_bytes(
-                                            batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv,
-                                            head_dim, dtype))
-      return TEENY_ERR_WORKSPACE;
+  if (few + more > 0) {
+    const size_t need = paged_part_bytes(few, head_dim) + paged_part_bytes(more, head_dim);
+    if (!workspace || workspace_bytes < need) return TEENY_ERR_WORKSPACE;
     if ((uintptr_t)workspace % 16 != 0) return TEENY_ERR_INVALID_VALUE;
-    const size_t each = align256(rows * shares * sizeof(float));
-    parts = {(float*)workspace, (float*)((char*)workspace + each),
-             (float*)((char*)workspace + 2 * each)};
+    char* w = (char*)workspace;
+    const size_t e = align256(few * sizeof(float)), e2 = align256(more * sizeof(float));
+    char* w2 = w + paged_part_bytes(few, head_dim);
+    parts = {(float*)w,  (float*)(w + e),   (float*)(w + 2 * e),
+             (float*)w2, (float*)(w2 + e2), (float*)(w2 + 2 * e2)};
   }
-  const long wgs = (long)p.splits * p.groups * batch * n_heads_kv;
-  const long many = (long)p.tiles * n_heads_kv * p.splits_many;
-  if (wgs >= (1L << 31) || many >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
   char name[64];
-  if (many > 0) {
+  long wgs;
+  if (dtype == TEENY_BF16 && (long)max_new * (n_heads_q / n_heads_kv) > 32) {
+    wgs = ((long)p.tiles * p.splits_many + (long)batch * p.splits) * n_heads_kv;
+    if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
     FwdPaged f{a, p, parts};
-    int total = (int)many;
+    int total = (int)wgs;
     snprintf(name, sizeof name, "teeny_fa2_fwd_bf16_d%d_paged", head_dim);
     void* args[] = {&q, &k_pages, &v_pages, &o, &total, &f};
-    rc = launch(name, dim3((unsigned)many), dim3(256), 0, stream, args);
-    if (rc) return rc;
-  }
-  // (all sequences alike: one of the two has work)
-  if (starts || many == 0) {
+    rc = launch(name, dim3((unsigned)wgs), dim3(256), 0, stream, args);
+  } else {
+    wgs = (long)p.splits * p.groups * batch * n_heads_kv;
+    if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
+    // (one share of many keys: 8 wavefronts)
+    const int nw = dtype == TEENY_F32 ? 1 : p.splits == 1 && max_keys > 128 ? 8 : 4;
     if (dtype == TEENY_BF16)
-      snprintf(name, sizeof name, "teeny_paged_attn_bf16_d%d_w4", head_dim);
+      snprintf(name, sizeof name, "teeny_paged_attn_bf16_d%d_w%d", head_dim, nw);
     else
       snprintf(name, sizeof name, "teeny_paged_attn_f32_d%d", head_dim);
     void* a0[] = {&q, &k_pages, &v_pages, &o, &a, &p, &parts};
-    rc = launch(name, dim3((unsigned)wgs), dim3(dtype == TEENY_BF16 ? 256 : 64), 0, stream, a0);
-    if (rc) return rc;
+    rc = launch(name, dim3((unsigned)wgs), dim3(64 * nw), 0, stream, a0);
   }
-  if (shares == 1) return TEENY_OK;
+  if (rc || few + more == 0) return rc;
   int lg_d = log2_of(head_dim);
+  // rows with a stride first, then those of all heads of all tokens
+  const size_t rows = (size_t)batch * n_heads_kv * p.stride +
+                      (p.stride == 0 || more > 0 ? (size_t)tokens * n_heads_q : 0);
   snprintf(name, sizeof name, "teeny_paged_merge_%s", dtype_tag(dtype));
   void* a1[] = {&parts, &o, &a, &p, &lg_d};
   return launch(name, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, a1);

@@ -94,8 +94,9 @@ struct FwdPrefix {
 // PAGED (teeny_paged_attention's sequences of many rows): the keys lie in the
 // sequence's pages, the rows of a kv head are its (token, q head of the group) pairs,
 // 32 NW consecutive ones a workgroup, and a workgroup walks a share of their keys.  The
-// page of each 16 keys comes from a register of 64 table entries; a load of a wavefront
-// lies in one page.  Workgroups go kv head by kv head, the last rows of a sequence first.
+// page of each 16 keys is read by scalar loads a tile ahead; a load of a wavefront lies in
+// one page.  Workgroups go kv head by kv head: the sequences of many rows, the last rows
+// first, then those of few, whose shares of the keys are read beside the others' products.
 struct FwdPaged {
   Paged a;
   PagedPlan pl;
@@ -108,7 +109,7 @@ struct FwdPaged {
 template <int D>
 DEVI void paged_rows(const bf16* q, const bf16* k, const bf16* v, bf16* o, const FwdPaged& pg,
                      const Seq& seq, int b, int hk, int split, int wrow0, int k_first, int k_last,
-                     bool direct) {
+                     bool direct, bool few) {
   constexpr int H = D / 2;
   const Paged& a = pg.a;
   const int ln = lane_now(), g = ln >> 5, group = a.hq / a.hkv;
@@ -158,14 +159,15 @@ DEVI void paged_rows(const bf16* q, const bf16* k, const bf16* v, bf16* o, const
     }
     return;
   }
-  const long to = (long)split * a.tokens * a.hq + row;
+  const long to = few ? few_row(a, pg.pl, split, b, hk, r, row) : (long)split * a.tokens * a.hq + row;
+  float* po = few ? pg.parts.o : pg.parts.o_many;
   if (g == 0) {
-    pg.parts.m[to] = m;
-    pg.parts.l[to] = l;
+    (few ? pg.parts.m : pg.parts.m_many)[to] = m;
+    (few ? pg.parts.l : pg.parts.l_many)[to] = l;
   }
 #pragma unroll
   for (int c = 0; c < H; c += 4)
-    *reinterpret_cast<f32x4*>(pg.parts.o + to * D + g * H + c) =
+    *reinterpret_cast<f32x4*>(po + to * D + g * H + c) =
         f32x4{acc[c], acc[c + 1], acc[c + 2], acc[c + 3]};
 }
 
@@ -203,46 +205,59 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   int mb = PREFIX ? rank : num_m_blocks - 1 - rank;
   Seq seq{};
   int group = 1, hk_p = 0, b_p = 0, split_p = 0, k_first = 0, k_last = 0;
-  bool direct = true;
+  bool direct = true, few_p = false;
   if constexpr (PAGED) {
     group = hq / hkv;
-    hk_p = id / (pg.pl.tiles * pg.pl.splits_many);
-    const int in = id - hk_p * pg.pl.tiles * pg.pl.splits_many;
-    split_p = in / pg.pl.tiles;
-    int left = in - split_p * pg.pl.tiles;
-    // the left-th row tile among those of the sequences of many rows
+    const int n_many = pg.pl.tiles * pg.pl.splits_many, per_head = n_many + pg.a.batch * pg.pl.splits;
+    hk_p = id / per_head;
+    const int in = id - hk_p * per_head;
     b_p = -1;
-    for (int b0 = 0; b0 < pg.a.batch && b_p < 0; b0 += 64) {
-      int tiles = 0;
-      if (b0 + lane < pg.a.batch) {
-        const long rows = (long)seq_of(pg.a, b0 + lane).n * group;
-        tiles = rows > pg.pl.few ? (int)((rows + BM - 1) / BM) : 0;
-      }
-      int run = tiles;
+    if (in >= n_many) {
+      split_p = (in - n_many) / pg.a.batch;
+      b_p = in - n_many - split_p * pg.a.batch;
+      mb = 0;
+    } else {
+      split_p = in / pg.pl.tiles;
+      int left = in - split_p * pg.pl.tiles;
+      // the left-th row tile among those of the sequences of many rows
+      for (int b0 = 0; b0 < pg.a.batch && b_p < 0; b0 += 64) {
+        int tiles = 0;
+        if (b0 + lane < pg.a.batch) {
+          const long rows = (long)seq_of(pg.a, b0 + lane).n * group;
+          tiles = rows > pg.pl.few ? (int)((rows + BM - 1) / BM) : 0;
+        }
+        int run = tiles;
 #pragma unroll
-      for (int off = 1; off < 64; off <<= 1) {
-        const int o = __shfl_up(run, off, 64);
-        run += lane >= off ? o : 0;
+        for (int off = 1; off < 64; off <<= 1) {
+          const int o = __shfl_up(run, off, 64);
+          run += lane >= off ? o : 0;
+        }
+        const uint64_t past = __ballot(run > left);
+        if (past) {
+          const int l = __builtin_ctzll(past);
+          b_p = b0 + l;
+          mb = __builtin_amdgcn_readlane(run, l) - 1 - left;  // the last rows first
+        } else {
+          left -= __builtin_amdgcn_readlane(run, 63);
+        }
       }
-      const uint64_t past = __ballot(run > left);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        b_p = b0 + l;
-        mb = __builtin_amdgcn_readlane(run, l) - 1 - left;  // the last rows first
-      } else {
-        left -= __builtin_amdgcn_readlane(run, 63);
-      }
+      if (b_p < 0) return;
     }
-    if (b_p < 0) return;
+    b_p = __builtin_amdgcn_readfirstlane(b_p);
     seq = seq_of(pg.a, b_p);
-    const int n_sh = paged_shares(seq, pg.pl.keys_many, pg.pl.splits_many);
+    const long rows = (long)seq.n * group;
+    few_p = rows <= pg.pl.few;
+    if (rows == 0 || few_p != (in >= n_many)) return;
+    const int share = few_p ? pg.pl.keys : pg.pl.keys_many;
+    const int most = few_p ? pg.pl.splits : pg.pl.splits_many;
+    const int n_sh = paged_shares(seq, share, most);
     if (split_p >= n_sh) return;
     direct = n_sh == 1;
     nq = seq.n * group;
     // the keys of this share that the workgroup's last row sees
     const int last = seq.keys((min(mb * BM + BM, nq) - 1) / group);
-    k_first = split_p * pg.pl.keys_many;
-    k_last = split_p + 1 < pg.pl.splits_many ? min(k_first + pg.pl.keys_many, last) : last;
+    k_first = split_p * share;
+    k_last = split_p + 1 < most ? min(k_first + share, last) : last;
     k_last = max(k_last, k_first);
   }
   // bhq: this wavefront's (b, q head); wrow0: its first query row; blk_end:
@@ -278,6 +293,11 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   }
   const int qrow = wrow0 + l32;
   const int wave_qmax = wrow0 + 31;
+  // PAGED: where the partials of row r go
+  auto paged_part = [&](int r, long row) {
+    return few_p ? few_row(pg.a, pg.pl, split_p, b_p, hk_p, r, row)
+                 : (long)split_p * pg.a.tokens * hq + row;
+  };
   // PAGED: the output row of row r of the kv head
   auto paged_row = [&](int r) {
     const int tok = r / group;
@@ -846,19 +866,20 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
       const int ln = lane_now(), r = wrow0 + (ln & 31), g = ln >> 5;
       if (r >= nq) return;
       if (bad) {
-        paged_rows<D>(q, k, v, o, pg, seq, b_p, hk_p, split_p, wrow0, k_first, k_last, direct);
+        paged_rows<D>(q, k, v, o, pg, seq, b_p, hk_p, split_p, wrow0, k_first, k_last, direct, few_p);
         return;
       }
-      const long row = (long)split_p * pg.a.tokens * hq + paged_row(r);
+      const long row = paged_part(r, paged_row(r));
+      float* po = few_p ? pg.parts.o : pg.parts.o_many;
       if (g == 0) {
-        pg.parts.m[row] = m_run;
-        pg.parts.l[row] = l_tot;
+        (few_p ? pg.parts.m : pg.parts.m_many)[row] = m_run;
+        (few_p ? pg.parts.l : pg.parts.l_many)[row] = l_tot;
       }
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<f32x4*>(pg.parts.o + row * D + 32 * t + 8 * j + 4 * g) =
+          *reinterpret_cast<f32x4*>(po + row * D + 32 * t + 8 * j + 4 * g) =
               f32x4{acc_o[t][4 * j], acc_o[t][4 * j + 1], acc_o[t][4 * j + 2], acc_o[t][4 * j + 3]};
       return;
     }
@@ -901,7 +922,7 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   }
   if constexpr (PAGED) {
     if (bad) {
-      paged_rows<D>(q, k, v, o, pg, seq, b_p, hk_p, split_p, wrow0, k_first, k_last, direct);
+      paged_rows<D>(q, k, v, o, pg, seq, b_p, hk_p, split_p, wrow0, k_first, k_last, direct, few_p);
       return;
     }
 #pragma unroll

@@ -73,13 +73,21 @@ struct PagedPlan {
   int keys_many, splits_many;  // of the others
   int few;
   int groups;                  // row tiles of a sequence in the few rows' grid
-  int tiles;                   // row tiles of all others, at most
+  int tiles;                   // row tiles of all sequences with more, at most
+  int stride;                  // rows of partials kept for each (sequence, kv head); 0: for all
+                               // heads of all tokens
 };
-// Partials [share][T Hq rows]; m in the log2 domain, -inf: no key.  Sequences of one
-// share write their output instead.
+// Partials; m in the log2 domain, -inf: no key.  Sequences of one share write their output
+// instead.  Sequences of few rows: share i of row r at [i][b][kv head][r] (stride > 0) or
+// at [i][token][head]; of many rows, at [i][token][head] of arrays of their own.
 struct PagedParts {
   float *m, *l, *o;
+  float *m_many, *l_many, *o_many;
 };
+DEVI long few_row(const Paged& a, const PagedPlan& pl, int split, int b, int hk, int r, long row) {
+  return pl.stride ? (((long)split * a.batch + b) * a.hkv + hk) * pl.stride + r
+                   : (long)split * a.tokens * a.hq + row;
+}
 // (the last share of the grid takes all that is left)
 DEVI int paged_shares(const Seq& s, int keys, int most) {
   return min(max(1, (s.keys(s.n - 1) + keys - 1) / keys), most);

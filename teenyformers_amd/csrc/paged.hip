@@ -284,7 +284,6 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
             st.acc[t][4 * j], st.acc[t][4 * j + 1], st.acc[t][4 * j + 2], st.acc[t][4 * j + 3]};
   }
   __syncthreads();
-  const long n_rows = (long)a.tokens * a.hq;
   for (int i = tid; i < n_here * (D / 4); i += NW * 64) {
     const int rr = i / (D / 4), d = (i - rr * (D / 4)) * 4;
     float mm = -INFINITY;
@@ -307,10 +306,11 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
           u32x2{pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv)};
       continue;
     }
-    *reinterpret_cast<f32x4*>(out.o + (split * n_rows + to) * D + d) = num;
+    const long at = few_row(a, pl, split, b, hk, ri, to);
+    *reinterpret_cast<f32x4*>(out.o + at * D + d) = num;
     if (d == 0) {
-      out.m[split * n_rows + to] = mm;
-      out.l[split * n_rows + to] = den;
+      out.m[at] = mm;
+      out.l[at] = den;
     }
   }
 }
@@ -463,7 +463,7 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
     store_col<D>(o + row * D, acc, g, [l](float x) { return l == 0.0f ? 0.0f : x / l; });
     return;
   }
-  const long to = (long)split * a.tokens * a.hq + row;
+  const long to = few_row(a, pl, split, b, hk, (int)rc, row);
   if (g == 0) {
     out.m[to] = m * kLog2e;
     out.l[to] = l;
@@ -472,22 +472,45 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
 }
 
 // The shares of a row, weighed by 2^(m - max m) and summed: a wavefront a row, whose
-// lanes hold four d each in groups that go over the shares side by side.
+// lanes hold four d each in groups that go over the shares side by side.  With a stride the
+// rows are those kept for each (sequence, kv head), then (the sequences of many rows, where
+// they have shares) those of all heads of all tokens; else the latter alone.
 template <typename T>
-__device__ void paged_merge(const PagedParts in, T* __restrict__ o, const Paged a, const PagedPlan pl, int lg_d) {
-  const int lane = threadIdx.x & 63;
+__device__ void paged_merge(const PagedParts parts, T* __restrict__ o, const Paged a,
+                            const PagedPlan pl, int lg_d) {
+  const int lane = threadIdx.x & 63, G = a.hq / a.hkv;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const long n_rows = (long)a.tokens * a.hq, row = (long)blockIdx.x * 4 + wave;
-  if (row >= n_rows) return;
-  const int t = (int)(row / a.hq), b = seq_at(a, t);
-  if (b < 0) return;
-  const Seq s = seq_of(a, b);
-  if (t < s.t0 || t >= s.t0 + s.n) return;
-  const bool many = (long)s.n * (a.hq / a.hkv) > pl.few;
-  const int n = many ? paged_shares(s, pl.keys_many, pl.splits_many) : paged_shares(s, pl.keys, pl.splits);
+  const long item = (long)blockIdx.x * 4 + wave, n_few = (long)a.batch * a.hkv * pl.stride;
+  PagedParts in = parts;
+  long row, first, step;  // the output row; the first share's partials, those to the next
+  int n;
+  if (item < n_few) {
+    const int bh = (int)(item / pl.stride), r = (int)(item - (long)bh * pl.stride);
+    const int b = bh / a.hkv, hk = bh - b * a.hkv;
+    const Seq s = seq_of(a, b);
+    const long rows = (long)s.n * G;
+    if (r >= rows || rows > pl.few) return;
+    n = paged_shares(s, pl.keys, pl.splits);
+    row = (long)(s.t0 + r / G) * a.hq + hk * G + r % G;
+    first = item;
+    step = n_few;
+  } else {
+    row = item - n_few;
+    step = (long)a.tokens * a.hq;
+    if (row >= step) return;
+    const int t = (int)(row / a.hq), b = seq_at(a, t);
+    if (b < 0) return;
+    const Seq s = seq_of(a, b);
+    if (t < s.t0 || t >= s.t0 + s.n) return;
+    const bool many = (long)s.n * G > pl.few;
+    if (pl.stride > 0 && !many) return;
+    n = many ? paged_shares(s, pl.keys_many, pl.splits_many) : paged_shares(s, pl.keys, pl.splits);
+    first = row;
+    if (many) in = PagedParts{in.m_many, in.l_many, in.o_many, nullptr, nullptr, nullptr};
+  }
   if (n <= 1) return;
   float mx = -INFINITY;
-  for (int i = lane; i < n; i += 64) mx = fmaxf(mx, in.m[i * n_rows + row]);
+  for (int i = lane; i < n; i += 64) mx = fmaxf(mx, in.m[first + i * step]);
   mx = wave_max(mx);
   const float ref = mx == -INFINITY ? 0.0f : mx;  // no key at all: zeros
   const int lanes = 1 << (lg_d - 2), grp = lane >> (lg_d - 2), groups = 64 >> (lg_d - 2);
@@ -500,7 +523,7 @@ __device__ void paged_merge(const PagedParts in, T* __restrict__ o, const Paged 
     float mi[U], li[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {  // (past the end: the last one, unweighed)
-      const long at = min(i0 + u * groups, n - 1) * n_rows + row;
+      const long at = first + min(i0 + u * groups, n - 1) * step;
       v[u] = *reinterpret_cast<const f32x4*>(in.o + (at << lg_d) + d);
       mi[u] = in.m[at];
       li[u] = in.l[at];
@@ -563,7 +586,9 @@ extern "C" __global__ __launch_bounds__(256) void teeny_copy_pages(char* pages, 
     paged_attn<D, NW>(q, kp, vp, o, a, pl, p);                                                   \
   }
 TEENY_PAGED_ATTN_BF16_INST(64, 4)
+TEENY_PAGED_ATTN_BF16_INST(64, 8)
 TEENY_PAGED_ATTN_BF16_INST(128, 4)
+TEENY_PAGED_ATTN_BF16_INST(128, 8)
 
 #define TEENY_PAGED_ATTN_F32_INST(D)                                                             \
   extern "C" __global__ __launch_bounds__(64) void teeny_paged_attn_f32_d##D(                    \
