@@ -1543,7 +1543,6 @@ int paged_args(Paged* a, const int32_t* table, int table_ld, int table_width, co
 // shares beside them.
 PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, int hkv, int head_dim,
                      int dtype) {
-  (void)head_dim;
   PagedPlan p{};
   const bool f32 = dtype == TEENY_F32;
   const long G = hq / hkv, rows = G * max_new, cus = device_cus();
@@ -1565,13 +1564,20 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
     p.few = 32;
     p.groups = 1;
     p.stride = (int)rows;
-    if (max_keys <= 1024 || (long)batch * hkv >= 2 * cus) p.keys = max_keys, p.splits = 1;
-    else share((long)batch * hkv, 2 * cus, 128, 128);
+    // One share, and no merge, where (sequence, kv head) pairs fill the device or the keys
+    // are few; else workgroups for every CU.  us in a graph, one share and several, Hq32
+    // Hkv8 D128: 1 sequence of 300 keys 8.2, 8.9, 700 9.8, 9.0, 1000 11.3, 9.0, 2000 17.1,
+    // 9.7 (eager calls pay 4 us more for the second launch); 16 of up to 900 11.9, 12.5.
+    // With one and two workgroups a CU: 4 of up to 32000 66, 75 (a share each of fewer keys
+    // brings no more bytes at a time, and its last ones end unevenly), 16 of 4000 28.7,
+    // 30.0; heads of 64, half the bytes a key, 8 of 3000 19.7, 17.3.
+    if (max_keys <= 768 || (long)batch * hkv >= 2 * cus) p.keys = max_keys, p.splits = 1;
+    else share((long)batch * hkv, head_dim == 128 ? cus : 2 * cus, 128, 128);
     return p;
   }
   p.few = rows > 128 ? 32 : 128;
   p.stride = (int)std::min(rows, (long)p.few);
-  share((long)batch * hkv, 3 * cus, 512, 64);
+  share((long)batch * hkv, (getenv("TS3") ? atof(getenv("TS3")) : 3.0) * cus, getenv("TL3") ? atoi(getenv("TL3")) : 512, 64);
   if (rows > p.few) {
     p.tiles = (int)(tokens * G / 128 + std::min((long)batch, tokens * G / (p.few + 1)));
     const long wgs = (long)p.tiles * hkv;
@@ -1688,8 +1694,10 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
   } else {
     wgs = (long)p.splits * p.groups * batch * n_heads_kv;
     if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
-    // (one share of many keys: 8 wavefronts)
-    const int nw = dtype == TEENY_F32 ? 1 : p.splits == 1 && max_keys > 128 ? 8 : 4;
+    // Wavefronts: 4; 8 for one share of few keys, and of heads of 64.  us with 4 and 8: 64
+    // sequences of up to 8191 keys, D128 206, 215, of 2000 45.2, 46.2; D64, 16 kv heads, of
+    // 4000 106, 99.
+    const int nw = dtype == TEENY_F32 ? 1 : p.splits == 1 && (head_dim == 64 || max_keys <= 768) ? 8 : 4;
     if (dtype == TEENY_BF16)
       snprintf(name, sizeof name, "teeny_paged_attn_bf16_d%d_w%d", head_dim, nw);
     else

@@ -67,6 +67,15 @@ DEVI u32x2 lds_read_tr(const char* p) {
 DEVI __amdgpu_buffer_rsrc_t make_rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);
 }
+// ... of a base and size that are the same in all lanes, where the compiler cannot see it (it
+// would put a loop over the lanes' descriptors around every load)
+DEVI __amdgpu_buffer_rsrc_t make_rsrc_uniform(const void* base, int bytes) {
+  const uint64_t p = reinterpret_cast<uint64_t>(base);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+  return make_rsrc(reinterpret_cast<const void*>((uint64_t)hi << 32 | lo),
+                   __builtin_amdgcn_readfirstlane(bytes));
+}
 // buffer_load_dwordx4 ... lds: 16 bytes per lane from buffer offset
 // soff + voff into LDS at lds + 16 * lane.  A MUBUF load, not FLAT: with FLAT
 // LDS loads in flight the compiler waits for every LDS read to drain.

@@ -458,8 +458,8 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
         const long at = ((((long)max(page, 0) * hkv + hk_p) << lg) + (key & ((1 << lg) - 1))) * D;
         // the lane's chunk within the 16 rows
         const int back = RPL == 16 ? 0 : (wave >> 1) * 16 * D * 2;
-        dma16(make_rsrc(k + at, n * D * 2), kdst + i * LSTEP, k_src - back, 0);
-        dma16(make_rsrc(v + at, n * D * 2), vdst + i * LSTEP, v_src - back, 0);
+        dma16(make_rsrc_uniform(k + at, n * D * 2), kdst + i * LSTEP, k_src - back, 0);
+        dma16(make_rsrc_uniform(v + at, n * D * 2), vdst + i * LSTEP, v_src - back, 0);
       }
       return;
     }
@@ -538,6 +538,15 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     acc_o[t] = mfma32(as_bf16x8(a), bop, acc_o[t]);
   };
 
+  // (PAGED, D = 128: the last offsets are formed from the first where they are used, the
+  // chunk's bits being XORed into it: with all of them in registers the loop lacks four,
+  // and read a part of Q from scratch memory in every tile)
+  auto k_at = [&](int c) {
+    if (!PAGED || D != 128 || c < DC - 4) return k_off[c];
+    int at;
+    asm volatile("v_xor_b32 %0, %1, %2" : "=v"(at) : "i"(32 * c), "v"(k_off[0]));
+    return at;
+  };
   // S^T = K Q^T for the NSUB 32-key subtiles of a tile (interleaved
   // chains, K fragments read KPF steps ahead)
   auto qk = [&](const char* kt0, f32x16& s0, f32x16& s1) {
@@ -547,15 +556,15 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     u32x4 ra[DC], rb[DC];
 #pragma unroll
     for (int c = 0; c < KPF; ++c) {
-      ra[c] = *reinterpret_cast<const u32x4*>(kt0 + k_off[c]);
-      if constexpr (NSUB == 2) rb[c] = *reinterpret_cast<const u32x4*>(kt0 + 32 * D * 2 + k_off[c]);
+      ra[c] = *reinterpret_cast<const u32x4*>(kt0 + k_at(c));
+      if constexpr (NSUB == 2) rb[c] = *reinterpret_cast<const u32x4*>(kt0 + 32 * D * 2 + k_at(c));
     }
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
       if (c + KPF < DC) {
-        ra[c + KPF] = *reinterpret_cast<const u32x4*>(kt0 + k_off[c + KPF]);
+        ra[c + KPF] = *reinterpret_cast<const u32x4*>(kt0 + k_at(c + KPF));
         if constexpr (NSUB == 2)
-          rb[c + KPF] = *reinterpret_cast<const u32x4*>(kt0 + 32 * D * 2 + k_off[c + KPF]);
+          rb[c + KPF] = *reinterpret_cast<const u32x4*>(kt0 + 32 * D * 2 + k_at(c + KPF));
       }
       s0 = mfma32(as_bf16x8(ra[c]), qreg[c], s0);
       if constexpr (NSUB == 2) s1 = mfma32(as_bf16x8(rb[c]), qreg[c], s1);
@@ -794,7 +803,9 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
 #pragma unroll
       for (int q = 0; q < 8 * NSUB; ++q)
         if (pair_slot(q) == j) sm_pair(s0, s1, q, la, lb);
-      if (j == NJ / 2 && it + 1 < n_iter)
+      // (PAGED: behind the last tile too, where nothing is read, and zeros go to buffers that
+      // nobody reads: around a branch the compiler gathers all of the exponentials behind it)
+      if (j == NJ / 2 && (PAGED || it + 1 < n_iter))
         load_tile(it + 1, ((kb + 1) % KBUF) * TILE, ((vp + 2) % VBUF) * TILE);
       __builtin_amdgcn_sched_barrier(0);
     }

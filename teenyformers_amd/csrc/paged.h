@@ -46,12 +46,17 @@ DEVI int seq_at(const Paged& a, int t) {
   return n > 0 && n <= a.batch ? n - 1 : -1;
 }
 
-// A wavefront's way along a sequence's table: 64 entries in a register.
+// A wavefront's way along a sequence's table: 64 entries in a register, the first ones
+// asked for at once (a short sequence's, beside the loads of its length).
 struct PageWalk {
   const int* row;
   int width, n_pages, first, mine;
   DEVI PageWalk(const Paged& a, int b)
-      : row(a.table + (long)b * a.ld), width(a.width), n_pages(a.n_pages), first(-1 << 20), mine(-1) {}
+      : row(a.table + (long)b * a.ld), width(a.width), n_pages(a.n_pages), first(0) {
+    const int j = threadIdx.x & 63;
+    mine = row[min(j, width - 1)];
+    if (j >= width || (unsigned)mine >= (unsigned)n_pages) mine = -1;
+  }
   // the page of table entry i (wave-uniform); -1: absent
   DEVI int at(int i) {
     if ((unsigned)(i - first) >= 64u) {
@@ -99,10 +104,14 @@ DEVI int paged_shares(const Seq& s, int keys, int most) {
 // tile in the SWZ_DUAL order; pb: their P; lim: the lane's keys, relative to vt's first.
 template <int D>
 DEVI void add_keys(f32x16* acc, const char* vt, const uint32_t* pb, int lim) {
+  typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
   const int g = lane_now() >> 5;
-#pragma unroll
+  const u32x8 p8 = {pb[0], pb[1], pb[2], pb[3], pb[4], pb[5], pb[6], pb[7]};
+  // (looped: it hardly ever runs, and code in the way of what does costs its fetches)
+#pragma unroll 1
   for (int r = 0; r < 16; ++r) {
-    const float mine = r & 1 ? bf16hi(pb[r >> 1]) : bf16lo(pb[r >> 1]), other = other_half(mine);
+    const uint32_t two = p8[r >> 1];
+    const float mine = r & 1 ? bf16hi(two) : bf16lo(two), other = other_half(mine);
 #pragma unroll 1
     for (int gg = 0; gg < 2; ++gg) {
       const int key = 8 * (r >> 2) + 4 * gg + (r & 3);

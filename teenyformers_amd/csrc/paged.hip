@@ -191,6 +191,7 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
   const int hk = id % a.hkv;
   id /= a.hkv;
   const int split = id % pl.splits, b = id / pl.splits;
+  PageWalk walk(a, b);
   const Seq s = seq_of(a, b);
   const int G = a.hq / a.hkv;
   const long all = (long)s.n * G;
@@ -210,7 +211,6 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
   const int kpw = ((max(0, s1 - s0) + NW - 1) / NW + TK - 1) / TK * TK;
   const int k0 = s0 + wave * kpw, end = min(k0 + kpw, s1);
   const int n_tiles = max(0, end - k0 + TK - 1) / TK;
-  PageWalk walk(a, b);
   // loads of a tile: 16 rows lie in one page (its rows at or past `end`, and absent
   // pages, lie outside the descriptor and load as zeros); returns the absent halves
   auto load = [&](const bf16* pool, char* to, int it, auto sw) __attribute__((always_inline)) {
@@ -220,7 +220,7 @@ __device__ void paged_attn(const bf16* __restrict__ q, const bf16* __restrict__ 
       const int key = k0 + it * TK + 16 * h, page = walk.at(key >> a.lg);
       const int n = page < 0 ? 0 : min(max(end - key, 0), 16);
       const long at = (((long)max(page, 0) * a.hkv + hk) << a.lg) + (key & ((1 << a.lg) - 1));
-      const auto rs = make_rsrc(pool + at * D, n * D * 2);
+      const auto rs = make_rsrc_uniform(pool + at * D, n * D * 2);
       absent |= (page < 0) << h;
 #pragma unroll
       for (int i = h * NLD / 2; i < (h + 1) * NLD / 2; ++i)
@@ -331,6 +331,7 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
   const int hk = id % a.hkv;
   id /= a.hkv;
   const int split = id % pl.splits, b = id / pl.splits;
+  PageWalk walk(a, b);
   const Seq s = seq_of(a, b);
   const int G = a.hq / a.hkv;
   const long rows = (long)s.n * G;
@@ -350,7 +351,6 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
   f32x4 acc[NH][VW];
   zero_acc<D>(acc);
   float m = -INFINITY, l = 0.0f;
-  PageWalk walk(a, b);
   for (int t0 = k0; t0 < end; t0 += 32) {
     f32x4 kf[2][NC];
     float vf[8][NH][VW];
