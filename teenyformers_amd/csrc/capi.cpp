@@ -1577,7 +1577,12 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
   }
   p.few = rows > 128 ? 32 : 128;
   p.stride = (int)std::min(rows, (long)p.few);
-  share((long)batch * hkv, (getenv("TS3") ? atof(getenv("TS3")) : 3.0) * cus, getenv("TL3") ? atoi(getenv("TL3")) : 512, 64);
+  // Shares of the sequences of few rows: three workgroups a CU, at least 512 keys; beside
+  // sequences of many, which fill the device already, one a CU.  us with 3, 2 and 1: 8 x 16
+  // tokens behind 4000 keys 28.5, 29.4, 34.4; 512 tokens among 32 single ones behind 1000
+  // 51.8, 46.5, 46.5; with least shares of 256 and 1024 keys the former 28.7, 34.9, 24
+  // tokens of one sequence behind 16000 (512: 26.8) 29.1, 35.7.
+  share((long)batch * hkv, rows > p.few ? cus : 3 * cus, 512, 64);
   if (rows > p.few) {
     p.tiles = (int)(tokens * G / 128 + std::min((long)batch, tokens * G / (p.few + 1)));
     const long wgs = (long)p.tiles * hkv;

@@ -803,9 +803,11 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
 #pragma unroll
       for (int q = 0; q < 8 * NSUB; ++q)
         if (pair_slot(q) == j) sm_pair(s0, s1, q, la, lb);
-      // (PAGED: behind the last tile too, where nothing is read, and zeros go to buffers that
-      // nobody reads: around a branch the compiler gathers all of the exponentials behind it)
-      if (j == NJ / 2 && (PAGED || it + 1 < n_iter))
+      // PAGED: before the PV products, since a tile of a long cache comes from HBM (2048 tokens
+      // behind 6144 among 32 one-token sequences 307 -> 287 us, 512 behind 32000 321 ->
+      // 311), and behind the last tile too, where nothing is read and zeros go to buffers that
+      // nobody reads: around a branch the compiler gathers all of the exponentials behind it.
+      if (j == (PAGED ? 0 : NJ / 2) && (PAGED || it + 1 < n_iter))
         load_tile(it + 1, ((kb + 1) % KBUF) * TILE, ((vp + 2) % VBUF) * TILE);
       __builtin_amdgcn_sched_barrier(0);
     }
