@@ -578,7 +578,8 @@ int teeny_qkv_rope_split_rows(const void* qkv, const float* parts, int n_parts, 
  * table's unused entries; pages given back behind a window).
  * The new tokens of all sequences are packed: tokens starts[b] .. starts[b+1]-1
  * are sequence b's (int32 device memory, batch+1 values that do not fall; none
- * for a sequence is allowed), or with starts null tokens / batch each.  Token i
+ * for a sequence is allowed; one whose starts fall, or lie outside 0 .. tokens, has
+ * none), or with starts null tokens / batch each.  Token i
  * of sequence b is at position n_past[b] + i (int32 device memory, one value per
  * sequence; null: n_past_host for all).  Tokens behind starts[batch] are nobody's:
  * their rows of the outputs are left as they were.  All tensors are 16-byte

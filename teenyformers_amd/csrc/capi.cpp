@@ -1557,13 +1557,17 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
   if (f32) {
     p.few = 0x7fffffff;
     p.groups = (int)((rows + 15) / 16);
-    share((long)batch * hkv * p.groups, 2 * cus, 32, 32);
+    // us in a graph, one share and several: 4 sequences of 4 heads of 64 and 64 keys 7.0,
+    // 8.7, 1 of 100 keys 10.1, 7.9 (an eager call pays 4 us for the merge's launch).  With 2,
+    // 4 and 8 wavefronts a CU: 16 sequences of 300 keys, Hkv8 D128, 16.3, 14.0, 14.2, 32 of
+    // 4000 208, 148, 153, 1 of 8000 26, 29, 41, 2 x 512 tokens behind 1000 94, 58, 52.
+    if (max_keys <= 96) p.keys = max_keys, p.splits = 1;
+    else share((long)batch * hkv * p.groups, 4 * cus, 32, 32);
     return p;
   }
   if (rows <= 32) {
-    p.few = 32;
+    p.few = p.stride = (int)rows;  // (sequences with more new tokens than max_new: not taken)
     p.groups = 1;
-    p.stride = (int)rows;
     // One share, and no merge, where (sequence, kv head) pairs fill the device or the keys
     // are few; else workgroups for every CU.  us in a graph, one share and several, Hq32
     // Hkv8 D128: 1 sequence of 300 keys 8.2, 8.9, 700 9.8, 9.0, 1000 11.3, 9.0, 2000 17.1,
@@ -1575,8 +1579,7 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
     else share((long)batch * hkv, head_dim == 128 ? cus : 2 * cus, 128, 128);
     return p;
   }
-  p.few = rows > 128 ? 32 : 128;
-  p.stride = (int)std::min(rows, (long)p.few);
+  p.few = p.stride = rows > 128 ? 32 : (int)rows;
   // Shares of the sequences of few rows: three workgroups a CU, at least 512 keys; beside
   // sequences of many, which fill the device already, one a CU.  us with 3, 2 and 1: 8 x 16
   // tokens behind 4000 keys 28.5, 29.4, 34.4; 512 tokens among 32 single ones behind 1000

@@ -14,8 +14,9 @@ struct Paged {
   int hq, hkv;
 };
 
-// What a kernel knows of a sequence, bounded whatever the device arrays hold:
-// tokens t0 .. t0 + n - 1 lie in the batch, and every count of keys in the table.
+// What a kernel knows of a sequence, bounded whatever the device arrays hold: tokens t0 ..
+// t0 + n - 1 lie in the batch (none where its starts do not, or fall), and every count of
+// keys in the table.
 struct Seq {
   int t0, n, past, cap;
   // keys that the sequence's first i + 1 new tokens see
@@ -25,13 +26,14 @@ DEVI Seq seq_of(const Paged& a, int b) {
   Seq s;
   const int t0 = a.starts ? a.starts[b] : b * a.each;
   const int t1 = a.starts ? a.starts[b + 1] : t0 + a.each;
-  s.t0 = min(max(t0, 0), a.tokens);
-  s.n = max(min(t1, a.tokens) - s.t0, 0);
+  const bool in = t0 >= 0 && t0 <= t1 && t1 <= a.tokens;
+  s.t0 = in ? t0 : 0;
+  s.n = in ? t1 - t0 : 0;
   s.cap = a.width << a.lg;
   s.past = min(max(a.past ? a.past[b] : a.past_all, -a.tokens), s.cap);
   return s;
 }
-// The sequence of token t (wave-uniform): the last one that starts at or before it;
+// The sequence of token t (wave-uniform): the one before the first that starts behind it;
 // -1: none.  A wavefront looks at 64 starts at a time.
 DEVI int seq_at(const Paged& a, int t) {
   if (!a.starts) return t < a.batch * a.each ? t / a.each : -1;
@@ -40,7 +42,7 @@ DEVI int seq_at(const Paged& a, int t) {
   for (int i = 0; i <= a.batch; i += 64) {
     const bool yes = i + lane <= a.batch && a.starts[min(i + lane, a.batch)] <= t;
     const uint64_t all = __ballot(yes);
-    n += __builtin_popcountll(all);
+    n += ~all ? __builtin_ctzll(~all) : 64;
     if (~all) break;
   }
   return n > 0 && n <= a.batch ? n - 1 : -1;

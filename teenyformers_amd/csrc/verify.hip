@@ -11,7 +11,7 @@
 //
 // Numbers: a weight is 2^(x c - K) in fp32, c = log2(e) / T rounded to fp32 and K = c
 // max x rounded (the exponent is one fused product: whatever rounds K is common to all
-// weights, c's rounding moves a weight d octaves down by d 2^-25); sums of eight in fp32
+// weights, c's rounding moves a weight d octaves down by d 2^-24); sums of eight in fp32
 // and from there in fp64; what decides (acceptance, the place of u among running sums) is
 // fp64.  A draw from one row sums unscaled weights, exact for equal logits.  One order
 // of sums: no atomics on them.
@@ -57,7 +57,8 @@ DEVI Factor factor_of(const Args& a, float ts) {
   const double t = a.ts ? (double)ts : a.t;
   Factor f;
   f.greedy = !(t > 0.0);  // (NaN too)
-  f.c = f.greedy ? (float)kLog2e : (float)(kLog2e / t);
+  // (a factor past 1e30 leaves the same tokens)
+  f.c = f.greedy ? (float)kLog2e : (float)fmin(kLog2e / t, 1e30);
   return f;
 }
 DEVI Factor factor_of(const Args& a, int b) { return factor_of(a, a.ts ? a.ts[b] : 0.0f); }
@@ -66,15 +67,28 @@ DEVI Factor factor_of(const Args& a, int b) { return factor_of(a, a.ts ? a.ts[b]
 DEVI float weight(float x, float ref, const Factor& f) {
   return __builtin_amdgcn_exp2f(fmaxf(__builtin_fmaf(x, f.c, -ref), -200.0f));
 }
-// ... where the largest may be infinite: then it and its equals alone
-DEVI float weight(float x, float xmax, float ref, const Factor& f) {
-  return xmax == INFINITY ? (x == INFINITY ? 1.0f : 0.0f) : weight(x, ref, f);
+// Whether K is small enough for that: its rounding, a factor of all weights, is 2^-9
+// octaves at most.  Else (tiny temperatures, huge logits) the exponent is (x - max x) c;
+// an infinite maximum and its equals have weight alone.  (A part without a token: any sum,
+// which `below` leaves out.)
+DEVI bool fused(float ref) { return fabsf(ref) < 65536.0f; }
+DEVI float weight_apart(float x, float xmax, const Factor& f) {
+  return __builtin_amdgcn_exp2f(x == xmax ? 0.0f : fmaxf((x - xmax) * f.c, -200.0f));
 }
-// 2^(a - b) of two references a <= b, those of maxima xa <= xb
+DEVI float weight(float x, float xmax, float ref, const Factor& f) {
+  if (fused(ref)) return weight(x, ref, f);
+  return xmax > -INFINITY ? weight_apart(x, xmax, f) : 0.0f;
+}
+// The reference of a row's, or a part's, weights as it was used
+DEVI double ref_of(float xmax, const Factor& f) {
+  const float k = f.ref(xmax);
+  return fused(k) ? (double)k : (double)xmax * (double)f.c;
+}
+// 2^(a - b) of the references of maxima xa <= xb
 DEVI float below(float xa, float xb, const Factor& f) {
   if (!(xa > -INFINITY)) return 0.0f;
   if (xa == xb) return 1.0f;
-  return __builtin_amdgcn_exp2f(fmaxf(f.ref(xa) - f.ref(xb), -200.0f));
+  return __builtin_amdgcn_exp2f(fmaxf((float)(ref_of(xa, f) - ref_of(xb, f)), -200.0f));
 }
 
 template <typename T> DEVI const T* target_row(const Args& a, int b, int i) {
@@ -216,12 +230,12 @@ __device__ void verify_scan(const Args& a, Rec* __restrict__ rec, int* __restric
     } else {
       const float ref = f.ref(mx);
       float s[kVec];
-      if (mx == INFINITY) {
+      if (!fused(ref)) {
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
           s[v] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < kTok; ++j) s[v] += x[v][j] == INFINITY ? 1.0f : 0.0f;
+          for (int j = 0; j < kTok; ++j) s[v] += weight_apart(x[v][j], mx, f);
         }
       } else {
 #pragma unroll
@@ -283,7 +297,7 @@ DEVI double prob(float x, int col, const Row& r, const Factor& f) {
   if (f.greedy) return r.xmax > -INFINITY && col == r.first ? 1.0 : 0.0;
   if (!(x > -INFINITY) || !(r.sum > 0.0)) return 0.0;
   if (r.xmax == INFINITY) return x == INFINITY ? 1.0 / r.sum : 0.0;
-  return exp2((double)x * f.c - (double)f.ref(r.xmax)) / r.sum;
+  return exp2((double)x * (double)f.c - ref_of(r.xmax, f)) / r.sum;
 }
 
 // What the token after the accepted ones is drawn from: max(p_n - q_n, 0), or p_n.
@@ -378,7 +392,7 @@ DEVI double weigh(const T* prow, const T* qrow, int cols, int ch, const Rest& r,
   const int c0 = ch * kChunk - misaligned(prow) + 2 * kTok * (int)threadIdx.x;
   double sum = 0.0;
   // (vectors of the two rows begin at other columns where they are aligned otherwise)
-  if (c0 >= 0 && c0 + 2 * kTok <= cols && r.pmax < INFINITY && r.qmax < INFINITY &&
+  if (c0 >= 0 && c0 + 2 * kTok <= cols && fused(r.pref) && fused(r.qref) &&
       (!r.minus_q || misaligned(qrow) == misaligned(prow))) {
     u32x4 x[2 * VW], y[2 * VW];
 #pragma unroll

@@ -689,9 +689,10 @@ class Llama:
         list of its new tokens, [] once it has n_new or its last one was eos (or -1, nothing
         to draw)."""
         n_new, B, per = u.shape
-        if not prompts or n_new < 1 or n_draft < 1 or samples < 1 or B != len(prompts) * samples:
-            raise ValueError("draft_steps: u is [n_new, len(prompts) * samples, ..], n_draft and samples "
-                             "at least 1")
+        if (not prompts or n_new < 1 or not 1 <= n_draft <= 64 or samples < 1
+                or B != len(prompts) * samples):
+            raise ValueError("draft_steps: u is [n_new, len(prompts) * samples, ..], n_draft 1 to 64, "
+                             "samples at least 1")
         if u.dtype != torch.float32 or per != (2 * n_draft + 1 if draft else n_draft + 1):
             raise ValueError("draft_steps: u is fp32 with n_draft + 1 numbers a step and sequence, n_draft "
                              "more with a draft model")

@@ -435,3 +435,56 @@ def test_refusals(cuda):
             ops.copy_pages(pages, src, dst)
     with pytest.raises(ValueError):
         ops.copy_pages(pages[0, 0], [0], [1])
+
+
+@pytest.mark.parametrize("dtype,lens,most", [(BF, [1, 7, 1], 1), (BF, [1, 1, 5], 2), (F32, [2, 40, 1], 2),
+                                             (BF, [9, 20, 3], 9), (BF, [40, 70, 1], 40)])
+def test_more_new_tokens_than_said(cuda, dtype, lens, most):
+    """A sequence with more new tokens than max_new: the others are as they should be, and nothing
+    behind the workspace is written."""
+    past = [3000, 2000, 2500]
+    c = Batch(dtype, 8, 2, 64, 16, past, lens)
+    T, Hq, D = c.q.shape
+    from teenyformers_amd import _lib
+    need = _lib.lib().teeny_paged_attention_workspace_bytes(3, T, most, 3000 + most, Hq, 2, D,
+                                                            1 if dtype == BF else 0)
+    assert need > 0
+    ws = torch.full((need + 65536,), 0x5a, dtype=torch.uint8, device="cuda")
+    out = torch.full_like(c.q, 7.0)
+    c.run(out=out, max_new=most, max_keys=3000 + most, workspace=ws)
+    assert (ws[need:] == 0x5a).all()
+    ref, tol = c.reference()
+    t = 0
+    for n in lens:
+        if n <= most:
+            assert ((out[t:t + n].double() - ref[t:t + n]).abs() <= tol[t:t + n]).all()
+        t += n
+
+
+def test_device_values_out_of_their_ranges(cuda):
+    """starts that fall or lie past the batch, lengths of any size: bounded, and a sequence that is
+    well described is not disturbed."""
+    for dtype in (BF, F32):
+        c = Batch(dtype, 8, 2, 64, 16, [100, 40, 40, 9], [5, 1, 1, 1])
+        ref, tol = c.reference()
+        c.starts.copy_(torch.tensor([0, 5, 2 ** 31 - 1, -7, 10 ** 6], dtype=torch.int32))
+        c.n_past.copy_(torch.tensor([100, 2 ** 31 - 1, -2 ** 31, 10 ** 9], dtype=torch.int32))
+        c.k.nan_to_num_(0.5)  # (any row may be read)
+        c.v.nan_to_num_(0.5)
+        out = c.run()
+        assert ((out[:5].double() - ref[:5]).abs() <= tol[:5]).all()
+        qkv = c.rnd(8, (8 + 2 * 2) * 64)
+        before = c.k.clone()
+        q = ops.paged_qkv_rope_split(qkv, c.k, c.v, c.table, c.n_past, 8, 1e4, starts=c.starts)
+        y, e = rotated(qkv[:5].view(5, 12, 64)[:, :10], torch.arange(100, 105, device="cuda"), 1e4)
+        assert ((q[:5].double() - y[:, :8]).abs() <= e[:, :8]).all()
+        changed = (c.k != before).flatten(1).any(1)
+        assert set(changed.nonzero().view(-1).tolist()) <= set(c.table[0].tolist())
+
+
+def test_far_lengths_of_one_sequence(cuda):
+    """One sequence of 100000 keys: shares of the keys, positions far out."""
+    for dtype, D in ((BF, 128), (F32, 32)):
+        c = Batch(dtype, 4, 1, D, 64, [100000], [1])
+        c.check(c.run(max_keys=100001))
+        c.check(c.run())

@@ -298,3 +298,30 @@ def test_refusals(cuda):
                           torch.zeros((1, n + 1), device="cuda"))
     t, a = ops.verify_drafts(x[:0], d[:0], u[:0], y[:0])
     assert t.shape == (0, 3) and a.shape == (0,)
+
+
+def test_extreme_temperatures_and_logits(cuda):
+    """Factors and logits whose product is past fp32: the largest logit and its equals share the
+    draw, as in the limit."""
+    x, d, u, y = case(F32, 16, 2, 300, 6, True)
+    x[8:, :, 7] = x[8:].amax(2)          # two equal maxima (at most; 7 may be one)
+    best = x == x.amax(2, keepdim=True)
+    for T in (1e-36, 1e-40, 1e-44):
+        tokens, accepted = ops.verify_drafts(x, d, u, None, T)
+        for b in range(16):
+            n = int(accepted[b])
+            assert best[b, n, tokens[b, n]] or (n < 2 and not best[b, n, d[b, n]])
+            assert best[b, n, tokens[b, n]]
+            for i in range(n):
+                assert best[b, i, d[b, i]]
+    low = torch.finfo(F32).min
+    z = torch.full((4, 2, 100), low, device="cuda")
+    z[1, :, 40] = 3e38
+    z[2, :, 10:12] = 1e38
+    z[3] = 0.0
+    drafts = torch.full((4, 1), -1, dtype=torch.int64, device="cuda")
+    uu = torch.tensor([[0.5, 0.5]] * 4, device="cuda")
+    tokens, _ = ops.verify_drafts(z, drafts, uu, None, 0.25)
+    assert tokens[:, 0].tolist() == [50, 40, 11, 50]
+    tokens, _ = ops.verify_drafts(z, drafts, uu, None, math.inf)
+    assert tokens[3, 0] == 50
