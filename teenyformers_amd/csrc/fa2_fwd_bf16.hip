@@ -97,6 +97,11 @@ struct FwdPrefix {
 // page of each 16 keys is read by scalar loads a tile ahead; a load of a wavefront lies in
 // one page.  Workgroups go kv head by kv head: the sequences of many rows, the last rows
 // first, then those of few, whose shares of the keys are read beside the others' products.
+// 2 x 4096 tokens behind 4096, Hq32 Hkv8 D128: 1069 TFLOP/s (the forward over contiguous
+// keys 1156, PREFIX 1104; pages of 16 or 256 rows, in order or not, make no difference); 8 x
+// 512 behind 7680 955 (1111, 1128): 1024 workgroups of equal length for 768 places.  64-key
+// tiles at two workgroups per CU: 974 there, but 1001 for the former, and a step of 2048
+// tokens behind 6144 among 32 single ones 365 us instead of 295.
 struct FwdPaged {
   Paged a;
   PagedPlan pl;
@@ -805,7 +810,8 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
         if (pair_slot(q) == j) sm_pair(s0, s1, q, la, lb);
       // PAGED: before the PV products, since a tile of a long cache comes from HBM (2048 tokens
       // behind 6144 among 32 one-token sequences 307 -> 287 us, 512 behind 32000 321 ->
-      // 311), and behind the last tile too, where nothing is read and zeros go to buffers that
+      // 311; K two tiles ahead in a third buffer and V one gained nothing more), and behind the
+      // last tile too, where nothing is read and zeros go to buffers that
       // nobody reads: around a branch the compiler gathers all of the exponentials behind it.
       if (j == (PAGED ? 0 : NJ / 2) && (PAGED || it + 1 < n_iter))
         load_tile(it + 1, ((kb + 1) % KBUF) * TILE, ((vp + 2) % VBUF) * TILE);

@@ -770,14 +770,15 @@ def paged_qkv_rope_split(qkv, k_pages, v_pages, page_table, n_past, n_heads_q: i
     kernel runs (for captured graphs).  Positions without a page are not written;
     tokens behind starts[B] are nobody's, their rows of q_out are left as they were."""
     parts = isinstance(qkv, Partials)
-    src = qkv.slabs if parts else qkv
-    T = math.prod(qkv.shape[:-1])
-    x = src if parts else src.reshape(T, qkv.shape[-1])
+    src = x = qkv.slabs if parts else qkv
+    T, W = math.prod(qkv.shape[:-1]), qkv.shape[-1]
+    if not parts and len(qkv.shape) != 2:
+        x = qkv.reshape(T, W)
     B, n_pages, hkv, size, D, where = _paged("paged_qkv_rope_split", x[0] if parts else x, k_pages,
                                              v_pages, page_table, n_past, starts)
     if qkv.dtype != k_pages.dtype:
         raise TypeError("paged_qkv_rope_split: the tensors share a dtype")
-    if n_heads_q < 1 or n_heads_q % hkv or qkv.shape[-1] != (n_heads_q + 2 * hkv) * D:
+    if n_heads_q < 1 or n_heads_q % hkv or W != (n_heads_q + 2 * hkv) * D:
         raise ValueError("paged_qkv_rope_split: qkv is [T, (Hq+2Hkv)*D] matching the pages")
     if q_out is None:
         q_out = torch.empty((T, n_heads_q, D), dtype=k_pages.dtype, device=k_pages.device)
