@@ -1555,7 +1555,7 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
     p.splits = std::max(1, (max_keys + p.keys - 1) / p.keys);
   };
   if (f32) {
-    p.few = 0x7fffffff;
+    p.few = (int)rows;  // (as below)
     p.groups = (int)((rows + 15) / 16);
     // us in a graph, one share and several: 4 sequences of 4 heads of 64 and 64 keys 7.0,
     // 8.7, 1 of 100 keys 10.1, 7.9 (an eager call pays 4 us for the merge's launch).  With 2,

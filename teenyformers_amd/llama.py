@@ -249,6 +249,8 @@ class PagedKVCache:
 
     def fork(self, seq: int, n: int = 1) -> list:
         """n sequences that go on from seq's keys, sharing its pages."""
+        if n < 0:
+            raise ValueError("fork: n is at least 0")
         table, length = self.tables[seq], self.lengths[seq]
         new = [self.add() for _ in range(n)]
         for i in new:

@@ -785,6 +785,8 @@ def paged_qkv_rope_split(qkv, k_pages, v_pages, page_table, n_past, n_heads_q: i
     elif (q_out.shape != (T, n_heads_q, D) or q_out.dtype != k_pages.dtype
           or q_out.get_device() != k_pages.get_device() or not q_out.is_contiguous()):
         raise ValueError("paged_qkv_rope_split: q_out is contiguous [T, Hq, D] on the pages' device")
+    if T == 0:
+        return q_out
     with _on_device_of(k_pages):
         call("teeny_paged_qkv_rope_split", None if parts else _p(x), _p(src) if parts else None,
              qkv.n if parts else 0, _p(q_out), _p(k_pages), _p(v_pages), *where, B, T, n_pages, size,
@@ -828,6 +830,8 @@ def paged_attention(q, k_pages, v_pages, page_table, n_past, softmax_scale: floa
     if workspace is not None and (workspace.get_device() != q.get_device()
                                   or not workspace.is_contiguous()):
         raise ValueError("paged_attention: workspace must be contiguous, on q's device")
+    if T == 0:
+        return out
     with _on_device_of(q):
         if workspace is None:  # (asked on q's device: the shares go by its CUs)
             need = _lib.lib().teeny_paged_attention_workspace_bytes(B, T, new, max(1, keys), Hq, hkv,

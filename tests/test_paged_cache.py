@@ -139,6 +139,16 @@ def test_refusals(cache):
             next(m.draft_steps(**a))
 
 
+def test_forks_are_counted(cache):
+    s = cache.add()
+    write(cache, [s], [[1.0] * 20])
+    with pytest.raises(ValueError):
+        cache.fork(s, -1)
+    assert cache.fork(s, 0) == []
+    cache.remove(s)
+    assert cache.free_pages == len(cache._uses)
+
+
 @pytest.mark.parametrize("text,n,want", [
     ([1, 2, 3, 9, 1, 2, 3], 2, [9, 1]), ([1, 2, 3, 9, 1, 2, 3], 9, [9, 1, 2, 3]), ([5, 1, 5, 2, 5], 1, [2]),
     ([1, 2, 3], 4, []), ([7], 3, []), ([7, 7], 3, [7]), ([1, 2, 1], 0, [])])

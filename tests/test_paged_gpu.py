@@ -461,6 +461,41 @@ def test_more_new_tokens_than_said(cuda, dtype, lens, most):
         t += n
 
 
+@pytest.mark.parametrize("dtype,lens,most", [(F32, [2, 40, 1], 2), (F32, [5, 6, 1], 5), (BF, [1, 7, 1], 1),
+                                             (BF, [9, 20, 3], 9)])
+def test_more_new_tokens_than_said_are_left_out(cuda, dtype, lens, most):
+    """... and such a sequence's rows stay as they were, in one share or several."""
+    for past in (40, 3000):
+        c = Batch(dtype, 8, 2, 64, 16, [past] * 3, lens)
+        out = torch.full_like(c.q, 7.0)
+        c.run(out=out, max_new=most, max_keys=past + most)
+        ref, tol = c.reference()
+        t = 0
+        for n in lens:
+            if n <= most:
+                assert ((out[t:t + n].double() - ref[t:t + n]).abs() <= tol[t:t + n]).all()
+            else:
+                assert (out[t:t + n] == 7.0).all()
+            t += n
+
+
+def test_no_new_tokens(cuda):
+    for dtype in (BF, F32):
+        c = Batch(dtype, 8, 2, 64, 16, [100, 40], [1, 1])
+        before = c.k.clone(), c.v.clone()
+        starts = torch.zeros_like(c.starts)
+        for kw in (dict(), dict(starts=starts)):
+            assert ops.paged_attention(c.q[:0], c.k, c.v, c.table, c.n_past, **kw).shape == (0, 8, 64)
+            qkv = c.rnd(0, (8 + 2 * 2) * 64)
+            assert ops.paged_qkv_rope_split(qkv, c.k, c.v, c.table, c.n_past, 8, 1e4, **kw).shape == (0, 8, 64)
+        out = torch.full_like(c.q, 7.0)  # tokens, but nobody's
+        c.starts = starts
+        c.run(out=out)
+        assert (out == 7.0).all()
+        assert torch.equal(c.k.view(torch.uint8), before[0].view(torch.uint8))
+        assert torch.equal(c.v.view(torch.uint8), before[1].view(torch.uint8))
+
+
 def test_device_values_out_of_their_ranges(cuda):
     """starts that fall or lie past the batch, lengths of any size: bounded, and a sequence that is
     well described is not disturbed."""
