@@ -642,7 +642,7 @@ int teeny_copy_pages(void* pages, int planes, long plane_bytes, long page_bytes,
  * (fp32 device memory, one per sequence); 0: p and q one-hot at the lowest index of
  * the row's maximum.  NaN and -inf logits have no weight; a row without any other
  * draws -1.  n_drafts 1 .. 64; workspace: teeny_verify_drafts_workspace_bytes bytes,
- * 16-byte aligned. */
+ * 16-byte aligned, that no call on another stream uses meanwhile. */
 size_t teeny_verify_drafts_workspace_bytes(int batch, int n_drafts, int cols, int with_draft);
 int teeny_verify_drafts(const void* target, long target_seq, long target_row, const void* draft,
                         long draft_seq, long draft_row, const int64_t* drafts, const float* u,

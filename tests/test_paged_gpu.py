@@ -192,6 +192,24 @@ def test_attention_later_tokens_have_no_influence(cuda, dtype, where, bad):
         assert not got[at:lens[0], 4:].isfinite().all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("page", [64, 256, 512, 1024])
+def test_page_sizes(cuda, dtype, page):
+    """Few rows, rows enough for the forward's walk, and keys written by the split, in large pages."""
+    c = Batch(dtype, 8, 2, 64, page, [2 * page - 1, page, 0, 700], [1, 3, 2, 1], seed=page)
+    c.check(c.run())
+    c = Batch(dtype, 8, 2, 64, page, [2 * page - 1, 0, 700], [60, 20, 1], seed=page)
+    c.check(c.run())
+    qkv = c.rnd(c.T, (8 + 2 * 2) * 64)
+    ops.paged_qkv_rope_split(qkv, c.k, c.v, c.table, c.n_past, 8, 1e4, starts=c.starts)
+    want, t = qkv.view(c.T, 12, 64)[:, 10:], 0
+    for b, (past, m) in enumerate(zip(c.past, c.lens)):
+        V = c.keys(b, past + m)[1]
+        assert torch.equal(V[:, past:].transpose(0, 1), want[t:t + m])
+        t += m
+    c.check(c.run())
+
+
 def test_attention_lowest_scores(cuda):
     """Rows whose scores lie far below zero, and keys of the type's lowest values."""
     for dtype in (F32, BF):
