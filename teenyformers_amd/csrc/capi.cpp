@@ -1560,9 +1560,12 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
     // us in a graph, one share and several: 4 sequences of 4 heads of 64 and 64 keys 7.0,
     // 8.7, 1 of 100 keys 10.1, 7.9 (an eager call pays 4 us for the merge's launch).  With 2,
     // 4 and 8 wavefronts a CU: 16 sequences of 300 keys, Hkv8 D128, 16.3, 14.0, 14.2, 32 of
-    // 4000 208, 148, 153, 1 of 8000 26, 29, 41, 2 x 512 tokens behind 1000 94, 58, 52.
+    // 4000 208, 148, 153, 1 of 8000 26, 29, 41, 2 x 512 tokens behind 1000 94, 58, 52.  The
+    // groups that have rows count (2278 tokens among 56 x 9 of one head of 32: all groups of
+    // all sequences counted 101, so 48).
+    const long tiles = std::min((long)batch * p.groups, tokens * G / 16 + batch);
     if (max_keys <= 96) p.keys = max_keys, p.splits = 1;
-    else share((long)batch * hkv * p.groups, 4 * cus, 32, 32);
+    else share(tiles * hkv, 4 * cus, 32, 32);
     return p;
   }
   if (rows <= 32) {
@@ -1588,12 +1591,33 @@ PagedPlan paged_plan(int batch, int tokens, int max_new, int max_keys, int hq, i
   share((long)batch * hkv, rows > p.few ? cus : 3 * cus, 512, 64);
   if (rows > p.few) {
     p.tiles = (int)(tokens * G / 128 + std::min((long)batch, tokens * G / (p.few + 1)));
-    const long wgs = (long)p.tiles * hkv;
-    const long n = std::max(1L, std::min(3 * cus / std::max(1L, wgs), (max_keys + 511L) / 512));
+    // Shares of their keys: the walk of the longest row against the partials, whose traffic
+    // costs most of what idle CUs would bring.  Estimated us: `walk` one share's (a key of
+    // 128 0.022, of 64 0.014, a workgroup a CU), `work` that of all workgroups at three a
+    // CU (0.8 of it a key), `part` a share's partials written and read (2 TB/s), a merge 4.
+    // us measured with one and more, D128: 1024 tokens behind 0, Hq32 Hkv8 32, 45, Hq8 Hkv1
+    // 30, 28; 1024 behind 2000, Hq32 Hkv8 74, 80, Hq16 Hkv16 76, 57; 512 behind 4000, Hq32
+    // Hkv8 99, 66; D64: 2048 behind 0, Hq16 Hkv16 38, 50; 128 behind 3000, Hq16 Hkv2 50, 20.
+    const double wgs = std::max(1.0, (double)tokens * G / 128) * hkv;
+    const double key = head_dim == 128 ? 0.022 : 0.014, walk = key * max_keys;
+    const double work = 0.8 * key * wgs / cus * (max_keys - 0.5 * std::min(max_new, max_keys));
+    const double part = 4e-6 * tokens * hq * head_dim;
+    auto us = [&](long n) {
+      return n == 1 ? std::max(walk, work) : std::max(walk / n, work) + n * part + 4;
+    };
+    const long most = (long)std::min({3 * cus / wgs, walk / work + 1, max_keys / 64.0});
+    long n = std::min((long)std::sqrt(walk / part), most);  // the best where the walk counts
+    if (n < most && us(n + 1) < us(std::max(n, 1L))) ++n;
+    if (n < 2 || us(n) >= us(1)) n = 1;
     p.keys_many = (int)(((max_keys + n - 1) / n + 63) / 64 * 64);
     p.splits_many = std::max(1, (max_keys + p.keys_many - 1) / p.keys_many);
   }
   return p;
+}
+// Workgroups of a grid whose kernel takes its place from paged_place (paged.h)
+long paged_grid(long per_head, int hkv) {
+  const int lg = std::min(__builtin_ctz((unsigned)hkv), 3);
+  return 8 * ((per_head * (hkv >> lg) + (8 >> lg) - 1) >> (3 - lg));
 }
 // Rows of partials: of sequences of few rows, of the others (0: none)
 size_t paged_rows_few(const PagedPlan& p, int batch, int tokens, int hq, int hkv) {
@@ -1692,7 +1716,7 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
   char name[64];
   long wgs;
   if (dtype == TEENY_BF16 && (long)max_new * (n_heads_q / n_heads_kv) > 32) {
-    wgs = ((long)p.tiles * p.splits_many + (long)batch * p.splits) * n_heads_kv;
+    wgs = paged_grid((long)p.tiles * p.splits_many + (long)batch * p.splits, n_heads_kv);
     if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
     FwdPaged f{a, p, parts};
     int total = (int)wgs;
@@ -1700,7 +1724,8 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
     void* args[] = {&q, &k_pages, &v_pages, &o, &total, &f};
     rc = launch(name, dim3((unsigned)wgs), dim3(256), 0, stream, args);
   } else {
-    wgs = (long)p.splits * p.groups * batch * n_heads_kv;
+    wgs = (long)p.splits * p.groups * batch;
+    wgs = dtype == TEENY_F32 ? paged_grid(wgs, n_heads_kv) : wgs * n_heads_kv;
     if (wgs >= (1L << 31)) return TEENY_ERR_INVALID_SHAPE;
     // Wavefronts: 4; 8 for one share of few keys, and of heads of 64.  us with 4 and 8: 64
     // sequences of up to 8191 keys, D128 206, 215, of 2000 45.2, 46.2; D64, 16 kv heads, of

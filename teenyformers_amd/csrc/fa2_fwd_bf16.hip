@@ -200,7 +200,7 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l32 = lane & 31, g = lane >> 5;
 
-  const int id = xcd_remap(blockIdx.x, total_blocks);
+  const int id = PAGED ? 0 : xcd_remap(blockIdx.x, total_blocks);
   int bh, rank;
   // causal blocks: heads in groups of 4 (measured 1.02-1.06x at B16 Hq32 Hkv8
   // S512 and B4 S2048 against pairs; equal blocks gain nothing from it)
@@ -214,8 +214,8 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
   if constexpr (PAGED) {
     group = hq / hkv;
     const int n_many = pg.pl.tiles * pg.pl.splits_many, per_head = n_many + pg.a.batch * pg.pl.splits;
-    hk_p = id / per_head;
-    const int in = id - hk_p * per_head;
+    int in;
+    if (!paged_place(hkv, per_head, &hk_p, &in)) return;
     b_p = -1;
     if (in >= n_many) {
       split_p = (in - n_many) / pg.a.batch;
@@ -253,16 +253,16 @@ __device__ __forceinline__ void fa2_fwd_bf16(const bf16* __restrict__ q, const b
     const long rows = (long)seq.n * group;
     few_p = rows <= pg.pl.few;
     if (rows == 0 || few_p != (in >= n_many)) return;
-    const int share = few_p ? pg.pl.keys : pg.pl.keys_many;
+    const int part = few_p ? pg.pl.keys : pg.pl.keys_many;
     const int most = few_p ? pg.pl.splits : pg.pl.splits_many;
-    const int n_sh = paged_shares(seq, share, most);
+    const int n_sh = paged_shares(seq, part, most);
     if (split_p >= n_sh) return;
     direct = n_sh == 1;
     nq = seq.n * group;
     // the keys of this share that the workgroup's last row sees
     const int last = seq.keys((min(mb * BM + BM, nq) - 1) / group);
-    k_first = split_p * share;
-    k_last = split_p + 1 < most ? min(k_first + share, last) : last;
+    k_first = split_p * part;
+    k_last = split_p + 1 < most ? min(k_first + part, last) : last;
     k_last = max(k_last, k_first);
   }
   // bhq: this wavefront's (b, q head); wrow0: its first query row; blk_end:

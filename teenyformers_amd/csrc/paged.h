@@ -72,6 +72,20 @@ struct PageWalk {
   }
 };
 
+// The kv head of a workgroup and its place among per_head of that head; false: none.
+// XCDs take heads of their own, or groups of 2, 4 or 8 share some, and their heads' places
+// in turn: a head's keys pass few L2 caches, and where a head's long rows come first, every
+// XCD and CU gets long and short ones.  us of bf16 chunks with runs of a head's places by
+// XCD and so: 2048 tokens behind 6144, Hq32 Hkv4 296, 254, Hq16 Hkv16 175, 163; 3548 behind
+// 0, Hq32 Hkv4 168, 129, Hq24 Hkv6 108, 103, Hq32 Hkv8 120, 120.
+DEVI bool paged_place(int hkv, int per_head, int* hk, int* in) {
+  const int lg = min(__builtin_ctz(hkv), 3), share = 3 - lg, heads = hkv >> lg;
+  const int x = blockIdx.x & 7, at = (blockIdx.x >> 3 << share) + (x & ((1 << share) - 1));
+  *in = at / heads;
+  *hk = (x >> share) * heads + at - *in * heads;
+  return *in < per_head;
+}
+
 // How a launch of the attention shares its work out.  The rows of a sequence and kv
 // head are r = i G + g: token i, q head g of the group.
 struct PagedPlan {

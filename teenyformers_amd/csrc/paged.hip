@@ -343,11 +343,10 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
                                const PagedPlan pl, const PagedParts out) {
   constexpr int NC = Geo<D>::NC, VW = Geo<D>::VW, NH = Geo<D>::NH;
   const int lane = threadIdx.x, j = lane & 15, g = lane >> 4;
-  int id = blockIdx.x;
+  int hk, id;
+  if (!paged_place(a.hkv, pl.splits * pl.groups * a.batch, &hk, &id)) return;
   const int rg = id % pl.groups;
   id /= pl.groups;
-  const int hk = id % a.hkv;
-  id /= a.hkv;
   const int split = id % pl.splits, b = id / pl.splits;
   PageWalk walk(a, b);
   const Seq s = seq_of(a, b);
