@@ -193,6 +193,17 @@ def test_attention_later_tokens_have_no_influence(cuda, dtype, where, bad):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("Hkv", [1, 2, 3, 4, 6, 8, 12, 16, 24])
+def test_kv_heads(cuda, dtype, Hkv):
+    """Every way of dealing kv heads to the caches' parts of the device: a long sequence among short
+    ones, its keys in one share or several."""
+    for past, lens in (([150, 0, 700], [1, 300, 2]), ([2500, 40], [130, 1])):
+        c = Batch(dtype, 2 * Hkv, Hkv, 64, 16, past, lens, seed=Hkv)
+        c.check(c.run(max_new=max(lens), max_keys=max(n + m for n, m in zip(past, lens))))
+        c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("page", [64, 256, 512, 1024])
 def test_page_sizes(cuda, dtype, page):
     """Few rows, rows enough for the forward's walk, and keys written by the split, in large pages."""
