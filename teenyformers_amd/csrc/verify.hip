@@ -383,28 +383,28 @@ DEVI Rest rest_of(const Args& a, const Rec* rec, int b, const Factor& f, RestSme
   r.qref = f.ref(r.qmax);
   return r;
 }
-// The weight of column c
-template <typename T>
-DEVI float weigh_one(const T* prow, const T* qrow, int c, const Rest& r, const Factor& f) {
-  float z = weight((float)prow[c], r.pmax, r.pref, f);
-  if (r.minus_q) z = surplus(z, r.ap, weight((float)qrow[c], r.qmax, r.qref, f), r.aq);
+// The weight of column c, logits x and y
+DEVI float weigh_one(float x, float y, int c, const Rest& r, const Factor& f) {
+  float z = weight(x, r.pmax, r.pref, f);
+  if (r.minus_q) z = surplus(z, r.ap, weight(y, r.qmax, r.qref, f), r.aq);
   return c == r.skip ? 0.0f : z;
 }
-// The sum of a thread's 16 columns of a chunk: those from 16 tid on
+// The sum of a thread's 16 columns of a chunk: those from 16 tid on, in the draft's row
+// wherever they lie in memory (rows of an odd number of columns: 48 sequences of 8 drafts
+// of 128255 97 us with such columns one by one, 67 so)
+typedef uint32_t u32x4any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 DEVI double weigh(const T* prow, const T* qrow, int cols, int ch, const Rest& r, const Factor& f) {
   constexpr int VW = kTok / Vec16<T>::N;
   const int c0 = ch * kChunk - misaligned(prow) + 2 * kTok * (int)threadIdx.x;
   double sum = 0.0;
-  // (vectors of the two rows begin at other columns where they are aligned otherwise)
-  if (c0 >= 0 && c0 + 2 * kTok <= cols && fused(r.pref) && fused(r.qref) &&
-      (!r.minus_q || misaligned(qrow) == misaligned(prow))) {
+  if (c0 >= 0 && c0 + 2 * kTok <= cols && fused(r.pref) && fused(r.qref)) {
     u32x4 x[2 * VW], y[2 * VW];
 #pragma unroll
     for (int v = 0; v < 2 * VW; ++v) x[v] = reinterpret_cast<const u32x4*>(prow + c0)[v];
     if (r.minus_q)
 #pragma unroll
-      for (int v = 0; v < 2 * VW; ++v) y[v] = reinterpret_cast<const u32x4*>(qrow + c0)[v];
+      for (int v = 0; v < 2 * VW; ++v) y[v] = reinterpret_cast<const u32x4any*>(qrow + c0)[v];
     auto at = [](const u32x4* z, int j) __attribute__((always_inline)) {
       const uint32_t w = VW == 2 ? z[j / 4][j % 4] : z[j / 8][j % 8 / 2];
       return VW == 2 ? __builtin_bit_cast(float, w) : j & 1 ? bf16hi(w) : bf16lo(w);
@@ -430,9 +430,19 @@ DEVI double weigh(const T* prow, const T* qrow, int cols, int ch, const Rest& r,
       sum += (double)part;
     }
   } else {
+    // a row's ends, and references too large to fuse: four columns' loads at a time
 #pragma unroll 1
-    for (int j = 0; j < 2 * kTok; ++j)
-      if (c0 + j >= 0 && c0 + j < cols) sum += (double)weigh_one(prow, qrow, c0 + j, r, f);
+    for (int j = c0; j < c0 + 2 * kTok; j += 4) {
+      float x[4], y[4] = {};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = (float)prow[max(min(j + i, cols - 1), 0)];
+      if (r.minus_q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = (float)qrow[max(min(j + i, cols - 1), 0)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j + i >= 0 && j + i < cols) sum += (double)weigh_one(x[i], y[i], j + i, r, f);
+    }
   }
   return sum;
 }
@@ -488,7 +498,9 @@ __device__ void verify_rest(const Args& a, const Rec* __restrict__ rec, double* 
       const int l = at ? __builtin_ctzll(at) : 63 - __builtin_clzll(any);
       const double t = target - lane_double(lo, l);
       const int c = ch * kChunk - misaligned(prow) + 2 * kTok * (wave * 64 + l) + lane;
-      const double v = lane < 2 * kTok && c >= 0 && c < a.cols ? (double)weigh_one(prow, qrow, c, r, f) : 0.0;
+      double v = 0.0;
+      if (lane < 2 * kTok && c >= 0 && c < a.cols)
+        v = (double)weigh_one((float)prow[c], (float)qrow[c], c, r, f);
       const double upto = wave_run(v);
       const u64 hit = __ballot(v > 0.0 && upto > t), some = __ballot(v > 0.0);
       if (lane == (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some))) out[r.n] = c;
