@@ -8,8 +8,8 @@ Shapes follow the reference with the batch split out:
 """
 from __future__ import annotations
 
+import array
 import contextlib
-import ctypes
 import functools
 import math
 import threading
@@ -853,7 +853,10 @@ def copy_pages(pages: torch.Tensor, src, dst) -> torch.Tensor:
     if pages.dim() < 4:
         raise ValueError("copy_pages: pages is [..., n_pages, Hkv, page_size, D]")
     _dev(pages)
-    src, dst = [int(i) for i in src], [int(i) for i in dst]
+    try:
+        src, dst = array.array("i", map(int, src)), array.array("i", map(int, dst))
+    except OverflowError:
+        raise ValueError("copy_pages: page numbers lie in the pool") from None
     if len(src) != len(dst):
         raise ValueError("copy_pages: as many sources as destinations")
     if not src or pages.numel() == 0:
@@ -867,10 +870,9 @@ def copy_pages(pages: torch.Tensor, src, dst) -> torch.Tensor:
         raise ValueError("copy_pages: a page is written once, and not both read and written")
     size = pages.element_size() * math.prod(pages.shape[-3:])
     planes = math.prod(pages.shape[:-4])
-    ints = ctypes.c_int32 * len(src)
     with _on_device_of(pages):
-        call("teeny_copy_pages", _p(pages), planes, size * n_pages, size, n_pages, ints(*src),
-             ints(*dst), len(src), _stream())
+        call("teeny_copy_pages", _p(pages), planes, size * n_pages, size, n_pages,
+             src.buffer_info()[0], dst.buffer_info()[0], len(src), _stream())
     return pages
 
 

@@ -508,6 +508,19 @@ def test_more_new_tokens_than_said_are_left_out(cuda, dtype, lens, most):
             t += n
 
 
+def test_copies_of_far_numbers(cuda):
+    pages = torch.arange(2 * 2000, device="cuda").view(2, 2000, 1, 1, 1).expand(2, 2000, 1, 16, 8).float().contiguous()
+    want = pages.clone()
+    for src, dst in (([2 ** 31], [0]), ([0], [2 ** 40]), ([0], [-2 ** 40])):
+        with pytest.raises(ValueError):
+            ops.copy_pages(pages, src, dst)
+    assert torch.equal(pages, want)
+    src, dst = range(1000, 2000), torch.arange(1000)  # more than one launch's pairs; any iterables of whole numbers
+    ops.copy_pages(pages, src, dst)
+    want[:, :1000] = want[:, 1000:]
+    assert torch.equal(pages, want)
+
+
 def test_no_new_tokens(cuda):
     for dtype in (BF, F32):
         c = Batch(dtype, 8, 2, 64, 16, [100, 40], [1, 1])
