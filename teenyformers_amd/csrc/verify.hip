@@ -339,7 +339,8 @@ DEVI Rest rest_of(const Args& a, const Rec* rec, int b, const Factor& f, RestSme
   const float u = a.u[(long)b * (a.k + 1) + mine];
   const float x = (float)target_row<T>(a, b, mine)[d];
   const float y = a.draft ? (float)draft_row<T>(a, b, mine)[d] : 0.0f;
-  const int rows = real + 1 + (a.draft ? real : 0);
+  // (all rows, whatever the drafts are: these loads do not wait for them)
+  const int rows = a.k + 1 + (a.draft ? a.k : 0);
   for (int r0 = wave; r0 < rows; r0 += U * kWaves) {
     Rec r[U];
 #pragma unroll
@@ -347,7 +348,7 @@ DEVI Rest rest_of(const Args& a, const Rec* rec, int b, const Factor& f, RestSme
       const int t = r0 + i * kWaves;
       r[i] = Rec{0.0, -INFINITY, 0x7fffffff};
       if (t < rows && lane < a.n_ch)
-        r[i] = (t <= real ? target_rec(a, rec, b, t) : draft_rec(a, rec, b, t - real - 1))[lane];
+        r[i] = (t <= a.k ? target_rec(a, rec, b, t) : draft_rec(a, rec, b, t - a.k - 1))[lane];
     }
 #pragma unroll
     for (int i = 0; i < U; ++i) {
@@ -359,7 +360,7 @@ DEVI Rest rest_of(const Args& a, const Rec* rec, int b, const Factor& f, RestSme
   __syncthreads();
   bool passed = false;
   if (lane < real) {
-    const double q = a.draft ? prob(y, d, sm.row[real + 1 + lane], f) : 1.0;
+    const double q = a.draft ? prob(y, d, sm.row[a.k + 1 + lane], f) : 1.0;
     passed = (double)u * q < prob(x, d, sm.row[lane], f);
   }
   Rest r;
@@ -375,7 +376,7 @@ DEVI Rest rest_of(const Args& a, const Rec* rec, int b, const Factor& f, RestSme
   r.qmax = 0.0f;
   r.aq = 0.0f;
   if (r.minus_q) {
-    const Row q = sm.row[real + 1 + r.n];
+    const Row q = sm.row[a.k + 1 + r.n];
     r.qmax = q.xmax;
     r.aq = q.sum > 0.0 ? (float)(1.0 / q.sum) : 0.0f;
   }
