@@ -19,14 +19,14 @@
 //   scan   workgroups take chunks of 8192 columns of the rows in turn: their maximum and
 //          the weights' sum below it, each wavefront's below its own first (one barrier a
 //          chunk), the next chunk's loads in flight meanwhile.  Reading the rows bounds it:
-//          48 sequences of 8 drafts, 816 rows of 128256 bf16, 209 MB, 44 us (4.7 TB/s); 144
-//          rows, 37 MB, 10.1 us; 5 rows 4.4 us.
+//          48 sequences of 8 drafts, 816 rows of 128256 bf16, 209 MB, 45 us (4.6 TB/s); 144
+//          rows, 37 MB, 11 us; 5 rows 4.2 us.
 //   rest   (chunk, sequence): each workgroup finds the sequence's accepted drafts from the
 //          scan's sums (a wavefront a draft, a lane a chunk) and sums its chunk of what the
 //          next token is drawn from; the one that ends last finds the chunk and the token.
 //          Bound by a chain: records and drafts' logits, the chunk's rows, the count, the
-//          sums, the drawn chunk once more: 1 and 16 sequences 8.4 and 11.5 us; 48, with 25
-//          MB of rows and two exponentials a column, 18.5.
+//          sums, the drawn chunk once more: 1 and 16 sequences 8.3 and 11.6 us; 48, with 25
+//          MB of rows and two exponentials a column, 18.
 #include "sample.h"
 
 namespace {
