@@ -345,7 +345,7 @@ __device__ void paged_attn_f32(const float* __restrict__ q, const float* __restr
   const int lane = threadIdx.x, j = lane & 15, g = lane >> 4;
   int hk, id;
   if (!paged_place(a.hkv, pl.splits * pl.groups * a.batch, &hk, &id)) return;
-  const int rg = id % pl.groups;
+  const int rg = pl.groups - 1 - id % pl.groups;  // the last rows, with the most keys, first
   id /= pl.groups;
   const int split = id % pl.splits, b = id / pl.splits;
   PageWalk walk(a, b);
