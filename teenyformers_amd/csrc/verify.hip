@@ -25,8 +25,9 @@
 //          scan's sums (a wavefront a draft, a lane a chunk) and sums its chunk of what the
 //          next token is drawn from; the one that ends last finds the chunk and the token.
 //          Bound by a chain: records and drafts' logits, the chunk's rows, the count, the
-//          sums, the drawn chunk once more: 1 and 16 sequences 8.3 and 11.6 us; 48, with 25
-//          MB of rows and two exponentials a column, 18.
+//          sums, the drawn chunk once more: 16 sequences 11.6 us, 1 without draft logits (no
+//          differences, no count) 6.6; 48, with 25 MB of rows and two exponentials a column,
+//          18.
 #include "sample.h"
 
 namespace {
@@ -467,21 +468,30 @@ __device__ void verify_rest(const Args& a, const Rec* __restrict__ rec, double* 
     if (tid == 0) accepted[b] = r.n;
   }
   if (r.greedy) return;
+  // p_n's own weights: one workgroup draws, the scan has the sums of the chunks, but that of
+  // the refused draft's chunk without it (1 sequence 8.1 -> 6.6 us)
+  const bool alone = !r.minus_q;
+  if (alone && blockIdx.x > 0) return;
   const T* prow = target_row<T>(a, b, r.n);
   const T* qrow = r.minus_q ? draft_row<T>(a, b, r.n) : prow;
+  const Rec* prec = target_rec(a, rec, b, r.n) + min(lane, n_ch - 1);
   // Twice through one body (code that runs once is fetched from memory as it goes): the
   // workgroup's own chunk, then, by the last workgroup of the sequence, the drawn one.
-  int ch = blockIdx.x;
+  int ch = !alone ? blockIdx.x : r.skip < 0 ? -1 : (r.skip + misaligned(prow)) / kChunk;
   double target = 0.0;
 #pragma unroll 1
   for (int pass = 0;; ++pass) {
-    const double mine = weigh<T>(prow, qrow, a.cols, ch, r, f), run = wave_run(mine);
-    if (lane == 63) sums[wave] = run;
-    __syncthreads();
-    double before = 0.0, all = 0.0;  // of the wavefront; of the chunk
-    for (int i = 0; i < kWaves; ++i) {
-      before += i < wave ? sums[i] : 0.0;
-      all += sums[i];
+    double mine = 0.0, run = 0.0;
+    double before = 0.0, all = 0.0;  // sums before the wavefront's; of the chunk
+    if (ch >= 0) {
+      mine = weigh<T>(prow, qrow, a.cols, ch, r, f);
+      run = wave_run(mine);
+      if (lane == 63) sums[wave] = run;
+      __syncthreads();
+      for (int i = 0; i < kWaves; ++i) {
+        before += i < wave ? sums[i] : 0.0;
+        all += sums[i];
+      }
     }
     if (pass == 1) {
       // the thread that the target falls into (rounding may leave none: the last that has any)
@@ -507,7 +517,7 @@ __device__ void verify_rest(const Args& a, const Rec* __restrict__ rec, double* 
       if (lane == (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some))) out[r.n] = c;
       return;
     }
-    if (tid == 0) {
+    if (tid == 0 && !alone) {
       // Store, count and the last one's loads are accesses of device scope, past the L2
       // caches; the store has been performed before the count is sent.  (Release and
       // acquire would write back and drop a whole L2 in every workgroup.)
@@ -517,14 +527,18 @@ __device__ void verify_rest(const Args& a, const Rec* __restrict__ rec, double* 
       count = __hip_atomic_fetch_add(arrived + b, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
-    if (count != n_ch - 1) return;
+    if (!alone && count != n_ch - 1) return;
     // every wavefront finds the chunk for itself
-    double s = lane < n_ch ? __hip_atomic_load(part + (long)b * kMaxChunks + lane, __ATOMIC_RELAXED,
-                                               __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    auto scanned = [&] { return lane < n_ch ? prec->sum * (double)below(prec->xmax, r.pmax, f) : 0.0; };
+    double s;
+    if (alone)
+      s = lane == ch ? all : scanned();
+    else
+      s = lane < n_ch ? __hip_atomic_load(part + (long)b * kMaxChunks + lane, __ATOMIC_RELAXED,
+                                          __HIP_MEMORY_SCOPE_AGENT) : 0.0;
     double at = wave_run(s), whole = lane_double(at, 63);
     if (!(whole > 0.0)) {  // p_n lies below q_n everywhere: then p_n itself
-      const Rec t = target_rec(a, rec, b, r.n)[min(lane, n_ch - 1)];
-      s = lane < n_ch ? t.sum * (double)below(t.xmax, r.pmax, f) : 0.0;
+      s = scanned();
       at = wave_run(s);
       whole = lane_double(at, 63);
       r.minus_q = false;

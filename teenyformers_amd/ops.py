@@ -984,10 +984,12 @@ def sample_rows(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0,
 
 def _logit_rows(name: str, x: torch.Tensor):
     """x [B, n, V] with its columns side by side, and the sequences' and rows' strides."""
-    V = x.shape[2]
-    if x.stride(2) != 1 and V > 1 or x.shape[1] > 1 and x.stride(1) < V or x.shape[0] > 1 and x.stride(0) < 0:
+    B, n, V = x.shape
+    seq, row, col = x.stride()
+    if col != 1 and V > 1 or n > 1 and row < V:
         x = x.contiguous()
-    return x, x.stride(0) if x.shape[0] > 1 else 0, x.stride(1) if x.shape[1] > 1 else V
+        seq, row, _ = x.stride()
+    return x, seq if B > 1 else 0, row if n > 1 else V
 
 
 def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor,
@@ -1010,9 +1012,10 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor,
     dev = logits.get_device()
     if dev < 0:
         raise ValueError("teenyformers_amd ops take device tensors (no CPU fallback)")
-    if logits.dim() != 3 or logits.shape[1] < 2 or logits.shape[2] < 1:
+    shape = logits.shape
+    if len(shape) != 3 or shape[1] < 2 or shape[2] < 1:
         raise ValueError("verify_drafts: logits are [B, K + 1, V] with K and V at least 1")
-    B, K, V = logits.shape[0], logits.shape[1] - 1, logits.shape[2]
+    B, K, V = shape[0], shape[1] - 1, shape[2]
     code = _code(logits)
 
     def of(name, t, shape, dtype):
