@@ -1026,7 +1026,7 @@ def verify_drafts(logits: torch.Tensor, drafts: torch.Tensor, u: torch.Tensor,
 
     of("drafts", drafts, (B, K), torch.int64)
     of("u", u, (B, K + 1), torch.float32)
-    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=logits.device) if tokens is None else \
+    tokens = torch.empty_like(u, dtype=torch.int64) if tokens is None else \
         of("tokens", tokens, (B, K + 1), torch.int64)
     accepted = torch.empty(B, dtype=torch.int32, device=logits.device) if accepted is None else \
         of("accepted", accepted, (B,), torch.int32)
