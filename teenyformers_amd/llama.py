@@ -278,15 +278,17 @@ class PagedKVCache:
 
     def reserve(self, seqs, counts):
         """Room for counts[i] more keys of seqs[i]: pages are taken, and those to be
-        written that other sequences share are replaced by copies.  All or nothing:
-        without enough free pages it raises and leaves everything as it was."""
+        written that other sequences share are replaced by copies.  Pages that a sequence
+        holds already count for it alone.  All or nothing: without enough free pages it
+        raises and leaves everything as it was."""
         if len(set(seqs)) != len(seqs) or len(seqs) != len(counts) or min(counts, default=0) < 0:
             raise ValueError("reserve: a count for each of different sequences")
         size, copies, grow, shared = self.page_size, [], 0, {}
         for seq, n in zip(seqs, counts):
             table, length = self.tables[seq], self.lengths[seq]
-            grow += -(-(length + n) // size) - len(table)
-            for i in range(length // size, len(table)) if n else ():
+            need = -(-(length + n) // size)
+            grow += max(0, need - len(table))
+            for i in range(length // size, min(need, len(table))) if n else ():
                 left = shared.get(table[i], self._uses[table[i]])
                 if left > 1:  # (the last one to write a page keeps it)
                     shared[table[i]] = left - 1

@@ -169,3 +169,135 @@ def test_default_temperature_with_drafts(monkeypatch):
     monkeypatch.setattr(generate, "generate_text", lambda args: seen.append((args.temperature, args.on_device)) or 0)
     assert generate.main(["--model-dir", "unread", "--draft-len", "4"]) == 0
     assert seen == [(0.0, True)]
+
+
+def state_of(cache):
+    return ({s: list(t) for s, t in cache.tables.items()}, dict(cache.lengths), list(cache._uses),
+            sorted(cache._free), cache.pages.clone())
+
+
+def same_state(a, b):
+    return a[:4] == b[:4] and torch.equal(a[4], b[4])
+
+
+def counted(cache):
+    """Uses and free pages are those of the tables, which may hold more than their keys need."""
+    uses = [0] * len(cache._uses)
+    for seq, table in cache.tables.items():
+        assert len(table) >= -(-cache.lengths[seq] // 16)
+        for page in table:
+            uses[page] += 1
+    assert uses == cache._uses
+    assert sorted(cache._free) == [i for i, n in enumerate(uses) if n == 0]
+
+
+@pytest.fixture
+def small(monkeypatch):
+    monkeypatch.setattr(ops, "copy_pages", copy_pages)
+    c = llama.PagedKVCache(CFG, 8, 16, torch.float32, "cpu")
+    c.pages.zero_()
+    return c
+
+
+def test_pages_held_ahead_are_not_others_room(small):
+    """A sequence that holds more pages than a call needs brings none to the others of the call."""
+    a, b = small.add(), small.add()
+    small.reserve([a], [96])
+    was = state_of(small)
+    with pytest.raises(RuntimeError, match="free pages"):
+        small.reserve([a, b], [1, 64])
+    assert same_state(was, state_of(small))
+    small.reserve([a, b], [1, 32])
+    assert small.free_pages == 0 and len(small.tables[a]) == 6 and len(small.tables[b]) == 2
+    counted(small)
+
+
+def test_no_room_leaves_a_fork_its_page(small):
+    """... nor takes it a fork's page away before the copy."""
+    a, b = small.add(), small.add()
+    write(small, [a], [[1.0, 2.0]])
+    small.reserve([a], [62])
+    (f,) = small.fork(a)
+    was = state_of(small)
+    with pytest.raises(RuntimeError, match="free pages"):
+        small.reserve([a, f, b], [1, 1, 64])
+    assert same_state(was, state_of(small))
+    assert read(small, f) == [1.0, 2.0]
+
+
+def test_forks_of_pages_held_ahead(small):
+    """Shared pages that a call does not write to are not copied by it, but by the one that does."""
+    a = small.add()
+    write(small, [a], [[float(i) for i in range(20)]])
+    small.reserve([a], [40])  # four pages, two without a key
+    (f,) = small.fork(a)
+    write(small, [f], [[100.0]])  # the second page alone
+    assert small.free_pages == 3 and small.tables[f][2:] == small.tables[a][2:]
+    write(small, [f, a], [[101.0] * 15, [200.0] * 15])  # ... and the third of each
+    counted(small)
+    assert read(small, f) == [float(i) for i in range(20)] + [100.0] + [101.0] * 15
+    assert read(small, a) == [float(i) for i in range(20)] + [200.0] * 15
+
+
+def test_a_pass_that_raises_behind_its_room(small, monkeypatch):
+    """run_paged reserves before it runs: after an error the keys are as they were and the pages count."""
+    m = llama.Llama(CFG, {})
+    a, b = small.add(), small.add()
+    write(small, [a], [[1.0, 2.0, 3.0]])
+    monkeypatch.setattr(m, "hidden", lambda *_: (_ for _ in ()).throw(TypeError("mixed types")))
+    with pytest.raises(TypeError):
+        m.run_paged(small, [a, b], [[1] * 60, [2]])
+    assert small.lengths == {a: 3, b: 0} and read(small, a) == [1.0, 2.0, 3.0]
+    counted(small)
+    was = state_of(small)
+    with pytest.raises(RuntimeError, match="free pages"):
+        small.reserve([a, b], [1, 6 * 16])
+    assert same_state(was, state_of(small))
+    small.truncate(a, 3)
+    assert small.free_pages == 6
+    counted(small)
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_use_with_room_ahead(cache, seed):
+    """As test_random_use, with pages reserved ahead, shared, given back and asked for in vain."""
+    rng = random.Random(1000 + seed)
+    want, counter = {}, iter(range(10 ** 6))
+    for _ in range(200):
+        what = rng.choice(["add", "fork", "write", "write", "write", "ahead", "ahead", "truncate", "remove", "compact"])
+        seqs = list(want)
+        was = state_of(cache)
+        if what == "add" and len(seqs) < 8:
+            want[cache.add()] = []
+        elif what == "fork" and seqs and len(seqs) < 8:
+            s = rng.choice(seqs)
+            for f in cache.fork(s, rng.randint(1, 2)):
+                want[f] = list(want[s])
+        elif what in ("write", "ahead") and seqs:
+            some = rng.sample(seqs, rng.randint(1, len(seqs)))
+            counts = [rng.choice([0, 1, 1, 3, 17, 40, 150]) for _ in some]
+            try:
+                if what == "ahead":
+                    cache.reserve(some, counts)
+                elif max(counts) > 0:
+                    values = [[float(next(counter)) for _ in range(n)] for n in counts]
+                    write(cache, some, values)
+                    for s, v in zip(some, values):
+                        want[s] += v
+            except RuntimeError:
+                assert [x for x in was[:4]] == [x for x in state_of(cache)[:4]]
+        elif what == "truncate" and seqs:
+            s = rng.choice(seqs)
+            n = rng.randint(0, len(want[s]))
+            cache.truncate(s, n)
+            want[s] = want[s][:n]
+        elif what == "remove" and seqs:
+            s = rng.choice(seqs)
+            cache.remove(s)
+            del want[s]
+        elif what == "compact":
+            n = cache.compact()
+            assert all(p < n for t in cache.tables.values() for p in t) and n == len(cache._uses) - cache.free_pages
+        counted(cache)
+        for s, v in want.items():
+            assert read(cache, s) == v
