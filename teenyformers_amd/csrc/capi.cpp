@@ -1672,8 +1672,8 @@ size_t teeny_paged_attention_workspace_bytes(int batch, int tokens, int max_new,
   if (batch <= 0 || tokens <= 0 || max_new <= 0 || max_keys <= 0 || n_heads_q <= 0 ||
       n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0 || head_dim <= 0 || !dtype_ok(dtype))
     return 0;
-  const PagedPlan p = paged_plan(batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv, head_dim,
-                                 dtype);
+  const PagedPlan p = paged_plan(batch, tokens, std::min(max_new, tokens), max_keys, n_heads_q,
+                                 n_heads_kv, head_dim, dtype);  // (as the call clamps it)
   return paged_part_bytes(paged_rows_few(p, batch, tokens, n_heads_q, n_heads_kv), head_dim) +
          paged_part_bytes(paged_rows_many(p, tokens, n_heads_q), head_dim);
 }
@@ -1695,7 +1695,7 @@ int teeny_paged_attention(const void* q, const void* k_pages, const void* v_page
   const uintptr_t at = (uintptr_t)q | (uintptr_t)o | (uintptr_t)k_pages | (uintptr_t)v_pages;
   if (at % 16 != 0) return TEENY_ERR_INVALID_VALUE;
   if (tokens == 0 || max_new == 0) return TEENY_OK;
-  max_new = starts ? std::min(max_new, tokens) : a.each;
+  max_new = std::min(std::max(max_new, a.each), tokens);  // (each: 0 with starts)
   max_keys = std::max(1, std::min(max_keys, table_width * page_size));
   PagedPlan p = paged_plan(batch, tokens, max_new, max_keys, n_heads_q, n_heads_kv, head_dim, dtype);
   p.scale = softmax_scale;

@@ -596,3 +596,36 @@ def test_verify_drafts_validation(L):
     assert verify(ws=None) == WS and verify(size=64) == WS
     ws = L.teeny_verify_drafts_workspace_bytes
     assert ws(2, 3, 100, 1) > 0 and ws(2, 65, 100, 1) == 0 and ws(0, 3, 100, 0) == 0 and ws(1 << 15, 3, 100, 0) == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_paged_workspace_is_enough(L, dtype):
+    """The bytes asked for with the arguments of a call are enough for it, also where max_new is
+    above the tokens, or above the new tokens of each without starts."""
+    import random
+
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("a call that no check refuses would launch")
+    rng = random.Random(dtype)
+    ws = L.teeny_paged_attention_workspace_bytes
+
+    def att(b, t, new, keys, hq, hkv, d, starts, size):
+        # (a misaligned workspace: refused behind the check of its size, before any launch)
+        return L.teeny_paged_attention(P, P, P, P, P, 4096, 4096, starts, P, 0, b, t, new, keys, 9, 16, hq, hkv,
+                                       d, 0.1, dtype, P + 8, size, None)
+
+    shares = 0
+    for _ in range(4000):
+        hkv = rng.choice([1, 2, 4, 8])
+        hq, d = hkv * rng.choice([1, 2, 4, 8]), rng.choice([64, 128])
+        b, each = rng.choice([1, 1, 2, 5, 16]), rng.choice([1, 1, 2, 4, 9, 40, 500])
+        new, keys = rng.choice([each, each, 2 * each, 7 * each, 4096]), rng.choice([64, 500, 4000, 30000])
+        a = (b, b * each, new, keys, hq, hkv, d)
+        need = ws(*a, dtype)
+        for starts in (None, P):
+            if need == 0:
+                continue  # (nothing to check it by: the call would launch)
+            shares += 1
+            assert att(*a, starts, need) == VALUE, a
+    assert shares > 1000
