@@ -548,8 +548,10 @@ __device__ void paged_merge(const PagedParts parts, T* __restrict__ o, const Pag
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const float e = i0 + u * groups < n ? fast_exp2(mi[u] - ref) : 0.0f;
-      if (e == 0.0f) continue;  // (a share without a key, or without weight)
+      if (i0 + u * groups >= n) continue;
+      // (a share without a key has sums of zero; one whose scores are all NaN has no maximum
+      // either, but NaN in its sums, which the row's are then)
+      const float e = fast_exp2(mi[u] - ref);
       acc += e * v[u];
       den += e * li[u];
     }

@@ -565,3 +565,26 @@ def test_far_lengths_of_one_sequence(cuda):
         c = Batch(dtype, 4, 1, D, 64, [100000], [1])
         c.check(c.run(max_keys=100001))
         c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,D", [(F32, 4, 2, 64), (BF, 8, 2, 64), (BF, 8, 2, 128)])
+@pytest.mark.parametrize("where", ["q", "k"])
+def test_attention_of_nan_is_nan(cuda, dtype, Hq, Hkv, D, where):
+    """A row whose scores are NaN, all of them or those of one share's keys, is NaN in one share and
+    in several; the others are as they were."""
+    for past, lens in (([40, 30], [2, 1]), ([9000, 30], [2, 1]), ([40, 3000], [60, 2]), ([9000, 30], [60, 1])):
+        c = Batch(dtype, Hq, Hkv, D, 16, past, lens)
+        keys = max(n + m for n, m in zip(past, lens))
+        ref = c.run(max_new=max(lens), max_keys=keys)
+        c.check(ref)
+        if where == "q":
+            c.q[1] = NAN  # one token of the first sequence
+        else:
+            c.k[c.table[0, :128 if past[0] > 2048 else 1].long()] = NAN  # its first keys: whole shares
+        got = c.run(max_new=max(lens), max_keys=keys)
+        if where == "q":
+            assert got[1].isnan().all()
+            assert torch.equal(got[:1], ref[:1]) and torch.equal(got[2:], ref[2:])
+        else:
+            assert got[:lens[0]].isnan().all()
+            assert torch.equal(got[lens[0]:], ref[lens[0]:])
