@@ -33,19 +33,17 @@ DEVI Seq seq_of(const Paged& a, int b) {
   s.past = min(max(a.past ? a.past[b] : a.past_all, -a.tokens), s.cap);
   return s;
 }
-// The sequence of token t (wave-uniform): the one before the first that starts behind it;
-// -1: none.  A wavefront looks at 64 starts at a time.
+// The sequence of token t (wave-uniform), the first that has it as seq_of sees it, whatever
+// the starts of others are; -1: none.  A wavefront looks at 64 sequences at a time.
 DEVI int seq_at(const Paged& a, int t) {
   if (!a.starts) return t < a.batch * a.each ? t / a.each : -1;
   const int lane = threadIdx.x & 63;
-  int n = 0;
-  for (int i = 0; i <= a.batch; i += 64) {
-    const bool yes = i + lane <= a.batch && a.starts[min(i + lane, a.batch)] <= t;
-    const uint64_t all = __ballot(yes);
-    n += ~all ? __builtin_ctzll(~all) : 64;
-    if (~all) break;
+  for (int i = 0; i < a.batch; i += 64) {
+    const int b = min(i + lane, a.batch - 1), t0 = a.starts[b], t1 = a.starts[b + 1];
+    const uint64_t has = __ballot(t0 >= 0 && t0 <= t && t < t1 && t1 <= a.tokens);
+    if (has) return i + (int)__builtin_ctzll(has);
   }
-  return n > 0 && n <= a.batch ? n - 1 : -1;
+  return -1;
 }
 
 // A wavefront's way along a sequence's table: 64 entries in a register, the first ones

@@ -588,3 +588,26 @@ def test_attention_of_nan_is_nan(cuda, dtype, Hq, Hkv, D, where):
         else:
             assert got[:lens[0]].isnan().all()
             assert torch.equal(got[lens[0]:], ref[lens[0]:])
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_sequences_behind_one_of_broken_starts(cuda, dtype):
+    """A sequence whose starts lie outside the batch, or fall, has no tokens; those behind it have
+    theirs, in the split as in the attention."""
+    past, lens = [20, 9, 2500, 50], [3, 0, 5, 2]
+    for broken in ([0, 10 ** 6, 3, 8, 10], [0, -9, 3, 8, 10], [7, 0, 3, 8, 10], [2 ** 31 - 1, -2 ** 31, 3, 8, 10]):
+        c = Batch(dtype, 8, 2, 64, 16, past, lens)
+        qkv = c.rnd(10, (8 + 2 * 2) * 64)
+        k, v = c.k.clone(), c.v.clone()
+        want_q = ops.paged_qkv_rope_split(qkv, k, v, c.table, c.n_past, 8, 1e4, starts=c.starts)
+        want = ops.paged_attention(c.q, k, v, c.table, c.n_past, starts=c.starts, max_keys=2600)
+        c.starts.copy_(torch.tensor(broken, dtype=torch.int64).to(torch.int32))
+        q = torch.full_like(want_q, 7.0)
+        ops.paged_qkv_rope_split(qkv, c.k, c.v, c.table, c.n_past, 8, 1e4, starts=c.starts, q_out=q)
+        assert torch.equal(q[3:], want_q[3:])
+        for b in (2, 3):
+            for got, there in zip((c.k, c.v), (k, v)):
+                pages = c.table[b][c.table[b] >= 0].long()
+                assert torch.equal(got[pages].nan_to_num(1.0), there[pages].nan_to_num(1.0))
+        out = torch.full_like(c.q, 7.0)
+        c.run(out=out, max_keys=2600)
+        assert torch.equal(out[3:], want[3:])
