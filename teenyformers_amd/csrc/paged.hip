@@ -58,13 +58,13 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
   if (wave < TOK) {
     const int t = tok0 + wave;
     const int b = t < a.tokens ? seq_at(a, t) : -1;
-    long row = -1;
-    int pos = 0, in = 0;
+    long row = -1, pos = 0;
+    int in = 0;
     if (b >= 0) {
       const Seq s = seq_of(a, b);
       const int i = t - s.t0;
       in = i >= 0 && i < s.n;
-      pos = s.past + i;
+      pos = (long)(a.past ? a.past[b] : a.past_all) + i;  // (behind the table too: q is rotated)
       if (in && pos >= 0 && pos < s.cap) {
         const int page = a.table[(long)b * a.ld + (pos >> a.lg)];
         if ((unsigned)page < (unsigned)a.n_pages)
@@ -77,7 +77,7 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
     }
     if (lane < head_dim / 2) {
       // turns, less whole ones: in [-1/2, 1/2]
-      double turn = pos * (exp(-2.0 * lane * ln_base / head_dim) * 0.15915494309189533577);
+      double turn = (double)pos * (exp(-2.0 * lane * ln_base / head_dim) * 0.15915494309189533577);
       turn -= rint(turn);
       double sn, cn;
       sincospi(2.0 * turn, &sn, &cn);

@@ -611,3 +611,22 @@ def test_sequences_behind_one_of_broken_starts(cuda, dtype):
         out = torch.full_like(c.q, 7.0)
         c.run(out=out, max_keys=2600)
         assert torch.equal(out[3:], want[3:])
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_split_far_behind_the_table(cuda, dtype):
+    """q is rotated by the token's own position, however far behind the table that lies."""
+    Hq, Hkv, D = 4, 2, 64
+    c = Batch(dtype, Hq, Hkv, D, 16, [30, 10, 60], [2, 2, 2], width=4)
+    before = c.k.clone(), c.v.clone()
+    qkv = c.rnd(6, (Hq + 2 * Hkv) * D)
+    x = qkv.view(6, -1, D)[:, :Hq]
+    for n in ([64, 65, 1000], [100, 300000, 10 ** 9]):
+        c.n_past.copy_(torch.tensor(n, dtype=torch.int32))
+        q = ops.paged_qkv_rope_split(qkv, c.k, c.v, c.table, c.n_past, Hq, 1e4)
+        pos = (torch.tensor(n)[:, None] + torch.arange(2)).view(-1).cuda()
+        y, tol = rotated(x, pos, 1e4)
+        # (angles of 1e9 in 64 bits: 1e9 times three roundings of 2^-53)
+        tol = tol + (4e-7 if n[2] > 10 ** 6 else 0.0) * x.abs().max().item()
+        assert ((q.double() - y).abs() <= tol).all()
+        for now, then in zip((c.k, c.v), before):
+            assert torch.equal(now.nan_to_num(1.0), then.nan_to_num(1.0))
