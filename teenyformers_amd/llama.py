@@ -683,9 +683,10 @@ class Llama:
         """Continuations of prompts (1-D ids each), several tokens a step: up to n_draft
         tokens are drafted for each sequence, by the model `draft` or looked up in its text
         (lookup_drafts), checked in one pass (run_paged) and accepted or replaced
-        (ops.verify_drafts), so that they are distributed as this model's own; greedy at
-        temperature 0.  With a filter the tokens are drawn row by row (ops.sample_rows) and
-        a draft stays while it is what was drawn.
+        (ops.verify_drafts), so that they are distributed as this model's own.  With a filter
+        the tokens are drawn row by row (ops.sample_rows) and a draft stays while it is what
+        was drawn; so, without one, at temperature 0, with generate's choice of each row
+        (ops.argmax_rows: the last of equal maxima).
 
         samples: continuations of each prompt, which runs once and whose pages they share.
         u: random numbers fp32 [n_new, B, n_draft + 1], B = len(prompts) * samples, with a
@@ -707,7 +708,14 @@ class Llama:
             raise ValueError("draft_steps: a prompt has at least one token")
         how = (temperature, top_k, top_p, min_p)
         filters = top_k > 0 or top_p < 1.0 or min_p > 0.0
+        greedy = temperature == 0.0 and not filters
         device = u.device
+
+        def choose(logits, un, how=how):
+            """A token of each row [.., vocab], as lists."""
+            if greedy:
+                return ops.argmax_rows(logits).view(logits.shape[:-1]).tolist()
+            return ops.sample_rows(logits, un, *how).tolist()
 
         def fill(model):
             """The prompts in a cache of their own, each forked -> cache, sequences, logits."""
@@ -722,7 +730,7 @@ class Llama:
         cache, seqs, logits = fill(self)
         if draft is not None:
             dcache, dseqs, _ = fill(draft)
-        nxt = ops.sample_rows(logits, u[0, :, n_draft].contiguous(), *how).tolist()
+        nxt = choose(logits, u[0, :, n_draft].contiguous())
         texts = [list(t) for t in texts for _ in range(samples)]
         made = [0] * B
         live = list(range(B))
@@ -759,14 +767,14 @@ class Llama:
                 guess, q = [[] for _ in now], []
                 for j in range(k):
                     q.append(draft.run_paged(dcache, [dseqs[b] for b in now], feed))
-                    drawn = ops.sample_rows(q[-1], un[:, n_draft + 1 + j].contiguous(), temperature).tolist()
+                    drawn = choose(q[-1], un[:, n_draft + 1 + j].contiguous(), (temperature,))
                     for x, t in zip(guess, drawn):
                         x.append(t)
                     feed = [[max(t, 0)] for t in drawn]
                 guess = [x[:r] for x, r in zip(guess, room)]
             if k == 0:
                 logits = self.run_paged(cache, [seqs[b] for b in now], [texts[b][-1:] for b in now])
-                tokens = ops.sample_rows(logits, un[:, n_draft].contiguous(), *how).view(-1, 1).tolist()
+                tokens = [[t] for t in choose(logits, un[:, n_draft].contiguous())]
                 accepted = [0] * len(now)
             else:
                 rows = [x + [-1] * (k - len(x)) for x in guess]
@@ -774,8 +782,8 @@ class Llama:
                 logits = self.run_paged(cache, [seqs[b] for b in now], ids, all_rows=True)
                 logits = logits.view(len(now), k + 1, -1)
                 pick = torch.cat([un[:, :k], un[:, n_draft:n_draft + 1]], 1)
-                if filters:
-                    tokens = ops.sample_rows(logits, pick.view(-1), *how).tolist()
+                if filters or greedy:
+                    tokens = choose(logits, pick.view(-1))
                     accepted = []
                     for t, x in zip(tokens, rows):
                         n = 0

@@ -234,3 +234,25 @@ def test_command_drafts(cuda, tmp_path):
     two = run("--draft-len", "3", "--num-samples", "2", "--temperature", "0.8")
     assert two.count("--- ") == 2
     assert run("--draft-len", "3", "--top-k", "5").startswith("w5 w17 w3 w5 w17")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_greedy_drafts_of_equal_logits(cuda, dtype):
+    """Every token has a twin of the same embedding, so of the same logit: greedy decoding takes the
+    last of them, with drafts as without."""
+    m = model_of(dtype, std=0.15)
+    m.w["model.embed_tokens.weight"][48:] = m.w["model.embed_tokens.weight"][:48]
+    d = llama.Llama(m.cfg, m.w)
+    prompts, n_new, K = [ids_of(9, seed=1, vocab=48), ids_of(20, seed=2, vocab=48)], 12, 3
+    for draft in (None, d):
+        u = torch.rand((n_new, 2, (2 if draft else 1) * K + 1), device="cuda")
+        got = m.generate_drafted(prompts, u, K, temperature=0.0, draft=draft, page_size=16)
+        for p, t in zip(prompts, got):
+            assert min(t) >= 48 and len(t) == n_new
+            assert int(m.generate(p[None], n_new).min()) >= 48
+            if dtype == F32:
+                seq, x = p.tolist(), None
+                for tok in t:
+                    x = m.forward(torch.tensor([seq], device="cuda"))[0, -1].double()
+                    assert x[tok] >= x.max() - 2 * CLOSE * x.norm()
+                    seq.append(tok)

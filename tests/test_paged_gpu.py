@@ -589,6 +589,7 @@ def test_attention_of_nan_is_nan(cuda, dtype, Hq, Hkv, D, where):
             assert got[:lens[0]].isnan().all()
             assert torch.equal(got[lens[0]:], ref[lens[0]:])
 
+
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_sequences_behind_one_of_broken_starts(cuda, dtype):
     """A sequence whose starts lie outside the batch, or fall, has no tokens; those behind it have
@@ -611,6 +612,7 @@ def test_sequences_behind_one_of_broken_starts(cuda, dtype):
         out = torch.full_like(c.q, 7.0)
         c.run(out=out, max_keys=2600)
         assert torch.equal(out[3:], want[3:])
+
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 def test_split_far_behind_the_table(cuda, dtype):
