@@ -707,6 +707,9 @@ class Llama:
         if min(len(t) for t in texts) < 1:
             raise ValueError("draft_steps: a prompt has at least one token")
         how = (temperature, top_k, top_p, min_p)
+        if any(isinstance(x, torch.Tensor) for x in how):
+            raise ValueError("draft_steps: temperature, top_k, top_p and min_p are numbers, those of all "
+                             "sequences")
         filters = top_k > 0 or top_p < 1.0 or min_p > 0.0
         greedy = temperature == 0.0 and not filters
         device = u.device

@@ -301,3 +301,13 @@ def test_random_use_with_room_ahead(cache, seed):
         counted(cache)
         for s, v in want.items():
             assert read(cache, s) == v
+
+
+def test_draft_settings_are_numbers():
+    """The batch of a run of drafts shrinks as sequences end: settings of each sequence are refused
+    before anything runs, not when the first one has ended."""
+    m = llama.Llama(CFG, {})
+    for kw in (dict(temperature=torch.ones(2)), dict(top_k=torch.ones(2, dtype=torch.int32)),
+               dict(top_p=torch.ones(2)), dict(min_p=torch.zeros(2))):
+        with pytest.raises(ValueError, match="are numbers"):
+            next(m.draft_steps([[1], [2]], torch.zeros((4, 2, 4)), 3, **kw))
