@@ -1,13 +1,10 @@
 // A row of logits in chunks, and wavefront sums: what the kernels that draw tokens
 // share (sample.hip, verify.hip).
 #pragma once
+#include "chunks.h"
 #include "common.h"
 
 typedef unsigned long long u64;
-
-constexpr int kTok = 8;                   // tokens of a thread's vector
-constexpr int kChunk = 8192;              // columns per chunk
-constexpr int kMaxChunks = 64;            // a lane each
 
 // The logits of thread slot `slot` of chunk ch: columns col .. col + 7, those
 // outside the row as -inf.  A chunk starts at a 16-byte aligned address, which

@@ -178,11 +178,9 @@ __device__ void verify_scan(const Args& a, Rec* __restrict__ rec, int* __restric
   u32x4 raw[kVec][VW];
   auto load = [&](const Place& p) __attribute__((always_inline)) {
     if (a.cols < 2 * kTok) return;
-    const T* some = p.row + (p.c0 < 0 ? p.c0 + kTok : 0);  // a whole vector of the row
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-      const int c = p.c0 + (v * kScan + tid) * kTok;
-      const T* src = c >= 0 && c + kTok <= a.cols ? p.row + c : some;
+      const T* src = p.row + vector_col(p.c0 + (v * kScan + tid) * kTok, a.cols);
 #pragma unroll
       for (int w = 0; w < VW; ++w)
         raw[v][w] = *reinterpret_cast<const u32x4*>(src + w * Vec16<T>::N);

@@ -629,3 +629,38 @@ def test_paged_workspace_is_enough(L, dtype):
             shares += 1
             assert att(*a, starts, need) == VALUE, a
     assert shares > 1000
+
+
+def test_logit_vectors_lie_in_their_row(tmp_path):
+    """Every vector that the scans of logits load lies in its row and is aligned, for rows of any
+    number of columns at any offset: the loader's own arithmetic, over all its threads."""
+    import os
+    import shutil
+    import subprocess
+    if not shutil.which("g++"):
+        pytest.skip("no host compiler")
+    src = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+    (tmp_path / "t.cpp").write_text(r"""
+#include <cstdio>
+#include "chunks.h"
+int main() {
+  long bad = 0, n = 0;
+  const int near[] = {16, 17, 23, 24, 31, 1000, 8176, 8184, 8185, 8190, 8191, 8192, 8193, 8194, 8196, 8199, 8200,
+                      8208, 16377, 16383, 16384, 16385, 32000, 32768, 50257, 65536, 128255, 128256, 131072};
+  for (int cols : near)
+    for (int per = 4; per <= 8; per += 4)       // elements of 16 bytes: fp32, bf16
+      for (int mis = 0; mis < per; ++mis)       // elements behind an aligned address
+        for (int ch = 0; ch < (cols + 7 + kChunk - 1) / kChunk; ++ch)
+          for (int slot = 0; slot < kChunk / kTok; ++slot, ++n) {
+            const int c = ch * kChunk - mis + slot * kTok, at = vector_col(c, cols);
+            if (at < 0 || at + kTok > cols || (at + mis) % per != 0) ++bad;
+            if (c >= 0 && c + kTok <= cols && at != c) ++bad;
+          }
+  std::printf("%ld %ld\n", bad, n);
+  return bad != 0;
+}
+""")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", src, str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")], check=True)
+    out = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True)
+    assert out.returncode == 0, out.stdout
+    assert int(out.stdout.split()[1]) > 100000
