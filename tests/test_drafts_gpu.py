@@ -256,3 +256,132 @@ def test_greedy_drafts_of_equal_logits(cuda, dtype):
                     x = m.forward(torch.tensor([seq], device="cuda"))[0, -1].double()
                     assert x[tok] >= x.max() - 2 * CLOSE * x.norm()
                     seq.append(tok)
+
+
+def recorded(model, log):
+    """The model's passes over pages, logged: their tokens by sequence, and their logits."""
+    run = model.run_paged
+
+    def wrapper(cache, seqs, ids, all_rows=False):
+        rows = run(cache, seqs, ids, all_rows)
+        log.append(([[int(t) for t in x] for x in ids], rows.clone()))
+        return rows
+
+    model.run_paged = wrapper
+
+
+@pytest.mark.parametrize("how", ["lookup", "model", "filter", "greedy", "greedy model"])
+@pytest.mark.parametrize("ends", [False, True])
+def test_steps_replayed_token_by_token(cuda, how, ends):
+    """Every pass of a run of drafts holds the tokens that it should and gives the logits of whole
+    passes over its sequences' texts, and every step's tokens are the definition's on those logits and
+    the step's random numbers, to the last one."""
+    from tests.test_verify_gpu import outcomes
+    m = model_of(F32)
+    d = model_of(F32, std=0.075) if "model" in how else None
+    T, more = (0.0 if "greedy" in how else 0.9), dict(top_k=9) if how == "filter" else {}
+    prompts, samples, K, n_new, V = [[5, 17, 3, 5, 17], ids_of(33, seed=2).tolist()], 2, 3, 14, 96
+    g = torch.Generator(device="cuda").manual_seed(4)
+    u = torch.rand((n_new, 4, (2 if d else 1) * K + 1), generator=g, device="cuda")
+    run = dict(temperature=T, draft=d, samples=samples, page_size=16, **more)
+    eos = m.generate_drafted(prompts, u, K, **run)[0][6] if ends else None
+    log, dlog = [], []
+    recorded(m, log)
+    if d:
+        recorded(d, dlog)
+    steps = list(m.draft_steps(prompts, u, K, eos=eos, **run))
+    log = iter(log)
+    un = u.double().cpu().numpy()
+
+    def drawn(row, at, got, **more):
+        """Whether got is what the row [V] gives for the random number u[at]."""
+        if T == 0.0:
+            return got == V - 1 - int(row.flip(0).argmax())
+        if more:
+            return got == int(ops.sample_rows(row[None], u[at].reshape(1), T, **more))
+        x = row.double().cpu().numpy()
+        return got in outcomes(np.stack([x, x]), [-1], [0.0, un[at]], None, T)[0]
+
+    ids, rows = next(log)
+    assert ids == prompts
+    for p, row in zip(prompts, rows):
+        assert off(row, m.forward(torch.tensor([p], device="cuda"))[0, -1]) < CLOSE
+    texts = [list(p) for p in prompts for _ in range(samples)]
+    if d:
+        assert dlog.pop(0)[0] == prompts
+    held = [len(t) for t in texts]  # of the draft model's keys
+    for b in range(4):
+        assert len(steps[0][b]) == 1 and drawn(rows[b // samples], (0, b, K), steps[0][b][0], **more)
+    made, live, text0 = [[] for _ in range(4)], list(range(4)), [len(t) for t in texts]
+
+    def take(step):
+        for b in list(live):
+            new = steps[step][b]
+            assert new and len(made[b]) + len(new) <= n_new and (eos is None or eos not in new[:-1])
+            made[b] += new
+            texts[b] += new
+            if len(made[b]) == n_new or new[-1] == eos:
+                live.remove(b)
+
+    take(0)
+    step = 1
+    while live:
+        now = list(live)
+        room = [min(K, n_new - len(made[b]) - 1) for b in now]
+        k, q = max(room), None
+        if d is None:
+            guess = [llama.lookup_drafts(texts[b], r) for b, r in zip(now, room)]
+            k = max(len(x) for x in guess)
+        elif k:
+            guess, q = [[] for _ in now], [[] for _ in now]
+            for j in range(k):
+                ids, rows = dlog.pop(0)
+                for i, b in enumerate(now):
+                    assert ids[i] == (guess[i][-1:] if j else texts[b][held[b]:])
+                    whole = texts[b] + guess[i]
+                    assert off(rows[i], d.forward(torch.tensor([whole], device="cuda"))[0, -1]) < CLOSE
+                    q[i].append(rows[i])
+                    if j + 1 < k:  # what was drawn: the next pass holds it, the last one's the check
+                        guess[i].append(dlog[0][0][i][-1])
+            held = [held[b] if b not in now else len(texts[b]) + k - 1 for b in range(4)]
+        ids, rows = next(log)
+        at = 0
+        for i, b in enumerate(now):
+            if d is not None and k:
+                mine = ids[i][1:1 + room[i]]
+                assert mine[:len(guess[i])] == guess[i][:room[i]]
+                for j, t in enumerate(mine):
+                    assert drawn(q[i][j], (step, b, K + 1 + j), t)
+            else:
+                mine = guess[i] if k else []
+            assert ids[i] == texts[b][-1:] + mine + [0] * (k - len(mine))
+            x = rows[at:at + k + 1]
+            at += k + 1
+            whole = m.forward(torch.tensor([texts[b] + mine], device="cuda"))[0, len(texts[b]) - 1:]
+            for r in range(len(mine) + 1):
+                assert off(x[r], whole[r]) < CLOSE
+            new = steps[step][b]
+            if more or T == 0.0:
+                for r, t in enumerate(new):
+                    uu = (step, b, r) if r < k else (step, b, K)
+                    assert drawn(x[r], uu, t, **more)
+                n = len(new) - 1
+                assert new[:n] == mine[:n]
+                assert len(new) == len(mine) + 1 or new[n] != mine[n] or new[n] == eos
+            else:
+                xs = x.double().cpu().numpy()
+                ys = None if q is None else np.stack([z.double().cpu().numpy() for z in q[i][:k]])
+                row = mine + [-1] * (k - len(mine))
+                may = outcomes(xs, row, np.append(un[step, b, :k], un[step, b, K]), ys, T)
+                n = len(new) - 1
+                assert new[:n] == mine[:n]
+                assert (n in may and new[n] in may[n]) or (n < len(mine) and new[n] == mine[n] == eos)
+            if d is not None and k:
+                held[b] = min(held[b], len(texts[b]) + len(new) - 1)
+        take(step)
+        assert all(steps[step][b] == [] for b in range(4) if b not in now)
+        step += 1
+    assert step == len(steps) and next(log, None) is None and not dlog
+    for b in range(4):
+        assert len(made[b]) == n_new or made[b][-1] == eos
+        assert texts[b] == (prompts[b // samples] + made[b]) and text0[b] == len(prompts[b // samples])

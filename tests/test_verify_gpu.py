@@ -325,3 +325,76 @@ def test_extreme_temperatures_and_logits(cuda):
     assert tokens[:, 0].tolist() == [50, 40, 11, 50]
     tokens, _ = ops.verify_drafts(z, drafts, uu, None, math.inf)
     assert tokens[3, 0] == 50
+
+
+def outcomes(x, d, u, y, T):
+    """One sequence: {accepted: the tokens that may be drawn there} for weights off by the derived
+    error: acceptance within EDGE relative, a running sum within EDGE of the whole.  Greedy: exact."""
+    n, V = x.shape
+    may, edge = {}, EDGE if T > 0 else 0.0
+
+    def draw(at, w, rest, but=-1):
+        c = np.cumsum(rest)
+        before = np.concatenate([[0.0], c[:-1]])
+        t = u[n - 1] * c[-1]
+        ok = (c > t - edge) & (before <= t + edge) & (w > 0)
+        if not T > 0:
+            ok = rest > 0
+        ok[[i for i in (but,) if i >= 0]] = False
+        may.setdefault(at, set()).update(np.nonzero(ok)[0].tolist() if c[-1] > 0 or ok.any() else [-1])
+
+    for i in range(n - 1):
+        p = probs(x[i], T)
+        if not 0 <= d[i] < V:
+            draw(i, p, p)
+            return may
+        q = np.zeros(V)
+        q[d[i]] = 1.0
+        if y is not None:
+            q = probs(y[i], T)
+        pd, qd = p[d[i]], q[d[i]]
+        slack = edge * max(pd, qd) if pd != qd else 0.0
+        if not u[i] * qd < pd - slack:  # may be refused
+            rest = np.maximum(p - q, 0.0)
+            if rest.sum() > 0:
+                draw(i, np.where(p > 0, 1.0, 0.0), rest, d[i])
+            if rest.sum() <= edge:
+                draw(i, p, p)
+        if not u[i] * qd < pd + slack:  # must be
+            return may
+    p = probs(x[n - 1], T)
+    draw(n - 1, p, p)
+    return may
+
+
+def check_every_row(x, drafts, u, y, T):
+    tokens, accepted = ops.verify_drafts(x, drafts, u, y, T)
+    tokens, accepted = tokens.cpu().numpy(), accepted.cpu().numpy()
+    x, d, un = x.double().cpu().numpy(), drafts.cpu().numpy(), u.double().cpu().numpy()
+    y = None if y is None else y.double().cpu().numpy()
+    T = np.broadcast_to(T.double().cpu().numpy() if torch.is_tensor(T) else float(T), len(x))
+    for b in range(len(x)):
+        may, n = outcomes(x[b], d[b], un[b], None if y is None else y[b], T[b]), int(accepted[b])
+        assert n in may, (b, n, sorted(may))
+        assert tokens[b, n] in may[n], (b, n, tokens[b, n], sorted(may[n])[:8])
+        assert (tokens[b, :n] == d[b, :n]).all() and (tokens[b, n + 1:] == -1).all()
+        assert (d[b, :n] >= 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("with_q", [False, True])
+@pytest.mark.parametrize("T", [0.0, 0.05, 0.8, 30.0])
+def test_every_row_is_the_definition_within_the_error(cuda, dtype, with_q, T):
+    """No sequence is left out: those next to a border have one of the outcomes beside it."""
+    for B, K, V in ((1, 1, 1), (40, 3, 3000), (60, 1, 300), (4, 2, 8193), (3, 5, 50257), (2, 64, 500)):
+        check_every_row(*case(dtype, B, K, V, 3 * B + V, with_q, T=max(T, 0.3)), T)
+    x, d, u, y = case(dtype, 32, 3, 700, 12, with_q)
+    x[:8, :, ::2] = -math.inf
+    x[8:10, 1] = -math.inf
+    x[10:12, :, 5] = float("nan")
+    d[12:15, 1] = -1
+    d[15, 0] = 700
+    if with_q:
+        y[16:20, :, ::3] = -math.inf
+        y[20:24] = x[20:24, :3]  # nearly every draft accepted
+    check_every_row(x, d, u, y, T)
