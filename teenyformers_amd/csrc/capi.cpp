@@ -1660,10 +1660,9 @@ int teeny_paged_qkv_rope_split(const void* qkv, const float* parts, int n_parts,
                     &ln_rope_base};
     return launch(name, dim3((unsigned)tokens), dim3(256), 0, stream, args);
   }
-  const bool one = tokens <= 4 * device_cus();
-  snprintf(name, sizeof name, "teeny_paged_split_%s%s", dtype_tag(dtype), one ? "_one" : "");
+  snprintf(name, sizeof name, "teeny_paged_split_%s", dtype_tag(dtype));
   void* args[] = {&qkv, &q_out, &k_pages, &v_pages, &a, &lg_d, &ln_rope_base};
-  return launch(name, dim3((unsigned)(one ? tokens : (tokens + 3) / 4)), dim3(256), 0, stream, args);
+  return launch(name, dim3((unsigned)tokens), dim3(256), 0, stream, args);
 }
 
 size_t teeny_paged_attention_workspace_bytes(int batch, int tokens, int max_new, int max_keys,

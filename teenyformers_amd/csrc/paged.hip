@@ -17,32 +17,32 @@
 namespace {
 
 // ---------------------------------------------------------------------------
-// split: TOK tokens a workgroup.  Their rows of the projection are one run of
-// memory; a thread's first loads are in flight while each wavefront finds a token's
-// sequence, position and page and its (cos, sin), once for all heads.
+// split: a workgroup a token.  Its row of the projection is one run of memory; a thread's
+// first loads are in flight while the first wavefront finds the token's sequence, position
+// and page and its (cos, sin), once for all heads.
 //
 // Angles are formed and reduced in 64 bits: of position p the fp32 product p base^
 // (-2k/D) is off by up to p 2^-24 radians (2e-3 at 32768), as much as a bf16 rounds.
 //
 // Bound by HBM where there are many tokens, else by one chain (starts, length, page table,
-// rows).  Hq32 Hkv8 D128 bf16: 8208 tokens, 202 MB read and written, 36 us (5.6 TB/s); 64
-// tokens of 64 sequences 3.9 us.
+// rows).  Hq32 Hkv8 D128, us with rows from HBM: bf16 512 tokens 6.4, 2048 13, 8208 40.5 (5.0
+// TB/s), 32768 150; fp32 9.5, 23, 80 (5.0 TB/s), 304; 64 tokens of 64 sequences, in caches,
+// 3.5, 4.1.  Workgroups of four tokens: 9.7, 16, 41.7, 158; 15, 26, 85, 318; 6.9, 9.9.
 // ---------------------------------------------------------------------------
-template <typename T, bool PARTS, int TOK>
+template <typename T, bool PARTS>
 __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__ parts, int n_parts,
                             long part_stride, T* __restrict__ q_out, T* __restrict__ kp,
                             T* __restrict__ vp, const Paged a, int lg_d, double ln_base) {
-  constexpr int NT = 256, VN = Vec16<T>::N, U = PARTS ? 1 : TOK == 1 ? 3 : 6;
-  static_assert(TOK <= NT / 64, "a wavefront a token");
-  __shared__ float2 cs[TOK][64];
-  __shared__ long at[TOK];  // element of the token's row in its page, head 0; -1: none
-  __shared__ int live[TOK];
+  constexpr int NT = 256, VN = Vec16<T>::N, U = PARTS ? 1 : 3;
+  __shared__ float2 cs[64];
+  __shared__ long at;  // element of the token's row in its page, head 0; -1: none
+  __shared__ int live;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int head_dim = 1 << lg_d, lg_v = lg_d - __builtin_ctz(VN);  // vectors of a head
-  const int vecs = (a.hq + 2 * a.hkv) << lg_v;                      // ... of a token
-  const int tok0 = blockIdx.x * TOK, total = min(TOK, a.tokens - tok0) * vecs;
-  const long src = (long)tok0 * vecs * VN;
+  const int total = (a.hq + 2 * a.hkv) << lg_v;                     // ... of the token
+  const int t = blockIdx.x;
+  const long src = (long)t * total * VN;
   u32x4 raw[U];
   float sum[VN];
   auto load = [&](int i0) __attribute__((always_inline)) {
@@ -55,9 +55,8 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
     }
   };
   load(tid);
-  if (wave < TOK) {
-    const int t = tok0 + wave;
-    const int b = t < a.tokens ? seq_at(a, t) : -1;
+  if (wave == 0) {
+    const int b = seq_at(a, t);
     long row = -1, pos = 0;
     int in = 0;
     if (b >= 0) {
@@ -72,8 +71,8 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
       }
     }
     if (lane == 0) {
-      at[wave] = row;
-      live[wave] = in;
+      at = row;
+      live = in;
     }
     if (lane < head_dim / 2) {
       // turns, less whole ones: in [-1/2, 1/2]
@@ -81,10 +80,11 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
       turn -= rint(turn);
       double sn, cn;
       sincospi(2.0 * turn, &sn, &cn);
-      cs[wave][lane] = make_float2((float)cn, (float)sn);
+      cs[lane] = make_float2((float)cn, (float)sn);
     }
   }
   __syncthreads();
+  if (!live) return;
   const long head_k = (long)1 << (a.lg + lg_d);  // elements between a page's kv heads
   for (int i0 = tid; i0 < total; i0 += U * NT) {
     if (i0 != tid) load(i0);
@@ -92,18 +92,14 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * NT;
       if (i >= total) break;
-      int tk = 0;
-#pragma unroll
-      for (int x = 1; x < TOK; ++x) tk += i >= x * vecs;
-      const int col = i - tk * vecs, head = col >> lg_v, v = col & ((1 << lg_v) - 1);
+      const int head = i >> lg_v, v = i & ((1 << lg_v) - 1);
       T* dst;
       if (head < a.hq) {
-        if (!live[tk]) continue;
-        dst = q_out + (((long)(tok0 + tk) * a.hq + head) << lg_d);
+        dst = q_out + (((long)t * a.hq + head) << lg_d);
       } else {
-        if (at[tk] < 0) continue;
+        if (at < 0) continue;
         const bool is_k = head < a.hq + a.hkv;
-        dst = (is_k ? kp : vp) + at[tk] + (head - a.hq - (is_k ? 0 : a.hkv)) * head_k;
+        dst = (is_k ? kp : vp) + at + (head - a.hq - (is_k ? 0 : a.hkv)) * head_k;
       }
       float in[VN], out[VN];
 #pragma unroll
@@ -114,7 +110,7 @@ __device__ void paged_split(const T* __restrict__ qkv, const float* __restrict__
         else in[j] = j & 1 ? bf16hi(w) : bf16lo(w);
       }
       if (head < a.hq + a.hkv) {
-        const float2* c = cs[tk] + v * (VN / 2);
+        const float2* c = cs + v * (VN / 2);
 #pragma unroll
         for (int j = 0; j < VN / 2; ++j)
           rope_rotate(in[2 * j], in[2 * j + 1], c[j].x, c[j].y, out[2 * j], out[2 * j + 1]);
@@ -574,21 +570,18 @@ __device__ void paged_merge(const PagedParts parts, T* __restrict__ o, const Pag
 
 }  // namespace
 
-#define TEENY_PAGED_SPLIT_INST(TN, T, SFX, TOK)                                                  \
-  extern "C" __global__ __launch_bounds__(256) void teeny_paged_split_##TN##SFX(                  \
+#define TEENY_PAGED_SPLIT_INST(TN, T)                                                            \
+  extern "C" __global__ __launch_bounds__(256) void teeny_paged_split_##TN(                       \
       const T* qkv, T* q_out, T* kp, T* vp, Paged a, int lg_d, double ln_base) {                  \
-    paged_split<T, false, TOK>(qkv, nullptr, 0, 0, q_out, kp, vp, a, lg_d, ln_base);              \
+    paged_split<T, false>(qkv, nullptr, 0, 0, q_out, kp, vp, a, lg_d, ln_base);                   \
   }
-TEENY_PAGED_SPLIT_INST(bf16, bf16, , 4)
-TEENY_PAGED_SPLIT_INST(bf16, bf16, _one, 1)
-TEENY_PAGED_SPLIT_INST(f32, float, , 4)
-TEENY_PAGED_SPLIT_INST(f32, float, _one, 1)
+TEENY_PAGED_SPLIT_INST(bf16, bf16)
+TEENY_PAGED_SPLIT_INST(f32, float)
 #define TEENY_PAGED_SPLIT_PARTS_INST(TN, T)                                                      \
   extern "C" __global__ __launch_bounds__(256) void teeny_paged_split_parts_##TN(                 \
       const float* parts, int n_parts, long part_stride, T* q_out, T* kp, T* vp, Paged a,         \
       int lg_d, double ln_base) {                                                                 \
-    paged_split<T, true, 1>(nullptr, parts, n_parts, part_stride, q_out, kp, vp, a, lg_d,         \
-                            ln_base);                                                             \
+    paged_split<T, true>(nullptr, parts, n_parts, part_stride, q_out, kp, vp, a, lg_d, ln_base);  \
   }
 TEENY_PAGED_SPLIT_PARTS_INST(bf16, bf16)
 TEENY_PAGED_SPLIT_PARTS_INST(f32, float)
