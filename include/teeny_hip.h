@@ -588,7 +588,7 @@ int teeny_qkv_rope_split_rows(const void* qkv, const float* parts, int n_parts, 
  * teeny_paged_qkv_rope_split: the QKV projection's rows (qkv [tokens, (Hq + 2 Hkv)
  * D], or qkv null and parts, K-split fp32 slabs as teeny_qkv_rope_split_partials_dev
  * takes them) to q_out [tokens, Hq, D] (rotated) and the rows of their pages (k
- * rotated, v).  Positions outside the table are not written.  Angles are formed in
+ * rotated, v).  Keys at positions outside the table are not written.  Angles are formed in
  * 64 bits (ln_rope_base too); the other splits form them in 32, as the reference
  * does, so far positions differ by up to p 2^-24 radians.
  *
@@ -596,7 +596,7 @@ int teeny_qkv_rope_split_rows(const void* qkv, const float* parts, int n_parts, 
  * token i of sequence b attends to keys 0 .. n_past[b] + i (its own is in its page
  * already) of the pages that are present, rows without a key give zeros.  Rows of
  * the pages behind the last key are never read, and a key has no influence on
- * tokens before it, whatever its values.  max_new: the most new tokens of a
+ * tokens before it, whatever its values; a row with a score of NaN is NaN.  max_new: the most new tokens of a
  * sequence (with more, their rows may be left as they were); max_keys: n_past plus
  * the new tokens at most, which only picks the number of shares.  workspace:
  * teeny_paged_attention_workspace_bytes bytes (for max_keys up to table_width *

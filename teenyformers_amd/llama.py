@@ -216,8 +216,9 @@ class PagedKVCache:
     page_size, D], taken as sequences grow and given back when they end.  A forked
     sequence shares its pages with the first one until one of them writes to a
     shared page, which is then copied (ops.copy_pages, all layers in one launch).
-    The host keeps tables, lengths and uses; nothing here waits for the GPU.  Calls
-    are of one stream: a page given back may be written by the next call on it."""
+    The host keeps tables, lengths and uses; of these calls only `batch`, whose copy to the
+    device is an ordinary one, waits for the stream.  Calls are of one stream: a page given
+    back may be written by the next call on it."""
 
     def __init__(self, cfg: LlamaConfig, n_pages: int, page_size: int = 64, dtype=torch.bfloat16,
                  device="cuda"):
