@@ -632,3 +632,21 @@ def test_split_far_behind_the_table(cuda, dtype):
         assert ((q.double() - y).abs() <= tol).all()
         for now, then in zip((c.k, c.v), before):
             assert torch.equal(now.nan_to_num(1.0), then.nan_to_num(1.0))
+
+
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (BF, 64), (BF, 128)])
+def test_one_key_of_nan(cuda, dtype, D):
+    """A key of NaN makes the rows that see it NaN, whatever share or tile it lies in, and no other."""
+    for past, lens in ((70, 3), (9000, 3), (70, 90), (3000, 90)):
+        c = Batch(dtype, 8, 2, D, 16, [past, 40], [lens, 1])
+        ref = c.run(max_new=lens, max_keys=past + lens)
+        for at in (0, past // 2, past - 1, past + 1, past + lens - 1):
+            page, row = c.table[0, at // 16], at % 16
+            was = c.k[page, 1, row].clone()
+            c.k[page, 1, row] = NAN
+            got = c.run(max_new=lens, max_keys=past + lens)
+            c.k[page, 1, row] = was
+            first = max(0, at - past)  # the first token that sees it
+            assert got[first:lens, 4:].isnan().all(), at
+            assert got[:first, 4:].isfinite().all(), at
+            assert torch.equal(got[:, :4], ref[:, :4]) and torch.equal(got[lens:], ref[lens:])
